@@ -137,9 +137,9 @@ def prepare(c, seed):
         tokens = torch.randint(0, V, (total,), generator=gen, device="cuda")
         judged = [b + j for b, n in zip(starts, rows) for j in range(n - 1)]   # the rows that judge a drafted token
         at = torch.tensor(judged, dtype=torch.int64, device="cuda")
-        draft = logits[at] + normal(len(judged), V, std=0.5) if c["draft"] else None
+        draft = logits + normal(total, V, std=0.5) if c["draft"] else None   # a sequence's last row judges nothing: unused
         # a draft model's tokens are drawn from its distribution; a text's own suggestions are often the most probable token
-        drawn = (draft if c["draft"] else logits[at] * 1.5) - torch.empty(len(judged), V, device="cuda").exponential_(generator=gen).log()
+        drawn = (draft[at] if c["draft"] else logits[at] * 1.5) - torch.empty(len(judged), V, device="cuda").exponential_(generator=gen).log()
         tokens[at + 1] = drawn.argmax(1)
         s.update(tokens=tokens, draft=draft)
         return s
@@ -300,8 +300,7 @@ def run_verify(s, c):
     chance = p[row, token]
     if c["draft"]:
         q = torch.softmax(s["draft"].double() / c["temperature"], 1)
-        drow = (row - torch.arange(B, device="cuda")[:, None]).clamp(max=max(0, q.shape[0] - 1))
-        q_of = q[drow, token] if q.shape[0] else torch.ones_like(chance)
+        q_of = q[row, token]
     else:
         q_of = torch.ones_like(chance)
     good = judged & (s["uniform"].double()[row] * q_of < chance)
@@ -309,8 +308,8 @@ def run_verify(s, c):
     last = start[:-1] + count
     left = p[last]
     refused = count < n - 1
-    if c["draft"] and q.shape[0]:
-        less = (left - q[(last - torch.arange(B, device="cuda")).clamp(max=q.shape[0] - 1)]).clamp(min=0)
+    if c["draft"]:
+        less = (left - q[last]).clamp(min=0)
     else:
         less = left.scatter(1, s["tokens"][(last + 1).clamp(max=s["logits"].shape[0] - 1)][:, None], 0.0)
     left = torch.where(refused[:, None], less, left)
@@ -403,7 +402,7 @@ def exact(c, seed):
                 p = e / e.sum()
                 if drafted is not None:
                     if c["draft"]:
-                        e = s["draft"][r - b].double()
+                        e = s["draft"][r].double()
                         e = ((e - e.max()) / T).exp()
                         q = e / e.sum()
                     else:
