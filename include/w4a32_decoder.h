@@ -251,6 +251,116 @@ int w4a32_op_matmul_nt(const float* d_a, const void* d_b, int b_dtype, float* d_
  * load and the f32 operators run on the result. */
 int w4a32_op_f16_to_f32(const void* d_in, float* d_out, size_t n, void* stream);
 
+/* ---- a batch of sequences on a paged cache ------------------------------------------------------
+ * Sequences of different lengths share pools of pages: token t of sequence b lies in page
+ * d_table[b][t / page] at t % page. A step takes rows of all of them at once: sequence b owns rows
+ * d_row_start[b] .. d_row_start[b + 1] (one token, a few drafted ones, a prompt's portion, or none), which
+ * stand behind its d_len[b] tokens. Lengths, tables and row starts are device memory: a launch sequence that was
+ * captured into a HIP graph serves later steps. Rows behind the last sequence's are left as they are, in every
+ * operator (a batch padded to a fixed size).
+ *
+ * What a device array may say wrongly is kept inside the pools: a page number outside [0, n_pages) stands for a page
+ * that is not there (its tokens are not seen and not written; pages that a window has left may be given back so), a
+ * negative length is 0, tokens behind the table's end are not there, and a sequence has at most max_rows rows.
+ *
+ * The reference has one sequence per model and caches of a fixed length (mllm/Backends/Arm/Ops/KVCacheOp.cpp:44-72). */
+#define W4A32_CACHE_F32 1
+#define W4A32_CACHE_F16 2
+#define W4A32_CACHE_BF16 3
+#define W4A32_PAGED_MAX_DIM 256
+
+/* Rows are f32 with any cache, or bf16 with a bf16 cache (`act_bf16`). dim % 8 == 0, dim <= 256; page is a power of two
+ * from 16 on; table_ld * page and the rows of a step stay below 2^30. Pools and rows on 16 bytes; row strides (ld*, in
+ * elements) are multiples of 8 that hold a row. Zero-initialise the structs before filling them. */
+typedef struct {
+  void *d_k, *d_v;        /* [n_pages][kv_heads][page][dim] of `dtype` */
+  float* d_weight;        /* [n_pages][kv_heads][page]: attention weight that each token has received; or NULL */
+  const int* d_table;     /* [n_seqs][table_ld] */
+  int* d_len;             /* [n_seqs]: tokens a sequence has in the cache, before this step's rows */
+  int dtype;              /* W4A32_CACHE_* */
+  int n_pages, page, kv_heads, dim, n_seqs, table_ld;
+} w4a32_paged_cache;
+
+typedef struct {
+  const int* d_row_start;   /* [n_seqs + 1] */
+  int rows;                 /* rows the buffers hold: no row number reaches it */
+  int max_rows;             /* most rows of one sequence */
+  int heads;                /* query heads, a multiple of kv_heads: head h reads kv head h / (heads / kv_heads) */
+  int act_bf16;
+  const void* d_q;          /* [rows][heads][dim] */
+  void* d_out;              /* [rows][heads][dim]: rotated q (append; may be d_q), attention's output */
+  int ldq, ldo;
+} w4a32_paged_rows;
+
+/* q and k of the rows are rotated (dimension i with i + rot_dims / 2, for i < rot_dims / 2; tables
+ * [table_rows][rot_dims / 2] as w4a32_op_rope_table builds them), k and v are written behind the sequences' tokens, and
+ * the added-up weight of the new tokens is set to 0. d_pos [n_seqs]: the position that a sequence's first row is rotated
+ * to (NULL: d_len; they differ once tokens were evicted). d_len stays as it is. rot_dims 0: no rotation (d_sin, d_cos
+ * unused). d_q NULL: keys and values alone. Rows at positions outside the tables are left out, as are rows without a slot
+ * in a page that is there (their q is rotated all the same). Rotation in f32, one rounding to each stored type.
+ * normal_hf_rope (rope.cpp:39-80) and ArmKVCacheOp::forward (KVCacheOp.cpp:44-72) per sequence. */
+int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, const void* d_k, int ldk,
+                          const void* d_v, int ldv, const int* d_pos, const float* d_sin, const float* d_cos,
+                          int rot_dims, int table_rows, void* stream);
+
+/* out = softmax(scale q K^T) V per head over what a row sees: row j of sequence b, which stands at slot s = d_len[b] + j
+ * (appended before the call), sees slots t <= s with t > s - window or t < first (window 0: all). A row that sees nothing
+ * gets zeros; values that are not finite reach only the rows that see them. With `accumulate` the weights are added to
+ * cache->d_weight: for every cached token the sum over the rows and over the heads of its kv head, in a fixed order
+ * (the same call gives the same bits).
+ *   Sums, maxima and products are f32 at f32 accuracy for f32 rows (a 16-bit cache's elements are exact operands of the
+ * 16-bit matrix instructions, q and the weights enter as two f16 or three bf16 terms); for bf16 rows the weights enter
+ * the second product as bf16, as the output is rounded.
+ *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes (contents need not be kept or cleared; calls
+ * that overlap in time need one each). That is 0 for a call that w4a32_op_paged_attention refuses.
+ * QWenAttention::forward, modeling_ds_qwen2.hpp:133-151, per sequence. */
+size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows,
+                                              int accumulate);
+int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale, int window,
+                             int first, int accumulate, void* d_scratch, size_t scratch_bytes, void* stream);
+
+/* Of every sequence's tokens `budget` stay, per kv head: the first `first` ones, the last `recent` ones and of the others
+ * those with the largest added-up weight (of equal ones the earlier; NaN counts as +infinity). Their keys, values and
+ * weights go in order to slots 0, 1, .. of the sequence in `to` (same sizes; pages that no table of `cache` names: what is
+ * read is not what is written), to->d_len becomes min(length, budget), and d_kept [n_seqs][kv_heads][budget] (int32, or
+ * NULL) the slots that stayed, -1 behind them. A sequence within its budget is copied whole. What lies in a page that is
+ * not there is lost: as a source it counts with weight 0 and is written as zeros, as a destination it is dropped.
+ * first + recent <= budget; both caches have weights. The slots of `to` are the order of the tokens and no longer their
+ * positions: give w4a32_op_paged_append d_pos from then on.
+ *   d_scratch: w4a32_op_paged_evict_scratch_bytes() bytes on 16 bytes, as above. */
+size_t w4a32_op_paged_evict_scratch_bytes(const w4a32_paged_cache* cache, int budget);
+int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache* to, int budget, int first, int recent,
+                         int* d_kept, void* d_scratch, size_t scratch_bytes, void* stream);
+
+/* Verification of drafted tokens. Sequence b's rows are its last token and then the tokens drafted behind it (d_tokens
+ * [rows]); row r's logits (f32 [rows][ldl]) judge token r + 1. With p = softmax(logits / temperature) and q the draft
+ * model's distribution, softmax(d_draft[r] / temperature) (f32 [rows][ldd], a sequence's last row is not read; NULL: the
+ * drafted token alone has q = 1), token t is accepted while uniform[r] q(t) < p(t). Behind the last
+ * accepted one the next token is drawn: where a token was refused from max(p - q, 0), else from p, as the least index whose
+ * running sum exceeds choice[b] times the whole sum. uniform [rows] and choice [n_seqs] are the caller's numbers from
+ * [0, 1). temperature 0: a token is accepted where it is the first maximum, and the next token is the first maximum (no
+ * draft logits or numbers are read; they may be NULL).
+ *   d_count[b] = accepted tokens + 1, the rows that stay; d_next[b] = the next token; d_len (may be NULL) += d_count.
+ * A sequence without rows gets count 0 and token -1, and a token that has no distribution to come from (no finite
+ * logit, a NaN, +infinity) is -1; -infinity is a probability of 0, and a drafted token outside [0, vocab) is refused.
+ * Exponentials and sums are held in 64 bits: the choice depends on neither the order of sums nor the sizes of the parts.
+ * Per sequence what AutoLLM.hpp:70-88 does for one token, with the test that keeps the target's distribution.
+ *   d_scratch: w4a32_op_verify_drafts_scratch_bytes() bytes on 16 bytes, as above. */
+typedef struct {
+  const float* d_logits;      /* [rows][ldl] */
+  const float* d_draft;       /* [rows][ldd], or NULL */
+  const int* d_row_start;     /* [n_seqs + 1] */
+  const int64_t* d_tokens;    /* [rows] */
+  const float *d_uniform, *d_choice;
+  int* d_count;               /* [n_seqs] */
+  int64_t* d_next;            /* [n_seqs] */
+  int* d_len;                 /* [n_seqs], or NULL */
+  int rows, max_rows, n_seqs, vocab, ldl, ldd;
+  float temperature;
+} w4a32_verify_args;
+size_t w4a32_op_verify_drafts_scratch_bytes(int rows, int vocab, int n_seqs);
+int w4a32_op_verify_drafts(const w4a32_verify_args* args, void* d_scratch, size_t scratch_bytes, void* stream);
+
 /* ---- decoder runner -------------------------------------------------------------------- */
 
 typedef struct {

@@ -92,6 +92,13 @@ ABI = {
     "w4a32_decoder_init": (_ci, [_vp, _vp, _vp]),
     "w4a32_decoder_prefill": (_ci, [_vp, _vp, _vp, _vp, _ci, _ci, _vp, _vp]),
     "w4a32_decoder_step": (_ci, [_vp, _vp, _vp, _vp, _vp, _vp]),
+    "w4a32_op_paged_append": (_ci, [_vp, _vp, _vp, _ci, _vp, _ci, _vp, _vp, _vp, _ci, _ci, _vp]),
+    "w4a32_op_paged_attention_scratch_bytes": (_sz, [_vp, _vp, _ci]),
+    "w4a32_op_paged_attention": (_ci, [_vp, _vp, ctypes.c_float, _ci, _ci, _ci, _vp, _sz, _vp]),
+    "w4a32_op_paged_evict_scratch_bytes": (_sz, [_vp, _ci]),
+    "w4a32_op_paged_evict": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _vp, _sz, _vp]),
+    "w4a32_op_verify_drafts_scratch_bytes": (_sz, [_ci, _ci, _ci]),
+    "w4a32_op_verify_drafts": (_ci, [_vp, _vp, _sz, _vp]),
     # include/w4a32_layered.h
     "w4a32_layered_check": (_ci, [_vp]),
     "w4a32_layered_head_rows": (_ci, [_ci, _ci]),
@@ -124,6 +131,30 @@ class DecodeLinearArgs(ctypes.Structure):
                 ("count", ctypes.c_int), ("d_packed", ctypes.c_void_p * 4), ("N", ctypes.c_int * 4),
                 ("d_y", ctypes.c_void_p * 4), ("silu_pair", ctypes.c_int), ("in_parts", ctypes.c_int),
                 ("out_parts", ctypes.c_int)]
+
+
+CACHE_F32, CACHE_F16, CACHE_BF16 = 1, 2, 3
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """w4a32_paged_cache"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_k", "d_v", "d_weight", "d_table", "d_len")] + \
+               [(n, ctypes.c_int) for n in ("dtype", "n_pages", "page", "kv_heads", "dim", "n_seqs", "table_ld")]
+
+
+class PagedRowsArgs(ctypes.Structure):
+    """w4a32_paged_rows"""
+    _fields_ = [("d_row_start", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int) for n in ("rows", "max_rows", "heads", "act_bf16")] + \
+               [("d_q", ctypes.c_void_p), ("d_out", ctypes.c_void_p), ("ldq", ctypes.c_int), ("ldo", ctypes.c_int)]
+
+
+class VerifyArgs(ctypes.Structure):
+    """w4a32_verify_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_logits", "d_draft", "d_row_start", "d_tokens", "d_uniform", "d_choice", "d_count",
+                                               "d_next", "d_len")] + \
+               [(n, ctypes.c_int) for n in ("rows", "max_rows", "n_seqs", "vocab", "ldl", "ldd")] + \
+               [("temperature", ctypes.c_float)]
 
 
 class DecoderConfig(ctypes.Structure):
@@ -758,6 +789,184 @@ def decode_linear(x, packed_list, n_list, norm_weight=None, eps=1e-6, delta=None
         a.d_y[i] = ys[i].data_ptr() if i < len(ys) else None
     _check(lib().w4a32_decode_linear(ctypes.byref(a), _stream()), "w4a32_decode_linear")
     return ys, total
+
+
+# ---- a batch of sequences on a paged cache (include/w4a32_decoder.h) ---------------------------
+
+def _on(t, what, *dtypes):
+    """Refuses a tensor of another type, or that is not on the current device, whose stream the call goes to."""
+    import torch
+
+    if t.dtype not in dtypes:
+        raise W4A32Error(f"{what}: {t.dtype} is not one of {', '.join(map(str, dtypes))}")
+    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
+        raise W4A32Error(f"{what}: not on the current device")
+    return t
+
+
+def _row_ld(t, what):
+    """Elements from one row to the next of a tensor [rows][width] whose rows are contiguous."""
+    if t.ndim != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise W4A32Error(f"{what}: rows of contiguous elements are wanted, got {tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _flat(t, what, shape=None):
+    if not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
+        raise W4A32Error(f"{what}: {tuple(t.shape)} with strides {t.stride()} is not what is wanted"
+                         + (f", {shape} contiguous" if shape is not None else ", contiguous"))
+    return t
+
+
+class PagedCache:
+    """A paged key / value cache that several sequences share: k and v [pages][kv_heads][page][dim] (f32, f16 or bf16), table
+    int32 [sequences][most pages of one] (a number outside the pool: no page), length int32 [sequences], and, where weights are
+    added up, weight f32 [pages][kv_heads][page]. The tensors stay the caller's: contents may change between calls (and between
+    the replays of a captured one), the memory may not."""
+
+    def __init__(self, k, v, table, length, weight=None):
+        import torch
+
+        kinds = {torch.float32: CACHE_F32, torch.float16: CACHE_F16, torch.bfloat16: CACHE_BF16}
+        _on(k, "k", *kinds), _on(v, "v", k.dtype), _on(table, "table", torch.int32), _on(length, "length", torch.int32)
+        if k.ndim != 4 or table.ndim != 2:
+            raise W4A32Error("k is [pages][kv_heads][page][dim] and table [sequences][pages]")
+        pages, kv, page, dim = k.shape
+        _flat(k, "k"), _flat(v, "v", tuple(k.shape)), _flat(table, "table"), _flat(length, "length", (table.shape[0],))
+        if weight is not None:
+            _flat(_on(weight, "weight", torch.float32), "weight", (pages, kv, page))
+        self.k, self.v, self.table, self.length, self.weight = k, v, table, length, weight
+        self.dtype, self.device, self.kv_heads, self.dim, self.n_seqs = k.dtype, k.get_device(), kv, dim, table.shape[0]
+        self.args = PagedCacheArgs(k.data_ptr(), v.data_ptr(), _ptr(weight), table.data_ptr(), length.data_ptr(), kinds[k.dtype],
+                                   pages, page, kv, dim, table.shape[0], table.shape[1])
+        self._ref = ctypes.byref(self.args)
+
+
+def _paged_rows(cache, q, row_start, max_rows, heads, out):
+    import torch
+
+    if cache.device != torch.cuda.current_device():
+        raise W4A32Error("the cache is not on the current device")
+    _on(q, "q", torch.float32, torch.bfloat16), _on(out, "out", q.dtype), _on(row_start, "row_start", torch.int32)
+    if heads < 1 or q.shape[1:] != (heads * cache.dim,) or out.shape != q.shape:
+        raise W4A32Error(f"rows of {heads} heads of {cache.dim}: got q {tuple(q.shape)} and out {tuple(out.shape)}")
+    _flat(row_start, "row_start", (cache.n_seqs + 1,))
+    return PagedRowsArgs(row_start.data_ptr(), q.shape[0], max_rows, heads, q.dtype == torch.bfloat16, q.data_ptr(), out.data_ptr(),
+                         _row_ld(q, "q"), _row_ld(out, "out"))
+
+
+def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max_rows=None, out=None):
+    """Rows q [rows][heads * dim], k and v [rows][kv_heads * dim] of all sequences (sequence b: row_start[b] .. row_start[b + 1]):
+    returns the rotated q and writes the rotated k, and v, behind the sequences' tokens. sin, cos [positions][rotated / 2]: none,
+    no rotation. pos int32 [sequences]: position of a sequence's first row where it is not cache.length."""
+    import torch
+
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    rows = q.shape[0]
+    r = _paged_rows(cache, q, row_start, max_rows or rows, q.shape[1] // cache.dim, out)
+    width = (rows, cache.kv_heads * cache.dim)
+    if k.shape != width or v.shape != width:
+        raise W4A32Error(f"k and v are {width}: got {tuple(k.shape)} and {tuple(v.shape)}")
+    _on(k, "k", q.dtype), _on(v, "v", q.dtype)
+    rot = positions = 0
+    if sin is not None:
+        _on(sin, "sin", torch.float32), _on(cos, "cos", torch.float32), _flat(sin, "sin"), _flat(cos, "cos", tuple(sin.shape))
+        positions, rot = sin.shape[0], 2 * sin.shape[1]
+    if pos is not None:
+        _flat(_on(pos, "pos", torch.int32), "pos", (cache.n_seqs,))
+    _check(lib().w4a32_op_paged_append(cache._ref, ctypes.byref(r), k.data_ptr(), _row_ld(k, "k"), v.data_ptr(), _row_ld(v, "v"),
+                                       _ptr(pos), _ptr(sin), _ptr(cos), rot, positions, _stream()), "w4a32_op_paged_append")
+    return out
+
+
+def op_paged_attention_scratch(cache, rows, max_rows, heads, accumulate=False):
+    """Scratch memory of op_paged_attention() for so many rows: kept between calls, not shared by calls that overlap in time."""
+    some = cache.args.d_k   # the sizes alone are asked about
+    r = PagedRowsArgs(some, rows, max_rows, heads, 0, some, some, heads * cache.dim, heads * cache.dim)
+    need = int(lib().w4a32_op_paged_attention_scratch_bytes(cache._ref, ctypes.byref(r), int(accumulate)))
+    if need == 0:
+        raise W4A32Error("w4a32_op_paged_attention_scratch_bytes: sizes that w4a32_op_paged_attention refuses")
+    return _dev_empty(need)
+
+
+def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, first=0, accumulate=False, scratch=None, out=None):
+    """Attention of rows q [rows][heads * dim] over their sequences' pages, the rows' own tokens included (appended before):
+    row j of sequence b sees slots t <= s = cache.length[b] + j with t > s - window or t < first (window 0: all). max_rows: most
+    rows of one sequence. accumulate: the weights that the cached tokens receive are added to cache.weight."""
+    import torch
+
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if scratch is None:
+        scratch = op_paged_attention_scratch(cache, q.shape[0], max_rows, heads, accumulate)
+    r = _paged_rows(cache, q, row_start, max_rows, heads, out)
+    _check(lib().w4a32_op_paged_attention(cache._ref, ctypes.byref(r), scale, window, first, int(accumulate), scratch.data_ptr(),
+                                          scratch.nbytes, _stream()), "w4a32_op_paged_attention")
+    return out
+
+
+def op_paged_evict_scratch(cache, budget):
+    """Scratch memory of op_paged_evict(), as op_paged_attention_scratch()."""
+    need = int(lib().w4a32_op_paged_evict_scratch_bytes(cache._ref, budget))
+    if need == 0:
+        raise W4A32Error("w4a32_op_paged_evict_scratch_bytes: sizes that w4a32_op_paged_evict refuses")
+    return _dev_empty(need)
+
+
+def op_paged_evict(cache, to, budget, first=0, recent=0, scratch=None):
+    """Of every sequence's tokens the first, the most recent and those with the largest added-up weight, `budget` in all per kv
+    head, go in order to the pages of `to`, whose lengths are set. Returns the slots that stayed, int32
+    [sequences][kv_heads][budget], -1 behind them."""
+    import torch
+
+    if cache.device != torch.cuda.current_device() or to.device != cache.device:
+        raise W4A32Error("the caches are not on the current device")
+    if scratch is None:
+        scratch = op_paged_evict_scratch(cache, budget)
+    kept = torch.empty((cache.n_seqs, cache.kv_heads, budget), dtype=torch.int32, device="cuda")
+    _check(lib().w4a32_op_paged_evict(cache._ref, to._ref, budget, first, recent, kept.data_ptr(), scratch.data_ptr(), scratch.nbytes,
+                                      _stream()), "w4a32_op_paged_evict")
+    return kept
+
+
+def op_verify_drafts_scratch(rows, vocab, n_seqs):
+    """Scratch memory of op_verify_drafts(), as op_paged_attention_scratch()."""
+    need = int(lib().w4a32_op_verify_drafts_scratch_bytes(rows, vocab, n_seqs))
+    if need == 0:
+        raise W4A32Error("w4a32_op_verify_drafts_scratch_bytes: sizes that w4a32_op_verify_drafts refuses")
+    return _dev_empty(need)
+
+
+def op_verify_drafts(logits, row_start, max_rows, tokens, uniform, choice, temperature, draft=None, length=None, scratch=None):
+    """logits [rows][vocab] of sequences' rows (their last token, then the drafted ones; tokens int64 [rows]) -> (count, next):
+    how many rows of each sequence stay (the accepted tokens and the one in front of them), and its next token. draft
+    [rows][vocab]: the draft model's logits; uniform [rows], choice [sequences]: random numbers from [0, 1) (temperature 0: the
+    greedy choice, they may be None). length int32 [sequences]: has the counts added."""
+    import torch
+
+    f32, n = (torch.float32,), row_start.numel() - 1
+    rows, vocab = logits.shape
+    _on(logits, "logits", *f32), _flat(_on(row_start, "row_start", torch.int32), "row_start")
+    _flat(_on(tokens, "tokens", torch.int64), "tokens", (rows,))
+    ldd = 0
+    if draft is not None:
+        ldd = _row_ld(_on(draft, "draft", *f32), "draft")
+        if draft.shape != logits.shape:
+            raise W4A32Error(f"draft is {tuple(logits.shape)}: got {tuple(draft.shape)}")
+    if uniform is not None:
+        _flat(_on(uniform, "uniform", *f32), "uniform", (rows,))
+    if choice is not None:
+        _flat(_on(choice, "choice", *f32), "choice", (n,))
+    if length is not None:
+        _flat(_on(length, "length", torch.int32), "length", (n,))
+    if scratch is None:
+        scratch = op_verify_drafts_scratch(rows, vocab, n)
+    count = torch.empty((n,), dtype=torch.int32, device="cuda")
+    token = torch.empty((n,), dtype=torch.int64, device="cuda")
+    a = VerifyArgs(logits.data_ptr(), _ptr(draft), row_start.data_ptr(), tokens.data_ptr(), _ptr(uniform), _ptr(choice),
+                   count.data_ptr(), token.data_ptr(), _ptr(length), rows, max_rows, n, vocab, _row_ld(logits, "logits"), ldd, temperature)
+    _check(lib().w4a32_op_verify_drafts(ctypes.byref(a), scratch.data_ptr(), scratch.nbytes, _stream()), "w4a32_op_verify_drafts")
+    return count, token
 
 
 class Decoder:

@@ -1,0 +1,350 @@
+// The paged cache: argument checks shared by its operators, the rows' append and the eviction of tokens.
+#include "w4a32_paged.h"
+
+namespace w4 {
+namespace paged {
+
+namespace {
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_ELAUNCH; }
+constexpr int kMost = 1 << 30;
+}  // namespace
+
+int check_cache(const w4a32_paged_cache* c) {
+  if (!c || !c->d_k || !c->d_v || !c->d_table || !c->d_len) return W4A32_EINVAL;
+  if (c->dtype < W4A32_CACHE_F32 || c->dtype > W4A32_CACHE_BF16) return W4A32_EINVAL;
+  if (c->n_pages < 1 || c->kv_heads < 1 || c->n_seqs < 1 || c->table_ld < 1 || c->dim < 1 || c->page < 1) return W4A32_EINVAL;
+  if (!aligned(c->d_k, 16) || !aligned(c->d_v, 16) || !aligned(c->d_weight, 4) || !aligned(c->d_table, 4) || !aligned(c->d_len, 4))
+    return W4A32_EINVAL;
+  if (c->page < 16 || c->page > kMost || (c->page & (c->page - 1)) || c->dim % 8) return W4A32_ESHAPE;
+  if (c->dim > W4A32_PAGED_MAX_DIM) return W4A32_ENOTSUP;
+  if ((long long)c->table_ld * c->page >= kMost || c->n_seqs >= kMost || (long long)c->n_pages * c->kv_heads >= kMost * 2ll)
+    return W4A32_ESHAPE;
+  return W4A32_OK;
+}
+
+int check_rows(const w4a32_paged_cache* c, const w4a32_paged_rows* r) {
+  if (int e = check_cache(c)) return e;
+  if (!r || !r->d_row_start || r->rows < 1 || r->max_rows < 1 || r->heads < 1) return W4A32_EINVAL;
+  if (!aligned(r->d_row_start, 4) || !aligned(r->d_q, 16) || !aligned(r->d_out, 16)) return W4A32_EINVAL;
+  if (r->rows >= kMost || r->heads >= kMost / c->dim || r->heads % c->kv_heads) return W4A32_ESHAPE;
+  if (r->act_bf16 && c->dtype != W4A32_CACHE_BF16) return W4A32_ENOTSUP;
+  if (r->d_q && (!r->d_out || r->ldq < r->heads * c->dim || r->ldo < r->heads * c->dim || r->ldq % 8 || r->ldo % 8)) return W4A32_EINVAL;
+  return W4A32_OK;
+}
+
+Cache view(const w4a32_paged_cache* c) {
+  return {c->d_k, c->d_v, c->d_weight, c->d_table, c->d_len, c->n_pages, log2_of(c->page), c->kv_heads, c->dim, c->n_seqs, c->table_ld,
+          c->table_ld * c->page};
+}
+
+// ---------------------------------------------------------------------------------------------
+// Append. A thread takes eight elements of one head of one row: four pairs (i, i + rot / 2) to be turned, or eight
+// elements that stay. Everything is read and written once; a step of few rows is bound by its chain of dependent loads
+// (row starts, length, page number) and prompts by memory.
+// ---------------------------------------------------------------------------------------------
+struct Append {
+  Cache c;
+  const int* row_start;
+  const int* pos;
+  const void *q, *k, *v;
+  void* q_out;
+  const float *sin_t, *cos_t;
+  int rows, max_rows, heads, ldq, ldo, ldk, ldv, rot, table_rows;
+};
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<float> {
+  static __device__ __forceinline__ void load4(const void* p, size_t at, float (&x)[4]) {
+    const f32x4 v = load_global<f32x4>((const float*)p + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  }
+  static __device__ __forceinline__ void store4(void* p, size_t at, const float (&x)[4]) {
+    *(W4_GLOBAL f32x4*)((float*)p + at) = f32x4{x[0], x[1], x[2], x[3]};
+  }
+};
+template <>
+struct Elem<__bf16> {
+  static __device__ __forceinline__ void load4(const void* p, size_t at, float (&x)[4]) {
+    const u32x2 v = load_global<u32x2>((const uint16_t*)p + at);
+    x[0] = __uint_as_float(v[0] << 16);
+    x[1] = __uint_as_float(v[0] & 0xffff0000u);
+    x[2] = __uint_as_float(v[1] << 16);
+    x[3] = __uint_as_float(v[1] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ void store4(void* p, size_t at, const float (&x)[4]) {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    *(W4_GLOBAL b4*)((uint16_t*)p + at) = b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+  }
+};
+template <>
+struct Elem<_Float16> {
+  static __device__ __forceinline__ void store4(void* p, size_t at, const float (&x)[4]) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    *(W4_GLOBAL h4*)((uint16_t*)p + at) = h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+  }
+};
+
+// The last sequence whose rows start at or in front of row r: 64 starts at a time, so that the search costs one load's
+// latency and not the six of a binary search over 64.
+__device__ __forceinline__ int owner_of(const int* row_start, int n_seqs, int r) {
+  int before = 0;
+  for (int b = 0; b < n_seqs; b += 64) {
+    const int i = b + (int)(threadIdx.x & 63);
+    before += __popcll(__ballot(i < n_seqs && row_start[i] <= r));
+  }
+  return before - 1;
+}
+
+template <typename Act, typename KV>
+__global__ __launch_bounds__(256) void append_kernel(Append a, int blocks_per_row) {
+  const int r = blockIdx.x / blocks_per_row;
+  const int unit = (blockIdx.x % blocks_per_row) * 256 + threadIdx.x;
+  const int per_head = a.c.dim / 8, q_heads = a.q ? a.heads : 0;
+  const int b = owner_of(a.row_start, a.c.n_seqs, r);
+  if (b < 0) return;
+  const Span s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
+  const int j = r - s.r0;
+  const int head = unit / per_head, e = unit - head * per_head;
+  if (j < 0 || j >= s.n || head >= q_heads + 2 * a.c.kv_heads) return;
+  const int p = (int)((unsigned)(a.pos ? a.pos[b] : s.len) + (unsigned)j), slot = s.len + j;
+  const bool is_q = head < q_heads, is_v = head >= q_heads + a.c.kv_heads;
+  if (a.rot && (unsigned)p >= (unsigned)a.table_rows) return;
+
+  const int half = a.rot / 2;
+  const bool turned = !is_v && 8 * e < a.rot;
+  const int d0 = turned ? 4 * e : 8 * e, d1 = turned ? 4 * e + half : 8 * e + 4;
+  const int h = is_q ? head : is_v ? head - q_heads - a.c.kv_heads : head - q_heads;
+  const void* src = is_q ? a.q : is_v ? a.v : a.k;
+  const size_t row = (size_t)r * (is_q ? a.ldq : is_v ? a.ldv : a.ldk) + (size_t)h * a.c.dim;
+  float x0[4], x1[4];
+  Elem<Act>::load4(src, row + d0, x0);
+  Elem<Act>::load4(src, row + d1, x1);
+  if (turned) {
+    float sn[4], cs[4];
+    Elem<float>::load4(a.sin_t, (size_t)p * half + d0, sn);
+    Elem<float>::load4(a.cos_t, (size_t)p * half + d0, cs);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float u = x0[i], w = x1[i];
+      x0[i] = u * cs[i] - w * sn[i];
+      x1[i] = w * cs[i] + u * sn[i];
+    }
+  }
+  if (is_q) {
+    const size_t to = (size_t)r * a.ldo + (size_t)h * a.c.dim;
+    Elem<Act>::store4(a.q_out, to + d0, x0);
+    Elem<Act>::store4(a.q_out, to + d1, x1);
+    return;
+  }
+  if (slot >= a.c.cap) return;
+  const int page = a.c.table[(size_t)b * a.c.table_ld + (slot >> a.c.shift)];
+  if (!page_there(a.c, page)) return;
+  const size_t at = slot_row(a.c, page, h, slot);
+  void* dst = is_v ? a.c.v : a.c.k;
+  Elem<KV>::store4(dst, at * a.c.dim + d0, x0);
+  Elem<KV>::store4(dst, at * a.c.dim + d1, x1);
+  if (!is_v && e == 0 && a.c.weight) a.c.weight[at] = 0.0f;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Eviction. One workgroup per (sequence, kv head) finds the weight of the last token that stays, eight bits of its
+// order-preserving key at a time (a histogram in LDS each), and lists the slots that stay in order; a second launch copies.
+// ---------------------------------------------------------------------------------------------
+struct Evict {
+  Cache c, to;
+  int budget, first, recent;
+  int* kept;  // [n_seqs][kv_heads][budget]
+  int* to_len;
+};
+
+// Larger weights have larger keys; NaN is +infinity and -0 is 0.
+__device__ __forceinline__ uint32_t key_of(float w) {
+  if (!(w == w)) w = INFINITY;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float weight_at(const Cache& c, int b, int head, int t) {
+  const int page = c.table[(size_t)b * c.table_ld + (t >> c.shift)];
+  return page_there(c, page) ? c.weight[slot_row(c, page, head, t)] : 0.0f;
+}
+
+constexpr int kSelect = 1024;
+__global__ __launch_bounds__(kSelect) void select_kernel(Evict a) {
+  __shared__ unsigned hist[256], in_wave[2][kSelect / 64], state[2];
+  const int b = blockIdx.x / a.c.kv_heads, head = blockIdx.x % a.c.kv_heads, tid = threadIdx.x;
+  const int n = min(max(a.c.len[b], 0), a.c.cap), stay = min(n, a.budget);
+  int* kept = a.kept + (size_t)blockIdx.x * a.budget;
+  if (head == 0 && tid == 0) a.to_len[b] = stay;
+  for (int i = stay + tid; i < a.budget; i += kSelect) kept[i] = -1;
+  if (n <= a.budget) {
+    for (int i = tid; i < n; i += kSelect) kept[i] = i;
+    return;
+  }
+  const int lo = a.first, hi = n - a.recent;
+  unsigned want = a.budget - a.first - a.recent, prefix = 0;  // of those in [lo, hi), of which there are more
+  uint32_t mask = 0;
+  if (want) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256) hist[tid] = 0;
+      __syncthreads();
+      for (int t = lo + tid; t < hi; t += kSelect) {
+        const uint32_t k = key_of(weight_at(a.c, b, head, t));
+        if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255], 1u);
+      }
+      __syncthreads();
+      if (tid < 64) {  // lane l: digits 255 - 4 l down to 252 - 4 l
+        unsigned sum = 0, h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += h[i] = hist[255 - 4 * tid - i];
+        unsigned upto = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const unsigned y = __shfl_up(upto, o);
+          if (tid >= o) upto += y;
+        }
+        unsigned above = upto - sum;
+        if (above < want && upto >= want) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (above < want && above + h[i] >= want) {
+              state[0] = 255 - 4 * tid - i;
+              state[1] = want - above;
+            }
+            above += h[i];
+          }
+        }
+      }
+      __syncthreads();
+      prefix |= state[0] << shift;
+      want = state[1];
+      mask |= 255u << shift;
+      __syncthreads();
+    }
+  }
+  // those above the key stay, and of those that have it the first `want`
+  const bool any = a.budget > a.first + a.recent;
+  unsigned at = 0, equal = 0;
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int t0 = 0; t0 < n; t0 += kSelect) {
+    const int t = t0 + tid;
+    bool sure = t < n && (t < lo || t >= hi), tie = false;
+    if (any && t >= lo && t < hi) {
+      const uint32_t k = key_of(weight_at(a.c, b, head, t));
+      sure = k > prefix;
+      tie = k == prefix;
+    }
+    const unsigned long long ties = __ballot(tie);
+    if (lane == 0) in_wave[0][wave] = __popcll(ties);
+    __syncthreads();
+    unsigned rank = equal + __popcll(ties & ((1ull << lane) - 1));
+    for (int w = 0; w < kSelect / 64; ++w) {
+      rank += w < wave ? in_wave[0][w] : 0;
+      equal += in_wave[0][w];
+    }
+    const bool stays = sure || (tie && rank < want);
+    const unsigned long long all = __ballot(stays);
+    if (lane == 0) in_wave[1][wave] = __popcll(all);
+    __syncthreads();
+    unsigned to = at + __popcll(all & ((1ull << lane) - 1));
+    for (int w = 0; w < kSelect / 64; ++w) {
+      to += w < wave ? in_wave[1][w] : 0;
+      at += in_wave[1][w];
+    }
+    if (stays && to < (unsigned)a.budget) kept[to] = t;
+    __syncthreads();
+  }
+}
+
+// A thread copies 16 bytes of a token's key and of its value.
+constexpr int kCopies = 4;
+__global__ __launch_bounds__(256) void copy_kernel(Evict a, int units, int blocks_per_head) {
+  const int bh = blockIdx.x / blocks_per_head, b = bh / a.c.kv_heads, head = bh % a.c.kv_heads;
+  const int per = 256 / units, u = threadIdx.x % units;
+  if ((int)threadIdx.x >= per * units) return;
+  const int first = (blockIdx.x % blocks_per_head) * per * kCopies + threadIdx.x / units;
+#pragma unroll
+  for (int x = 0; x < kCopies; ++x) {
+    const int i = first + x * per;
+    const int t = i < a.budget ? a.kept[(size_t)bh * a.budget + i] : -1;
+    if (t < 0) continue;
+    const int from = a.c.table[(size_t)b * a.c.table_ld + (t >> a.c.shift)];
+    const int dst = a.to.table[(size_t)b * a.to.table_ld + (i >> a.to.shift)];
+    if (!page_there(a.to, dst)) continue;
+    const bool there = page_there(a.c, from);
+    const size_t src = slot_row(a.c, there ? from : 0, head, t), out = slot_row(a.to, dst, head, i);
+    const u32x4 zero = {0, 0, 0, 0};
+    u32x4 k = load_global<u32x4>((const u32x4*)a.c.k + src * units + u), v = load_global<u32x4>((const u32x4*)a.c.v + src * units + u);
+    *(W4_GLOBAL u32x4*)((u32x4*)a.to.k + out * units + u) = there ? k : zero;
+    *(W4_GLOBAL u32x4*)((u32x4*)a.to.v + out * units + u) = there ? v : zero;
+    if (u == 0) a.to.weight[out] = there ? a.c.weight[src] : 0.0f;
+  }
+}
+
+}  // namespace paged
+}  // namespace w4
+
+using namespace w4::paged;
+
+extern "C" {
+
+int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, const void* d_k, int ldk, const void* d_v,
+                          int ldv, const int* d_pos, const float* d_sin, const float* d_cos, int rot_dims, int table_rows,
+                          void* stream) {
+  if (int e = check_rows(cache, rows)) return e;
+  if (!d_k || !d_v || !aligned(d_k, 16) || !aligned(d_v, 16) || !aligned(d_pos, 4)) return W4A32_EINVAL;
+  const int width = cache->kv_heads * cache->dim;
+  if (cache->kv_heads >= kMost / cache->dim) return W4A32_ESHAPE;
+  if (ldk < width || ldv < width || ldk % 8 || ldv % 8) return W4A32_EINVAL;
+  if (rot_dims < 0 || rot_dims > cache->dim || rot_dims % 8) return W4A32_ESHAPE;
+  if (rot_dims && (!d_sin || !d_cos || table_rows < 1 || !aligned(d_sin, 16) || !aligned(d_cos, 16))) return W4A32_EINVAL;
+  const Append a{view(cache),   rows->d_row_start, d_pos,    rows->d_q, d_k, d_v, rows->d_out, d_sin, d_cos, rows->rows, rows->max_rows,
+                 rows->heads, rows->ldq, rows->ldo, ldk, ldv, rot_dims, table_rows};
+  const long long units = (long long)((rows->d_q ? rows->heads : 0) + 2 * cache->kv_heads) * (cache->dim / 8);
+  const long long per_row = (units + 255) / 256;
+  if (per_row * rows->rows >= (1ll << 31)) return W4A32_ESHAPE;
+  const dim3 grid((unsigned)(per_row * rows->rows)), block(256);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (rows->act_bf16)
+    hipLaunchKernelGGL((append_kernel<__bf16, __bf16>), grid, block, 0, s, a, (int)per_row);
+  else if (cache->dtype == W4A32_CACHE_F32)
+    hipLaunchKernelGGL((append_kernel<float, float>), grid, block, 0, s, a, (int)per_row);
+  else if (cache->dtype == W4A32_CACHE_F16)
+    hipLaunchKernelGGL((append_kernel<float, _Float16>), grid, block, 0, s, a, (int)per_row);
+  else
+    hipLaunchKernelGGL((append_kernel<float, __bf16>), grid, block, 0, s, a, (int)per_row);
+  return from_hip(hipGetLastError());
+}
+
+size_t w4a32_op_paged_evict_scratch_bytes(const w4a32_paged_cache* cache, int budget) {
+  if (check_cache(cache) || budget < 1 || budget >= kMost) return 0;
+  return (size_t)cache->n_seqs * cache->kv_heads * budget * sizeof(int);
+}
+
+int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache* to, int budget, int first, int recent, int* d_kept,
+                         void* d_scratch, size_t scratch_bytes, void* stream) {
+  if (int e = check_cache(cache)) return e;
+  if (int e = check_cache(to)) return e;
+  if (!cache->d_weight || !to->d_weight || budget < 1 || first < 0 || recent < 0 || !aligned(d_kept, 4)) return W4A32_EINVAL;
+  if (cache->dtype != to->dtype || cache->dim != to->dim || cache->kv_heads != to->kv_heads || cache->n_seqs != to->n_seqs)
+    return W4A32_ESHAPE;
+  if ((long long)first + recent > budget || budget > (long long)to->table_ld * to->page) return W4A32_ESHAPE;
+  if (cache->d_len == to->d_len) return W4A32_EINVAL;
+  const size_t need = w4a32_op_paged_evict_scratch_bytes(cache, budget);
+  if (!d_kept && (!d_scratch || !aligned(d_scratch, 16) || scratch_bytes < need)) return W4A32_EINVAL;
+  const Evict a{view(cache), view(to), budget, first, recent, d_kept ? d_kept : static_cast<int*>(d_scratch), to->d_len};
+  const long long heads = (long long)cache->n_seqs * cache->kv_heads;
+  const int units = cache->dim * (cache->dtype == W4A32_CACHE_F32 ? 4 : 2) / 16, per = 256 / units * kCopies;
+  const long long blocks = (budget + per - 1) / per;
+  if (heads * blocks >= (1ll << 31)) return W4A32_ESHAPE;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(select_kernel, dim3((unsigned)heads), dim3(kSelect), 0, s, a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return W4A32_ELAUNCH;
+  hipLaunchKernelGGL(copy_kernel, dim3((unsigned)(heads * blocks)), dim3(256), 0, s, a, units, (int)blocks);
+  return from_hip(hipGetLastError());
+}
+
+}  // extern "C"

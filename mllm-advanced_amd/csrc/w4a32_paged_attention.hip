@@ -1,0 +1,789 @@
+// Attention of a ragged batch over a paged cache: rows of one token, of a few drafted ones or of a prompt's portion.
+//
+// Work is cut into items of 16 query rows that read the same kv head: of a sequence with n rows, the n * G pairs (token, head
+// of the group of G) in that order, 16 at a time. An item's keys are cut into tiles (32 keys of a 16-bit cache, 16 of an f32
+// one) and the tiles into chunks, one chunk per workgroup; its four wavefronts take the chunk's tiles in turn and join their
+// softmax states through LDS, and a second launch joins the chunks of an item. How many tiles a chunk has follows on the
+// device from the lengths: the batch's tiles over about kTarget workgroups. So a batch of short and long sequences is dealt
+// evenly, one long sequence fills the chip, and a captured launch serves lengths that nobody knew when it was captured.
+//
+// Both products are transposed, so that a lane stands for one query row (lane % 16) and keeps its softmax state:
+//   S^T = K Q^T     A = K: lane = key l % 16, 8 dims (16-bit) or 4 (f32) straight from the row in memory
+//   O^T += V^T P^T  A = V^T: the tile goes through LDS, where ds_read_b64_tr_b16 turns it (f32: plain reads of 4 bytes);
+//                   B = the softmaxed S^T as it lies in the registers: lane group g holds keys 4 g .. 4 g + 3 of a half
+// The matrix instruction's 16 columns are what a group of 6 or 7 heads needs; a kv head with one query head uses one of 16,
+// which costs no time: a 16-bit tile of head size 128 is 16 kilobytes for 16 to 48 instructions of 16 clocks.
+#include "w4a32_paged.h"
+
+namespace w4 {
+namespace paged {
+
+namespace {
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_ELAUNCH; }
+
+constexpr int kRows = 16;         // query rows of an item
+constexpr int kWaves = 4;         // wavefronts of a workgroup
+constexpr int kTargetLog2 = 9;    // workgroups that a batch is dealt to: two per CU
+constexpr int kMinTiles = kWaves; // least tiles of a chunk that is one of several
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned long long u64;
+
+struct Attend {
+  Cache c;
+  const void* q;
+  void* out;
+  const int* row_start;
+  int ldq, ldo, rows, max_rows, heads, group;
+  int window, first;
+  long long most_items;  // what the scratch memory holds: row starts that overlap could ask for more
+  float scale;   // of the scores, times log2 e
+  float* part;   // [workgroup][16][dt]: a chunk's sums, relative to its maximum
+  float* state;  // [workgroup][16][2]: its maximum (log2) and sum
+  float* lse;    // [item][16] (accumulate)
+  float* dump;   // [tile of an item][lane][keys of the tile / 4]: scores (accumulate)
+};
+
+// The keys that a sequence's rows can see, in tiles: [0, ft) of the first tokens, then [w0, w0 + nt - ft).
+struct Seq {
+  Span s;
+  int keys;        // tokens there are once the rows are appended
+  int ft, w0, nt;  // tiles
+  int items;       // per kv head
+};
+
+template <int KT>
+__device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
+  Seq q;
+  q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
+  q.keys = min(q.s.len + q.s.n, a.c.cap);
+  q.items = (int)(((long long)q.s.n * a.group + kRows - 1) / kRows);
+  q.w0 = 0;
+  q.ft = 0;
+  if (a.window) {
+    q.w0 = max(0, q.s.len - a.window + 1) / KT;
+    q.ft = min((min(a.first, a.c.cap) + KT - 1) / KT, q.w0);
+  }
+  q.nt = q.s.n ? q.ft + max(0, (q.keys + KT - 1) / KT - q.w0) : 0;
+  return q;
+}
+
+__device__ __forceinline__ u64 wave_sum(u64 x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// What a workgroup, an item or a group of key tiles is: found by adding up the sequences, 64 at a time, which every wavefront
+// does for itself.
+enum Unit { kChunks, kItems, kKeyTiles };
+struct Place {
+  int b;            // -1: none
+  unsigned inner;   // which one of the sequence
+  unsigned chunk0;  // chunks and items in front of the sequence
+  unsigned item0;
+  u64 tile0;        // tiles of items in front of the sequence
+  int nchunk;       // chunks of each of the sequence's items
+  Seq q;
+};
+
+template <int KT>
+__device__ __forceinline__ Place place_of(const Attend& a, unsigned id, Unit unit) {
+  const int lane = threadIdx.x & 63, kv = a.c.kv_heads;
+  u64 total = 0;
+  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+    u64 mine = 0;
+    if (b0 + lane < a.c.n_seqs) {
+      const Seq q = seq_of<KT>(a, b0 + lane);
+      mine = (u64)q.items * kv * q.nt;
+    }
+    total += wave_sum(mine);
+  }
+  const unsigned per = (unsigned)max((u64)kMinTiles, (total + (1u << kTargetLog2) - 1) >> kTargetLog2);
+  Place p;
+  p.b = -1;
+  p.chunk0 = p.item0 = 0;
+  p.tile0 = 0;
+  unsigned before = 0;
+  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+    Seq q = {};
+    unsigned items = 0, chunks = 0, count = 0;
+    int nchunk = 0;
+    if (b0 + lane < a.c.n_seqs) {
+      q = seq_of<KT>(a, b0 + lane);
+      nchunk = q.nt ? (int)((q.nt + per - 1) / per) : 1;
+      items = (unsigned)q.items * kv;
+      chunks = items * nchunk;
+      count = unit == kChunks ? chunks : unit == kItems ? items : (unsigned)kv * ((q.nt + kWaves - 1) / kWaves);
+    }
+    const unsigned upto = wave_scan(count);
+    const u64 found = __ballot(before + upto > id);
+    const int at = found ? __builtin_ctzll(found) : 64;
+    p.chunk0 += (unsigned)wave_sum(lane < at ? chunks : 0);
+    p.item0 += (unsigned)wave_sum(lane < at ? items : 0);
+    p.tile0 += wave_sum(lane < at ? (u64)items * q.nt : 0);
+    if (found) {
+      auto from = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+      p.b = b0 + at;
+      p.inner = id - before - (unsigned)from((int)(upto - count));
+      p.nchunk = from(nchunk);
+      p.q.s.r0 = from(q.s.r0);
+      p.q.s.n = from(q.s.n);
+      p.q.s.len = from(q.s.len);
+      p.q.keys = from(q.keys);
+      p.q.ft = from(q.ft);
+      p.q.w0 = from(q.w0);
+      p.q.nt = from(q.nt);
+      p.q.items = from(q.items);
+      break;
+    }
+    before += (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
+  }
+  return p;
+}
+
+__device__ __forceinline__ float group_max(float x) {  // over the four lane groups: all lanes of one query row
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float group_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---- element types ---------------------------------------------------------------------------------------------------------
+// kTerms operands stand for one f32 operand of the 16-bit matrix instruction. kScale: exponent that the softmaxed scores
+// carry until the sums are divided (they cancel there).
+template <typename Act, typename KV>
+struct Math;
+
+// bf16: three truncations hold the 24 bits of an f32 whatever its exponent
+template <typename Act>
+struct Math<Act, __bf16> {
+  static constexpr int kTerms = sizeof(Act) == 4 ? 3 : 1;
+  static constexpr int kScale = 0;
+  typedef bf8 V8;
+  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ void split(const float (&x)[8], V8 (&t)[kTerms]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (kTerms == 1) {
+        t[0][i] = (__bf16)x[i];
+      } else {
+        float r = x[i];
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) {
+          const uint32_t top = __float_as_uint(r) & 0xffff0000u;
+          t[k][i] = __builtin_bit_cast(__bf16, (uint16_t)(top >> 16));
+          r -= __uint_as_float(top);
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among two elements
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  }
+  static __device__ __forceinline__ float widen(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
+};
+// f16: two roundings hold 22 to 24 bits of a number that is scaled near the type's largest, and of a smaller one whatever
+// lies above 2^-40 of the row's largest
+template <typename Act>
+struct Math<Act, _Float16> {
+  static constexpr int kTerms = 2;
+  static constexpr int kScale = 15;
+  typedef h8 V8;
+  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ void split(const float (&x)[8], V8 (&t)[kTerms]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      t[0][i] = (_Float16)x[i];
+      t[1][i] = (_Float16)(x[i] - (float)t[0][i]);
+    }
+  }
+  static __device__ __forceinline__ bool odd(uint32_t w) {
+    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+  }
+  static __device__ __forceinline__ float widen(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+};
+// f32: the f32 matrix instruction, operands as they are
+template <>
+struct Math<float, float> {
+  static constexpr int kTerms = 1;
+  static constexpr int kScale = 0;
+  static __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+};
+
+template <typename KV>
+constexpr int tile_keys() { return sizeof(KV) == 2 ? 32 : 16; }
+template <typename KV, int DT>
+constexpr int v_stride() { return sizeof(KV) == 2 ? DT + 16 : DT + 4; }  // elements of an LDS row: its reads meet no bank twice
+template <typename KV, int DT>
+constexpr size_t wave_lds() {  // a wavefront's tile of V; at the end its 16 rows of sums
+  constexpr size_t v = (size_t)tile_keys<KV>() * v_stride<KV, DT>() * sizeof(KV), o = (size_t)kRows * (DT + 4) * 4;
+  return v > o ? v : o;
+}
+template <typename KV, int DT>
+constexpr size_t lds_bytes() { return kWaves * (wave_lds<KV, DT>() + kRows * 2 * sizeof(float)); }
+
+template <typename Act>
+__device__ __forceinline__ void load8(const void* p, size_t at, float (&x)[8]) {
+  if constexpr (sizeof(Act) == 4) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 v = load_global<f32x4>((const float*)p + at + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * h + i] = v[i];
+    }
+  } else {
+    const u32x4 v = load_global<u32x4>((const uint16_t*)p + at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i & 1 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
+  }
+}
+template <typename Act>
+__device__ __forceinline__ void store4(void* p, size_t at, f32x4 x) {
+  if constexpr (sizeof(Act) == 4) {
+    *(W4_GLOBAL f32x4*)((float*)p + at) = x;
+  } else {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    *(W4_GLOBAL b4*)((uint16_t*)p + at) = b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+  }
+}
+
+// DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up.
+template <typename Act, typename KV, int DT, bool kDump>
+__global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(Attend a) {
+  using M = Math<Act, KV>;
+  constexpr int KT = tile_keys<KV>(), NT = M::kTerms, kHalves = KT / 16;
+  constexpr bool k16 = sizeof(KV) == 2;
+  constexpr int kSteps = k16 ? DT / 32 : DT / 16;         // 16-byte loads of a lane per 16 keys of K
+  constexpr int kVLoads = KT * DT * (int)sizeof(KV) / 1024;  // 16-byte loads of a lane per tile of V
+  constexpr int kVS = v_stride<KV, DT>();
+  constexpr int kE = 16 / (int)sizeof(KV);                // elements of a load
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, grp = lane >> 4;
+
+  const Place p = place_of<KT>(a, blockIdx.x, kChunks);
+  if (p.b < 0) return;
+  const Span s = p.q.s;
+  const int item = p.inner / p.nchunk, chunk = p.inner % p.nchunk;  // of the sequence
+  if ((long long)p.item0 + item >= a.most_items) return;
+  const int hk = item / p.q.items, rt = item % p.q.items;
+  const int dim = a.c.dim;
+  // tiles of this chunk
+  const int t_lo = (int)((long long)p.q.nt * chunk / p.nchunk), t_hi = (int)((long long)p.q.nt * (chunk + 1) / p.nchunk);
+  // this lane's query row, and the rows of the item
+  const int in_seq = rt * kRows + row, all_rows = s.n * a.group;
+  const bool real = in_seq < all_rows;
+  const int j = real ? in_seq / a.group : s.n - 1, head = hk * a.group + (real ? in_seq % a.group : 0);
+  const int j_min = rt * kRows / a.group, j_max = min(rt * kRows + kRows - 1, all_rows - 1) / a.group;
+  const int pos = min(s.len + j, a.c.cap - 1);
+  const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
+
+  // ---- q ----
+  typedef typename std::conditional<k16, u32x4, f32x4>::type Raw;
+  float row_scale = a.scale;
+  u32x4 qt[k16 ? NT : 1][k16 ? kSteps : 1];
+  f32x4 qf[k16 ? 1 : kSteps];
+  {
+    const size_t at = (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
+    if constexpr (k16) {
+      float x[kSteps][8], most = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const int d = 32 * c + 8 * grp;
+        if (real && d < dim) {
+          load8<Act>(a.q, at + d, x[c]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[c][i] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
+      }
+      if constexpr (M::kScale != 0) {  // a power of two that brings the row's largest to 2^14 .. 2^15
+        most = group_max(most);
+        int e = 0;
+        if (most > 0.0f && most < INFINITY) e = min(max(14 - ilogbf(most), -100), 100);
+        const float up = ldexpf(1.0f, e);
+        row_scale *= ldexpf(1.0f, -e);
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[c][i] *= up;
+      }
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        typename M::V8 t[NT];
+        M::split(x[c], t);
+#pragma unroll
+        for (int k = 0; k < NT; ++k) qt[k][c] = __builtin_bit_cast(u32x4, t[k]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const int d = 16 * c + 4 * grp;
+        qf[c] = real && d < dim ? load_global<f32x4>((const float*)a.q + at + d) : f32x4{0, 0, 0, 0};
+      }
+    }
+  }
+
+  const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
+  auto key_of = [&](int t) { return (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT; };
+  // page of a half of a tile (-1: not there)
+  auto page_at = [&](int t, int h) {
+    const int i = (key_of(t) + 16 * h) >> a.c.shift;
+    const int pg = t < t_hi && i < a.c.table_ld ? table[i] : -1;
+    return __builtin_amdgcn_readfirstlane(page_there(a.c, pg) ? pg : -1);
+  };
+
+  Raw kr[kHalves][kSteps], vr[kVLoads];
+  int page[kHalves];
+  auto load_k = [&](int t) {
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const KV* base = (const KV*)a.c.k + slot_row(a.c, max(page[h], 0), hk, key_of(t) + 16 * h) * dim;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const int d = (k16 ? 32 : 16) * c + kE * grp;
+        kr[h][c] = DT == dim || d < dim ? load_global<Raw>(base + row * dim + d) : Raw{0, 0, 0, 0};
+      }
+    }
+  };
+  auto load_v = [&](int t) {
+    constexpr int kPerKey = DT / kE;
+#pragma unroll
+    for (int i = 0; i < kVLoads; ++i) {
+      const int key = (64 * i + lane) / kPerKey, d = (64 * i + lane) % kPerKey * kE;
+      const int h = kHalves == 1 ? 0 : (64 * i) / (16 * kPerKey);
+      const KV* base = (const KV*)a.c.v + slot_row(a.c, max(page[h], 0), hk, key_of(t) + 16 * h) * dim;
+      vr[i] = DT == dim || d < dim ? load_global<Raw>(base + (key - 16 * h) * dim + d) : Raw{0, 0, 0, 0};
+    }
+  };
+
+  KV* vs = (KV*)(lds + wave * wave_lds<KV, DT>());
+  f32x4 o[DT / 16];
+#pragma unroll
+  for (int d = 0; d < DT / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
+  float m = -INFINITY, l = 0.0f;
+
+  int t = t_lo + wave;
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) page[h] = page_at(t, h);
+  if (t < t_hi) {
+    load_k(t);
+    load_v(t);
+  }
+  for (; t < t_hi; t += kWaves) {
+    const int k0 = key_of(t);
+    bool there = true;
+    int cur[kHalves], next[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      cur[h] = page[h];
+      there = there && cur[h] >= 0;
+      next[h] = page_at(t + kWaves, h);
+    }
+    // every key seen by every row, or each looked at
+    const bool whole = there && k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
+    bool apart = false;  // a value that is not finite, of a key that some rows see and others do not
+    if (!whole) {
+      constexpr int kPerKey = DT / kE;
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i) {
+        const int in = (64 * i + lane) / kPerKey, key = k0 + in;
+        const bool none = (kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0 || key > pos_max ||
+                          (a.window != 0 && key <= pos_min - a.window && key >= a.first);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if constexpr (k16) {
+            vr[i][w] = none ? 0u : vr[i][w];
+            apart = apart || M::odd(vr[i][w]);
+          } else {
+            vr[i][w] = none ? 0.0f : vr[i][w];
+            apart = apart || M::odd(__float_as_uint(vr[i][w]));
+          }
+        }
+      }
+      apart = j_min != j_max && __any(apart);
+    }
+    {
+      constexpr int kPerKey = DT / kE;
+#pragma unroll
+      for (int i = 0; i < kVLoads; ++i)
+        *(Raw*)(vs + (64 * i + lane) / kPerKey * kVS + (64 * i + lane) % kPerKey * kE) = vr[i];
+    }
+    // ---- scores ----
+    f32x4 sc[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      sc[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        if constexpr (k16) {
+#pragma unroll
+          for (int k = NT - 1; k >= 0; --k)  // small terms first
+            sc[h] = M::mfma(__builtin_bit_cast(typename M::V8, kr[h][c]), __builtin_bit_cast(typename M::V8, qt[k][c]), sc[h]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[h] = M::mfma(kr[h][c][i], qf[c][i], sc[h]);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) page[h] = next[h];
+    if (t + kWaves < t_hi) {
+      load_k(t + kWaves);
+      load_v(t + kWaves);
+    }
+    uint32_t seen = 0xff;  // bit 4 h + i: key 16 h + 4 grp + i
+    if (!whole) {
+      seen = 0;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 16 * h + 4 * grp + i;
+          const bool sees = real && cur[h] >= 0 && key <= pos && (a.window == 0 || key > pos - a.window || key < a.first);
+          seen |= sees ? 1u << (4 * h + i) : 0u;
+        }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = sc[h][i] * row_scale;
+        sc[h][i] = seen >> (4 * h + i) & 1 ? x : -INFINITY;
+        mx = fmaxf(mx, sc[h][i]);
+      }
+    if constexpr (kDump) {
+      const u64 at = p.tile0 + (u64)item * p.q.nt + t;
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) *(W4_GLOBAL f32x4*)(a.dump + (at * 64 + lane) * (4 * kHalves) + 4 * h) = sc[h];
+    }
+    const float m_new = fmaxf(m, group_max(mx));
+    const float base = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: exp2(-inf) is 0
+    if (__any(m_new > m)) {
+      const float down = pow2(m - base);
+      l *= down;
+#pragma unroll
+      for (int d = 0; d < DT / 16; ++d) o[d] *= down;
+    }
+    m = m_new;
+    float pr[8] = {};
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pr[4 * h + i] = pow2(sc[h][i] - base + (float)M::kScale);
+        l += pr[4 * h + i];
+      }
+    // ---- values ----
+    if (__builtin_expect(apart, 0)) {
+      // 0 times a value that is not finite must not reach a row that does not see it: key by key
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          for (int g = 0; g < 4; ++g) {
+            const float w = __shfl(pr[4 * h + i], 16 * g + row);
+            const bool mine = __shfl((int)seen, 16 * g + row) >> (4 * h + i) & 1;
+            const KV* v = vs + (16 * h + 4 * g + i) * kVS + 4 * grp;
+#pragma unroll
+            for (int d = 0; d < DT / 16; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                float x;
+                if constexpr (k16)
+                  x = M::widen(__builtin_bit_cast(uint16_t, v[16 * d + e]));
+                else
+                  x = v[16 * d + e];
+                o[d][e] += mine ? w * x : 0.0f;
+              }
+          }
+    } else if constexpr (k16) {
+      typename M::V8 pt[NT];
+      M::split(pr, pt);
+      const KV* v = vs + (4 * grp + (row >> 2)) * kVS + 4 * (row & 3);
+#pragma unroll
+      for (int d = 0; d < DT / 16; ++d) {
+        union {
+          s4 half[2];
+          typename M::V8 v8;
+        } vt;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          vt.half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(v + 16 * h * kVS + 16 * d));
+#pragma unroll
+        for (int k = NT - 1; k >= 0; --k) o[d] = M::mfma(vt.v8, pt[k], o[d]);
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT / 16; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d] = M::mfma(vs[(4 * grp + i) * kVS + 16 * d + row], pr[i], o[d]);
+    }
+  }
+
+  // ---- join the wavefronts ----
+  l = group_sum(l) * ldexpf(1.0f, -M::kScale);
+  float* sums = (float*)(lds + wave * wave_lds<KV, DT>());
+  float* states = (float*)(lds + kWaves * wave_lds<KV, DT>());
+#pragma unroll
+  for (int d = 0; d < DT / 16; ++d) *(f32x4*)(sums + row * (DT + 4) + 16 * d + 4 * grp) = o[d] * ldexpf(1.0f, -M::kScale);
+  if (grp == 0) {
+    states[(wave * kRows + row) * 2] = m;
+    states[(wave * kRows + row) * 2 + 1] = l;
+  }
+  __syncthreads();
+  constexpr int kPer = DT / 4;  // threads of a row
+  for (int i = threadIdx.x; i < kRows * kPer; i += 64 * kWaves) {
+    const int r = i / kPer, d = i % kPer * 4, of = rt * kRows + r;
+    if (of >= all_rows) continue;
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, states[(w * kRows + r) * 2]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = pow2(states[(w * kRows + r) * 2] - base);
+      sum += f * states[(w * kRows + r) * 2 + 1];
+      acc += f * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + r * (DT + 4) + d);
+    }
+    if (p.nchunk > 1) {
+      const size_t at = (size_t)blockIdx.x * kRows + r;
+      *(W4_GLOBAL f32x4*)(a.part + at * DT + d) = acc;
+      if (d == 0) {
+        a.state[2 * at] = top;
+        a.state[2 * at + 1] = sum;
+      }
+    } else {
+      if (d < dim) {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const size_t at = (size_t)(s.r0 + of / a.group) * a.ldo + (size_t)(hk * a.group + of % a.group) * dim;
+        store4<Act>(a.out, at + d, acc * inv);
+      }
+      if (kDump && d == 0) a.lse[(size_t)(p.item0 + item) * kRows + r] = sum == 0.0f ? INFINITY : base + __log2f(sum);
+    }
+  }
+}
+
+// Joins the chunks of an item: a workgroup per query row, its threads a quarter of the head's values each and, eight (or
+// four, sixteen) of them to a value, every eighth chunk.
+template <typename Act, typename KV, int DT, bool kDump>
+__global__ __launch_bounds__(256) void join_kernel(Attend a) {
+  constexpr int kPer = DT / 4, kAtOnce = 256 / kPer;
+  __shared__ __attribute__((aligned(16))) float sums[kAtOnce][DT];
+  __shared__ float tops[4], totals[kAtOnce];
+  const Place p = place_of<tile_keys<KV>()>(a, blockIdx.x / kRows, kItems);
+  if (p.b < 0 || p.nchunk == 1) return;
+  const int item = p.inner, hk = item / p.q.items, rt = item % p.q.items, r = blockIdx.x % kRows, of = rt * kRows + r;
+  if (of >= p.q.s.n * a.group || (long long)p.item0 + item >= a.most_items) return;
+  const size_t at = ((size_t)p.chunk0 + (size_t)item * p.nchunk) * kRows + r;
+  float top = -INFINITY;
+  for (int c = threadIdx.x; c < p.nchunk; c += 256) top = fmaxf(top, a.state[2 * (at + (size_t)c * kRows)]);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float base = top == -INFINITY ? 0.0f : top;
+  const int d = threadIdx.x % kPer * 4, first = threadIdx.x / kPer;
+  f32x4 acc = {0, 0, 0, 0};
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int c = first; c < p.nchunk; c += kAtOnce) {
+    const size_t from = at + (size_t)c * kRows;
+    const float f = pow2(a.state[2 * from] - base);
+    sum += f * a.state[2 * from + 1];
+    acc += f * load_global<f32x4>(a.part + from * DT + d);
+  }
+  *(f32x4*)&sums[first][d] = acc;
+  if (d == 0) totals[first] = sum;
+  __syncthreads();
+  if (first != 0) return;
+#pragma unroll
+  for (int i = 1; i < kAtOnce; ++i) {
+    acc += *(const f32x4*)&sums[i][d];
+    sum += totals[i];
+  }
+  if (d < a.c.dim) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const size_t to = (size_t)(p.q.s.r0 + of / a.group) * a.ldo + (size_t)(hk * a.group + of % a.group) * a.c.dim;
+    store4<Act>(a.out, to + d, acc * inv);
+  }
+  if (kDump && d == 0) a.lse[(size_t)(p.item0 + item) * kRows + r] = sum == 0.0f ? INFINITY : base + __log2f(sum);
+}
+
+// Adds the weights of a tile's keys up: a wavefront per tile of a kv head, over its items in order.
+template <typename KV>
+__global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
+  constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
+  const Place p = place_of<KT>(a, blockIdx.x, kKeyTiles);
+  if (p.b < 0) return;
+  const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = p.inner / per_head;
+  const int t = p.inner % per_head * kWaves + (threadIdx.x >> 6);
+  if (t >= p.q.nt) return;
+  const int lane = threadIdx.x & 63, row = lane & 15, grp = lane >> 4;
+  float w[4 * kHalves] = {};
+  for (int rt = 0; rt < p.q.items; ++rt) {
+    const int item = hk * p.q.items + rt;
+    if ((long long)p.item0 + item >= a.most_items) break;
+    const bool real = rt * kRows + row < p.q.s.n * a.group;
+    const float lse = real ? a.lse[(size_t)(p.item0 + item) * kRows + row] : INFINITY;
+    const float* from = a.dump + ((p.tile0 + (u64)item * p.q.nt + t) * 64 + lane) * (4 * kHalves);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const f32x4 x = load_global<f32x4>(from + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[4 * h + i] += real ? pow2(x[i] - lse) : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4 * kHalves; ++i)
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) w[i] += __shfl_xor(w[i], x);
+  if (row != 0) return;
+  const int k0 = (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT;
+#pragma unroll
+  for (int h = 0; h < kHalves; ++h) {
+    const int key = k0 + 16 * h + 4 * grp;
+    if (key >= p.q.keys) continue;
+    const int page = a.c.table[(size_t)p.b * a.c.table_ld + (key >> a.c.shift)];
+    if (!page_there(a.c, page)) continue;
+    float* to = a.c.weight + slot_row(a.c, page, hk, key);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (key + i < p.q.keys) to[i] += w[4 * h + i];
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+struct Plan {
+  long long items, grid, key_groups;  // workgroups of the three launches (the join: 16 per item)
+  bool join;
+  int dt;
+  size_t part_off, state_off, lse_off, dump_off, total;
+};
+
+inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// W4A32_OK and what a call takes at most, whatever the device arrays say
+int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, int first, bool accumulate, Plan& p) {
+  const int kt = c->dtype == W4A32_CACHE_F32 ? 16 : 32;
+  const long long group = r->heads / c->kv_heads, cap = (long long)c->table_ld * c->page;
+  const long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
+  const long long by_seq = (most * group + kRows - 1) / kRows * c->n_seqs, by_rows = (long long)r->rows * group / kRows + c->n_seqs;
+  p.items = (by_seq < by_rows ? by_seq : by_rows) * c->kv_heads;
+  long long tiles = (cap + kt - 1) / kt;
+  if (window) {
+    const long long near = ((long long)first + kt - 1) / kt + (window + most) / kt + 2;
+    tiles = near < tiles ? near : tiles;
+  }
+  const long long chunks = (tiles + kMinTiles - 1) / kMinTiles;
+  p.join = chunks > 1;
+  p.grid = p.items * chunks < p.items + (1ll << kTargetLog2) ? p.items * chunks : p.items + (1ll << kTargetLog2);
+  p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
+  p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
+  if (p.grid >= (1ll << 31) || p.items * kRows >= (1ll << 31) || p.key_groups >= (1ll << 31)) return W4A32_ESHAPE;
+  size_t at = 0;
+  p.part_off = at;
+  if (p.join) at = up256(at + (size_t)p.grid * kRows * p.dt * 4);
+  p.state_off = at;
+  if (p.join) at = up256(at + (size_t)p.grid * kRows * 2 * 4);
+  p.lse_off = at;
+  if (accumulate) at = up256(at + (size_t)p.items * kRows * 4);
+  p.dump_off = at;
+  if (accumulate) {
+    if (p.items * tiles >= (1ll << 40)) return W4A32_ESHAPE;
+    at = up256(at + (size_t)p.items * tiles * kRows * kt * 4);
+  }
+  p.total = at ? at : 256;
+  return W4A32_OK;
+}
+
+template <typename Act, typename KV, int DT>
+hipError_t launch(const Attend& a, const Plan& p, bool accumulate, hipStream_t s) {
+  constexpr size_t lds = lds_bytes<KV, DT>();
+  auto kernel = accumulate ? rows_kernel<Act, KV, DT, true> : rows_kernel<Act, KV, DT, false>;
+  if constexpr (lds > 64 * 1024) {
+    static LdsLimitOnce limit[2];
+    if (hipError_t e = limit[accumulate].raise((const void*)kernel, lds); e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)p.grid), dim3(64 * kWaves), lds, s, a);
+  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  if (p.join) {
+    auto join = accumulate ? join_kernel<Act, KV, DT, true> : join_kernel<Act, KV, DT, false>;
+    hipLaunchKernelGGL(join, dim3((unsigned)(p.items * kRows)), dim3(256), 0, s, a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  if (accumulate) {
+    hipLaunchKernelGGL((weights_kernel<KV>), dim3((unsigned)p.key_groups), dim3(64 * kWaves), 0, s, a);
+    return hipGetLastError();
+  }
+  return hipSuccess;
+}
+template <typename Act, typename KV>
+hipError_t launch_dim(const Attend& a, const Plan& p, bool accumulate, hipStream_t s) {
+  if (p.dt == 64) return launch<Act, KV, 64>(a, p, accumulate, s);
+  if (p.dt == 128) return launch<Act, KV, 128>(a, p, accumulate, s);
+  return launch<Act, KV, 256>(a, p, accumulate, s);
+}
+
+int check(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accumulate) {
+  if (int e = check_rows(cache, rows)) return e;
+  if (!rows->d_q || !rows->d_out) return W4A32_EINVAL;
+  if (accumulate && !cache->d_weight) return W4A32_EINVAL;
+  return W4A32_OK;
+}
+}  // namespace
+
+}  // namespace paged
+}  // namespace w4
+
+using namespace w4::paged;
+
+extern "C" {
+
+size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accumulate) {
+  Plan p;
+  if (check(cache, rows, accumulate) || plan_of(cache, rows, 0, 0, accumulate != 0, p)) return 0;
+  return p.total;
+}
+
+int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale, int window, int first,
+                             int accumulate, void* d_scratch, size_t scratch_bytes, void* stream) {
+  if (int e = check(cache, rows, accumulate)) return e;
+  if (window < 0 || first < 0 || !(scale == scale) || !d_scratch || !aligned(d_scratch, 16)) return W4A32_EINVAL;
+  Plan p;
+  if (int e = plan_of(cache, rows, window, first, accumulate != 0, p)) return e;
+  if (scratch_bytes < p.total) return W4A32_EINVAL;
+  uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
+  const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows, rows->max_rows, rows->heads,
+                 rows->heads / cache->kv_heads, window, first, p.items, scale * 1.44269504088896340736f, (float*)(scratch + p.part_off),
+                 (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool acc = accumulate != 0;
+  if (rows->act_bf16) return from_hip(launch_dim<__bf16, __bf16>(a, p, acc, s));
+  if (cache->dtype == W4A32_CACHE_F32) return from_hip(launch_dim<float, float>(a, p, acc, s));
+  if (cache->dtype == W4A32_CACHE_F16) return from_hip(launch_dim<float, _Float16>(a, p, acc, s));
+  return from_hip(launch_dim<float, __bf16>(a, p, acc, s));
+}
+
+}  // extern "C"
