@@ -166,7 +166,8 @@ def prepare(c, seed):
 
 def handle(s, which=""):
     """The caches and scratch memory that a program keeps between its steps."""
-    pkg, c, kept = importlib.import_module("mllm-advanced_amd"), s["case"], s["kept"]
+    c, kept = s["case"], s["kept"]
+    pkg = kept.get("pkg") or kept.setdefault("pkg", importlib.import_module("mllm-advanced_amd"))   # a program imports it once
     if which not in kept:
         kept[which] = pkg.PagedCache(s[which + "k"], s[which + "v"], s[which + "table"], s[which + "len"], s.get(which + "weight"))
     if "scratch" not in kept:
@@ -277,7 +278,7 @@ def run_evict(s, c):
 
 def run_verify(s, c):
     if own:
-        pkg = importlib.import_module("mllm-advanced_amd")
+        pkg = s["kept"].get("pkg") or s["kept"].setdefault("pkg", importlib.import_module("mllm-advanced_amd"))
         if "scratch" not in s["kept"]:
             s["kept"]["scratch"] = pkg.op_verify_drafts_scratch(s["logits"].shape[0], c["vocab"], c["seqs"])
         return list(pkg.op_verify_drafts(s["logits"], s["row_start"], s["max_rows"], s["tokens"], s["uniform"], s["choice"],
