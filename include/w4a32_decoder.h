@@ -311,8 +311,8 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
  *   Sums, maxima and products are f32 at f32 accuracy for f32 rows (a 16-bit cache's elements are exact operands of the
  * 16-bit matrix instructions, q and the weights enter as two f16 or three bf16 terms); for bf16 rows the weights enter
  * the second product as bf16, as the output is rounded.
- *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes (contents need not be kept or cleared; calls
- * that overlap in time need one each). That is 0 for a call that w4a32_op_paged_attention refuses.
+ *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time (calls that
+ * overlap in time, on two streams or in two graphs, need one each). That is 0 for a call that w4a32_op_paged_attention refuses.
  * QWenAttention::forward, modeling_ds_qwen2.hpp:133-151, per sequence. */
 size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows,
                                               int accumulate);
@@ -327,7 +327,7 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
  * not there is lost: as a source it counts with weight 0 and is written as zeros, as a destination it is dropped.
  * first + recent <= budget; both caches have weights. The slots of `to` are the order of the tokens and no longer their
  * positions: give w4a32_op_paged_append d_pos from then on.
- *   d_scratch: w4a32_op_paged_evict_scratch_bytes() bytes on 16 bytes, as above. */
+ *   d_scratch: w4a32_op_paged_evict_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time. */
 size_t w4a32_op_paged_evict_scratch_bytes(const w4a32_paged_cache* cache, int budget);
 int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache* to, int budget, int first, int recent,
                          int* d_kept, void* d_scratch, size_t scratch_bytes, void* stream);
@@ -345,7 +345,7 @@ int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache
  * logit, a NaN, +infinity) is -1; -infinity is a probability of 0, and a drafted token outside [0, vocab) is refused.
  * Exponentials and sums are held in 64 bits: the choice depends on neither the order of sums nor the sizes of the parts.
  * Per sequence what AutoLLM.hpp:70-88 does for one token, with the test that keeps the target's distribution.
- *   d_scratch: w4a32_op_verify_drafts_scratch_bytes() bytes on 16 bytes, as above. */
+ *   d_scratch: w4a32_op_verify_drafts_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time. */
 typedef struct {
   const float* d_logits;      /* [rows][ldl] */
   const float* d_draft;       /* [rows][ldd], or NULL */

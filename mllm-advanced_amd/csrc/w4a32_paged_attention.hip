@@ -1,13 +1,17 @@
 // Attention of a ragged batch over a paged cache: rows of one token, of a few drafted ones or of a prompt's portion.
 //
-// Work is cut into items of 16 query rows that read the same kv head: of a sequence with n rows, the n * G pairs (token, head
-// of the group of G) in that order, 16 at a time. An item's keys are cut into tiles (32 keys of a 16-bit cache, 16 of an f32
-// one) and the tiles into chunks, one chunk per workgroup; its four wavefronts take the chunk's tiles in turn and join their
-// softmax states through LDS, and a second launch joins the chunks of an item. How many tiles a chunk has follows on the
-// device from the lengths: the batch's tiles over about kTarget workgroups. So a batch of short and long sequences is dealt
-// evenly, one long sequence fills the chip, and a captured launch serves lengths that nobody knew when it was captured.
+// Work is cut into items of 16, 32 or 64 query rows that read the same kv head: of a sequence with n rows, the n * G pairs
+// (token, head of the group of G) in that order. An item's keys are cut into tiles (32 keys of a 16-bit cache, 16 of an f32
+// one), and the tiles of all items, in one row, are dealt to the workgroups in equal shares, whatever item they belong to. So a
+// batch of short and long sequences is dealt evenly, one long sequence fills the chip, and a captured launch serves lengths
+// that nobody knew when it was captured: every wavefront works the shares out from the lengths. Where an item is shared, its
+// workgroups leave their sums in scratch memory and a second launch joins them. (The last workgroup to arrive can join them
+// without it, but took longer: its stores, its count and its loads each go through to memory, and it is one workgroup of many.
+// 40 us against 33 for 16 sequences of 2 to 5 rows, 15 against 13 for one row of 200 tokens.)
 //
-// Both products are transposed, so that a lane stands for one query row (lane % 16) and keeps its softmax state:
+// A wavefront has 16 query rows and takes its item's tiles in turn with the others that have the same rows; those join their
+// softmax states through LDS. Both products are transposed, so that a lane stands for one query row (lane % 16) and keeps its
+// softmax state:
 //   S^T = K Q^T     A = K: lane = key l % 16, 8 dims (16-bit) or 4 (f32) straight from the row in memory
 //   O^T += V^T P^T  A = V^T: the tile goes through LDS, where ds_read_b64_tr_b16 turns it (f32: plain reads of 4 bytes);
 //                   B = the softmaxed S^T as it lies in the registers: lane group g holds keys 4 g .. 4 g + 3 of a half
@@ -22,15 +26,22 @@ namespace {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_ELAUNCH; }
 
-constexpr int kRows = 16;         // query rows of an item
+constexpr int kRows = 16;         // query rows of a wavefront
 constexpr int kWaves = 4;         // wavefronts of a workgroup
-constexpr int kTargetLog2 = 9;    // workgroups that a batch is dealt to: two per CU
-constexpr int kMinTiles = kWaves; // least tiles of a chunk that is one of several
+constexpr int kGrid = 512;        // workgroups that a batch is dealt to: two per CU, all there at once
+constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
+constexpr int kAlone = 16;        // tiles of an item that is not shared, where there are workgroups enough for all items
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
+
+// What the second launch has to know of an item
+struct Item {
+  int first, shares;  // workgroup that has its first tile, and how many have a part of it
+  int r0, row0, rows, head;  // first row of the sequence, first of the item among (token, head of the group), their number, kv head
+};
 
 struct Attend {
   Cache c;
@@ -39,19 +50,23 @@ struct Attend {
   const int* row_start;
   int ldq, ldo, rows, max_rows, heads, group;
   int window, first;
-  long long most_items;  // what the scratch memory holds: row starts that overlap could ask for more
-  float scale;   // of the scores, times log2 e
-  float* part;   // [workgroup][16][dt]: a chunk's sums, relative to its maximum
-  float* state;  // [workgroup][16][2]: its maximum (log2) and sum
-  float* lse;    // [item][16] (accumulate)
-  float* dump;   // [tile of an item][lane][keys of the tile / 4]: scores (accumulate)
+  int wide;             // wavefronts with rows of their own: 1, 2 or 4; an item has 16 times so many rows
+  int slot_rows;        // rows of an item that can be there: what a slot of scratch memory holds
+  unsigned most_items, most_tiles;  // what the scratch memory holds: row starts that overlap could ask for more, and get nothing
+  float scale;          // of the scores, times log2 e
+  struct Item* item;    // [most_items]
+  unsigned* count;      // how many there are
+  float* part;          // [2 grid][slot_rows][dt]: sums of a share, relative to its maxima
+  float* state;         // [2 grid][slot_rows][2]: maxima (log2) and sums of weights
+  float* lse;           // [item][slot_rows] (accumulate)
+  float* dump;          // [tile of an item][wide][lane][keys of the tile / 4]: scores (accumulate)
 };
 
 // The keys that a sequence's rows can see, in tiles: [0, ft) of the first tokens, then [w0, w0 + nt - ft).
 struct Seq {
   Span s;
   int keys;        // tokens there are once the rows are appended
-  int ft, w0, nt;  // tiles
+  int ft, w0, nt;  // tiles; at least one where there are rows
   int items;       // per kv head
 };
 
@@ -60,96 +75,116 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   Seq q;
   q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
   q.keys = min(q.s.len + q.s.n, a.c.cap);
-  q.items = (int)(((long long)q.s.n * a.group + kRows - 1) / kRows);
+  q.items = (int)(((long long)q.s.n * a.group + kRows * a.wide - 1) / (kRows * a.wide));
   q.w0 = 0;
   q.ft = 0;
   if (a.window) {
-    q.w0 = max(0, q.s.len - a.window + 1) / KT;
+    q.w0 = max(0, min(q.s.len, a.c.cap - 1) - a.window + 1) / KT;
     q.ft = min((min(a.first, a.c.cap) + KT - 1) / KT, q.w0);
   }
-  q.nt = q.s.n ? q.ft + max(0, (q.keys + KT - 1) / KT - q.w0) : 0;
+  q.nt = q.s.n ? q.ft + (q.keys + KT - 1) / KT - q.w0 : 0;
   return q;
 }
 
-__device__ __forceinline__ u64 wave_sum(u64 x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+// Sums over the wavefront's lanes up to this one, by moves within the register file; sums that do not fit stay at the most.
+__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
+  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
+  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
+  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
+  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
+  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));
   return x;
 }
-__device__ __forceinline__ unsigned wave_scan(unsigned x) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  return x;
-}
+__device__ __forceinline__ unsigned last_lane(unsigned x) { return (unsigned)__builtin_amdgcn_readlane((int)x, 63); }
 
-// What a workgroup, an item or a group of key tiles is: found by adding up the sequences, 64 at a time, which every wavefront
-// does for itself.
-enum Unit { kChunks, kItems, kKeyTiles };
+// How a batch is dealt, and what is counted: tiles of items, items, or tiles of a kv head in fours (for the launch that adds
+// weights up).
+enum Unit { kTiles, kItems, kKeyTiles };
+struct Deal {
+  unsigned total, items, per;  // tiles, items, tiles of a share; per = 0: nothing can be done
+  bool alone;                  // a share is an item
+};
 struct Place {
-  int b;            // -1: none
+  bool there;
+  int b;
   unsigned inner;   // which one of the sequence
-  unsigned chunk0;  // chunks and items in front of the sequence
-  unsigned item0;
-  u64 tile0;        // tiles of items in front of the sequence
-  int nchunk;       // chunks of each of the sequence's items
+  unsigned tile0;   // tiles of items in front of the sequence
+  unsigned item0;   // items in front of the sequence
   Seq q;
 };
 
+// The sequences of a block of 64, one of each lane: kept where there is one block only.
 template <int KT>
-__device__ __forceinline__ Place place_of(const Attend& a, unsigned id, Unit unit) {
-  const int lane = threadIdx.x & 63, kv = a.c.kv_heads;
-  u64 total = 0;
-  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
-    u64 mine = 0;
-    if (b0 + lane < a.c.n_seqs) {
-      const Seq q = seq_of<KT>(a, b0 + lane);
-      mine = (u64)q.items * kv * q.nt;
+struct Seqs {
+  Seq q;
+  unsigned tiles, items;
+  __device__ __forceinline__ void load(const Attend& a, int b0) {
+    const int b = b0 + (int)(threadIdx.x & 63);
+    q = {};
+    tiles = items = 0;
+    if (b < a.c.n_seqs) {
+      q = seq_of<KT>(a, b);
+      const u64 n = (u64)q.items * a.c.kv_heads;
+      items = (unsigned)min(n, (u64)0xffffffffu);
+      tiles = (unsigned)min(n * q.nt, (u64)0xffffffffu);
     }
-    total += wave_sum(mine);
   }
-  const unsigned per = (unsigned)max((u64)kMinTiles, (total + (1u << kTargetLog2) - 1) >> kTargetLog2);
+};
+
+template <int KT>
+__device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
+  Deal d = {0, 0, 0, false};
+  int longest = 0;
+  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+    s.load(a, b0);
+    d.total = add_sat(d.total, last_lane(wave_scan(s.tiles)));
+    d.items = add_sat(d.items, last_lane(wave_scan(s.items)));
+    longest = max(longest, __any(s.q.nt > kAlone) ? kAlone + 1 : 1);
+  }
+  if (d.total == 0 || d.total > a.most_tiles || d.items > a.most_items) return d;
+  const unsigned even = (d.total + kGrid - 1) / kGrid;
+  const unsigned few = min((unsigned)kMinTiles, (d.total + d.items - 1) / d.items);
+  d.per = max(even, few);
+  d.alone = longest <= kAlone && d.items <= gridDim.x;
+  return d;
+}
+
+template <int KT>
+__device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT>& s, unsigned u, Unit unit) {
   Place p;
-  p.b = -1;
-  p.chunk0 = p.item0 = 0;
-  p.tile0 = 0;
+  p.there = false;
+  p.tile0 = p.item0 = 0;
   unsigned before = 0;
   for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
-    Seq q = {};
-    unsigned items = 0, chunks = 0, count = 0;
-    int nchunk = 0;
-    if (b0 + lane < a.c.n_seqs) {
-      q = seq_of<KT>(a, b0 + lane);
-      nchunk = q.nt ? (int)((q.nt + per - 1) / per) : 1;
-      items = (unsigned)q.items * kv;
-      chunks = items * nchunk;
-      count = unit == kChunks ? chunks : unit == kItems ? items : (unsigned)kv * ((q.nt + kWaves - 1) / kWaves);
-    }
-    const unsigned upto = wave_scan(count);
-    const u64 found = __ballot(before + upto > id);
-    const int at = found ? __builtin_ctzll(found) : 64;
-    p.chunk0 += (unsigned)wave_sum(lane < at ? chunks : 0);
-    p.item0 += (unsigned)wave_sum(lane < at ? items : 0);
-    p.tile0 += wave_sum(lane < at ? (u64)items * q.nt : 0);
+    if (a.c.n_seqs > 64) s.load(a, b0);
+    const unsigned keys = (unsigned)a.c.kv_heads * ((s.q.nt + kWaves - 1) / kWaves);
+    const unsigned items = wave_scan(s.items), tiles = wave_scan(s.tiles);
+    const unsigned count = unit == kTiles ? s.tiles : unit == kItems ? s.items : keys;
+    const unsigned upto = unit == kTiles ? tiles : unit == kItems ? items : wave_scan(count);
+    const u64 found = __ballot(add_sat(before, upto) > u);
     if (found) {
-      auto from = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+      const int at = __builtin_ctzll(found);
+      auto from = [&](unsigned x) { return __builtin_amdgcn_readlane((int)x, at); };
+      p.there = true;
       p.b = b0 + at;
-      p.inner = id - before - (unsigned)from((int)(upto - count));
-      p.nchunk = from(nchunk);
-      p.q.s.r0 = from(q.s.r0);
-      p.q.s.n = from(q.s.n);
-      p.q.s.len = from(q.s.len);
-      p.q.keys = from(q.keys);
-      p.q.ft = from(q.ft);
-      p.q.w0 = from(q.w0);
-      p.q.nt = from(q.nt);
-      p.q.items = from(q.items);
-      break;
+      p.inner = u - before - (unsigned)from(upto - count);
+      p.tile0 += (unsigned)from(tiles - s.tiles);
+      p.item0 += (unsigned)from(items - s.items);
+      p.q.s.r0 = from(s.q.s.r0);
+      p.q.s.n = from(s.q.s.n);
+      p.q.s.len = from(s.q.s.len);
+      p.q.keys = from(s.q.keys);
+      p.q.ft = from(s.q.ft);
+      p.q.w0 = from(s.q.w0);
+      p.q.nt = from(s.q.nt);
+      p.q.items = from(s.q.items);
+      return p;
     }
-    before += (unsigned)__builtin_amdgcn_readlane((int)upto, 63);
+    before = add_sat(before, last_lane(upto));
+    p.tile0 = add_sat(p.tile0, last_lane(tiles));
+    p.item0 = add_sat(p.item0, last_lane(items));
   }
   return p;
 }
@@ -264,6 +299,17 @@ __device__ __forceinline__ void store4(void* p, size_t at, f32x4 x) {
   }
 }
 
+// A row's result, from its sums and the sum of its weights
+template <typename Act, bool kDump>
+__device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, size_t lse_at, int d, f32x4 acc, float base, float sum) {
+  if (d < a.c.dim) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const size_t at = (size_t)(r0 + of / a.group) * a.ldo + (size_t)(hk * a.group + of % a.group) * a.c.dim;
+    store4<Act>(a.out, at + d, acc * inv);
+  }
+  if (kDump && d == 0) a.lse[lse_at] = sum == 0.0f ? INFINITY : base + __log2f(sum);
+}
+
 // DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up.
 template <typename Act, typename KV, int DT, bool kDump>
 __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(Attend a) {
@@ -275,384 +321,421 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
   constexpr int kVS = v_stride<KV, DT>();
   constexpr int kE = 16 / (int)sizeof(KV);                // elements of a load
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, grp = lane >> 4;
+  float* states = (float*)(lds + kWaves * wave_lds<KV, DT>());
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, grp = lane >> 4, dim = a.c.dim;
+  const int streams = kWaves / a.wide, stream = wave / a.wide;  // wavefronts that share rows, and which of them this one is
 
-  const Place p = place_of<KT>(a, blockIdx.x, kChunks);
-  if (p.b < 0) return;
-  const Span s = p.q.s;
-  const int item = p.inner / p.nchunk, chunk = p.inner % p.nchunk;  // of the sequence
-  if ((long long)p.item0 + item >= a.most_items) return;
-  const int hk = item / p.q.items, rt = item % p.q.items;
-  const int dim = a.c.dim;
-  // tiles of this chunk
-  const int t_lo = (int)((long long)p.q.nt * chunk / p.nchunk), t_hi = (int)((long long)p.q.nt * (chunk + 1) / p.nchunk);
-  // this lane's query row, and the rows of the item
-  const int in_seq = rt * kRows + row, all_rows = s.n * a.group;
-  const bool real = in_seq < all_rows;
-  const int j = real ? in_seq / a.group : s.n - 1, head = hk * a.group + (real ? in_seq % a.group : 0);
-  const int j_min = rt * kRows / a.group, j_max = min(rt * kRows + kRows - 1, all_rows - 1) / a.group;
-  const int pos = min(s.len + j, a.c.cap - 1);
-  const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
+  Seqs<KT> seqs;
+  const Deal deal = deal_of<KT>(a, seqs);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = deal.per ? deal.items : 0;
+  if (deal.per == 0) return;
+  unsigned u = blockIdx.x, u_end = min(deal.items, u + 1);
+  if (!deal.alone) {
+    u *= deal.per;
+    u_end = min(deal.total, u + deal.per);
+  }
+  while (u < u_end) {
+    Place p = place_of<KT>(a, seqs, u, deal.alone ? kItems : kTiles);
+    if (!p.there) return;
+    const Span s = p.q.s;
+    if (deal.alone) p.inner *= p.q.nt;
+    const int item = (int)(p.inner / p.q.nt);  // of the sequence
+    const int hk = item / p.q.items;
+    // tiles of this share
+    const int t_lo = (int)(p.inner % p.q.nt), t_hi = deal.alone ? p.q.nt : (int)min((unsigned)p.q.nt, t_lo + (u_end - u));
+    // this lane's query row, and the rows of its wavefront
+    const int all_rows = s.n * a.group, row0 = ((item % p.q.items) * a.wide + wave % a.wide) * kRows;
+    const int in_seq = row0 + row;
+    const bool real = in_seq < all_rows, busy = row0 < all_rows;
+    const int j = real ? in_seq / a.group : s.n - 1, head = hk * a.group + (real ? in_seq % a.group : 0);
+    const int j_min = min(row0, all_rows - 1) / a.group, j_max = min(row0 + kRows - 1, all_rows - 1) / a.group;
+    const int pos = min(s.len + j, a.c.cap - 1);
+    const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
 
-  // ---- q ----
-  typedef typename std::conditional<k16, u32x4, f32x4>::type Raw;
-  float row_scale = a.scale;
-  u32x4 qt[k16 ? NT : 1][k16 ? kSteps : 1];
-  f32x4 qf[k16 ? 1 : kSteps];
-  {
-    const size_t at = (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
-    if constexpr (k16) {
-      float x[kSteps][8], most = 0.0f;
+    // ---- q ----
+    typedef typename std::conditional<k16, u32x4, f32x4>::type Raw;
+    float row_scale = a.scale;
+    u32x4 qt[k16 ? NT : 1][k16 ? kSteps : 1];
+    f32x4 qf[k16 ? 1 : kSteps];
+    {
+      const size_t at = (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
+      if constexpr (k16) {
+        float x[kSteps][8], most = 0.0f;
 #pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        const int d = 32 * c + 8 * grp;
-        if (real && d < dim) {
-          load8<Act>(a.q, at + d, x[c]);
-        } else {
+        for (int c = 0; c < kSteps; ++c) {
+          const int d = 32 * c + 8 * grp;
+          if (real && d < dim) {
+            load8<Act>(a.q, at + d, x[c]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[c][i] = 0.0f;
+            for (int i = 0; i < 8; ++i) x[c][i] = 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
+        }
+        if constexpr (M::kScale != 0) {  // a power of two that brings the row's largest to 2^14 .. 2^15
+          most = group_max(most);
+          int e = 0;
+          if (most > 0.0f && most < INFINITY) e = min(max(14 - ilogbf(most), -100), 100);
+          const float up = ldexpf(1.0f, e);
+          row_scale *= ldexpf(1.0f, -e);
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[c][i] *= up;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
-      }
-      if constexpr (M::kScale != 0) {  // a power of two that brings the row's largest to 2^14 .. 2^15
-        most = group_max(most);
-        int e = 0;
-        if (most > 0.0f && most < INFINITY) e = min(max(14 - ilogbf(most), -100), 100);
-        const float up = ldexpf(1.0f, e);
-        row_scale *= ldexpf(1.0f, -e);
+        for (int c = 0; c < kSteps; ++c) {
+          typename M::V8 t[NT];
+          M::split(x[c], t);
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c)
+          for (int k = 0; k < NT; ++k) qt[k][c] = __builtin_bit_cast(u32x4, t[k]);
+        }
+      } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[c][i] *= up;
-      }
-#pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        typename M::V8 t[NT];
-        M::split(x[c], t);
-#pragma unroll
-        for (int k = 0; k < NT; ++k) qt[k][c] = __builtin_bit_cast(u32x4, t[k]);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        const int d = 16 * c + 4 * grp;
-        qf[c] = real && d < dim ? load_global<f32x4>((const float*)a.q + at + d) : f32x4{0, 0, 0, 0};
+        for (int c = 0; c < kSteps; ++c) {
+          const int d = 16 * c + 4 * grp;
+          qf[c] = real && d < dim ? load_global<f32x4>((const float*)a.q + at + d) : f32x4{0, 0, 0, 0};
+        }
       }
     }
-  }
 
-  const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
-  auto key_of = [&](int t) { return (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT; };
-  // page of a half of a tile (-1: not there)
-  auto page_at = [&](int t, int h) {
-    const int i = (key_of(t) + 16 * h) >> a.c.shift;
-    const int pg = t < t_hi && i < a.c.table_ld ? table[i] : -1;
-    return __builtin_amdgcn_readfirstlane(page_there(a.c, pg) ? pg : -1);
-  };
+    const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
+    auto key_of = [&](int t) { return (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT; };
+    // page of a half of a tile (-1: not there)
+    auto page_at = [&](int t, int h) {
+      const int i = (key_of(t) + 16 * h) >> a.c.shift;
+      const int pg = t < t_hi && i < a.c.table_ld ? table[i] : -1;
+      return __builtin_amdgcn_readfirstlane(page_there(a.c, pg) ? pg : -1);
+    };
 
-  Raw kr[kHalves][kSteps], vr[kVLoads];
-  int page[kHalves];
-  auto load_k = [&](int t) {
+    Raw kr[kHalves][kSteps], vr[kVLoads];
+    int page[kHalves];
+    auto load_k = [&](int t) {
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const KV* base = (const KV*)a.c.k + slot_row(a.c, max(page[h], 0), hk, key_of(t) + 16 * h) * dim;
+      for (int h = 0; h < kHalves; ++h) {
+        const KV* base = (const KV*)a.c.k + slot_row(a.c, max(page[h], 0), hk, key_of(t) + 16 * h) * dim;
 #pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        const int d = (k16 ? 32 : 16) * c + kE * grp;
-        kr[h][c] = DT == dim || d < dim ? load_global<Raw>(base + row * dim + d) : Raw{0, 0, 0, 0};
+        for (int c = 0; c < kSteps; ++c) {
+          const int d = (k16 ? 32 : 16) * c + kE * grp;
+          kr[h][c] = DT == dim || d < dim ? load_global<Raw>(base + row * dim + d) : Raw{0, 0, 0, 0};
+        }
       }
-    }
-  };
-  auto load_v = [&](int t) {
-    constexpr int kPerKey = DT / kE;
-#pragma unroll
-    for (int i = 0; i < kVLoads; ++i) {
-      const int key = (64 * i + lane) / kPerKey, d = (64 * i + lane) % kPerKey * kE;
-      const int h = kHalves == 1 ? 0 : (64 * i) / (16 * kPerKey);
-      const KV* base = (const KV*)a.c.v + slot_row(a.c, max(page[h], 0), hk, key_of(t) + 16 * h) * dim;
-      vr[i] = DT == dim || d < dim ? load_global<Raw>(base + (key - 16 * h) * dim + d) : Raw{0, 0, 0, 0};
-    }
-  };
-
-  KV* vs = (KV*)(lds + wave * wave_lds<KV, DT>());
-  f32x4 o[DT / 16];
-#pragma unroll
-  for (int d = 0; d < DT / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
-  float m = -INFINITY, l = 0.0f;
-
-  int t = t_lo + wave;
-#pragma unroll
-  for (int h = 0; h < kHalves; ++h) page[h] = page_at(t, h);
-  if (t < t_hi) {
-    load_k(t);
-    load_v(t);
-  }
-  for (; t < t_hi; t += kWaves) {
-    const int k0 = key_of(t);
-    bool there = true;
-    int cur[kHalves], next[kHalves];
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      cur[h] = page[h];
-      there = there && cur[h] >= 0;
-      next[h] = page_at(t + kWaves, h);
-    }
-    // every key seen by every row, or each looked at
-    const bool whole = there && k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
-    bool apart = false;  // a value that is not finite, of a key that some rows see and others do not
-    if (!whole) {
+    };
+    auto load_v = [&](int t) {
       constexpr int kPerKey = DT / kE;
 #pragma unroll
       for (int i = 0; i < kVLoads; ++i) {
-        const int in = (64 * i + lane) / kPerKey, key = k0 + in;
-        const bool none = (kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0 || key > pos_max ||
-                          (a.window != 0 && key <= pos_min - a.window && key >= a.first);
+        const int key = (64 * i + lane) / kPerKey, d = (64 * i + lane) % kPerKey * kE;
+        const int h = kHalves == 1 ? 0 : (64 * i) / (16 * kPerKey);
+        const KV* base = (const KV*)a.c.v + slot_row(a.c, max(page[h], 0), hk, key_of(t) + 16 * h) * dim;
+        vr[i] = DT == dim || d < dim ? load_global<Raw>(base + (key - 16 * h) * dim + d) : Raw{0, 0, 0, 0};
+      }
+    };
+
+    KV* vs = (KV*)(lds + wave * wave_lds<KV, DT>());
+    f32x4 o[DT / 16];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+    for (int d = 0; d < DT / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+
+    int t = busy ? t_lo + stream : t_hi;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) page[h] = page_at(t, h);
+    if (t < t_hi) {
+      load_k(t);
+      load_v(t);
+    }
+    for (; t < t_hi; t += streams) {
+      const int k0 = key_of(t);
+      bool there = true;
+      int cur[kHalves], next[kHalves];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        cur[h] = page[h];
+        there = there && cur[h] >= 0;
+        next[h] = page_at(t + streams, h);
+      }
+      // every key seen by every row, or each looked at
+      const bool whole = there && k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
+      bool apart = false;  // a value that is not finite, of a key that some rows see and others do not
+      if (!whole) {
+        constexpr int kPerKey = DT / kE;
+#pragma unroll
+        for (int i = 0; i < kVLoads; ++i) {
+          const int in = (64 * i + lane) / kPerKey, key = k0 + in;
+          const bool none = (kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0 || key > pos_max ||
+                            (a.window != 0 && key <= pos_min - a.window && key >= a.first);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (k16) {
+              vr[i][w] = none ? 0u : vr[i][w];
+              apart = apart || M::odd(vr[i][w]);
+            } else {
+              vr[i][w] = none ? 0.0f : vr[i][w];
+              apart = apart || M::odd(__float_as_uint(vr[i][w]));
+            }
+          }
+        }
+        apart = j_min != j_max && __any(apart);
+      }
+      {
+        constexpr int kPerKey = DT / kE;
+#pragma unroll
+        for (int i = 0; i < kVLoads; ++i)
+          *(Raw*)(vs + (64 * i + lane) / kPerKey * kVS + (64 * i + lane) % kPerKey * kE) = vr[i];
+      }
+      // ---- scores ----
+      f32x4 sc[kHalves];
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        sc[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
           if constexpr (k16) {
-            vr[i][w] = none ? 0u : vr[i][w];
-            apart = apart || M::odd(vr[i][w]);
+#pragma unroll
+            for (int k = NT - 1; k >= 0; --k)  // small terms first
+              sc[h] = M::mfma(__builtin_bit_cast(typename M::V8, kr[h][c]), __builtin_bit_cast(typename M::V8, qt[k][c]), sc[h]);
           } else {
-            vr[i][w] = none ? 0.0f : vr[i][w];
-            apart = apart || M::odd(__float_as_uint(vr[i][w]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[h] = M::mfma(kr[h][c][i], qf[c][i], sc[h]);
           }
         }
       }
-      apart = j_min != j_max && __any(apart);
-    }
-    {
-      constexpr int kPerKey = DT / kE;
 #pragma unroll
-      for (int i = 0; i < kVLoads; ++i)
-        *(Raw*)(vs + (64 * i + lane) / kPerKey * kVS + (64 * i + lane) % kPerKey * kE) = vr[i];
-    }
-    // ---- scores ----
-    f32x4 sc[kHalves];
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      sc[h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        if constexpr (k16) {
-#pragma unroll
-          for (int k = NT - 1; k >= 0; --k)  // small terms first
-            sc[h] = M::mfma(__builtin_bit_cast(typename M::V8, kr[h][c]), __builtin_bit_cast(typename M::V8, qt[k][c]), sc[h]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[h] = M::mfma(kr[h][c][i], qf[c][i], sc[h]);
-        }
+      for (int h = 0; h < kHalves; ++h) page[h] = next[h];
+      if (t + streams < t_hi) {
+        load_k(t + streams);
+        load_v(t + streams);
       }
-    }
+      uint32_t seen = 0xff;  // bit 4 h + i: key 16 h + 4 grp + i
+      if (!whole) {
+        seen = 0;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) page[h] = next[h];
-    if (t + kWaves < t_hi) {
-      load_k(t + kWaves);
-      load_v(t + kWaves);
-    }
-    uint32_t seen = 0xff;  // bit 4 h + i: key 16 h + 4 grp + i
-    if (!whole) {
-      seen = 0;
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = k0 + 16 * h + 4 * grp + i;
+            const bool sees = real && cur[h] >= 0 && key <= pos && (a.window == 0 || key > pos - a.window || key < a.first);
+            seen |= sees ? 1u << (4 * h + i) : 0u;
+          }
+      }
+      float mx = -INFINITY;
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = k0 + 16 * h + 4 * grp + i;
-          const bool sees = real && cur[h] >= 0 && key <= pos && (a.window == 0 || key > pos - a.window || key < a.first);
-          seen |= sees ? 1u << (4 * h + i) : 0u;
+          const float x = sc[h][i] * row_scale;
+          sc[h][i] = seen >> (4 * h + i) & 1 ? x : -INFINITY;
+          mx = fmaxf(mx, sc[h][i]);
         }
-    }
-    float mx = -INFINITY;
+      if constexpr (kDump) {
+        const u64 at = ((u64)p.tile0 + (u64)item * p.q.nt + t) * a.wide + wave % a.wide;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = sc[h][i] * row_scale;
-        sc[h][i] = seen >> (4 * h + i) & 1 ? x : -INFINITY;
-        mx = fmaxf(mx, sc[h][i]);
+        for (int h = 0; h < kHalves; ++h) *(W4_GLOBAL f32x4*)(a.dump + (at * 64 + lane) * (4 * kHalves) + 4 * h) = sc[h];
       }
-    if constexpr (kDump) {
-      const u64 at = p.tile0 + (u64)item * p.q.nt + t;
+      const float m_new = fmaxf(m, group_max(mx));
+      const float base = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: exp2(-inf) is 0
+      if (__any(m_new > m)) {
+        const float down = pow2(m - base);
+        l *= down;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) *(W4_GLOBAL f32x4*)(a.dump + (at * 64 + lane) * (4 * kHalves) + 4 * h) = sc[h];
-    }
-    const float m_new = fmaxf(m, group_max(mx));
-    const float base = m_new == -INFINITY ? 0.0f : m_new;  // nothing seen yet: exp2(-inf) is 0
-    if (__any(m_new > m)) {
-      const float down = pow2(m - base);
-      l *= down;
-#pragma unroll
-      for (int d = 0; d < DT / 16; ++d) o[d] *= down;
-    }
-    m = m_new;
-    float pr[8] = {};
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        pr[4 * h + i] = pow2(sc[h][i] - base + (float)M::kScale);
-        l += pr[4 * h + i];
+        for (int d = 0; d < DT / 16; ++d) o[d] *= down;
       }
-    // ---- values ----
-    if (__builtin_expect(apart, 0)) {
-      // 0 times a value that is not finite must not reach a row that does not see it: key by key
+      m = m_new;
+      float pr[8] = {};
 #pragma unroll
       for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          for (int g = 0; g < 4; ++g) {
-            const float w = __shfl(pr[4 * h + i], 16 * g + row);
-            const bool mine = __shfl((int)seen, 16 * g + row) >> (4 * h + i) & 1;
-            const KV* v = vs + (16 * h + 4 * g + i) * kVS + 4 * grp;
+        for (int i = 0; i < 4; ++i) {
+          pr[4 * h + i] = pow2(sc[h][i] - base + (float)M::kScale);
+          l += pr[4 * h + i];
+        }
+      // ---- values ----
+      if (__builtin_expect(apart, 0)) {
+        // 0 times a value that is not finite must not reach a row that does not see it: key by key
 #pragma unroll
-            for (int d = 0; d < DT / 16; ++d)
+        for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float x;
-                if constexpr (k16)
-                  x = M::widen(__builtin_bit_cast(uint16_t, v[16 * d + e]));
-                else
-                  x = v[16 * d + e];
-                o[d][e] += mine ? w * x : 0.0f;
-              }
-          }
-    } else if constexpr (k16) {
-      typename M::V8 pt[NT];
-      M::split(pr, pt);
-      const KV* v = vs + (4 * grp + (row >> 2)) * kVS + 4 * (row & 3);
+          for (int i = 0; i < 4; ++i)
+            for (int g = 0; g < 4; ++g) {
+              const float w = __shfl(pr[4 * h + i], 16 * g + row);
+              const bool mine = __shfl((int)seen, 16 * g + row) >> (4 * h + i) & 1;
+              const KV* v = vs + (16 * h + 4 * g + i) * kVS + 4 * grp;
 #pragma unroll
-      for (int d = 0; d < DT / 16; ++d) {
-        union {
-          s4 half[2];
-          typename M::V8 v8;
-        } vt;
+              for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          vt.half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(v + 16 * h * kVS + 16 * d));
+                for (int e = 0; e < 4; ++e) {
+                  float x;
+                  if constexpr (k16)
+                    x = M::widen(__builtin_bit_cast(uint16_t, v[16 * d + e]));
+                  else
+                    x = v[16 * d + e];
+                  o[d][e] += mine ? w * x : 0.0f;
+                }
+            }
+      } else if constexpr (k16) {
+        typename M::V8 pt[NT];
+        M::split(pr, pt);
+        const KV* v = vs + (4 * grp + (row >> 2)) * kVS + 4 * (row & 3);
 #pragma unroll
-        for (int k = NT - 1; k >= 0; --k) o[d] = M::mfma(vt.v8, pt[k], o[d]);
+        for (int d = 0; d < DT / 16; ++d) {
+          union {
+            s4 half[2];
+            typename M::V8 v8;
+          } vt;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            vt.half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(v + 16 * h * kVS + 16 * d));
+#pragma unroll
+          for (int k = NT - 1; k >= 0; --k) o[d] = M::mfma(vt.v8, pt[k], o[d]);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < DT / 16; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d] = M::mfma(vs[(4 * grp + i) * kVS + 16 * d + row], pr[i], o[d]);
       }
-    } else {
-#pragma unroll
-      for (int d = 0; d < DT / 16; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[d] = M::mfma(vs[(4 * grp + i) * kVS + 16 * d + row], pr[i], o[d]);
     }
-  }
 
-  // ---- join the wavefronts ----
-  l = group_sum(l) * ldexpf(1.0f, -M::kScale);
-  float* sums = (float*)(lds + wave * wave_lds<KV, DT>());
-  float* states = (float*)(lds + kWaves * wave_lds<KV, DT>());
+    // ---- join the wavefronts ----
+    l = group_sum(l) * ldexpf(1.0f, -M::kScale);
+    float* sums = (float*)(lds + wave * wave_lds<KV, DT>());
 #pragma unroll
-  for (int d = 0; d < DT / 16; ++d) *(f32x4*)(sums + row * (DT + 4) + 16 * d + 4 * grp) = o[d] * ldexpf(1.0f, -M::kScale);
-  if (grp == 0) {
-    states[(wave * kRows + row) * 2] = m;
-    states[(wave * kRows + row) * 2 + 1] = l;
-  }
-  __syncthreads();
-  constexpr int kPer = DT / 4;  // threads of a row
-  for (int i = threadIdx.x; i < kRows * kPer; i += 64 * kWaves) {
-    const int r = i / kPer, d = i % kPer * 4, of = rt * kRows + r;
-    if (of >= all_rows) continue;
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, states[(w * kRows + r) * 2]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = pow2(states[(w * kRows + r) * 2] - base);
-      sum += f * states[(w * kRows + r) * 2 + 1];
-      acc += f * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + r * (DT + 4) + d);
+    for (int d = 0; d < DT / 16; ++d) *(f32x4*)(sums + row * (DT + 4) + 16 * d + 4 * grp) = o[d] * ldexpf(1.0f, -M::kScale);
+    if (grp == 0) {
+      states[(wave * kRows + row) * 2] = m;
+      states[(wave * kRows + row) * 2 + 1] = l;
     }
-    if (p.nchunk > 1) {
-      const size_t at = (size_t)blockIdx.x * kRows + r;
-      *(W4_GLOBAL f32x4*)(a.part + at * DT + d) = acc;
-      if (d == 0) {
-        a.state[2 * at] = top;
-        a.state[2 * at + 1] = sum;
+    __syncthreads();
+    // ---- and the shares of the item, where it is not this workgroup's alone ----
+    // The share that has an item's first tile lies in slot 2 w + 1 and the others in 2 w: of two items that meet in a
+    // workgroup one begins there and the other does not.
+    const int of0 = (item % p.q.items) * kRows * a.wide, rows = min(all_rows - of0, kRows * a.wide);
+    const unsigned begin = p.tile0 + (unsigned)item * p.q.nt;
+    const int w_first = deal.alone ? (int)blockIdx.x : (int)(begin / deal.per);
+    const int shares = deal.alone ? 1 : (int)((begin + p.q.nt - 1) / deal.per) - w_first + 1;
+    const int slot = 2 * (int)blockIdx.x + (t_lo == 0);
+    if (t_lo == 0 && threadIdx.x == 0) a.item[p.item0 + item] = Item{w_first, shares, s.r0, of0, rows, hk};
+    constexpr int kPer = DT / 4;  // threads of a row
+    for (int i = threadIdx.x; i < rows * kPer; i += 64 * kWaves) {
+      const int r = i / kPer, d = i % kPer * 4, w0 = r / kRows;
+      float top = -INFINITY, sum = 0.0f;
+      f32x4 acc = {0, 0, 0, 0};
+      for (int w = w0; w < kWaves; w += a.wide) top = fmaxf(top, states[(w * kRows + r % kRows) * 2]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      for (int w = w0; w < kWaves; w += a.wide) {
+        const float f = pow2(states[(w * kRows + r % kRows) * 2] - base);
+        sum += f * states[(w * kRows + r % kRows) * 2 + 1];
+        acc += f * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + (r % kRows) * (DT + 4) + d);
       }
-    } else {
-      if (d < dim) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const size_t at = (size_t)(s.r0 + of / a.group) * a.ldo + (size_t)(hk * a.group + of % a.group) * dim;
-        store4<Act>(a.out, at + d, acc * inv);
+      if (shares > 1) {
+        const size_t at = (size_t)slot * a.slot_rows + r;
+        *(W4_GLOBAL f32x4*)(a.part + at * DT + d) = acc;
+        if (d == 0) {
+          a.state[2 * at] = top;
+          a.state[2 * at + 1] = sum;
+        }
+      } else {
+        finish<Act, kDump>(a, s.r0, of0 + r, hk, (size_t)(p.item0 + item) * a.slot_rows + r, d, acc, base, sum);
       }
-      if (kDump && d == 0) a.lse[(size_t)(p.item0 + item) * kRows + r] = sum == 0.0f ? INFINITY : base + __log2f(sum);
     }
+    u += deal.alone ? 1 : t_hi - t_lo;
+    if (u < u_end) __syncthreads();  // the next item's tiles go where these sums were read
   }
 }
 
-// Joins the chunks of an item: a workgroup per query row, its threads a quarter of the head's values each and, eight (or
-// four, sixteen) of them to a value, every eighth chunk.
-template <typename Act, typename KV, int DT, bool kDump>
+// Joins the shares of an item: a workgroup per query row and kSlice of its values, its threads four values of every 256 /
+// (kSlice / 4)th share each.
+template <typename Act, int DT, int kSlice, bool kDump>
 __global__ __launch_bounds__(256) void join_kernel(Attend a) {
-  constexpr int kPer = DT / 4, kAtOnce = 256 / kPer;
-  __shared__ __attribute__((aligned(16))) float sums[kAtOnce][DT];
-  __shared__ float tops[4], totals[kAtOnce];
-  const Place p = place_of<tile_keys<KV>()>(a, blockIdx.x / kRows, kItems);
-  if (p.b < 0 || p.nchunk == 1) return;
-  const int item = p.inner, hk = item / p.q.items, rt = item % p.q.items, r = blockIdx.x % kRows, of = rt * kRows + r;
-  if (of >= p.q.s.n * a.group || (long long)p.item0 + item >= a.most_items) return;
-  const size_t at = ((size_t)p.chunk0 + (size_t)item * p.nchunk) * kRows + r;
-  float top = -INFINITY;
-  for (int c = threadIdx.x; c < p.nchunk; c += 256) top = fmaxf(top, a.state[2 * (at + (size_t)c * kRows)]);
-#pragma unroll
-  for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  const float base = top == -INFINITY ? 0.0f : top;
-  const int d = threadIdx.x % kPer * 4, first = threadIdx.x / kPer;
+  constexpr int kPer = kSlice / 4, kAtOnce = 256 / kPer;
+  __shared__ __attribute__((aligned(16))) float sums[kAtOnce][kSlice];
+  __shared__ float tops[kAtOnce], totals[kAtOnce];
+  const int slice = blockIdx.x % (DT / kSlice), r = blockIdx.x / (DT / kSlice) % a.slot_rows;
+  const unsigned item = blockIdx.x / (DT / kSlice) / a.slot_rows;
+  const unsigned count = *a.count;
+  const Item it = a.item[item];
+  if (item >= count || it.shares == 1 || r >= it.rows) return;
+  const int d = slice * kSlice + threadIdx.x % kPer * 4, mine = threadIdx.x / kPer;
+  float top = -INFINITY, sum = 0.0f;
   f32x4 acc = {0, 0, 0, 0};
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int c = first; c < p.nchunk; c += kAtOnce) {
-    const size_t from = at + (size_t)c * kRows;
-    const float f = pow2(a.state[2 * from] - base);
-    sum += f * a.state[2 * from + 1];
-    acc += f * load_global<f32x4>(a.part + from * DT + d);
-  }
-  *(f32x4*)&sums[first][d] = acc;
-  if (d == 0) totals[first] = sum;
-  __syncthreads();
-  if (first != 0) return;
+  for (int x0 = mine; x0 < it.shares; x0 += 8 * kAtOnce) {
+    float m[8], l[8];
+    f32x4 v[8];
 #pragma unroll
-  for (int i = 1; i < kAtOnce; ++i) {
-    acc += *(const f32x4*)&sums[i][d];
-    sum += totals[i];
+    for (int x = 0; x < 8; ++x) {
+      const int i = x0 + x * kAtOnce;
+      m[x] = -INFINITY;
+      l[x] = 0.0f;
+      v[x] = f32x4{0, 0, 0, 0};
+      if (i < it.shares) {
+        const size_t at = (size_t)(2 * (it.first + i) + (i == 0)) * a.slot_rows + r;
+        m[x] = load_global<float>(a.state + 2 * at);
+        l[x] = load_global<float>(a.state + 2 * at + 1);
+        v[x] = load_global<f32x4>(a.part + at * DT + d);
+      }
+    }
+    float most = top;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) most = fmaxf(most, m[x]);
+    const float base = most == -INFINITY ? 0.0f : most, down = pow2(top - base);
+    sum *= down;
+    acc *= down;
+    top = most;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const float f = pow2(m[x] - base);
+      sum += f * l[x];
+      acc += f * v[x];
+    }
   }
-  if (d < a.c.dim) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const size_t to = (size_t)(p.q.s.r0 + of / a.group) * a.ldo + (size_t)(hk * a.group + of % a.group) * a.c.dim;
-    store4<Act>(a.out, to + d, acc * inv);
+  *(f32x4*)&sums[mine][threadIdx.x % kPer * 4] = acc;
+  if (threadIdx.x % kPer == 0) {
+    tops[mine] = top;
+    totals[mine] = sum;
   }
-  if (kDump && d == 0) a.lse[(size_t)(p.item0 + item) * kRows + r] = sum == 0.0f ? INFINITY : base + __log2f(sum);
+  __syncthreads();
+  if (mine != 0) return;
+  const int n = min(it.shares, kAtOnce);
+  for (int i = 1; i < n; ++i) top = fmaxf(top, tops[i]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float f = pow2(tops[0] - base);
+  acc *= f;
+  sum *= f;
+  for (int i = 1; i < n; ++i) {
+    f = pow2(tops[i] - base);
+    acc += f * *(const f32x4*)&sums[i][threadIdx.x % kPer * 4];
+    sum += f * totals[i];
+  }
+  finish<Act, kDump>(a, it.r0, it.row0 + r, it.head, (size_t)item * a.slot_rows + r, d, acc, base, sum);
 }
 
 // Adds the weights of a tile's keys up: a wavefront per tile of a kv head, over its items in order.
 template <typename KV>
 __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
-  const Place p = place_of<KT>(a, blockIdx.x, kKeyTiles);
-  if (p.b < 0) return;
-  const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = p.inner / per_head;
-  const int t = p.inner % per_head * kWaves + (threadIdx.x >> 6);
+  Seqs<KT> seqs;
+  if (deal_of<KT>(a, seqs).per == 0) return;
+  const Place p = place_of<KT>(a, seqs, blockIdx.x, kKeyTiles);
+  if (!p.there) return;
+  const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = (int)p.inner / per_head;
+  const int t = (int)p.inner % per_head * kWaves + (threadIdx.x >> 6);
   if (t >= p.q.nt) return;
   const int lane = threadIdx.x & 63, row = lane & 15, grp = lane >> 4;
   float w[4 * kHalves] = {};
-  for (int rt = 0; rt < p.q.items; ++rt) {
-    const int item = hk * p.q.items + rt;
-    if ((long long)p.item0 + item >= a.most_items) break;
-    const bool real = rt * kRows + row < p.q.s.n * a.group;
-    const float lse = real ? a.lse[(size_t)(p.item0 + item) * kRows + row] : INFINITY;
-    const float* from = a.dump + ((p.tile0 + (u64)item * p.q.nt + t) * 64 + lane) * (4 * kHalves);
+  for (int i = 0; i < p.q.items * a.wide; ++i) {
+    const int item = hk * p.q.items + i / a.wide, r = i % a.wide * kRows + row;
+    const u64 tile = (u64)p.tile0 + (u64)item * p.q.nt + t;
+    if (i * kRows >= p.q.s.n * a.group) break;
+    const bool real = i * kRows + row < p.q.s.n * a.group;
+    const float lse = real ? a.lse[((size_t)p.item0 + item) * a.slot_rows + r] : INFINITY;
+    const float* from = a.dump + ((tile * a.wide + i % a.wide) * 64 + lane) * (4 * kHalves);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       const f32x4 x = load_global<f32x4>(from + 4 * h);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[4 * h + i] += real ? pow2(x[i] - lse) : 0.0f;
+      for (int e = 0; e < 4; ++e) w[4 * h + e] += real ? pow2(x[e] - lse) : 0.0f;
     }
   }
 #pragma unroll
@@ -676,10 +759,10 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
-  long long items, grid, key_groups;  // workgroups of the three launches (the join: 16 per item)
-  bool join;
-  int dt;
-  size_t part_off, state_off, lse_off, dump_off, total;
+  long long items, tiles, grid, key_groups;
+  int dt, wide, slot_rows;
+  bool join, sliced;
+  size_t item_off, part_off, state_off, lse_off, dump_off, total;
 };
 
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -689,32 +772,39 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   const int kt = c->dtype == W4A32_CACHE_F32 ? 16 : 32;
   const long long group = r->heads / c->kv_heads, cap = (long long)c->table_ld * c->page;
   const long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
-  const long long by_seq = (most * group + kRows - 1) / kRows * c->n_seqs, by_rows = (long long)r->rows * group / kRows + c->n_seqs;
+  // 32 or 64 rows of an item are two or four wavefronts' that ask for the same keys at about the same time: the caches serve
+  // all but the first, where as items of their own each would have the keys from memory again
+  p.wide = most * group <= kRows ? 1 : most * group <= 2 * kRows ? 2 : 4;
+  const long long of_item = kRows * p.wide;
+  p.slot_rows = (int)(most * group < of_item ? most * group : of_item);
+  const long long by_seq = (most * group + of_item - 1) / of_item * c->n_seqs, by_rows = (long long)r->rows * group / of_item + c->n_seqs;
   p.items = (by_seq < by_rows ? by_seq : by_rows) * c->kv_heads;
   long long tiles = (cap + kt - 1) / kt;
   if (window) {
     const long long near = ((long long)first + kt - 1) / kt + (window + most) / kt + 2;
     tiles = near < tiles ? near : tiles;
   }
-  const long long chunks = (tiles + kMinTiles - 1) / kMinTiles;
-  p.join = chunks > 1;
-  p.grid = p.items * chunks < p.items + (1ll << kTargetLog2) ? p.items * chunks : p.items + (1ll << kTargetLog2);
+  p.tiles = p.items * tiles;
+  p.grid = p.tiles < kGrid ? p.tiles : kGrid;
   p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
   p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
-  if (p.grid >= (1ll << 31) || p.items * kRows >= (1ll << 31) || p.key_groups >= (1ll << 31)) return W4A32_ESHAPE;
-  size_t at = 0;
+  if (p.tiles >= (1ll << 31) || p.items * p.slot_rows * (p.dt / 32) >= (1ll << 31) || p.key_groups >= (1ll << 31)) return W4A32_ESHAPE;
+  // Nothing is shared where every item is short and has a workgroup. Where a join of one workgroup per row leaves most CUs
+  // without work, a row's values are dealt to several.
+  p.join = tiles > kAlone || p.items > p.grid;
+  p.sliced = p.items * p.slot_rows <= 128;
+  size_t at = 256;
+  p.item_off = at;
+  at = up256(at + (size_t)p.items * sizeof(Item));
   p.part_off = at;
-  if (p.join) at = up256(at + (size_t)p.grid * kRows * p.dt * 4);
+  if (p.join) at = up256(at + (size_t)2 * kGrid * p.slot_rows * p.dt * 4);
   p.state_off = at;
-  if (p.join) at = up256(at + (size_t)p.grid * kRows * 2 * 4);
+  if (p.join) at = up256(at + (size_t)2 * kGrid * p.slot_rows * 2 * 4);
   p.lse_off = at;
-  if (accumulate) at = up256(at + (size_t)p.items * kRows * 4);
+  if (accumulate) at = up256(at + (size_t)p.items * p.slot_rows * 4);
   p.dump_off = at;
-  if (accumulate) {
-    if (p.items * tiles >= (1ll << 40)) return W4A32_ESHAPE;
-    at = up256(at + (size_t)p.items * tiles * kRows * kt * 4);
-  }
-  p.total = at ? at : 256;
+  if (accumulate) at = up256(at + (size_t)p.tiles * p.wide * kRows * kt * 4);
+  p.total = at;
   return W4A32_OK;
 }
 
@@ -729,15 +819,14 @@ hipError_t launch(const Attend& a, const Plan& p, bool accumulate, hipStream_t s
   hipLaunchKernelGGL(kernel, dim3((unsigned)p.grid), dim3(64 * kWaves), lds, s, a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (p.join) {
-    auto join = accumulate ? join_kernel<Act, KV, DT, true> : join_kernel<Act, KV, DT, false>;
-    hipLaunchKernelGGL(join, dim3((unsigned)(p.items * kRows)), dim3(256), 0, s, a);
+    auto join = p.sliced ? (accumulate ? join_kernel<Act, DT, 32, true> : join_kernel<Act, DT, 32, false>)
+                         : (accumulate ? join_kernel<Act, DT, DT, true> : join_kernel<Act, DT, DT, false>);
+    hipLaunchKernelGGL(join, dim3((unsigned)(p.items * p.slot_rows * (p.sliced ? DT / 32 : 1))), dim3(256), 0, s, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  if (accumulate) {
-    hipLaunchKernelGGL((weights_kernel<KV>), dim3((unsigned)p.key_groups), dim3(64 * kWaves), 0, s, a);
-    return hipGetLastError();
-  }
-  return hipSuccess;
+  if (!accumulate) return hipSuccess;
+  hipLaunchKernelGGL((weights_kernel<KV>), dim3((unsigned)p.key_groups), dim3(64 * kWaves), 0, s, a);
+  return hipGetLastError();
 }
 template <typename Act, typename KV>
 hipError_t launch_dim(const Attend& a, const Plan& p, bool accumulate, hipStream_t s) {
@@ -776,7 +865,8 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows, rows->max_rows, rows->heads,
-                 rows->heads / cache->kv_heads, window, first, p.items, scale * 1.44269504088896340736f, (float*)(scratch + p.part_off),
+                 rows->heads / cache->kv_heads, window, first, p.wide, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
+                 (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool acc = accumulate != 0;
