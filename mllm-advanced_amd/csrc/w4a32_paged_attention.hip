@@ -30,7 +30,8 @@ constexpr int kRows = 16;         // query rows of a wavefront
 constexpr int kWaves = 4;         // wavefronts of a workgroup
 constexpr int kGrid = 512;        // workgroups that a batch is dealt to: two per CU, all there at once
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
-constexpr int kAlone = 16;        // tiles of an item that is not shared, where there are workgroups enough for all items
+constexpr int kAlone = 8;         // tiles of an item that is not shared, where there are workgroups enough for all items
+constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
 
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -50,7 +51,7 @@ struct Attend {
   const int* row_start;
   int ldq, ldo, rows, max_rows, heads, group;
   int window, first;
-  int wide;             // wavefronts with rows of their own: 1, 2 or 4; an item has 16 times so many rows
+  int wide;             // log2 of the wavefronts with rows of their own (1, 2 or 4): an item has 16 << wide rows
   int slot_rows;        // rows of an item that can be there: what a slot of scratch memory holds
   unsigned most_items, most_tiles;  // what the scratch memory holds: row starts that overlap could ask for more, and get nothing
   float scale;          // of the scores, times log2 e
@@ -75,7 +76,7 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   Seq q;
   q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
   q.keys = min(q.s.len + q.s.n, a.c.cap);
-  q.items = (int)(((long long)q.s.n * a.group + kRows * a.wide - 1) / (kRows * a.wide));
+  q.items = (int)(((long long)q.s.n * a.group + (kRows << a.wide) - 1) >> (4 + a.wide));
   q.w0 = 0;
   q.ft = 0;
   if (a.window) {
@@ -99,12 +100,12 @@ __device__ __forceinline__ unsigned wave_scan(unsigned x) {
 }
 __device__ __forceinline__ unsigned last_lane(unsigned x) { return (unsigned)__builtin_amdgcn_readlane((int)x, 63); }
 
-// How a batch is dealt, and what is counted: tiles of items, items, or tiles of a kv head in fours (for the launch that adds
-// weights up).
-enum Unit { kTiles, kItems, kKeyTiles };
+// How a batch is dealt, and what is counted: tiles of items, shares of one item, or tiles of a kv head, one for each wavefront
+// (for the launch that adds weights up).
+enum Unit { kTiles, kShares, kKeyTiles };
 struct Deal {
   unsigned total, items, per;  // tiles, items, tiles of a share; per = 0: nothing can be done
-  bool alone;                  // a share is an item
+  bool apart;                  // a share has tiles of one item only: ceil(nt / per) of them per item
 };
 struct Place {
   bool there;
@@ -136,33 +137,52 @@ struct Seqs {
 template <int KT>
 __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
   Deal d = {0, 0, 0, false};
-  int longest = 0;
-  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+  bool all_short = true;
+  if (a.c.n_seqs == 1) {  // nothing to add up: a decode step of one sequence is all latency
+    s.load(a, 0);
+    d.total = (unsigned)__builtin_amdgcn_readfirstlane((int)s.tiles);
+    d.items = (unsigned)__builtin_amdgcn_readfirstlane((int)s.items);
+    all_short = __builtin_amdgcn_readfirstlane(s.q.nt) <= kAlone;
+  } else for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
     s.load(a, b0);
     d.total = add_sat(d.total, last_lane(wave_scan(s.tiles)));
     d.items = add_sat(d.items, last_lane(wave_scan(s.items)));
-    longest = max(longest, __any(s.q.nt > kAlone) ? kAlone + 1 : 1);
+    all_short = all_short && !__any(s.q.nt > kAlone);
   }
   if (d.total == 0 || d.total > a.most_tiles || d.items > a.most_items) return d;
-  const unsigned even = (d.total + kGrid - 1) / kGrid;
-  const unsigned few = min((unsigned)kMinTiles, (d.total + d.items - 1) / d.items);
-  d.per = max(even, few);
-  d.alone = longest <= kAlone && d.items <= gridDim.x;
+  d.per = max((d.total + kGrid - 1) / kGrid, (unsigned)kMinTiles);
+  const unsigned more = gridDim.x - min(gridDim.x, d.items);  // workgroups beyond one per item
+  if (all_short && d.items <= gridDim.x) {
+    d.per = kAlone;
+    d.apart = true;
+  } else if (more && (d.total + more - 1) / more <= kFew) {
+    d.per = max((d.total + more - 1) / more, (unsigned)kMinTiles);
+    d.apart = true;
+  }
   return d;
 }
 
 template <int KT>
-__device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT>& s, unsigned u, Unit unit) {
+__device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT>& s, unsigned u, Unit unit, unsigned per) {
   Place p;
   p.there = false;
   p.tile0 = p.item0 = 0;
+  if (a.c.n_seqs == 1) {
+    auto from = [&](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    p.b = 0;
+    p.inner = u;
+    p.q = {{from(s.q.s.r0), from(s.q.s.n), from(s.q.s.len)}, from(s.q.keys), from(s.q.ft), from(s.q.w0), from(s.q.nt), from(s.q.items)};
+    const unsigned each = unit == kTiles ? p.q.nt : unit == kShares ? (p.q.nt + per - 1) / per : (p.q.nt + kWaves - 1) / kWaves;
+    p.there = u < each * (unsigned)a.c.kv_heads * (unit == kKeyTiles ? 1 : p.q.items);
+    return p;
+  }
   unsigned before = 0;
   for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
     if (a.c.n_seqs > 64) s.load(a, b0);
     const unsigned keys = (unsigned)a.c.kv_heads * ((s.q.nt + kWaves - 1) / kWaves);
     const unsigned items = wave_scan(s.items), tiles = wave_scan(s.tiles);
-    const unsigned count = unit == kTiles ? s.tiles : unit == kItems ? s.items : keys;
-    const unsigned upto = unit == kTiles ? tiles : unit == kItems ? items : wave_scan(count);
+    const unsigned count = unit == kTiles ? s.tiles : unit == kShares ? s.items * ((s.q.nt + per - 1) / per) : keys;
+    const unsigned upto = unit == kTiles ? tiles : wave_scan(count);
     const u64 found = __ballot(add_sat(before, upto) > u);
     if (found) {
       const int at = __builtin_ctzll(found);
@@ -304,7 +324,8 @@ template <typename Act, bool kDump>
 __device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, size_t lse_at, int d, f32x4 acc, float base, float sum) {
   if (d < a.c.dim) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const size_t at = (size_t)(r0 + of / a.group) * a.ldo + (size_t)(hk * a.group + of % a.group) * a.c.dim;
+    const int j = (int)((unsigned)of / (unsigned)a.group);
+    const size_t at = (size_t)(r0 + j) * a.ldo + (size_t)(hk * a.group + of - j * a.group) * a.c.dim;
     store4<Act>(a.out, at + d, acc * inv);
   }
   if (kDump && d == 0) a.lse[lse_at] = sum == 0.0f ? INFINITY : base + __log2f(sum);
@@ -323,32 +344,46 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   float* states = (float*)(lds + kWaves * wave_lds<KV, DT>());
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, grp = lane >> 4, dim = a.c.dim;
-  const int streams = kWaves / a.wide, stream = wave / a.wide;  // wavefronts that share rows, and which of them this one is
+  const int streams = kWaves >> a.wide, stream = wave >> a.wide, wide = 1 << a.wide;  // wavefronts that share rows, and which of them this one is
 
   Seqs<KT> seqs;
   const Deal deal = deal_of<KT>(a, seqs);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = deal.per ? deal.items : 0;
   if (deal.per == 0) return;
-  unsigned u = blockIdx.x, u_end = min(deal.items, u + 1);
-  if (!deal.alone) {
+  unsigned u = blockIdx.x, u_end = u + 1;
+  if (!deal.apart) {
     u *= deal.per;
     u_end = min(deal.total, u + deal.per);
   }
   while (u < u_end) {
-    Place p = place_of<KT>(a, seqs, u, deal.alone ? kItems : kTiles);
+    const Place p = place_of<KT>(a, seqs, u, deal.apart ? kShares : kTiles, deal.per);
     if (!p.there) return;
     const Span s = p.q.s;
-    if (deal.alone) p.inner *= p.q.nt;
-    const int item = (int)(p.inner / p.q.nt);  // of the sequence
-    const int hk = item / p.q.items;
-    // tiles of this share
-    const int t_lo = (int)(p.inner % p.q.nt), t_hi = deal.alone ? p.q.nt : (int)min((unsigned)p.q.nt, t_lo + (u_end - u));
+    // the item (of the sequence), the tiles of this share, the workgroups that share the item
+    int item, t_lo, t_hi, w_first, shares;
+    if (deal.apart) {
+      shares = (int)((p.q.nt + deal.per - 1) / deal.per);
+      item = (int)(p.inner / (unsigned)shares);
+      const int mine = (int)p.inner - item * shares;
+      t_lo = (int)((unsigned)(p.q.nt * mine) / (unsigned)shares);  // at most kFew kGrid tiles
+      t_hi = (int)((unsigned)(p.q.nt * (mine + 1)) / (unsigned)shares);
+      w_first = (int)blockIdx.x - mine;
+    } else {
+      item = (int)(p.inner / p.q.nt);
+      t_lo = (int)(p.inner - (unsigned)item * p.q.nt);
+      t_hi = (int)min((unsigned)p.q.nt, t_lo + (u_end - u));
+      const unsigned begin = p.tile0 + (unsigned)item * p.q.nt;
+      w_first = (int)(begin / deal.per);
+      shares = (int)((begin + p.q.nt - 1) / deal.per) - w_first + 1;
+    }
+    const unsigned group = a.group;
+    const int hk = (int)((unsigned)item / (unsigned)p.q.items), of0 = (item - hk * p.q.items) * (kRows << a.wide);
     // this lane's query row, and the rows of its wavefront
-    const int all_rows = s.n * a.group, row0 = ((item % p.q.items) * a.wide + wave % a.wide) * kRows;
+    const int all_rows = s.n * a.group, row0 = of0 + (wave & (wide - 1)) * kRows;
     const int in_seq = row0 + row;
     const bool real = in_seq < all_rows, busy = row0 < all_rows;
-    const int j = real ? in_seq / a.group : s.n - 1, head = hk * a.group + (real ? in_seq % a.group : 0);
-    const int j_min = min(row0, all_rows - 1) / a.group, j_max = min(row0 + kRows - 1, all_rows - 1) / a.group;
+    const int j = (int)((unsigned)min(in_seq, all_rows - 1) / group), head = hk * a.group + (real ? in_seq - j * a.group : 0);
+    const int j_min = (int)((unsigned)min(row0, all_rows - 1) / group), j_max = (int)((unsigned)min(row0 + kRows - 1, all_rows - 1) / group);
     const int pos = min(s.len + j, a.c.cap - 1);
     const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
 
@@ -530,7 +565,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
           mx = fmaxf(mx, sc[h][i]);
         }
       if constexpr (kDump) {
-        const u64 at = ((u64)p.tile0 + (u64)item * p.q.nt + t) * a.wide + wave % a.wide;
+        const u64 at = ((u64)p.tile0 + (u64)item * p.q.nt + t) * wide + (wave & (wide - 1));
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) *(W4_GLOBAL f32x4*)(a.dump + (at * 64 + lane) * (4 * kHalves) + 4 * h) = sc[h];
       }
@@ -554,26 +589,28 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       // ---- values ----
       if (__builtin_expect(apart, 0)) {
         // 0 times a value that is not finite must not reach a row that does not see it: key by key
+#pragma unroll 1
+        for (int n = 0; n < 4 * kHalves; ++n) {
+#pragma unroll 1
+          for (int g = 0; g < 4; ++g) {
+            const float w = __shfl(pr[0], 16 * g + row);
+            const bool mine = __shfl((int)seen, 16 * g + row) >> n & 1;
+            const KV* v = vs + (16 * (n >> 2) + 4 * g + (n & 3)) * kVS + 4 * grp;
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
+            for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            for (int g = 0; g < 4; ++g) {
-              const float w = __shfl(pr[4 * h + i], 16 * g + row);
-              const bool mine = __shfl((int)seen, 16 * g + row) >> (4 * h + i) & 1;
-              const KV* v = vs + (16 * h + 4 * g + i) * kVS + 4 * grp;
+              for (int e = 0; e < 4; ++e) {
+                float x;
+                if constexpr (k16)
+                  x = M::widen(__builtin_bit_cast(uint16_t, v[16 * d + e]));
+                else
+                  x = v[16 * d + e];
+                o[d][e] += mine ? w * x : 0.0f;
+              }
+          }
 #pragma unroll
-              for (int d = 0; d < DT / 16; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float x;
-                  if constexpr (k16)
-                    x = M::widen(__builtin_bit_cast(uint16_t, v[16 * d + e]));
-                  else
-                    x = v[16 * d + e];
-                  o[d][e] += mine ? w * x : 0.0f;
-                }
-            }
+          for (int i = 0; i < 7; ++i) pr[i] = pr[i + 1];
+        }
       } else if constexpr (k16) {
         typename M::V8 pt[NT];
         M::split(pr, pt);
@@ -611,10 +648,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     // ---- and the shares of the item, where it is not this workgroup's alone ----
     // The share that has an item's first tile lies in slot 2 w + 1 and the others in 2 w: of two items that meet in a
     // workgroup one begins there and the other does not.
-    const int of0 = (item % p.q.items) * kRows * a.wide, rows = min(all_rows - of0, kRows * a.wide);
-    const unsigned begin = p.tile0 + (unsigned)item * p.q.nt;
-    const int w_first = deal.alone ? (int)blockIdx.x : (int)(begin / deal.per);
-    const int shares = deal.alone ? 1 : (int)((begin + p.q.nt - 1) / deal.per) - w_first + 1;
+    const int rows = min(all_rows - of0, kRows << a.wide);
     const int slot = 2 * (int)blockIdx.x + (t_lo == 0);
     if (t_lo == 0 && threadIdx.x == 0) a.item[p.item0 + item] = Item{w_first, shares, s.r0, of0, rows, hk};
     constexpr int kPer = DT / 4;  // threads of a row
@@ -622,9 +656,9 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       const int r = i / kPer, d = i % kPer * 4, w0 = r / kRows;
       float top = -INFINITY, sum = 0.0f;
       f32x4 acc = {0, 0, 0, 0};
-      for (int w = w0; w < kWaves; w += a.wide) top = fmaxf(top, states[(w * kRows + r % kRows) * 2]);
+      for (int w = w0; w < kWaves; w += wide) top = fmaxf(top, states[(w * kRows + r % kRows) * 2]);
       const float base = top == -INFINITY ? 0.0f : top;
-      for (int w = w0; w < kWaves; w += a.wide) {
+      for (int w = w0; w < kWaves; w += wide) {
         const float f = pow2(states[(w * kRows + r % kRows) * 2] - base);
         sum += f * states[(w * kRows + r % kRows) * 2 + 1];
         acc += f * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + (r % kRows) * (DT + 4) + d);
@@ -640,7 +674,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         finish<Act, kDump>(a, s.r0, of0 + r, hk, (size_t)(p.item0 + item) * a.slot_rows + r, d, acc, base, sum);
       }
     }
-    u += deal.alone ? 1 : t_hi - t_lo;
+    u += deal.apart ? 1 : t_hi - t_lo;
     if (u < u_end) __syncthreads();  // the next item's tiles go where these sums were read
   }
 }
@@ -717,20 +751,20 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
   Seqs<KT> seqs;
   if (deal_of<KT>(a, seqs).per == 0) return;
-  const Place p = place_of<KT>(a, seqs, blockIdx.x, kKeyTiles);
+  const Place p = place_of<KT>(a, seqs, blockIdx.x, kKeyTiles, 1);
   if (!p.there) return;
   const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = (int)p.inner / per_head;
   const int t = (int)p.inner % per_head * kWaves + (threadIdx.x >> 6);
   if (t >= p.q.nt) return;
   const int lane = threadIdx.x & 63, row = lane & 15, grp = lane >> 4;
   float w[4 * kHalves] = {};
-  for (int i = 0; i < p.q.items * a.wide; ++i) {
-    const int item = hk * p.q.items + i / a.wide, r = i % a.wide * kRows + row;
+  for (int i = 0; i < p.q.items << a.wide; ++i) {
+    const int item = hk * p.q.items + (i >> a.wide), rt = i & ((1 << a.wide) - 1), r = rt * kRows + row;
     const u64 tile = (u64)p.tile0 + (u64)item * p.q.nt + t;
     if (i * kRows >= p.q.s.n * a.group) break;
     const bool real = i * kRows + row < p.q.s.n * a.group;
     const float lse = real ? a.lse[((size_t)p.item0 + item) * a.slot_rows + r] : INFINITY;
-    const float* from = a.dump + ((tile * a.wide + i % a.wide) * 64 + lane) * (4 * kHalves);
+    const float* from = a.dump + (((tile << a.wide) + rt) * 64 + lane) * (4 * kHalves);
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       const f32x4 x = load_global<f32x4>(from + 4 * h);
@@ -865,7 +899,7 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows, rows->max_rows, rows->heads,
-                 rows->heads / cache->kv_heads, window, first, p.wide, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
+                 rows->heads / cache->kv_heads, window, first, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
                  (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
   hipStream_t s = static_cast<hipStream_t>(stream);
