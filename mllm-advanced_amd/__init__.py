@@ -7,6 +7,7 @@ is missing or a call fails, an exception is raised.
 """
 import ctypes
 import os
+import struct
 import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -793,29 +794,40 @@ def decode_linear(x, packed_list, n_list, norm_weight=None, eps=1e-6, delta=None
 
 # ---- a batch of sequences on a paged cache (include/w4a32_decoder.h) ---------------------------
 
-def _on(t, what, *dtypes):
-    """Refuses a tensor of another type, or that is not on the current device, whose stream the call goes to."""
+# These calls take as long on the host as on the GPU where a step is small, so the checks stay plain comparisons, the structs are
+# packed (ctypes fills one field by field) and torch is looked up once.
+_torch = _device = _kinds = None
+_ROWS_STRUCT = struct.Struct("@P4iPP2i")                # w4a32_paged_rows
+_VERIFY_STRUCT = struct.Struct("@9P6if4x")              # w4a32_verify_args
+
+
+def _setup():
+    global _torch, _device, _kinds
     import torch
 
-    if t.dtype not in dtypes:
-        raise W4A32Error(f"{what}: {t.dtype} is not one of {', '.join(map(str, dtypes))}")
-    if not t.is_cuda or t.get_device() != torch.cuda.current_device():
-        raise W4A32Error(f"{what}: not on the current device")
-    return t
+    torch.cuda.current_stream()  # initialises the device
+    _device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _kinds = {torch.float32: CACHE_F32, torch.float16: CACHE_F16, torch.bfloat16: CACHE_BF16}
+    _torch = torch
 
 
-def _row_ld(t, what):
+def _need(t, what, dtype, device, shape=None):
+    """Refuses a tensor that is not contiguous, of the type and shape, and on the device whose stream the call goes to."""
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise W4A32Error(f"{what}: {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, contiguous, on device {device} is wanted: "
+                         f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _row_ld(t, what, dtype, device):
     """Elements from one row to the next of a tensor [rows][width] whose rows are contiguous."""
-    if t.ndim != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2:
+        raise W4A32Error(f"{what}: rows of {dtype} on device {device} are wanted: got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.is_contiguous():
+        return t.shape[1]
+    ld, one = t.stride()
+    if one != 1 and t.shape[1] > 1:
         raise W4A32Error(f"{what}: rows of contiguous elements are wanted, got {tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _flat(t, what, shape=None):
-    if not t.is_contiguous() or (shape is not None and tuple(t.shape) != shape):
-        raise W4A32Error(f"{what}: {tuple(t.shape)} with strides {t.stride()} is not what is wanted"
-                         + (f", {shape} contiguous" if shape is not None else ", contiguous"))
-    return t
+    return ld if t.shape[0] > 1 else t.shape[1]
 
 
 class PagedCache:
@@ -825,57 +837,58 @@ class PagedCache:
     the replays of a captured one), the memory may not."""
 
     def __init__(self, k, v, table, length, weight=None):
-        import torch
-
-        kinds = {torch.float32: CACHE_F32, torch.float16: CACHE_F16, torch.bfloat16: CACHE_BF16}
-        _on(k, "k", *kinds), _on(v, "v", k.dtype), _on(table, "table", torch.int32), _on(length, "length", torch.int32)
-        if k.ndim != 4 or table.ndim != 2:
-            raise W4A32Error("k is [pages][kv_heads][page][dim] and table [sequences][pages]")
+        if _torch is None:
+            _setup()
+        if k.ndim != 4 or table.ndim != 2 or k.dtype not in _kinds:
+            raise W4A32Error("k is [pages][kv_heads][page][dim] of f32, f16 or bf16 and table [sequences][pages]")
+        device = k.get_device()
         pages, kv, page, dim = k.shape
-        _flat(k, "k"), _flat(v, "v", tuple(k.shape)), _flat(table, "table"), _flat(length, "length", (table.shape[0],))
+        _need(k, "k", k.dtype, device), _need(v, "v", k.dtype, device, k.shape), _need(table, "table", _torch.int32, device)
+        _need(length, "length", _torch.int32, device, table.shape[:1])
         if weight is not None:
-            _flat(_on(weight, "weight", torch.float32), "weight", (pages, kv, page))
+            _need(weight, "weight", _torch.float32, device, k.shape[:3])
         self.k, self.v, self.table, self.length, self.weight = k, v, table, length, weight
-        self.dtype, self.device, self.kv_heads, self.dim, self.n_seqs = k.dtype, k.get_device(), kv, dim, table.shape[0]
-        self.args = PagedCacheArgs(k.data_ptr(), v.data_ptr(), _ptr(weight), table.data_ptr(), length.data_ptr(), kinds[k.dtype],
+        self.dtype, self.device, self.kv_heads, self.dim, self.n_seqs = k.dtype, device, kv, dim, table.shape[0]
+        self.args = PagedCacheArgs(k.data_ptr(), v.data_ptr(), _ptr(weight), table.data_ptr(), length.data_ptr(), _kinds[k.dtype],
                                    pages, page, kv, dim, table.shape[0], table.shape[1])
         self._ref = ctypes.byref(self.args)
 
 
 def _paged_rows(cache, q, row_start, max_rows, heads, out):
-    import torch
-
-    if cache.device != torch.cuda.current_device():
-        raise W4A32Error("the cache is not on the current device")
-    _on(q, "q", torch.float32, torch.bfloat16), _on(out, "out", q.dtype), _on(row_start, "row_start", torch.int32)
-    if heads < 1 or q.shape[1:] != (heads * cache.dim,) or out.shape != q.shape:
+    device, dtype = _device(), q.dtype
+    if cache.device != device:
+        raise W4A32Error(f"the cache is on device {cache.device}, the current one is {device}")
+    if dtype is not _torch.float32 and dtype is not _torch.bfloat16:
+        raise W4A32Error(f"rows are f32 or bf16, not {dtype}")
+    ldq, ldo = _row_ld(q, "q", dtype, device), _row_ld(out, "out", dtype, device)
+    rows, width = q.shape
+    if heads < 1 or width != heads * cache.dim or out.shape != q.shape:
         raise W4A32Error(f"rows of {heads} heads of {cache.dim}: got q {tuple(q.shape)} and out {tuple(out.shape)}")
-    _flat(row_start, "row_start", (cache.n_seqs + 1,))
-    return PagedRowsArgs(row_start.data_ptr(), q.shape[0], max_rows, heads, q.dtype == torch.bfloat16, q.data_ptr(), out.data_ptr(),
-                         _row_ld(q, "q"), _row_ld(out, "out"))
+    _need(row_start, "row_start", _torch.int32, device, (cache.n_seqs + 1,))
+    return _ROWS_STRUCT.pack(row_start.data_ptr(), rows, max_rows, heads, dtype is _torch.bfloat16, q.data_ptr(), out.data_ptr(), ldq, ldo)
 
 
 def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max_rows=None, out=None):
     """Rows q [rows][heads * dim], k and v [rows][kv_heads * dim] of all sequences (sequence b: row_start[b] .. row_start[b + 1]):
     returns the rotated q and writes the rotated k, and v, behind the sequences' tokens. sin, cos [positions][rotated / 2]: none,
     no rotation. pos int32 [sequences]: position of a sequence's first row where it is not cache.length."""
-    import torch
-
-    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    rows = q.shape[0]
+    if out is None:
+        out = _torch.empty_like(q)
+    rows, dtype, device = q.shape[0], q.dtype, cache.device
     r = _paged_rows(cache, q, row_start, max_rows or rows, q.shape[1] // cache.dim, out)
+    ldk, ldv = _row_ld(k, "k", dtype, device), _row_ld(v, "v", dtype, device)
     width = (rows, cache.kv_heads * cache.dim)
     if k.shape != width or v.shape != width:
         raise W4A32Error(f"k and v are {width}: got {tuple(k.shape)} and {tuple(v.shape)}")
-    _on(k, "k", q.dtype), _on(v, "v", q.dtype)
-    rot = positions = 0
+    rot = positions = d_sin = d_cos = 0
     if sin is not None:
-        _on(sin, "sin", torch.float32), _on(cos, "cos", torch.float32), _flat(sin, "sin"), _flat(cos, "cos", tuple(sin.shape))
-        positions, rot = sin.shape[0], 2 * sin.shape[1]
+        _need(sin, "sin", _torch.float32, device), _need(cos, "cos", _torch.float32, device, sin.shape)
+        positions, rot = sin.shape
+        d_sin, d_cos, rot = sin.data_ptr(), cos.data_ptr(), 2 * rot
     if pos is not None:
-        _flat(_on(pos, "pos", torch.int32), "pos", (cache.n_seqs,))
-    _check(lib().w4a32_op_paged_append(cache._ref, ctypes.byref(r), k.data_ptr(), _row_ld(k, "k"), v.data_ptr(), _row_ld(v, "v"),
-                                       _ptr(pos), _ptr(sin), _ptr(cos), rot, positions, _stream()), "w4a32_op_paged_append")
+        _need(pos, "pos", _torch.int32, device, (cache.n_seqs,))
+    _check(lib().w4a32_op_paged_append(cache._ref, r, k.data_ptr(), ldk, v.data_ptr(), ldv, _ptr(pos), d_sin or None, d_cos or None, rot,
+                                       positions, _stream()), "w4a32_op_paged_append")
     return out
 
 
@@ -893,15 +906,13 @@ def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, fi
     """Attention of rows q [rows][heads * dim] over their sequences' pages, the rows' own tokens included (appended before):
     row j of sequence b sees slots t <= s = cache.length[b] + j with t > s - window or t < first (window 0: all). max_rows: most
     rows of one sequence. accumulate: the weights that the cached tokens receive are added to cache.weight."""
-    import torch
-
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = _torch.empty_like(q)
     if scratch is None:
         scratch = op_paged_attention_scratch(cache, q.shape[0], max_rows, heads, accumulate)
     r = _paged_rows(cache, q, row_start, max_rows, heads, out)
-    _check(lib().w4a32_op_paged_attention(cache._ref, ctypes.byref(r), scale, window, first, int(accumulate), scratch.data_ptr(),
-                                          scratch.nbytes, _stream()), "w4a32_op_paged_attention")
+    _check(lib().w4a32_op_paged_attention(cache._ref, r, scale, window, first, accumulate, scratch.data_ptr(), scratch.nbytes, _stream()),
+           "w4a32_op_paged_attention")
     return out
 
 
@@ -917,13 +928,11 @@ def op_paged_evict(cache, to, budget, first=0, recent=0, scratch=None):
     """Of every sequence's tokens the first, the most recent and those with the largest added-up weight, `budget` in all per kv
     head, go in order to the pages of `to`, whose lengths are set. Returns the slots that stayed, int32
     [sequences][kv_heads][budget], -1 behind them."""
-    import torch
-
-    if cache.device != torch.cuda.current_device() or to.device != cache.device:
+    if cache.device != _device() or to.device != cache.device:
         raise W4A32Error("the caches are not on the current device")
     if scratch is None:
         scratch = op_paged_evict_scratch(cache, budget)
-    kept = torch.empty((cache.n_seqs, cache.kv_heads, budget), dtype=torch.int32, device="cuda")
+    kept = cache.table.new_empty((cache.n_seqs, cache.kv_heads, budget))
     _check(lib().w4a32_op_paged_evict(cache._ref, to._ref, budget, first, recent, kept.data_ptr(), scratch.data_ptr(), scratch.nbytes,
                                       _stream()), "w4a32_op_paged_evict")
     return kept
@@ -942,30 +951,29 @@ def op_verify_drafts(logits, row_start, max_rows, tokens, uniform, choice, tempe
     how many rows of each sequence stay (the accepted tokens and the one in front of them), and its next token. draft
     [rows][vocab]: the draft model's logits; uniform [rows], choice [sequences]: random numbers from [0, 1) (temperature 0: the
     greedy choice, they may be None). length int32 [sequences]: has the counts added."""
-    import torch
-
-    f32, n = (torch.float32,), row_start.numel() - 1
+    if _torch is None:
+        _setup()
+    f32, i32, device, n = _torch.float32, _torch.int32, _device(), row_start.numel() - 1
+    ldl, ldd = _row_ld(logits, "logits", f32, device), 0
     rows, vocab = logits.shape
-    _on(logits, "logits", *f32), _flat(_on(row_start, "row_start", torch.int32), "row_start")
-    _flat(_on(tokens, "tokens", torch.int64), "tokens", (rows,))
-    ldd = 0
+    _need(row_start, "row_start", i32, device, (n + 1,)), _need(tokens, "tokens", _torch.int64, device, (rows,))
     if draft is not None:
-        ldd = _row_ld(_on(draft, "draft", *f32), "draft")
+        ldd = _row_ld(draft, "draft", f32, device)
         if draft.shape != logits.shape:
             raise W4A32Error(f"draft is {tuple(logits.shape)}: got {tuple(draft.shape)}")
     if uniform is not None:
-        _flat(_on(uniform, "uniform", *f32), "uniform", (rows,))
+        _need(uniform, "uniform", f32, device, (rows,))
     if choice is not None:
-        _flat(_on(choice, "choice", *f32), "choice", (n,))
+        _need(choice, "choice", f32, device, (n,))
     if length is not None:
-        _flat(_on(length, "length", torch.int32), "length", (n,))
+        _need(length, "length", i32, device, (n,))
     if scratch is None:
         scratch = op_verify_drafts_scratch(rows, vocab, n)
-    count = torch.empty((n,), dtype=torch.int32, device="cuda")
-    token = torch.empty((n,), dtype=torch.int64, device="cuda")
-    a = VerifyArgs(logits.data_ptr(), _ptr(draft), row_start.data_ptr(), tokens.data_ptr(), _ptr(uniform), _ptr(choice),
-                   count.data_ptr(), token.data_ptr(), _ptr(length), rows, max_rows, n, vocab, _row_ld(logits, "logits"), ldd, temperature)
-    _check(lib().w4a32_op_verify_drafts(ctypes.byref(a), scratch.data_ptr(), scratch.nbytes, _stream()), "w4a32_op_verify_drafts")
+    count, token = row_start.new_empty(n), tokens.new_empty(n)
+    a = _VERIFY_STRUCT.pack(logits.data_ptr(), _ptr(draft) or 0, row_start.data_ptr(), tokens.data_ptr(), _ptr(uniform) or 0,
+                            _ptr(choice) or 0, count.data_ptr(), token.data_ptr(), _ptr(length) or 0, rows, max_rows, n, vocab, ldl, ldd,
+                            temperature)
+    _check(lib().w4a32_op_verify_drafts(a, scratch.data_ptr(), scratch.nbytes, _stream()), "w4a32_op_verify_drafts")
     return count, token
 
 
