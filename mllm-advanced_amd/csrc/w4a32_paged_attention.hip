@@ -17,7 +17,7 @@
 //                   B = the softmaxed S^T as it lies in the registers: lane group g holds keys 4 g .. 4 g + 3 of a half
 // The matrix instruction's 16 columns are what a group of 6 or 7 heads needs; a kv head with one query head uses one of 16,
 // which costs no time: a 16-bit tile of head size 128 is 16 kilobytes for 16 to 48 instructions of 16 clocks.
-#include "w4a32_paged.h"
+#include "w4a32_paged_attention.h"
 
 namespace w4 {
 namespace paged {
@@ -26,113 +26,12 @@ namespace {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_ELAUNCH; }
 
-constexpr int kRows = 16;         // query rows of a wavefront
-constexpr int kWaves = 4;         // wavefronts of a workgroup
 constexpr int kGrid = 512;        // workgroups that a batch is dealt to: two per CU, all there at once
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
 constexpr int kAlone = 8;         // tiles of an item that is not shared, where there are workgroups enough for all items
+constexpr int kPromptRows = 64;   // pairs of token and head from which on a sequence is the prompts' kernel's
+constexpr int kPromptBlocks = 128;  // ... where that has so many workgroups
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
-
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef unsigned long long u64;
-
-// What the second launch has to know of an item
-struct Item {
-  int first, shares;  // workgroup that has its first tile, and how many have a part of it
-  int r0, row0, rows, head;  // first row of the sequence, first of the item among (token, head of the group), their number, kv head
-};
-
-struct Attend {
-  Cache c;
-  const void* q;
-  void* out;
-  const int* row_start;
-  int ldq, ldo, rows, max_rows, heads, group;
-  int window, first;
-  int wide;             // log2 of the wavefronts with rows of their own (1, 2 or 4): an item has 16 << wide rows
-  int slot_rows;        // rows of an item that can be there: what a slot of scratch memory holds
-  unsigned most_items, most_tiles;  // what the scratch memory holds: row starts that overlap could ask for more, and get nothing
-  float scale;          // of the scores, times log2 e
-  struct Item* item;    // [most_items]
-  unsigned* count;      // how many there are
-  float* part;          // [2 grid][slot_rows][dt]: sums of a share, relative to its maxima
-  float* state;         // [2 grid][slot_rows][2]: maxima (log2) and sums of weights
-  float* lse;           // [item][slot_rows] (accumulate)
-  float* dump;          // [tile of an item][wide][lane][keys of the tile / 4]: scores (accumulate)
-};
-
-// The keys that a sequence's rows can see, in tiles: [0, ft) of the first tokens, then [w0, w0 + nt - ft).
-struct Seq {
-  Span s;
-  int keys;        // tokens there are once the rows are appended
-  int ft, w0, nt;  // tiles; at least one where there are rows
-  int items;       // per kv head
-};
-
-template <int KT>
-__device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
-  Seq q;
-  q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
-  q.keys = min(q.s.len + q.s.n, a.c.cap);
-  q.items = (int)(((long long)q.s.n * a.group + (kRows << a.wide) - 1) >> (4 + a.wide));
-  q.w0 = 0;
-  q.ft = 0;
-  if (a.window) {
-    q.w0 = max(0, min(q.s.len, a.c.cap - 1) - a.window + 1) / KT;
-    q.ft = min((min(a.first, a.c.cap) + KT - 1) / KT, q.w0);
-  }
-  q.nt = q.s.n ? q.ft + (q.keys + KT - 1) / KT - q.w0 : 0;
-  return q;
-}
-
-// Sums over the wavefront's lanes up to this one, by moves within the register file; sums that do not fit stay at the most.
-__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return __builtin_elementwise_add_sat(a, b); }
-__device__ __forceinline__ unsigned wave_scan(unsigned x) {
-  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));  // row_shr 1, 2, 4, 8
-  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
-  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
-  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
-  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast 15, 31
-  x = add_sat(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));
-  return x;
-}
-__device__ __forceinline__ unsigned last_lane(unsigned x) { return (unsigned)__builtin_amdgcn_readlane((int)x, 63); }
-
-// How a batch is dealt, and what is counted: tiles of items, shares of one item, or tiles of a kv head, one for each wavefront
-// (for the launch that adds weights up).
-enum Unit { kTiles, kShares, kKeyTiles };
-struct Deal {
-  unsigned total, items, per;  // tiles, items, tiles of a share; per = 0: nothing can be done
-  bool apart;                  // a share has tiles of one item only: ceil(nt / per) of them per item
-};
-struct Place {
-  bool there;
-  int b;
-  unsigned inner;   // which one of the sequence
-  unsigned tile0;   // tiles of items in front of the sequence
-  unsigned item0;   // items in front of the sequence
-  Seq q;
-};
-
-// The sequences of a block of 64, one of each lane: kept where there is one block only.
-template <int KT>
-struct Seqs {
-  Seq q;
-  unsigned tiles, items;
-  __device__ __forceinline__ void load(const Attend& a, int b0) {
-    const int b = b0 + (int)(threadIdx.x & 63);
-    q = {};
-    tiles = items = 0;
-    if (b < a.c.n_seqs) {
-      q = seq_of<KT>(a, b);
-      const u64 n = (u64)q.items * a.c.kv_heads;
-      items = (unsigned)min(n, (u64)0xffffffffu);
-      tiles = (unsigned)min(n * q.nt, (u64)0xffffffffu);
-    }
-  }
-};
 
 template <int KT>
 __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
@@ -162,125 +61,6 @@ __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
   return d;
 }
 
-template <int KT>
-__device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT>& s, unsigned u, Unit unit, unsigned per) {
-  Place p;
-  p.there = false;
-  p.tile0 = p.item0 = 0;
-  if (a.c.n_seqs == 1) {
-    auto from = [&](int x) { return __builtin_amdgcn_readfirstlane(x); };
-    p.b = 0;
-    p.inner = u;
-    p.q = {{from(s.q.s.r0), from(s.q.s.n), from(s.q.s.len)}, from(s.q.keys), from(s.q.ft), from(s.q.w0), from(s.q.nt), from(s.q.items)};
-    const unsigned each = unit == kTiles ? p.q.nt : unit == kShares ? (p.q.nt + per - 1) / per : (p.q.nt + kWaves - 1) / kWaves;
-    p.there = u < each * (unsigned)a.c.kv_heads * (unit == kKeyTiles ? 1 : p.q.items);
-    return p;
-  }
-  unsigned before = 0;
-  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
-    if (a.c.n_seqs > 64) s.load(a, b0);
-    const unsigned keys = (unsigned)a.c.kv_heads * ((s.q.nt + kWaves - 1) / kWaves);
-    const unsigned items = wave_scan(s.items), tiles = wave_scan(s.tiles);
-    const unsigned count = unit == kTiles ? s.tiles : unit == kShares ? s.items * ((s.q.nt + per - 1) / per) : keys;
-    const unsigned upto = unit == kTiles ? tiles : wave_scan(count);
-    const u64 found = __ballot(add_sat(before, upto) > u);
-    if (found) {
-      const int at = __builtin_ctzll(found);
-      auto from = [&](unsigned x) { return __builtin_amdgcn_readlane((int)x, at); };
-      p.there = true;
-      p.b = b0 + at;
-      p.inner = u - before - (unsigned)from(upto - count);
-      p.tile0 += (unsigned)from(tiles - s.tiles);
-      p.item0 += (unsigned)from(items - s.items);
-      p.q.s.r0 = from(s.q.s.r0);
-      p.q.s.n = from(s.q.s.n);
-      p.q.s.len = from(s.q.s.len);
-      p.q.keys = from(s.q.keys);
-      p.q.ft = from(s.q.ft);
-      p.q.w0 = from(s.q.w0);
-      p.q.nt = from(s.q.nt);
-      p.q.items = from(s.q.items);
-      return p;
-    }
-    before = add_sat(before, last_lane(upto));
-    p.tile0 = add_sat(p.tile0, last_lane(tiles));
-    p.item0 = add_sat(p.item0, last_lane(items));
-  }
-  return p;
-}
-
-__device__ __forceinline__ float group_max(float x) {  // over the four lane groups: all lanes of one query row
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float group_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
-__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// ---- element types ---------------------------------------------------------------------------------------------------------
-// kTerms operands stand for one f32 operand of the 16-bit matrix instruction. kScale: exponent that the softmaxed scores
-// carry until the sums are divided (they cancel there).
-template <typename Act, typename KV>
-struct Math;
-
-// bf16: three truncations hold the 24 bits of an f32 whatever its exponent
-template <typename Act>
-struct Math<Act, __bf16> {
-  static constexpr int kTerms = sizeof(Act) == 4 ? 3 : 1;
-  static constexpr int kScale = 0;
-  typedef bf8 V8;
-  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ void split(const float (&x)[8], V8 (&t)[kTerms]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (kTerms == 1) {
-        t[0][i] = (__bf16)x[i];
-      } else {
-        float r = x[i];
-#pragma unroll
-        for (int k = 0; k < kTerms; ++k) {
-          const uint32_t top = __float_as_uint(r) & 0xffff0000u;
-          t[k][i] = __builtin_bit_cast(__bf16, (uint16_t)(top >> 16));
-          r -= __uint_as_float(top);
-        }
-      }
-    }
-  }
-  static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among two elements
-    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-  }
-  static __device__ __forceinline__ float widen(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
-};
-// f16: two roundings hold 22 to 24 bits of a number that is scaled near the type's largest, and of a smaller one whatever
-// lies above 2^-40 of the row's largest
-template <typename Act>
-struct Math<Act, _Float16> {
-  static constexpr int kTerms = 2;
-  static constexpr int kScale = 15;
-  typedef h8 V8;
-  static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ void split(const float (&x)[8], V8 (&t)[kTerms]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      t[0][i] = (_Float16)x[i];
-      t[1][i] = (_Float16)(x[i] - (float)t[0][i]);
-    }
-  }
-  static __device__ __forceinline__ bool odd(uint32_t w) {
-    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
-  }
-  static __device__ __forceinline__ float widen(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
-};
-// f32: the f32 matrix instruction, operands as they are
-template <>
-struct Math<float, float> {
-  static constexpr int kTerms = 1;
-  static constexpr int kScale = 0;
-  static __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
-};
 
 template <typename KV>
 constexpr int tile_keys() { return sizeof(KV) == 2 ? 32 : 16; }
@@ -293,43 +73,6 @@ constexpr size_t wave_lds() {  // a wavefront's tile of V; at the end its 16 row
 }
 template <typename KV, int DT>
 constexpr size_t lds_bytes() { return kWaves * (wave_lds<KV, DT>() + kRows * 2 * sizeof(float)); }
-
-template <typename Act>
-__device__ __forceinline__ void load8(const void* p, size_t at, float (&x)[8]) {
-  if constexpr (sizeof(Act) == 4) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 v = load_global<f32x4>((const float*)p + at + 4 * h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * h + i] = v[i];
-    }
-  } else {
-    const u32x4 v = load_global<u32x4>((const uint16_t*)p + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i & 1 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
-  }
-}
-template <typename Act>
-__device__ __forceinline__ void store4(void* p, size_t at, f32x4 x) {
-  if constexpr (sizeof(Act) == 4) {
-    *(W4_GLOBAL f32x4*)((float*)p + at) = x;
-  } else {
-    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-    *(W4_GLOBAL b4*)((uint16_t*)p + at) = b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
-  }
-}
-
-// A row's result, from its sums and the sum of its weights
-template <typename Act, bool kDump>
-__device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, size_t lse_at, int d, f32x4 acc, float base, float sum) {
-  if (d < a.c.dim) {
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int j = (int)((unsigned)of / (unsigned)a.group);
-    const size_t at = (size_t)(r0 + j) * a.ldo + (size_t)(hk * a.group + of - j * a.group) * a.c.dim;
-    store4<Act>(a.out, at + d, acc * inv);
-  }
-  if (kDump && d == 0) a.lse[lse_at] = sum == 0.0f ? INFINITY : base + __log2f(sum);
-}
 
 // DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up.
 template <typename Act, typename KV, int DT, bool kDump>
@@ -356,7 +99,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     u_end = min(deal.total, u + deal.per);
   }
   while (u < u_end) {
-    const Place p = place_of<KT>(a, seqs, u, deal.apart ? kShares : kTiles, deal.per);
+    const Place p = place_of(a, seqs, u, deal.apart ? kShares : kTiles, deal.per);
     if (!p.there) return;
     const Span s = p.q.s;
     // the item (of the sequence), the tiles of this share, the workgroups that share the item
@@ -408,12 +151,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll
           for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
         }
-        if constexpr (M::kScale != 0) {  // a power of two that brings the row's largest to 2^14 .. 2^15
-          most = group_max(most);
-          int e = 0;
-          if (most > 0.0f && most < INFINITY) e = min(max(14 - ilogbf(most), -100), 100);
-          const float up = ldexpf(1.0f, e);
-          row_scale *= ldexpf(1.0f, -e);
+        if constexpr (M::kScale != 0) {
+          const float up = M::row_scale(group_max(most), row_scale);
 #pragma unroll
           for (int c = 0; c < kSteps; ++c)
 #pragma unroll
@@ -751,7 +490,7 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
   Seqs<KT> seqs;
   if (deal_of<KT>(a, seqs).per == 0) return;
-  const Place p = place_of<KT>(a, seqs, blockIdx.x, kKeyTiles, 1);
+  const Place p = place_of(a, seqs, blockIdx.x, kKeyTiles, 1);
   if (!p.there) return;
   const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = (int)p.inner / per_head;
   const int t = (int)p.inner % per_head * kWaves + (threadIdx.x >> 6);
@@ -795,7 +534,9 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
 struct Plan {
   long long items, tiles, grid, key_groups;
   int dt, wide, slot_rows;
-  bool join, sliced;
+  bool join, sliced, others;  // others: rows that are not the prompts' kernel's
+  int prompt_rows;
+  long long prompts;          // its workgroups
   size_t item_off, part_off, state_off, lse_off, dump_off, total;
 };
 
@@ -819,6 +560,14 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
     tiles = near < tiles ? near : tiles;
   }
   p.tiles = p.items * tiles;
+  p.prompts = (long long)r->rows * group / (1 << kPromptLog2) * c->kv_heads + (long long)c->n_seqs * c->kv_heads;
+  p.prompt_rows = 0;
+  p.others = true;
+  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && p.prompts >= kPromptBlocks) {
+    // where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then
+    p.others = r->rows < (long long)r->max_rows * c->n_seqs;
+    p.prompt_rows = p.others ? kPromptRows : 1;
+  }
   p.grid = p.tiles < kGrid ? p.tiles : kGrid;
   p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
   p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
@@ -850,6 +599,7 @@ hipError_t launch(const Attend& a, const Plan& p, bool accumulate, hipStream_t s
     static LdsLimitOnce limit[2];
     if (hipError_t e = limit[accumulate].raise((const void*)kernel, lds); e != hipSuccess) return e;
   }
+  if (!p.others) return hipSuccess;
   hipLaunchKernelGGL(kernel, dim3((unsigned)p.grid), dim3(64 * kWaves), lds, s, a);
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   if (p.join) {
@@ -899,11 +649,14 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows, rows->max_rows, rows->heads,
-                 rows->heads / cache->kv_heads, window, first, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
+                 rows->heads / cache->kv_heads, window, first, p.prompt_rows, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
                  (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool acc = accumulate != 0;
+  if (p.prompt_rows)
+    if (hipError_t e = launch_prompts(a, cache->dtype, rows->act_bf16 != 0, p.dt, (unsigned)p.prompts, s); e != hipSuccess)
+      return W4A32_ELAUNCH;
   if (rows->act_bf16) return from_hip(launch_dim<__bf16, __bf16>(a, p, acc, s));
   if (cache->dtype == W4A32_CACHE_F32) return from_hip(launch_dim<float, float>(a, p, acc, s));
   if (cache->dtype == W4A32_CACHE_F16) return from_hip(launch_dim<float, _Float16>(a, p, acc, s));

@@ -1,0 +1,347 @@
+// Attention of prompts over a paged cache of 16-bit elements: the sequences of a batch that have so many rows that products bound
+// them and not the cache.
+//
+// A workgroup has 128 query rows of one kv head (pairs of token and head of the group, 32 to a wavefront) and takes the keys that
+// they can see, 64 (32 where an f32 operand is two or three terms, or the head has 256 dims) at a time through LDS: the next
+// tile's loads are in flight in registers while this one is multiplied. Both products are transposed as in the rows' kernel, on
+// v_mfma_f32_32x32x16: a lane stands for query row lane % 32, and lanes l and l + 32 share it.
+//   S^T = K Q^T     A = K from LDS: lane = key l % 32, dims 16 c + 8 (l / 32) ..; B = Q in registers
+//   O^T += V^T P^T  B = the softmaxed S^T registers: half h of the wavefront has keys 8 b + 4 h .. + 3 of a block of 32;
+//                   A = V^T: ds_read_b64_tr_b16 of the same keys
+// What bounds it: a tile of 64 keys and 128 dims costs a SIMD 32 x 32 = 1024 clocks of bf16 products per wavefront, and about as
+// many of maxima, exponentials and sums, which run under the other wavefront's products (two per SIMD).
+// LDS rows: K on 16 bytes more than its dims (a read of 16 rows meets every bank once), V on 64 bytes more (so do the 8 rows of
+// 64 bytes that a transposing read takes).
+// Rows of one kv head lie together, so that a group of heads reads a key once; workgroups of consecutive numbers have
+// consecutive kv heads, which the dispatcher deals to the XCDs in turn: an L2 sees few heads. Late rows, which see most keys,
+// come first.
+#include "w4a32_paged_attention.h"
+
+namespace w4 {
+namespace paged {
+
+namespace {
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int kBlock = 1 << kPromptLog2;
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+
+template <typename Act, typename KV, int DT>
+struct Shape {
+  static constexpr int kTerms = Math<Act, KV>::kTerms;
+  static constexpr int kKeys = kTerms == 1 && DT <= 128 ? 64 : 32;
+  static constexpr int kKS = DT + 8, kVS = DT + 32;  // elements of LDS rows
+  static constexpr int kBuffer = kKeys * (kKS + kVS);
+  static constexpr size_t kLds = (size_t)2 * kBuffer * 2 + 2 * 4 * sizeof(int);
+};
+
+template <typename Act, typename KV, int DT>
+__global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Attend a) {
+  using M = Math<Act, KV>;
+  using Sh = Shape<Act, KV, DT>;
+  constexpr int NT = Sh::kTerms, KB = Sh::kKeys, kSub = KB / 32, kSteps = DT / 16, kDims = DT / 32;
+  constexpr int kPerKey = DT / 8;                      // 16-byte loads of a key
+  constexpr int kLoads = KB * kPerKey / kThreads;      // of a thread, for K and for V
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int* odd_flags = (int*)(lds + (size_t)2 * Sh::kBuffer * 2);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 31, half = lane >> 5, dim = a.c.dim;
+
+  // ---- which rows ----
+  Seqs<KB, true> seqs;
+  unsigned total = 0;
+  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+    seqs.load(a, b0);
+    total = add_sat(total, last_lane(wave_scan(seqs.items)));
+  }
+  if (blockIdx.x >= total) return;
+  const Place p = place_of(a, seqs, total - 1 - blockIdx.x, kItems, 1);
+  if (!p.there) return;
+  const Span s = p.q.s;
+  const unsigned group = a.group;
+  const int block = (int)(p.inner / (unsigned)a.c.kv_heads), hk = (int)p.inner - block * a.c.kv_heads;
+  const int all_rows = s.n * a.group, of0 = block * kBlock, row0 = of0 + 32 * wave, in_seq = row0 + row;
+  const bool real = in_seq < all_rows;
+  auto slot_of = [&](int r) { return min(s.len + (int)((unsigned)min(r, all_rows - 1) / group), a.c.cap - 1); };
+  const int j = (int)((unsigned)min(in_seq, all_rows - 1) / group), head = hk * a.group + (real ? in_seq - j * a.group : 0);
+  const int pos = min(s.len + j, a.c.cap - 1), pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
+  const int block_min = slot_of(of0), block_max = slot_of(of0 + kBlock - 1);
+  // tiles that the workgroup's rows can see: [0, ft) and [w0, ..)
+  const int w0 = a.window ? max(0, block_min - a.window + 1) / KB : 0;
+  const int ft = a.window ? min((min(a.first, a.c.cap) + KB - 1) / KB, w0) : 0;
+  const int nt = ft + block_max / KB + 1 - w0;
+  auto key_of = [&](int t) { return (t < ft ? t : t - ft + w0) * KB; };
+
+  // ---- q ----
+  float row_scale = a.scale;
+  typename M::V8 q[NT][kSteps];
+  {
+    const size_t at = (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
+    float x[kSteps][8], most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
+      const int d = 16 * c + 8 * half;
+      if (real && d < dim) {
+        load8<Act>(a.q, at + d, x[c]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[c][i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
+    }
+    float up = 1.0f;
+    if constexpr (M::kScale != 0) {
+      most = fmaxf(most, __shfl_xor(most, 32));
+      up = M::row_scale(most, row_scale);
+    }
+#pragma unroll
+    for (int c = 0; c < kSteps; ++c) {
+      typename M::V8 t[NT];
+      if constexpr (M::kScale != 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[c][i] *= up;
+      }
+      M::split(x[c], t);
+#pragma unroll
+      for (int k = 0; k < NT; ++k) q[k][c] = t[k];
+    }
+  }
+
+  // ---- tiles ----
+  const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
+  u32x4 kr[kLoads], vr[kLoads];
+  // A wavefront's 64 loads lie in one page: they are at most 16 keys that begin at a multiple of 8 or less
+  auto wave_key = [&](int i) { return (kThreads * i + 64 * wave) / kPerKey; };
+  int page[kLoads];
+  auto find = [&](int t) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int at = (key_of(t) + wave_key(i)) >> a.c.shift;
+      const int pg = t < nt && at < a.c.table_ld ? table[at] : -1;
+      page[i] = __builtin_amdgcn_readfirstlane(page_there(a.c, pg) ? pg : -1);
+    }
+  };
+  int kept_key0 = 0, missing = 0;
+  auto load = [&](int t) {
+    missing = 0;
+    kept_key0 = key_of(t);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = (kThreads * i + tid) / kPerKey, d = (kThreads * i + tid) % kPerKey * 8;
+      missing |= page[i] < 0 ? 1 << i : 0;
+      const size_t at = slot_row(a.c, max(page[i], 0), hk, kept_key0 + key) * dim + d;
+      const bool in = DT == dim || d < dim;
+      kr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.k + at) : u32x4{0, 0, 0, 0};
+      vr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.v + at) : u32x4{0, 0, 0, 0};
+    }
+  };
+  // Whether all of the workgroup's rows see all keys from k0 on
+  auto all_seen = [&](int k0, int lo, int hi) {
+    return k0 + KB - 1 <= lo && (a.window == 0 || k0 > hi - a.window || k0 + KB - 1 < a.first);
+  };
+  auto put = [&](int buffer) {
+    uint16_t* ks = (uint16_t*)lds + buffer * Sh::kBuffer;
+    uint16_t* vs = ks + KB * Sh::kKS;
+    bool odd = false;
+    const bool look = missing || !all_seen(kept_key0, block_min, block_max);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int key = (kThreads * i + tid) / kPerKey, d = (kThreads * i + tid) % kPerKey * 8, at = kept_key0 + key;
+      if (look) {  // what no row sees must not meet a weight of 0 as an infinity or NaN
+        const bool none = missing >> i & 1 || at > block_max || (a.window != 0 && at <= block_min - a.window && at >= a.first);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          vr[i][w] = none ? 0u : vr[i][w];
+          odd = odd || M::odd(vr[i][w]);
+        }
+      }
+      *(u32x4*)(ks + key * Sh::kKS + d) = kr[i];
+      *(u32x4*)(vs + key * Sh::kVS + d) = vr[i];
+    }
+    // bit 0: values that are not finite; bits 1 ..: loads of this wavefront whose page is not there
+    const int any = __any(odd) ? 1 : 0;
+    if (lane == 0) odd_flags[4 * buffer + wave] = any | missing << 1;
+  };
+
+  f32x16 o[kDims];
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  find(0);
+  load(0);
+  find(1);
+  put(0);
+  __syncthreads();
+  for (int t = 0; t < nt; ++t) {
+    if (t + 1 < nt) load(t + 1);
+    find(t + 2);
+    const uint16_t* ks = (const uint16_t*)lds + (t & 1) * Sh::kBuffer;
+    const uint16_t* vs = ks + KB * Sh::kKS;
+    const int k0 = key_of(t);
+    int flags = 0, gone = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int f = odd_flags[4 * (t & 1) + w];
+      flags |= f;
+      gone |= f >> 1;
+    }
+    flags = __builtin_amdgcn_readfirstlane(flags);
+    gone = __builtin_amdgcn_readfirstlane(gone);
+    const bool whole = gone == 0 && all_seen(k0, pos_min, pos_max);
+    const bool none = row0 >= all_rows || k0 > pos_max;  // of this wavefront
+    if (!none) {
+      // ---- scores ----
+      f32x16 sc[kSub];
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[u][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c) {
+          const typename M::V8 kf = *(const typename M::V8*)(ks + (32 * u + row) * Sh::kKS + 16 * c + 8 * half);
+#pragma unroll
+          for (int k = NT - 1; k >= 0; --k) sc[u] = mfma32(kf, q[k][c], sc[u]);
+        }
+      }
+      uint32_t seen[kSub];  // bit i: key 32 u + 8 (i / 4) + 4 half + i % 4
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) seen[u] = 0xffff;
+      if (!whole) {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+          seen[u] = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int in = 32 * u + 8 * (i / 4) + 4 * half + i % 4, key = k0 + in;
+            bool sees = real && key <= pos && (a.window == 0 || key > pos - a.window || key < a.first);
+            if (gone) {
+              const int at = key >> a.c.shift;
+              sees = sees && at < a.c.table_ld && page_there(a.c, table[at < a.c.table_ld ? at : 0]);
+            }
+            seen[u] |= sees ? 1u << i : 0u;
+            sc[u][i] = sees ? sc[u][i] : -INFINITY;
+          }
+        }
+      }
+      // ---- softmax: with c the scale of the row (times log2 e), 2^(c s - c m) ----
+      float mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < kSub; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[u][i] *= row_scale;
+          mx = fmaxf(mx, sc[u][i]);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new;
+      if (__any(m_new > m)) {
+        const float down = pow2(m - base);
+        l *= down;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[d] *= down;
+      }
+      m = m_new;
+      const float off = (float)M::kScale - base;
+      const bool apart = !whole && (flags & 1);
+#pragma unroll
+      for (int u = 0; u < kSub; ++u) {
+        float pr[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          pr[i] = pow2(sc[u][i] + off);
+          l += pr[i];
+        }
+        if (__builtin_expect(apart, 0)) {
+          // 0 times a value that is not finite must not reach a row that does not see it: key by key
+#pragma unroll 1
+          for (int n = 0; n < 16; ++n) {
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              const float w = __shfl(pr[0], 32 * h + row);
+              const bool mine = __shfl((int)seen[u], 32 * h + row) >> n & 1;
+              const uint16_t* v = vs + (32 * u + 8 * (n >> 2) + 4 * h + (n & 3)) * Sh::kVS + 4 * half;
+#pragma unroll
+              for (int d = 0; d < kDims; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const float x = M::widen(v[32 * d + 8 * (i / 4) + i % 4]);
+                  o[d][i] += mine ? w * x : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 15; ++i) pr[i] = pr[i + 1];
+          }
+          continue;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {  // 16 keys
+          float p8[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p8[i] = pr[8 * c + i];
+          typename M::V8 pt[NT];
+          M::split(p8, pt);
+          const uint16_t* v = vs + (32 * u + 16 * c + 4 * half + ((lane & 15) >> 2)) * Sh::kVS + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+          for (int d = 0; d < kDims; ++d) {
+            union {
+              s4 part[2];
+              typename M::V8 v8;
+            } vt;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              vt.part[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(v + 8 * x * Sh::kVS + 32 * d));
+#pragma unroll
+            for (int k = NT - 1; k >= 0; --k) o[d] = mfma32(vt.v8, pt[k], o[d]);
+          }
+        }
+      }
+    }
+    if (t + 1 < nt) put((t + 1) & 1);
+    __syncthreads();
+  }
+
+  // ---- results: lane = row, four dims at a time ----
+  l += __shfl_xor(l, 32);
+  if (!real) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const size_t at = (size_t)(s.r0 + j) * a.ldo + (size_t)head * dim;
+#pragma unroll
+  for (int d = 0; d < kDims; ++d)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int to = 32 * d + 8 * b + 4 * half;
+      if (DT == dim || to < dim) store4<Act>(a.out, at + to, f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]} * inv);
+    }
+}
+
+template <typename Act, typename KV, int DT>
+hipError_t launch(const Attend& a, unsigned items, hipStream_t s) {
+  constexpr size_t lds = Shape<Act, KV, DT>::kLds;
+  if constexpr (lds > 64 * 1024) {
+    static LdsLimitOnce limit;
+    if (hipError_t e = limit.raise((const void*)prompt_kernel<Act, KV, DT>, lds); e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT>), dim3(items), dim3(kThreads), lds, s, a);
+  return hipGetLastError();
+}
+template <typename Act, typename KV>
+hipError_t launch_dim(const Attend& a, int dt, unsigned items, hipStream_t s) {
+  if (dt == 64) return launch<Act, KV, 64>(a, items, s);
+  if (dt == 128) return launch<Act, KV, 128>(a, items, s);
+  return launch<Act, KV, 256>(a, items, s);
+}
+}  // namespace
+
+hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s) {
+  if (act_bf16) return launch_dim<__bf16, __bf16>(a, dt, items, s);
+  if (dtype == W4A32_CACHE_F16) return launch_dim<float, _Float16>(a, dt, items, s);
+  return launch_dim<float, __bf16>(a, dt, items, s);
+}
+
+}  // namespace paged
+}  // namespace w4

@@ -60,11 +60,14 @@ def attend(B, q, k, v, heads, scale, window=0, first=0):
     for b, n in enumerate(B.lens):
         for j in range(B.rows[b]):
             s = n + j
-            seen = [t for t in range(min(s + 1, B.ld * B.page)) if (window == 0 or t > s - window or t < first) and B.there(b, t)]
-            if not seen:
+            t = np.arange(min(s + 1, B.ld * B.page))
+            page = B.table[b, t // B.page]
+            seen = (page >= 0) & (page < B.n_pages)
+            if window:
+                seen &= (t > s - window) | (t < first)
+            if not seen.any():
                 continue
-            at = [B.slot(b, t) for t in seen]
-            pages, slots = [p for p, _ in at], [i for _, i in at]
+            pages, slots = page[seen], t[seen] % B.page
             for h in range(heads):
                 kk, vv = k[pages, h // G, slots], v[pages, h // G, slots]
                 with np.errstate(invalid="ignore", over="ignore"):

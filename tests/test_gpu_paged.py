@@ -100,6 +100,59 @@ def test_attention(pkg, act, kind, heads, kv, dim, page, lens, rows):
 
 
 @pytest.mark.parametrize("act,kind", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,page,lens,rows,window,first", [
+    (8, 8, 128, 32, [0, 70], [600, 601], 0, 0),              # enough workgroups for the prompts' kernel, all sequences alike
+    (14, 2, 64, 16, [33, 200, 5, 0], [300, 3, 1, 250], 0, 0),  # beside sequences that are not its own
+    (16, 8, 80, 64, [100, 0], [257, 333], 50, 5),
+    (8, 8, 256, 16, [31], [700], 200, 40),
+    (12, 12, 8, 128, [0], [1100], 0, 0),
+    (7, 7, 96, 16, [130, 0], [450, 449], 1, 0),
+])
+def test_prompts(pkg, act, kind, heads, kv, dim, page, lens, rows, window, first):
+    B = pm.Batch(25, lens, rows, kv, dim, page)
+    fill_new(B)
+    run_attention(pkg, B, act, kind, heads, window, first, pad_rows=3, stride=16)
+
+
+@pytest.mark.parametrize("act,kind", TYPES)
+def test_prompts_with_missing_pages_and_odd_values(pkg, act, kind):
+    B = pm.Batch(26, [90, 40], [500, 400], 16, 64, 16)
+    fill_new(B)
+    B.table[0, 3], B.table[0, 20], B.table[1, 0] = -1, B.n_pages + 7, -2 ** 31
+    run_attention(pkg, B, act, kind, 16)
+    run_attention(pkg, B, act, kind, 16, window=100, first=70)
+    for bad, t in ((np.inf, 200), (np.nan, 89), (-np.inf, 10)):
+        B = pm.Batch(27, [90], [600], 16, 64, 16)
+        fill_new(B)
+        p, i = B.slot(0, t)
+        B.v[p, 5, i, 7] = bad
+        q64, q = held(B.rng.standard_normal((600, 16 * 64)), act)
+        cache, k64, v64 = on_gpu(pkg, B, kind)
+        for window, first in ((0, 0), (64, 4)):
+            got = pkg.op_paged_attention(cache, q, dev(B.row_start), 600, 16, 0.125, window=window, first=first).double().cpu().numpy()
+            want = pm.attend(B, q64.reshape(600, 16, 64), k64, v64, 16, 0.125, window, first)[0].reshape(600, -1)
+            ok = np.isfinite(want)
+            assert np.array_equal(np.isfinite(got), ok)
+            assert np.all(np.abs(got[ok] - want[ok]) <= (2 ** -6 if act == "bf16" else 1e-5))
+
+
+def test_a_padded_prompt_that_turns_out_short(pkg):
+    """Buffers and max_rows for 900 rows, of which the device says there are 2, then none"""
+    B = pm.Batch(28, [50], [2], 16, 64, 16)
+    fill_new(B)
+    q = torch.randn(900, 16 * 64, device="cuda")
+    cache, k64, v64 = on_gpu(pkg, B, "bf16")
+    for rows in (2, 0):
+        out = torch.full_like(q, 7.5)
+        pkg.op_paged_attention(cache, q, dev(np.array([0, rows], np.int32)), 900, 16, 0.125, out=out)
+        got = out.double().cpu().numpy()
+        assert np.all(got[rows:] == 7.5)
+        B.total, B.rows = rows, [rows]
+        want = pm.attend(B, q.double().cpu().numpy().reshape(900, 16, 64), k64, v64, 16, 0.125)[0].reshape(rows, 1024)
+        assert np.all(np.abs(got[:rows] - want) <= 1e-5)
+
+
+@pytest.mark.parametrize("act,kind", TYPES)
 @pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (5, 2), (16, 4), (33, 37), (64, 500), (100000, 3), (2 ** 31 - 1, 2 ** 31 - 1)])
 def test_window_and_first_tokens(pkg, act, kind, window, first):
     B = pm.Batch(2, [150, 31, 0, 64, 90], [1, 3, 5, 0, 2], 2, 64, 16)
