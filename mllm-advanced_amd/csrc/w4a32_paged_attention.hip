@@ -142,12 +142,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           const int d = 32 * c + 8 * grp;
-          if (real && d < dim) {
-            load8<Act>(a.q, at + d, x[c]);
-          } else {
+          load8<Act>(a.q, at + (DT == dim || d < dim ? d : 0), x[c]);
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[c][i] = 0.0f;
-          }
+        for (int c = 0; c < kSteps; ++c) {
+          const int d = 32 * c + 8 * grp;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[c][i] = DT == dim || d < dim ? x[c][i] : 0.0f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
         }
@@ -169,22 +170,32 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll
         for (int c = 0; c < kSteps; ++c) {
           const int d = 16 * c + 4 * grp;
-          qf[c] = real && d < dim ? load_global<f32x4>((const float*)a.q + at + d) : f32x4{0, 0, 0, 0};
+          qf[c] = load_global<f32x4>((const float*)a.q + at + (DT == dim || d < dim ? d : 0));
+          if (DT != dim && d >= dim) qf[c] = f32x4{0, 0, 0, 0};
         }
       }
     }
 
     const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
     auto key_of = [&](int t) { return (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT; };
-    // page of a half of a tile (-1: not there)
-    auto page_at = [&](int t, int h) {
-      const int i = (key_of(t) + 16 * h) >> a.c.shift;
-      const int pg = t < t_hi && i < a.c.table_ld ? table[i] : -1;
-      return __builtin_amdgcn_readfirstlane(page_there(a.c, pg) ? pg : -1);
+    // Lane h has the page of half h of a tile (-1: not there). It is asked for a tile ahead of the loads that need it, and in front
+    // of the loads of the tile between: loads return in order, and behind these it would take as long as all of them.
+    int pages = -1;
+    auto find = [&](int t) {
+      const int i = (key_of(t) + 16 * min(lane, kHalves - 1)) >> a.c.shift;
+      pages = t < t_hi && i < a.c.table_ld ? table[i] : -1;
     };
 
     Raw kr[kHalves][kSteps], vr[kVLoads];
     int page[kHalves];
+    auto turn = [&](int t) {  // to the pages of tile t, and asks for those of the next
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const int pg = __builtin_amdgcn_readlane(pages, h);
+        page[h] = page_there(a.c, pg) ? pg : -1;
+      }
+      find(t + streams);
+    };
     auto load_k = [&](int t) {
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
@@ -214,21 +225,20 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     float m = -INFINITY, l = 0.0f;
 
     int t = busy ? t_lo + stream : t_hi;
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) page[h] = page_at(t, h);
+    find(t);
     if (t < t_hi) {
+      turn(t);
       load_k(t);
       load_v(t);
     }
     for (; t < t_hi; t += streams) {
       const int k0 = key_of(t);
       bool there = true;
-      int cur[kHalves], next[kHalves];
+      int cur[kHalves];
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
         cur[h] = page[h];
         there = there && cur[h] >= 0;
-        next[h] = page_at(t + streams, h);
       }
       // every key seen by every row, or each looked at
       const bool whole = there && k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
@@ -276,9 +286,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
           }
         }
       }
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) page[h] = next[h];
       if (t + streams < t_hi) {
+        turn(t + streams);
         load_k(t + streams);
         load_v(t + streams);
       }

@@ -9,7 +9,9 @@
 //   O^T += V^T P^T  B = the softmaxed S^T registers: half h of the wavefront has keys 8 b + 4 h .. + 3 of a block of 32;
 //                   A = V^T: ds_read_b64_tr_b16 of the same keys
 // What bounds it: a tile of 64 keys and 128 dims costs a SIMD 32 x 32 = 1024 clocks of bf16 products per wavefront, and about as
-// many of maxima, exponentials and sums, which run under the other wavefront's products (two per SIMD).
+// many of maxima, exponentials and sums, which run under the other wavefront's products (two per SIMD). So the sums' reference
+// follows a row's maximum only when that has grown by more than 2^kSlack: the 64 products that bring the sums to a new reference
+// are then rare, and weights of up to 2^kSlack are as exact as those up to 1 (f16 has its weights' scale lowered for them).
 // LDS rows: K on 16 bytes more than its dims (a read of 16 rows meets every bank once), V on 64 bytes more (so do the 8 rows of
 // 64 bytes that a transposing read takes).
 // Rows of one kv head lie together, so that a group of heads reads a key once; workgroups of consecutive numbers have
@@ -24,6 +26,7 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kBlock = 1 << kPromptLog2;
 constexpr int kThreads = 256;
+constexpr int kSlack = 8;
 
 __device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -42,6 +45,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
   using M = Math<Act, KV>;
   using Sh = Shape<Act, KV, DT>;
   constexpr int NT = Sh::kTerms, KB = Sh::kKeys, kSub = KB / 32, kSteps = DT / 16, kDims = DT / 32;
+  constexpr int kWeight = M::kScale ? M::kScale - kSlack : 0;  // exponent that weights carry
   constexpr int kPerKey = DT / 8;                      // 16-byte loads of a key
   constexpr int kLoads = KB * kPerKey / kThreads;      // of a thread, for K and for V
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -56,12 +60,45 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
     total = add_sat(total, last_lane(wave_scan(seqs.items)));
   }
   if (blockIdx.x >= total) return;
-  const Place p = place_of(a, seqs, total - 1 - blockIdx.x, kItems, 1);
-  if (!p.there) return;
+  const unsigned group = a.group, kv = a.c.kv_heads;
+  const unsigned order = blockIdx.x / kv;
+  const int hk = (int)(blockIdx.x - order * kv);
+  Place p;
+  int block;
+  if (a.c.n_seqs > 1 && a.c.n_seqs <= 64) {
+    // The blocks of all sequences by the last key that they see, most keys first: the position from which on `order` blocks
+    // or fewer are left is searched for, all sequences counting at once.
+    const Seq& q = seqs.q;
+    auto from = [&](int end) {  // this lane's blocks whose last row stands at `end` or behind
+      if (!q.items || end > q.s.len + q.s.n - 1) return 0u;
+      const long long need = (long long)(end - q.s.len) * a.group + 1;  // pairs up to the first that stands there
+      return (unsigned)(q.items - (need <= 0 ? 0 : (int)((need + kBlock - 1) >> kPromptLog2) - 1));
+    };
+    int lo = 0, hi = a.c.cap + a.max_rows;  // from(lo) counts more than `order`, from(hi) does not
+    while (hi - lo > 1) {
+      const int mid = lo + (hi - lo) / 2;
+      if (last_lane(wave_scan(from(mid))) > order)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const unsigned more = from(hi), mine = from(lo) - more;
+    const unsigned before = last_lane(wave_scan(more)), upto = wave_scan(mine);
+    const u64 found = __ballot(before + upto > order);
+    if (!found) return;
+    const int at = __builtin_ctzll(found);
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+    p.b = at;
+    p.q.s = {of(q.s.r0), of(q.s.n), of(q.s.len)};
+    const unsigned nth = order - before - (unsigned)of((int)(upto - mine));
+    block = of(q.items) - 1 - of((int)more) - (int)nth;
+  } else {
+    p = place_of(a, seqs, (total / kv - 1 - order) * kv + hk, kItems, 1);
+    if (!p.there) return;
+    block = (int)(p.inner / kv);
+  }
   const Span s = p.q.s;
-  const unsigned group = a.group;
-  const int block = (int)(p.inner / (unsigned)a.c.kv_heads), hk = (int)p.inner - block * a.c.kv_heads;
-  const int all_rows = s.n * a.group, of0 = block * kBlock, row0 = of0 + 32 * wave, in_seq = row0 + row;
+  const int all_rows = s.n * (int)group, of0 = block * kBlock, row0 = of0 + 32 * wave, in_seq = row0 + row;
   const bool real = in_seq < all_rows;
   auto slot_of = [&](int r) { return min(s.len + (int)((unsigned)min(r, all_rows - 1) / group), a.c.cap - 1); };
   const int j = (int)((unsigned)min(in_seq, all_rows - 1) / group), head = hk * a.group + (real ? in_seq - j * a.group : 0);
@@ -74,7 +111,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
   auto key_of = [&](int t) { return (t < ft ? t : t - ft + w0) * KB; };
 
   // ---- q ----
-  float row_scale = a.scale;
+  float row_scale = fabsf(a.scale);
   typename M::V8 q[NT][kSteps];
   {
     const size_t at = (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
@@ -82,27 +119,30 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) {
       const int d = 16 * c + 8 * half;
-      if (real && d < dim) {
-        load8<Act>(a.q, at + d, x[c]);
-      } else {
+      load8<Act>(a.q, at + (DT == dim || d < dim ? d : 0), x[c]);
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[c][i] = 0.0f;
-      }
+    for (int c = 0; c < kSteps; ++c) {
+      const int d = 16 * c + 8 * half;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[c][i] = DT == dim || d < dim ? x[c][i] : 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
     }
-    float up = 1.0f;
+    float up = a.scale < 0.0f ? -1.0f : 1.0f;  // the sign is q's, so that a larger product is a larger score
     if constexpr (M::kScale != 0) {
       most = fmaxf(most, __shfl_xor(most, 32));
-      up = M::row_scale(most, row_scale);
+      up *= M::row_scale(most, row_scale);
+    }
+    if (a.scale == 0.0f) {  // all alike: scores of 0, not infinity times 0 where a key is not seen
+      up = 0.0f;
+      row_scale = 1.0f;
     }
 #pragma unroll
     for (int c = 0; c < kSteps; ++c) {
       typename M::V8 t[NT];
-      if constexpr (M::kScale != 0) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[c][i] *= up;
-      }
+      for (int i = 0; i < 8; ++i) x[c][i] *= up;
       M::split(x[c], t);
 #pragma unroll
       for (int k = 0; k < NT; ++k) q[k][c] = t[k];
@@ -114,27 +154,34 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
   u32x4 kr[kLoads], vr[kLoads];
   // A wavefront's 64 loads lie in one page: they are at most 16 keys that begin at a multiple of 8 or less
   auto wave_key = [&](int i) { return (kThreads * i + 64 * wave) / kPerKey; };
-  int page[kLoads];
+  // Lane i has the page of load i. They are asked for a tile ahead of the loads that need them, and in front of the loads of the
+  // tile between: loads return in order, so a page asked for behind these would be waited for as long as all of them.
+  int pages = -1;
   auto find = [&](int t) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int at = (key_of(t) + wave_key(i)) >> a.c.shift;
-      const int pg = t < nt && at < a.c.table_ld ? table[at] : -1;
-      page[i] = __builtin_amdgcn_readfirstlane(page_there(a.c, pg) ? pg : -1);
-    }
+    const int at = (key_of(t) + wave_key(min(lane, kLoads - 1))) >> a.c.shift;
+    pages = t < nt && at < a.c.table_ld ? table[at] : -1;
   };
   int kept_key0 = 0, missing = 0;
+  const unsigned lane_at = lane / kPerKey * dim + lane % kPerKey * 8;  // of a wavefront's 64 loads
+  const bool in = DT == dim || lane % kPerKey * 8 < dim;
   auto load = [&](int t) {
+    int page[kLoads];
     missing = 0;
     kept_key0 = key_of(t);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int key = (kThreads * i + tid) / kPerKey, d = (kThreads * i + tid) % kPerKey * 8;
-      missing |= page[i] < 0 ? 1 << i : 0;
-      const size_t at = slot_row(a.c, max(page[i], 0), hk, kept_key0 + key) * dim + d;
-      const bool in = DT == dim || d < dim;
-      kr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.k + at) : u32x4{0, 0, 0, 0};
-      vr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.v + at) : u32x4{0, 0, 0, 0};
+      page[i] = __builtin_amdgcn_readlane(pages, i);
+      if (!page_there(a.c, page[i])) {
+        missing |= 1 << i;
+        page[i] = 0;
+      }
+    }
+    find(t + 1);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const size_t at = slot_row(a.c, page[i], hk, kept_key0 + __builtin_amdgcn_readfirstlane(wave_key(i))) * dim;
+      kr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.k + at + lane_at) : u32x4{0, 0, 0, 0};
+      vr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.v + at + lane_at) : u32x4{0, 0, 0, 0};
     }
   };
   // Whether all of the workgroup's rows see all keys from k0 on
@@ -174,12 +221,10 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
 
   find(0);
   load(0);
-  find(1);
   put(0);
   __syncthreads();
   for (int t = 0; t < nt; ++t) {
     if (t + 1 < nt) load(t + 1);
-    find(t + 2);
     const uint16_t* ks = (const uint16_t*)lds + (t & 1) * Sh::kBuffer;
     const uint16_t* vs = ks + KB * Sh::kKS;
     const int k0 = key_of(t);
@@ -228,32 +273,28 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
           }
         }
       }
-      // ---- softmax: with c the scale of the row (times log2 e), 2^(c s - c m) ----
+      // ---- softmax: with c the scale of the row (times log2 e) and r its reference, 2^(c s - r) ----
       float mx = -INFINITY;
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sc[u][i] *= row_scale;
-          mx = fmaxf(mx, sc[u][i]);
-        }
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float m_new = fmaxf(m, mx), base = m_new == -INFINITY ? 0.0f : m_new;
-      if (__any(m_new > m)) {
-        const float down = pow2(m - base);
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[u][i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32)) * row_scale;
+      if (__any(mx > m + (float)kSlack)) {
+        const float m_new = fmaxf(m, mx), down = m == -INFINITY ? 0.0f : pow2(m - m_new);
+        m = m_new;
         l *= down;
 #pragma unroll
         for (int d = 0; d < kDims; ++d) o[d] *= down;
       }
-      m = m_new;
-      const float off = (float)M::kScale - base;
+      const float off = m == -INFINITY ? 0.0f : (float)kWeight - m;  // nothing seen yet: 2^-infinity is 0
       const bool apart = !whole && (flags & 1);
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
         float pr[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          pr[i] = pow2(sc[u][i] + off);
+          pr[i] = pow2(__fmaf_rn(sc[u][i], row_scale, off));
           l += pr[i];
         }
         if (__builtin_expect(apart, 0)) {
