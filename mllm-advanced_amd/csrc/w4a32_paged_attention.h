@@ -176,6 +176,9 @@ __device__ __forceinline__ float group_sum(float x) {
 __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- element types ---------------------------------------------------------------------------------------------------------
+// Values that are not finite must reach only rows that see their key, and 0 times one would reach all. In a tile that not every
+// row sees whole they are zeros to the product; where there were some, they are added behind the last tile, key by key.
+
 // kTerms operands stand for one f32 operand of the 16-bit matrix instruction. kScale: exponent that the softmaxed scores
 // carry until the sums are divided (they cancel there).
 template <typename Act, typename KV>
@@ -204,8 +207,9 @@ struct Math<Act, __bf16> {
       }
     }
   }
-  static __device__ __forceinline__ bool odd(uint32_t w) {  // an infinity or NaN among two elements
-    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  static constexpr uint32_t kSize = 0x7fff7fffu, kStep = 0x00800080u;  // a largest exponent and kStep give the sign's bit
+  static __device__ __forceinline__ uint32_t finite(uint32_t w) {  // two elements, those that are not finite as 0
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
   }
   static __device__ __forceinline__ float widen(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
 };
@@ -231,8 +235,9 @@ struct Math<Act, _Float16> {
       t[1][i] = (_Float16)(x[i] - (float)t[0][i]);
     }
   }
-  static __device__ __forceinline__ bool odd(uint32_t w) {
-    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+  static constexpr uint32_t kSize = 0x7fff7fffu, kStep = 0x04000400u;
+  static __device__ __forceinline__ uint32_t finite(uint32_t w) {
+    return ((w & 0x7c00u) == 0x7c00u ? 0u : w & 0xffffu) | ((w & 0x7c000000u) == 0x7c000000u ? 0u : w & 0xffff0000u);
   }
   static __device__ __forceinline__ float widen(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
 };
@@ -242,7 +247,9 @@ struct Math<float, float> {
   static constexpr int kTerms = 1;
   static constexpr int kScale = 0;
   static __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ bool odd(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+  static constexpr uint32_t kSize = 0x7fffffffu, kStep = 0x00800000u;
+  static __device__ __forceinline__ uint32_t finite(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u ? 0u : w; }
+  static __device__ __forceinline__ float widen(float x) { return x; }
 };
 
 template <typename Act>

@@ -223,6 +223,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
+    bool odd = false;  // values that are not finite, in a tile that not every row sees whole
 
     int t = busy ? t_lo + stream : t_hi;
     find(t);
@@ -242,26 +243,32 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       }
       // every key seen by every row, or each looked at
       const bool whole = there && k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
-      bool apart = false;  // a value that is not finite, of a key that some rows see and others do not
       if (!whole) {
+        asm volatile("");
+        uint32_t top = 0;  // the signs' places: whether a value is not finite
         constexpr int kPerKey = DT / kE;
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i) {
           const int in = (64 * i + lane) / kPerKey, key = k0 + in;
-          const bool none = (kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0 || key > pos_max ||
-                            (a.window != 0 && key <= pos_min - a.window && key >= a.first);
+          const bool none = ((kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0) | (key > pos_max) |
+                            ((a.window != 0) & (key <= pos_min - a.window) & (key >= a.first));
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            if constexpr (k16) {
-              vr[i][w] = none ? 0u : vr[i][w];
-              apart = apart || M::odd(vr[i][w]);
-            } else {
-              vr[i][w] = none ? 0.0f : vr[i][w];
-              apart = apart || M::odd(__float_as_uint(vr[i][w]));
-            }
+            const uint32_t x = none ? 0u : __builtin_bit_cast(u32x4, vr[i])[w];
+            top |= ((x & M::kSize) + M::kStep) & ~M::kSize;
+            vr[i][w] = __builtin_bit_cast(Raw, u32x4{x, x, x, x})[0];
           }
         }
-        apart = j_min != j_max && __any(apart);
+        if (__any(top != 0)) {
+          odd = true;
+#pragma unroll
+          for (int i = 0; i < kVLoads; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t x = M::finite(__builtin_bit_cast(u32x4, vr[i])[w]);
+              vr[i][w] = __builtin_bit_cast(Raw, u32x4{x, x, x, x})[0];
+            }
+        }
       }
       {
         constexpr int kPerKey = DT / kE;
@@ -293,13 +300,14 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       }
       uint32_t seen = 0xff;  // bit 4 h + i: key 16 h + 4 grp + i
       if (!whole) {
+        asm volatile("");  // a branch: the compiler would rather do this for every tile
         seen = 0;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = k0 + 16 * h + 4 * grp + i;
-            const bool sees = real && cur[h] >= 0 && key <= pos && (a.window == 0 || key > pos - a.window || key < a.first);
+            const bool sees = real & (cur[h] >= 0) & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first));
             seen |= sees ? 1u << (4 * h + i) : 0u;
           }
       }
@@ -335,31 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
           l += pr[4 * h + i];
         }
       // ---- values ----
-      if (__builtin_expect(apart, 0)) {
-        // 0 times a value that is not finite must not reach a row that does not see it: key by key
-#pragma unroll 1
-        for (int n = 0; n < 4 * kHalves; ++n) {
-#pragma unroll 1
-          for (int g = 0; g < 4; ++g) {
-            const float w = __shfl(pr[0], 16 * g + row);
-            const bool mine = __shfl((int)seen, 16 * g + row) >> n & 1;
-            const KV* v = vs + (16 * (n >> 2) + 4 * g + (n & 3)) * kVS + 4 * grp;
-#pragma unroll
-            for (int d = 0; d < DT / 16; ++d)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                float x;
-                if constexpr (k16)
-                  x = M::widen(__builtin_bit_cast(uint16_t, v[16 * d + e]));
-                else
-                  x = v[16 * d + e];
-                o[d][e] += mine ? w * x : 0.0f;
-              }
-          }
-#pragma unroll
-          for (int i = 0; i < 7; ++i) pr[i] = pr[i + 1];
-        }
-      } else if constexpr (k16) {
+      if constexpr (k16) {
         typename M::V8 pt[NT];
         M::split(pr, pt);
         const KV* v = vs + (4 * grp + (row >> 2)) * kVS + 4 * (row & 3);
@@ -380,6 +364,37 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[d] = M::mfma(vs[(4 * grp + i) * kVS + 16 * d + row], pr[i], o[d]);
+      }
+    }
+
+    if (odd) {
+#pragma unroll 1
+      for (t = t_lo + stream; t < t_hi; t += streams) {
+#pragma unroll 1
+        for (int k = 0; k < KT; ++k) {
+          const int k0 = key_of(t), key = k0 + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
+          const bool sees = real & page_there(a.c, pg) & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first));
+          bool whole = k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
+          for (int h = 0; h < kHalves; ++h) {
+            const int i = (k0 + 16 * h) >> a.c.shift;
+            whole = whole && i < a.c.table_ld && page_there(a.c, table[i]);
+          }
+          if (whole || !sees) continue;  // whole: they were in the product as they are
+          const KV* v = (const KV*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
+#pragma unroll
+          for (int d = 0; d < DT / 16; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int x = 16 * d + 4 * grp + e;
+              if constexpr (k16) {
+                const uint32_t bits = x < dim ? ((const uint16_t*)v)[x] : 0u;
+                if (M::finite(bits) != bits) o[d][e] += M::widen((uint16_t)bits);
+              } else {
+                const uint32_t bits = x < dim ? ((const uint32_t*)v)[x] : 0u;
+                if (M::finite(bits) != bits) o[d][e] += __uint_as_float(bits);
+              }
+            }
+        }
       }
     }
 
@@ -555,7 +570,21 @@ inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, int first, bool accumulate, Plan& p) {
   const int kt = c->dtype == W4A32_CACHE_F32 ? 16 : 32;
   const long long group = r->heads / c->kv_heads, cap = (long long)c->table_ld * c->page;
-  const long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
+  long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
+  p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
+  p.prompts = ((long long)r->rows * group / (1 << kPromptLog2) + c->n_seqs) * c->kv_heads;
+  p.prompt_rows = 0;
+  p.others = true;
+  if (p.prompts >= (1ll << 31)) return W4A32_ESHAPE;
+  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && p.prompts >= kPromptBlocks) {
+    // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then. Else the rows'
+    // kernel has what is left, of so few rows.
+    const bool ragged = r->rows < (long long)r->max_rows * c->n_seqs;
+    p.prompt_rows = ragged ? kPromptRows : 1;
+    most = (kPromptRows - 1) / group;
+    p.others = ragged && most > 0;
+    if (!p.others) most = 1;
+  }
   // 32 or 64 rows of an item are two or four wavefronts' that ask for the same keys at about the same time: the caches serve
   // all but the first, where as items of their own each would have the keys from memory again
   p.wide = most * group <= kRows ? 1 : most * group <= 2 * kRows ? 2 : 4;
@@ -569,17 +598,8 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
     tiles = near < tiles ? near : tiles;
   }
   p.tiles = p.items * tiles;
-  p.prompts = (long long)r->rows * group / (1 << kPromptLog2) * c->kv_heads + (long long)c->n_seqs * c->kv_heads;
-  p.prompt_rows = 0;
-  p.others = true;
-  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && p.prompts >= kPromptBlocks) {
-    // where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then
-    p.others = r->rows < (long long)r->max_rows * c->n_seqs;
-    p.prompt_rows = p.others ? kPromptRows : 1;
-  }
   p.grid = p.tiles < kGrid ? p.tiles : kGrid;
   p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
-  p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
   if (p.tiles >= (1ll << 31) || p.items * p.slot_rows * (p.dt / 32) >= (1ll << 31) || p.key_groups >= (1ll << 31)) return W4A32_ESHAPE;
   // Nothing is shared where every item is short and has a workgroup. Where a join of one workgroup per row leaves most CUs
   // without work, a row's values are dealt to several.

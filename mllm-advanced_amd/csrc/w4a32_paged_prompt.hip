@@ -3,7 +3,7 @@
 //
 // A workgroup has 128 query rows of one kv head (pairs of token and head of the group, 32 to a wavefront) and takes the keys that
 // they can see, 64 (32 where an f32 operand is two or three terms, or the head has 256 dims) at a time through LDS: the next
-// tile's loads are in flight in registers while this one is multiplied. Both products are transposed as in the rows' kernel, on
+// tile goes from memory straight to the other half of it (global_load_lds_dwordx4) while this one is multiplied. Both products are transposed as in the rows' kernel, on
 // v_mfma_f32_32x32x16: a lane stands for query row lane % 32, and lanes l and l + 32 share it.
 //   S^T = K Q^T     A = K from LDS: lane = key l % 32, dims 16 c + 8 (l / 32) ..; B = Q in registers
 //   O^T += V^T P^T  B = the softmaxed S^T registers: half h of the wavefront has keys 8 b + 4 h .. + 3 of a block of 32;
@@ -12,8 +12,10 @@
 // many of maxima, exponentials and sums, which run under the other wavefront's products (two per SIMD). So the sums' reference
 // follows a row's maximum only when that has grown by more than 2^kSlack: the 64 products that bring the sums to a new reference
 // are then rare, and weights of up to 2^kSlack are as exact as those up to 1 (f16 has its weights' scale lowered for them).
-// LDS rows: K on 16 bytes more than its dims (a read of 16 rows meets every bank once), V on 64 bytes more (so do the 8 rows of
-// 64 bytes that a transposing read takes).
+// A wavefront's load fills 1024 bytes of LDS in lane order, so rows have no padding between them; instead the 16-byte pieces of a
+// row of K lie exchanged by its number (a read of 16 rows then meets every bank once), and so do the 32-byte pieces of a row of V
+// (the 8 rows of 64 bytes of a transposing read meet every bank twice, which is what they take): each lane asks for the piece that
+// belongs where its 16 bytes go.
 // Rows of one kv head lie together, so that a group of heads reads a key once; workgroups of consecutive numbers have
 // consecutive kv heads, which the dispatcher deals to the XCDs in turn: an L2 sees few heads. Late rows, which see most keys,
 // come first.
@@ -35,10 +37,23 @@ template <typename Act, typename KV, int DT>
 struct Shape {
   static constexpr int kTerms = Math<Act, KV>::kTerms;
   static constexpr int kKeys = kTerms == 1 && DT <= 128 ? 64 : 32;
-  static constexpr int kKS = DT + 8, kVS = DT + 32;  // elements of LDS rows
-  static constexpr int kBuffer = kKeys * (kKS + kVS);
-  static constexpr size_t kLds = (size_t)2 * kBuffer * 2 + 2 * 4 * sizeof(int);
+  static constexpr int kTile = kKeys * DT;            // elements of a tile of K or V
+  static constexpr size_t kLds = (size_t)4 * kTile * 2 + 4 * sizeof(int);
+  // by which the pieces of row r are exchanged: 16 bytes of K, 32 bytes of V
+  static __device__ __forceinline__ int k_turn(int r) { return DT == 64 ? r >> 1 & 7 : r & 15; }
+  static __device__ __forceinline__ int v_turn(int r) { return DT == 64 ? r >> 1 & 3 : r & 7; }
 };
+
+// 16 bytes of every lane, from `base` + `at` (or, second form, from `from`) to LDS from `to` on. The wait for it is the caller's:
+// the compiler does not see these loads, whose arrival it would otherwise wait for at the next read of any LDS. (M0 holds their
+// place in LDS and is the compiler's to set in front of each of its own uses.)
+__device__ __forceinline__ void load_lds(const void* base, unsigned at, unsigned to) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(to) : "memory");
+}
+__device__ __forceinline__ void load_lds(const void* from, unsigned to) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+}
+__device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 template <typename Act, typename KV, int DT>
 __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Attend a) {
@@ -49,7 +64,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
   constexpr int kPerKey = DT / 8;                      // 16-byte loads of a key
   constexpr int kLoads = KB * kPerKey / kThreads;      // of a thread, for K and for V
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int* odd_flags = (int*)(lds + (size_t)2 * Sh::kBuffer * 2);
+  int* odd_flags = (int*)(lds + (size_t)4 * Sh::kTile * 2);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 31, half = lane >> 5, dim = a.c.dim;
 
   // ---- which rows ----
@@ -151,65 +166,90 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
 
   // ---- tiles ----
   const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
-  u32x4 kr[kLoads], vr[kLoads];
-  // A wavefront's 64 loads lie in one page: they are at most 16 keys that begin at a multiple of 8 or less
-  auto wave_key = [&](int i) { return (kThreads * i + 64 * wave) / kPerKey; };
-  // Lane i has the page of load i. They are asked for a tile ahead of the loads that need them, and in front of the loads of the
-  // tile between: loads return in order, so a page asked for behind these would be waited for as long as all of them.
+  // Lane b has the page of the tile's b-th 16 keys. They are asked for a tile ahead of the loads that need them, and in front of
+  // the loads of the tile between: loads return in order, so a page asked for behind these would be waited for as long as all.
+  constexpr int kBlocks = KB / 16;
   int pages = -1;
   auto find = [&](int t) {
-    const int at = (key_of(t) + wave_key(min(lane, kLoads - 1))) >> a.c.shift;
+    const int at = (key_of(t) + 16 * min(lane, kBlocks - 1)) >> a.c.shift;
     pages = t < nt && at < a.c.table_ld ? table[at] : -1;
   };
-  int kept_key0 = 0, missing = 0;
-  const unsigned lane_at = lane / kPerKey * dim + lane % kPerKey * 8;  // of a wavefront's 64 loads
-  const bool in = DT == dim || lane % kPerKey * 8 < dim;
-  auto load = [&](int t) {
-    int page[kLoads];
-    missing = 0;
-    kept_key0 = key_of(t);
+  // Where this lane's 16 bytes of a wavefront's load come from, in a row of the load
+  const int lane_row = lane / kPerKey, piece = lane % kPerKey, wave_row = 64 * wave / kPerKey;
+  unsigned k_at[2], v_at;  // the turn of K's rows in a load of odd number differs where a load has 8 rows
+  bool k_in[2], v_in;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      page[i] = __builtin_amdgcn_readlane(pages, i);
-      if (!page_there(a.c, page[i])) {
-        missing |= 1 << i;
-        page[i] = 0;
+  for (int x = 0; x < 2; ++x) {
+    const int r = x * kThreads / kPerKey + wave_row + lane_row, from = piece ^ Sh::k_turn(r);
+    k_in[x] = 8 * from < dim;
+    k_at[x] = (unsigned)(lane_row * dim + 8 * from) * 2;
+  }
+  {
+    const int from = ((piece >> 1) ^ Sh::v_turn(wave_row + lane_row)) << 1 | (piece & 1);
+    v_in = 8 * from < dim;
+    v_at = (unsigned)(lane_row * dim + 8 * from) * 2;
+  }
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+  // Tile t to buffer t & 1; returns the sixteens of keys whose page is not there.
+  auto load = [&](int t) {
+    int page[kBlocks], gone = 0;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      page[b] = __builtin_amdgcn_readlane(pages, b);
+      if (!page_there(a.c, page[b])) {
+        gone |= 1 << b;
+        page[b] = 0;
       }
     }
     find(t + 1);
+    const unsigned to = lds0 + (t & 1) * (4 * Sh::kTile) + __builtin_amdgcn_readfirstlane(wave) * 1024;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const size_t at = slot_row(a.c, page[i], hk, kept_key0 + __builtin_amdgcn_readfirstlane(wave_key(i))) * dim;
-      kr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.k + at + lane_at) : u32x4{0, 0, 0, 0};
-      vr[i] = in ? load_global<u32x4>((const uint16_t*)a.c.v + at + lane_at) : u32x4{0, 0, 0, 0};
+      const int r = i * kThreads / kPerKey + __builtin_amdgcn_readfirstlane(wave_row);
+      int pg = page[0];
+#pragma unroll
+      for (int b = 1; b < kBlocks; ++b) pg = r / 16 == b ? page[b] : pg;
+      const size_t at = slot_row(a.c, pg, hk, key_of(t) + r) * dim;
+      const uint16_t *k = (const uint16_t*)a.c.k + at, *v = (const uint16_t*)a.c.v + at;
+      if (DT == dim) {
+        load_lds(k, k_at[i & 1], to + 4096 * i);
+        load_lds(v, v_at, to + 4096 * i + 2 * Sh::kTile);
+      } else {  // zeros past the head's size
+        load_lds(k_in[i & 1] ? (const uint8_t*)k + k_at[i & 1] : (const uint8_t*)&kZeros, to + 4096 * i);
+        load_lds(v_in ? (const uint8_t*)v + v_at : (const uint8_t*)&kZeros, to + 4096 * i + 2 * Sh::kTile);
+      }
     }
+    return gone;
   };
-  // Whether all of the workgroup's rows see all keys from k0 on
+  // Whether rows that stand from lo to hi all see all keys from k0 on
   auto all_seen = [&](int k0, int lo, int hi) {
     return k0 + KB - 1 <= lo && (a.window == 0 || k0 > hi - a.window || k0 + KB - 1 < a.first);
   };
-  auto put = [&](int buffer) {
-    uint16_t* ks = (uint16_t*)lds + buffer * Sh::kBuffer;
-    uint16_t* vs = ks + KB * Sh::kKS;
+  // The tile has arrived, for all wavefronts. Where not all rows see all of it: zeros for what no row sees, and for values that
+  // are not finite; whether there were any of those is noted.
+  if (tid < 4) odd_flags[tid] = 0;
+  auto arrive = [&](int t, int gone) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    const int k0 = key_of(t);
+    if (gone == 0 && all_seen(k0, block_min, block_max)) return;
+    u32x4* vs = (u32x4*)((uint16_t*)lds + (t & 1) * (2 * Sh::kTile) + Sh::kTile);
     bool odd = false;
-    const bool look = missing || !all_seen(kept_key0, block_min, block_max);
+#pragma unroll 1
+    for (int i = tid; i < KB * kPerKey; i += kThreads) {
+      const int key = i / kPerKey, at = k0 + key;
+      const bool none = (gone >> key / 16 & 1) | (at > block_max) | ((a.window != 0) & (at <= block_min - a.window) & (at >= a.first));
+      u32x4 x = vs[i];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int key = (kThreads * i + tid) / kPerKey, d = (kThreads * i + tid) % kPerKey * 8, at = kept_key0 + key;
-      if (look) {  // what no row sees must not meet a weight of 0 as an infinity or NaN
-        const bool none = missing >> i & 1 || at > block_max || (a.window != 0 && at <= block_min - a.window && at >= a.first);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          vr[i][w] = none ? 0u : vr[i][w];
-          odd = odd || M::odd(vr[i][w]);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t y = none ? 0u : M::finite(x[e]);
+        odd = odd | (!none & (y != x[e]));
+        x[e] = y;
       }
-      *(u32x4*)(ks + key * Sh::kKS + d) = kr[i];
-      *(u32x4*)(vs + key * Sh::kVS + d) = vr[i];
+      vs[i] = x;
     }
-    // bit 0: values that are not finite; bits 1 ..: loads of this wavefront whose page is not there
-    const int any = __any(odd) ? 1 : 0;
-    if (lane == 0) odd_flags[4 * buffer + wave] = any | missing << 1;
+    if (__any(odd) && lane == 0) odd_flags[wave] = 1;
+    __syncthreads();
   };
 
   f32x16 o[kDims];
@@ -220,58 +260,50 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
   float m = -INFINITY, l = 0.0f;
 
   find(0);
-  load(0);
-  put(0);
-  __syncthreads();
+  int gone = load(0);
+  arrive(0, gone);
   for (int t = 0; t < nt; ++t) {
-    if (t + 1 < nt) load(t + 1);
-    const uint16_t* ks = (const uint16_t*)lds + (t & 1) * Sh::kBuffer;
-    const uint16_t* vs = ks + KB * Sh::kKS;
+    const int next_gone = t + 1 < nt ? load(t + 1) : 0;
+    const uint16_t* ks = (const uint16_t*)lds + (t & 1) * (2 * Sh::kTile);
+    const uint16_t* vs = ks + Sh::kTile;
     const int k0 = key_of(t);
-    int flags = 0, gone = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int f = odd_flags[4 * (t & 1) + w];
-      flags |= f;
-      gone |= f >> 1;
-    }
-    flags = __builtin_amdgcn_readfirstlane(flags);
-    gone = __builtin_amdgcn_readfirstlane(gone);
     const bool whole = gone == 0 && all_seen(k0, pos_min, pos_max);
     const bool none = row0 >= all_rows || k0 > pos_max;  // of this wavefront
     if (!none) {
       // ---- scores ----
+      const int k_turn = 8 * Sh::k_turn(row);  // of rows 32 u + row
       f32x16 sc[kSub];
 #pragma unroll
-      for (int u = 0; u < kSub; ++u) {
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[u][i] = 0.0f;
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          const typename M::V8 kf = *(const typename M::V8*)(ks + (32 * u + row) * Sh::kKS + 16 * c + 8 * half);
+      for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+          const typename M::V8 kf = *(const typename M::V8*)(ks + (32 * u + row) * DT + (8 * (2 * c + half) ^ k_turn));
 #pragma unroll
           for (int k = NT - 1; k >= 0; --k) sc[u] = mfma32(kf, q[k][c], sc[u]);
         }
+      // four reads ahead of the products
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < kSteps * kSub - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
-      uint32_t seen[kSub];  // bit i: key 32 u + 8 (i / 4) + 4 half + i % 4
-#pragma unroll
-      for (int u = 0; u < kSub; ++u) seen[u] = 0xffff;
+      __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 0);
       if (!whole) {
+        int first_key = k0 + 4 * half;
+        asm volatile("" : "+v"(first_key));  // here, not in front of the loop in a register for each key
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
-          seen[u] = 0;
+        for (int u = 0; u < kSub; ++u)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int in = 32 * u + 8 * (i / 4) + 4 * half + i % 4, key = k0 + in;
-            bool sees = real && key <= pos && (a.window == 0 || key > pos - a.window || key < a.first);
-            if (gone) {
-              const int at = key >> a.c.shift;
-              sees = sees && at < a.c.table_ld && page_there(a.c, table[at < a.c.table_ld ? at : 0]);
-            }
-            seen[u] |= sees ? 1u << i : 0u;
+            const int key = first_key + 32 * u + 8 * (i / 4) + i % 4;
+            const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !(gone >> (2 * u + i / 8) & 1);
             sc[u][i] = sees ? sc[u][i] : -INFINITY;
           }
-        }
       }
       // ---- softmax: with c the scale of the row (times log2 e) and r its reference, 2^(c s - r) ----
       float mx = -INFINITY;
@@ -288,67 +320,76 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
         for (int d = 0; d < kDims; ++d) o[d] *= down;
       }
       const float off = m == -INFINITY ? 0.0f : (float)kWeight - m;  // nothing seen yet: 2^-infinity is 0
-      const bool apart = !whole && (flags & 1);
+      float pr[kSub][16];
 #pragma unroll
-      for (int u = 0; u < kSub; ++u) {
-        float pr[16];
+      for (int u = 0; u < kSub; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          pr[i] = pow2(__fmaf_rn(sc[u][i], row_scale, off));
-          l += pr[i];
-        }
-        if (__builtin_expect(apart, 0)) {
-          // 0 times a value that is not finite must not reach a row that does not see it: key by key
-#pragma unroll 1
-          for (int n = 0; n < 16; ++n) {
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h) {
-              const float w = __shfl(pr[0], 32 * h + row);
-              const bool mine = __shfl((int)seen[u], 32 * h + row) >> n & 1;
-              const uint16_t* v = vs + (32 * u + 8 * (n >> 2) + 4 * h + (n & 3)) * Sh::kVS + 4 * half;
-#pragma unroll
-              for (int d = 0; d < kDims; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                  const float x = M::widen(v[32 * d + 8 * (i / 4) + i % 4]);
-                  o[d][i] += mine ? w * x : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 15; ++i) pr[i] = pr[i + 1];
-          }
-          continue;
+          pr[u][i] = pow2(__fmaf_rn(sc[u][i], row_scale, off));
+          l += pr[u][i];
         }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {  // 16 keys
-          float p8[8];
+      for (int c = 0; c < 2 * kSub; ++c) {  // 16 keys
+        float p8[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) p8[i] = pr[8 * c + i];
-          typename M::V8 pt[NT];
-          M::split(p8, pt);
-          const uint16_t* v = vs + (32 * u + 16 * c + 4 * half + ((lane & 15) >> 2)) * Sh::kVS + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        for (int i = 0; i < 8; ++i) p8[i] = pr[c / 2][8 * (c % 2) + i];
+        typename M::V8 pt[NT];
+        M::split(p8, pt);
+        const int r0 = 4 * half + ((lane & 15) >> 2);  // of rows 16 c + 8 x + r0
 #pragma unroll
-          for (int d = 0; d < kDims; ++d) {
-            union {
-              s4 part[2];
-              typename M::V8 v8;
-            } vt;
+        for (int d = 0; d < kDims; ++d) {
+          union {
+            s4 part[2];
+            typename M::V8 v8;
+          } vt;
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              vt.part[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(v + 8 * x * Sh::kVS + 32 * d));
+          for (int x = 0; x < 2; ++x)
+            vt.part[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(
+                vs + (16 * c + 8 * x + r0) * DT + ((2 * d + (lane >> 4 & 1)) ^ Sh::v_turn(8 * x + r0)) * 16 + 4 * (lane & 3)));
 #pragma unroll
-            for (int k = NT - 1; k >= 0; --k) o[d] = mfma32(vt.v8, pt[k], o[d]);
-          }
+          for (int k = NT - 1; k >= 0; --k) o[d] = mfma32(vt.v8, pt[k], o[d]);
         }
       }
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+#pragma unroll
+      for (int i = 0; i < 2 * kSub * kDims - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NT, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 1);
     }
-    if (t + 1 < nt) put((t + 1) & 1);
-    __syncthreads();
+    if (t + 1 < nt) arrive(t + 1, next_gone);
+    gone = next_gone;
   }
 
   // ---- results: lane = row, four dims at a time ----
   l += __shfl_xor(l, 32);
   if (!real) return;
+  if (odd_flags[0] | odd_flags[1] | odd_flags[2] | odd_flags[3]) {  // behind a barrier at the last tile's arrival
+#pragma unroll 1
+    for (int t = 0; t < nt; ++t) {
+#pragma unroll 1
+      for (int k = 0; k < KB; ++k) {
+        const int key = key_of(t) + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
+        if (!page_there(a.c, pg) || key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
+        bool all_there = true;  // then its values were in the product as they are
+        for (int b = 0; b < kBlocks; ++b) {
+          const int i = (key_of(t) + 16 * b) >> a.c.shift;
+          all_there = all_there && i < a.c.table_ld && page_there(a.c, table[i]);
+        }
+        if (all_there && all_seen(key_of(t), block_min, block_max)) continue;
+        const uint16_t* v = (const uint16_t*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int x = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
+            const uint32_t bits = x < dim ? v[x] : 0u;
+            if (M::finite(bits) != bits) o[d][i] += M::widen((uint16_t)bits);
+          }
+      }
+    }
+  }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const size_t at = (size_t)(s.r0 + j) * a.ldo + (size_t)head * dim;
 #pragma unroll
