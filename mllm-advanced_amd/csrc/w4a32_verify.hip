@@ -5,9 +5,9 @@
 // sequence and, where one was refused, adds up max(p - q, 0) over the segments of its row; the third finds the segment and
 // then the index that the given number falls on.
 //
-// Exponentials and sums are f64: an f64 instruction runs at the rate of an f32 one here, an exponential takes about 16 of
-// them, and with two logits per 8 bytes read the launch stays bound by memory. In f32 the sums' rounding would decide which
-// token a number falls on whenever it lies within 1e-7 of a border, as one of 150000 tokens' borders often does.
+// Exponentials and sums are f64: an f64 sum or product takes as long as an f32 one here, an exponential 16 of them, and so the
+// first launch stays near what memory gives. In f32 the sums' rounding would decide which token a number falls on whenever it
+// lies within 1e-7 of a border, as one of 150000 tokens' borders often does.
 #include "w4a32_internal.h"
 #include "w4a32_decoder.h"
 
@@ -17,6 +17,7 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 
 constexpr int kSegment = 4096;  // logits of a segment: 16 of each thread, all requested at once
 constexpr int kEach = kSegment / 256;
+constexpr int kTestWaves = 8;   // wavefronts of the second launch: rows of a sequence that are tested at once
 
 struct Part {
   double sum;
@@ -24,9 +25,9 @@ struct Part {
   int at;  // greedy: index of the maximum
 };
 struct Found {  // what the second launch leaves for the third
-  double zp, zq;
+  double rp, rq;  // one over the sums of the row's exponentials, target and draft
   float mp, mq;
-  int count, refused;
+  int count, refused, row;
 };
 struct Verify {
   const float *logits, *draft;
@@ -62,6 +63,30 @@ __device__ __forceinline__ double exp_neg(double x) {
   return __builtin_amdgcn_ldexp(y, (int)k);
 }
 
+// The same for sums alone, 7e-12 relative: k from the low bits of a sum that has no bits behind the point, 2^f by the Taylor
+// polynomial of degree 9 on |f| <= 1/2, and k added to the exponent. At least 2^-1000 where x is less (-infinity, NaN).
+__device__ __forceinline__ double exp_sum(float l, double c, double offset) {
+  constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
+  const double y = fmax(__builtin_fma((double)l, c, offset), -1000.0);
+  const double t = y + kMagic, f = y - (t - kMagic);
+  constexpr double L = 0.69314718055994530942;
+  constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6, c7 = c6 * L / 7,
+                   c8 = c7 * L / 8, c9 = c8 * L / 9;
+  double p = c9;
+  p = __builtin_fma(p, f, c8);
+  p = __builtin_fma(p, f, c7);
+  p = __builtin_fma(p, f, c6);
+  p = __builtin_fma(p, f, c5);
+  p = __builtin_fma(p, f, c4);
+  p = __builtin_fma(p, f, c3);
+  p = __builtin_fma(p, f, c2);
+  p = __builtin_fma(p, f, c1);
+  p = __builtin_fma(p, f, 1.0);
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, p);
+  const unsigned k = (unsigned)__builtin_bit_cast(unsigned long long, t);
+  return __builtin_bit_cast(double, (bits & 0xffffffffull) | (unsigned long long)((unsigned)(bits >> 32) + (k << 20)) << 32);
+}
+
 struct Rows {
   int r0, n;
 };
@@ -72,16 +97,42 @@ __device__ __forceinline__ Rows rows_of(const Verify& a, int b) {
   return s;
 }
 
-template <typename T>
-__device__ __forceinline__ T wave_add(T x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+// Sums, maxima and minima over a wavefront by moves within the register file; scan: up to this lane.
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ double moved(double x) {  // 0 where no lane is
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, kCtrl, kRowMask, 0xf, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), kCtrl, kRowMask, 0xf, false);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan(double x) {
+  x += moved<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);  // row_bcast 15, 31
+  x += moved<0x143, 0xc>(x);
   return x;
 }
+__device__ __forceinline__ double of_lane(double x, int lane) {
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), lane);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_add(double x) { return of_lane(wave_scan(x), 63); }
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ float most(float x) {
+  const int y = __builtin_amdgcn_update_dpp((int)0xff800000, __float_as_int(x), kCtrl, kRowMask, 0xf, false);  // -infinity where no lane is
+  return fmaxf(x, __int_as_float(y));
+}
 __device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
+  x = most<0x111, 0xf>(x);
+  x = most<0x112, 0xf>(x);
+  x = most<0x114, 0xf>(x);
+  x = most<0x118, 0xf>(x);
+  x = most<0x142, 0xa>(x);
+  x = most<0x143, 0xc>(x);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
 // blockIdx: segment, row, target or draft
@@ -100,17 +151,30 @@ __global__ __launch_bounds__(256) void stats_kernel(Verify a) {
   const float* x = of_draft ? a.draft + (size_t)r * a.ldd : a.logits + (size_t)r * a.ldl;
   const int base = seg * kSegment;
   float v[kEach];
+  // four values of a thread together, 1024 apart
+  if (((uintptr_t)x & 15) == 0 && base + kSegment <= a.vocab) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int at = base + i * 256 + (int)threadIdx.x;
-    v[i] = at < a.vocab ? load_global<float>(x + at) : -INFINITY;
+    for (int i = 0; i < kEach; i += 4) {
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      const f4 w = load_global<f4>(x + base + i * 256 + 4 * (int)threadIdx.x);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[i + e] = w[e];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int at = base + (i & ~3) * 256 + 4 * (int)threadIdx.x + (i & 3);
+      v[i] = at < a.vocab ? load_global<float>(x + at) : -INFINITY;
+    }
   }
   float top = -INFINITY;
   int where = 0x7fffffff;
+  bool nan = false;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
-    if (kGreedy && v[i] > top) where = base + i * 256 + (int)threadIdx.x;
+    if (kGreedy && v[i] > top) where = base + (i & ~3) * 256 + 4 * (int)threadIdx.x + (i & 3);
     top = fmaxf(top, v[i]);
+    nan |= v[i] != v[i];
   }
   const float mine = top;
   top = wave_max(top);
@@ -135,10 +199,12 @@ __global__ __launch_bounds__(256) void stats_kernel(Verify a) {
     return;
   }
   double sum = 0.0;
-  const double m = all == -INFINITY ? 0.0 : (double)all;
+  const double c = a.inv_t * 1.4426950408889634074;
+  const double offset = all == -INFINITY ? 0.0 : -(double)all * c;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sum += exp_neg(((double)v[i] - m) * a.inv_t);
-  sum = wave_add(sum);
+  for (int i = 0; i < kEach; ++i) sum += exp_sum(v[i], c, offset);
+  if (nan || all == INFINITY) sum = (double)NAN;  // no distribution
+  sum = all == -INFINITY ? 0.0 : wave_add(sum);
   if (lane == 0) sums[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -147,89 +213,105 @@ __global__ __launch_bounds__(256) void stats_kernel(Verify a) {
   }
 }
 
-// A row's maximum and sum from its segments', by one wavefront
-__device__ __forceinline__ void combine(const Verify& a, const Part* parts, float& m, double& z) {
+// The maximum and sum of a row, or of two at once, from their segments', by one wavefront
+template <int kRows>
+__device__ __forceinline__ void combine(const Verify& a, const Part* const (&parts)[kRows], float (&m)[kRows], double (&z)[kRows]) {
   const int lane = threadIdx.x & 63;
-  m = -INFINITY;
-  for (int i = lane; i < a.segs; i += 64) m = fmaxf(m, parts[i].top);
-  m = wave_max(m);
-  const double base = m == -INFINITY ? 0.0 : (double)m;
-  z = 0.0;
-  for (int i = lane; i < a.segs; i += 64) z += parts[i].sum * exp_neg(((double)parts[i].top - base) * a.inv_t);
-  z = wave_add(z);
+  Part mine[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    mine[r] = lane < a.segs ? parts[r][lane] : Part{0.0, -INFINITY, 0};
+    m[r] = mine[r].top;
+  }
+  for (int i = lane + 64; i < a.segs; i += 64)
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) m[r] = fmaxf(m[r], parts[r][i].top);
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    m[r] = wave_max(m[r]);
+    const double base = m[r] == -INFINITY ? 0.0 : (double)m[r];
+    z[r] = mine[r].sum * exp_neg(((double)mine[r].top - base) * a.inv_t);
+    for (int i = lane + 64; i < a.segs; i += 64) z[r] += parts[r][i].sum * exp_neg(((double)parts[r][i].top - base) * a.inv_t);
+    z[r] = wave_add(z[r]);
+  }
 }
 
-// What is left for the next token at index i of the row that refused
-__device__ __forceinline__ double left_at(const Verify& a, const Found& f, const float* p, const float* q, int64_t token, int i) {
-  const double x = exp_neg(((double)p[i] - (double)f.mp) * a.inv_t) / f.zp;
-  if (!q) return i == token ? 0.0 : x;
-  const double y = x - exp_neg(((double)q[i] - (double)f.mq) * a.inv_t) / f.zq;
+// What is left for the next token at an index with these logits, in the row that refused
+__device__ __forceinline__ double left_of(const Verify& a, const Found& f, float p, float q, bool draft, bool drafted) {
+  const double x = exp_neg(((double)p - (double)f.mp) * a.inv_t) * f.rp;
+  if (!draft) return drafted ? 0.0 : x;
+  const double y = x - exp_neg(((double)q - (double)f.mq) * a.inv_t) * f.rq;
   return y < 0.0 ? 0.0 : y;
 }
 
-// blockIdx: segment, sequence. Every workgroup tests its sequence's tokens by itself.
-__global__ __launch_bounds__(256) void test_kernel(Verify a) {
-  __shared__ Found f;
-  __shared__ double sums[4];
-  __shared__ int refused[4];
+// blockIdx: segment, sequence. Every workgroup tests its sequence's tokens by itself, a row of each wavefront at a time.
+__global__ __launch_bounds__(64 * kTestWaves) void test_kernel(Verify a) {
+  __shared__ Found found[kTestWaves];
+  __shared__ double sums[kTestWaves];
+  __shared__ int stops[kTestWaves];
   const int seg = blockIdx.x % a.segs, b = blockIdx.x / a.segs, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Rows s = rows_of(a, b);
   if (s.n == 0) {
-    if (seg == 0 && threadIdx.x == 0) a.found[b] = Found{0.0, 0.0, 0.0f, 0.0f, 0, 0};
+    if (seg == 0 && threadIdx.x == 0) a.found[b] = Found{0.0, 0.0, 0.0f, 0.0f, 0, 0, 0};
     return;
   }
-  int stop = s.n - 1;  // tokens accepted
-  for (int j0 = 0; j0 < s.n - 1; j0 += 4) {
-    bool bad = false;
-    const int r = s.r0 + j0 + wave;
-    if (j0 + wave < s.n - 1) {
-      float mp, mq = 0.0f;
-      double zp, zq = 1.0, qt = 1.0;
-      combine(a, a.p + (size_t)r * a.segs, mp, zp);
-      const int64_t t = a.tokens[r + 1];
-      const bool in = t >= 0 && t < a.vocab;
-      if (a.draft && in) {
-        combine(a, a.q + (size_t)r * a.segs, mq, zq);
-        qt = exp_neg(((double)a.draft[(size_t)r * a.ldd + t] - (double)mq) * a.inv_t) / zq;
-      }
-      const double pt = in ? exp_neg(((double)a.logits[(size_t)r * a.ldl + t] - (double)mp) * a.inv_t) / zp : 0.0;
-      bad = !((double)a.uniform[r] * qt < pt);
+  int at = 0;  // the wavefront that had the first row behind which it ends
+  for (int j0 = 0; j0 < s.n; j0 += kTestWaves) {
+    const int j = j0 + wave, r = s.r0 + j;
+    int stop = 0;
+    if (j < s.n) {
+      const bool judges = j < s.n - 1;  // the last row has no token behind it
+      const int64_t t = judges ? a.tokens[r + 1] : 0;
+      const float u = judges ? a.uniform[r] : 0.0f;
+      const bool known = t >= 0 && t < a.vocab, both = judges && a.draft;
+      const Part* const parts[2] = {a.p + (size_t)r * a.segs, (both ? a.q : a.p) + (size_t)r * a.segs};
+      const float lt = a.logits[(size_t)r * a.ldl + (known ? t : 0)], dt = both ? a.draft[(size_t)r * a.ldd + (known ? t : 0)] : 0.0f;
+      float m[2];
+      double z[2];
+      combine(a, parts, m, z);
+      const double rp = 1.0 / z[0], rq = 1.0 / z[1];
+      const double pt = exp_neg(((double)lt - (double)m[0]) * a.inv_t) * rp;
+      const double qt = both ? exp_neg(((double)dt - (double)m[1]) * a.inv_t) * rq : 1.0;
+      stop = !(judges && known && (double)u * qt < pt);
+      if (lane == 0) found[wave] = Found{rp, both ? rq : 1.0, m[0], both ? m[1] : 0.0f, j + 1, judges, r};
     }
-    if (lane == 0) refused[wave] = bad;
+    if (lane == 0) stops[wave] = stop;
     __syncthreads();
-    int first = 4;
+    at = kTestWaves;
 #pragma unroll
-    for (int w = 3; w >= 0; --w) first = refused[w] ? w : first;
+    for (int w = kTestWaves - 1; w >= 0; --w) at = stops[w] ? w : at;
+    if (at < kTestWaves) break;  // the last row stops at the latest
     __syncthreads();
-    if (first < 4) {
-      stop = j0 + first;
-      break;
-    }
   }
-  const int r = s.r0 + stop;
-  const bool no = stop < s.n - 1;
-  if (wave == 0) {
-    float m, mq = 0.0f;
-    double z, zq = 1.0;
-    combine(a, a.p + (size_t)r * a.segs, m, z);
-    if (no && a.draft) combine(a, a.q + (size_t)r * a.segs, mq, zq);
-    if (lane == 0) f = Found{z, zq, m, mq, stop + 1, no};
-  }
-  __syncthreads();
+  const Found f = found[at];
   if (seg == 0 && threadIdx.x == 0) a.found[b] = f;
-  if (!no) return;  // p itself: its segments' sums are there
-  const float *p = a.logits + (size_t)r * a.ldl, *q = a.draft ? a.draft + (size_t)r * a.ldd : nullptr;
-  const int64_t token = a.tokens[r + 1];
+  if (!f.refused) return;  // p itself: its segments' sums are there
+  const float *p = a.logits + (size_t)f.row * a.ldl, *q = a.draft ? a.draft + (size_t)f.row * a.ldd : nullptr;
+  const int64_t token = a.tokens[f.row + 1];
+  constexpr int kMine = kSegment / (64 * kTestWaves);
+  const int base = seg * kSegment + (int)threadIdx.x;
+  float x[kMine], y[kMine];
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int k = min(base + i * 64 * kTestWaves, a.vocab - 1);
+    x[i] = load_global<float>(p + k);
+    y[i] = q ? load_global<float>(q + k) : 0.0f;
+  }
   double sum = 0.0;
-#pragma unroll 4
-  for (int i = 0; i < kEach; ++i) {
-    const int at = seg * kSegment + i * 256 + (int)threadIdx.x;
-    if (at < a.vocab) sum += left_at(a, f, p, q, token, at);
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int k = base + i * 64 * kTestWaves;
+    if (k < a.vocab) sum += left_of(a, f, x[i], y[i], q != nullptr, k == token);
   }
   sum = wave_add(sum);
   if (lane == 0) sums[wave] = sum;
   __syncthreads();
-  if (threadIdx.x == 0) a.left[(size_t)b * a.segs + seg] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  if (threadIdx.x == 0) {
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < kTestWaves; ++w) sum += sums[w];
+    a.left[(size_t)b * a.segs + seg] = sum;
+  }
 }
 
 // A workgroup per sequence
@@ -237,43 +319,58 @@ __global__ __launch_bounds__(256) void choose_kernel(Verify a) {
   __shared__ double in_wave[4], before, target;
   __shared__ int seg, last[4], hit[4];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Rows s = rows_of(a, b);
-  if (s.n == 0) {
+  Found f = a.found[b];
+  const float choice = a.choice[b];
+  if (f.count == 0) {  // no rows
     if (threadIdx.x == 0) {
       a.count[b] = 0;
       a.next[b] = -1;
     }
     return;
   }
-  Found f = a.found[b];
-  const int r = s.r0 + f.count - 1;
+  const int r = f.row;
   const Part* parts = a.p + (size_t)r * a.segs;
   auto sum_of = [&](int i) {
     return f.refused ? a.left[(size_t)b * a.segs + i]
-                     : parts[i].sum * exp_neg(((double)parts[i].top - (f.mp == -INFINITY ? 0.0 : (double)f.mp)) * a.inv_t) / f.zp;
+                     : parts[i].sum * exp_neg(((double)parts[i].top - (f.mp == -INFINITY ? 0.0 : (double)f.mp)) * a.inv_t) * f.rp;
   };
-  if (threadIdx.x == 0) {
-    double total = 0.0;
-    for (int i = 0; i < a.segs; ++i) total += sum_of(i);
+  if (wave == 0) {
+    double mine = lane < a.segs ? sum_of(lane) : 0.0;  // of the first 64 segments
+    auto whole = [&]() {
+      double sum = mine;
+      for (int i = lane + 64; i < a.segs; i += 64) sum += sum_of(i);
+      return wave_add(sum);
+    };
+    double total = whole();
     if (f.refused && total == 0.0) {  // p and q are the same: nothing is left over but p
       f.refused = 0;
-      for (int i = 0; i < a.segs; ++i) total += sum_of(i);
+      mine = lane < a.segs ? sum_of(lane) : 0.0;
+      total = whole();
     }
-    seg = -1;
-    if (total > 0.0 && total < INFINITY) {
-      target = (double)a.choice[b] * total;
+    int at = -1;
+    double in_front = 0.0;
+    const double mark = (double)choice * total;
+    if (total > 0.0 && total < (double)INFINITY) {
       double up = 0.0;
-      for (int i = 0; i < a.segs; ++i) {
-        const double x = sum_of(i);
-        if (x > 0.0) {
-          seg = i;
-          before = up;
+      for (int i0 = 0; i0 < a.segs; i0 += 64) {
+        const double x = i0 == 0 ? mine : i0 + lane < a.segs ? sum_of(i0 + lane) : 0.0, upto = up + wave_scan(x);
+        // the first whose sum passes the mark, and until there is one the last that has a share
+        const unsigned long long past = __ballot(upto > mark && x > 0.0), some = __ballot(x > 0.0);
+        if (some) {
+          const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+          at = i0 + l;
+          in_front = of_lane(upto - x, l);
         }
-        up += x;
-        if (up > target) break;
+        if (past) break;
+        up = of_lane(upto, 63);
       }
     }
-    last[0] = f.refused;
+    if (lane == 0) {
+      seg = at;
+      before = in_front;
+      target = mark;
+      last[0] = f.refused;
+    }
   }
   __syncthreads();
   f.refused = last[0];
@@ -283,20 +380,22 @@ __global__ __launch_bounds__(256) void choose_kernel(Verify a) {
     const float *p = a.logits + (size_t)r * a.ldl, *q = a.draft && f.refused ? a.draft + (size_t)r * a.ldd : nullptr;
     const int64_t not_this = f.refused ? a.tokens[r + 1] : -1;
     const int base = seg * kSegment + (int)threadIdx.x * kEach;
+    float lp[kEach], lq[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int k = min(base + i, a.vocab - 1);
+      lp[i] = load_global<float>(p + k);
+      lq[i] = q ? load_global<float>(q + k) : 0.0f;
+    }
     double x[kEach], sum = 0.0;
     int positive = -1;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      x[i] = base + i < a.vocab ? left_at(a, f, p, q, not_this, base + i) : 0.0;
+      x[i] = base + i < a.vocab ? left_of(a, f, lp[i], lq[i], q != nullptr, base + i == not_this) : 0.0;
       sum += x[i];
       if (x[i] > 0.0) positive = base + i;
     }
-    double upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(upto, o);
-      if (lane >= o) upto += y;
-    }
+    const double upto = wave_scan(sum);
     if (lane == 63) in_wave[wave] = upto;
     __syncthreads();
     double up = before + (upto - sum);
@@ -412,7 +511,7 @@ int w4a32_op_verify_drafts(const w4a32_verify_args* v, void* d_scratch, size_t s
   } else {
     hipLaunchKernelGGL((stats_kernel<false>), stats, dim3(256), 0, s, a);
     if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
-    hipLaunchKernelGGL(test_kernel, dim3((unsigned)(v->n_seqs * (long long)l.segs)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(test_kernel, dim3((unsigned)(v->n_seqs * (long long)l.segs)), dim3(64 * kTestWaves), 0, s, a);
     if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
     hipLaunchKernelGGL(choose_kernel, dim3((unsigned)v->n_seqs), dim3(256), 0, s, a);
   }
