@@ -151,8 +151,11 @@ __global__ __launch_bounds__(256) void append_kernel(Append a, int blocks_per_ro
 }
 
 // ---------------------------------------------------------------------------------------------
-// Eviction. One workgroup per (sequence, kv head) finds the weight of the last token that stays, eight bits of its
-// order-preserving key at a time (a histogram in LDS each), and lists the slots that stay in order; a second launch copies.
+// Eviction. One workgroup per (sequence, kv head) finds the weight of the last token that stays, 12, 10 and 10 bits of its
+// order-preserving key at a time (a histogram in LDS each: 12 first, so that weights of similar size, which have few exponents,
+// do not all count in the same place), and lists the slots that stay in order; a second launch copies. Up to kHeld keys lie in
+// LDS; beyond them every pass has the weights from memory. The selection is all latency, the copy all memory. (The first and the
+// last tokens copied by other workgroups of the first launch took as much longer there as the second took less.)
 // ---------------------------------------------------------------------------------------------
 struct Evict {
   Cache c, to;
@@ -172,9 +175,50 @@ __device__ __forceinline__ float weight_at(const Cache& c, int b, int head, int 
   return page_there(c, page) ? c.weight[slot_row(c, page, head, t)] : 0.0f;
 }
 
+// Threads copy 16 bytes of a token's key and of its value each: token t of a sequence's head to slot i.
+__device__ __forceinline__ void copy_token(const Evict& a, int b, int head, int t, int i, int units, int u) {
+  const int from = a.c.table[(size_t)b * a.c.table_ld + (t >> a.c.shift)];
+  const int dst = a.to.table[(size_t)b * a.to.table_ld + (i >> a.to.shift)];
+  if (!page_there(a.to, dst)) return;
+  const bool there = page_there(a.c, from);
+  const size_t src = slot_row(a.c, there ? from : 0, head, t), out = slot_row(a.to, dst, head, i);
+  const u32x4 zero = {0, 0, 0, 0};
+  const u32x4 k = load_global<u32x4>((const u32x4*)a.c.k + src * units + u), v = load_global<u32x4>((const u32x4*)a.c.v + src * units + u);
+  *(W4_GLOBAL u32x4*)((u32x4*)a.to.k + out * units + u) = there ? k : zero;
+  *(W4_GLOBAL u32x4*)((u32x4*)a.to.v + out * units + u) = there ? v : zero;
+  if (u == 0) a.to.weight[out] = there ? a.c.weight[src] : 0.0f;
+}
+constexpr int kCopies = 4;  // tokens of a thread
+
 constexpr int kSelect = 1024;
+constexpr int kHeld = 32 * 1024;
+
+// Sums of all threads up to this one, and of all
+__device__ __forceinline__ unsigned block_scan(unsigned x, unsigned* in_wave, unsigned& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned upto = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned y = __shfl_up(upto, o);
+    if (lane >= o) upto += y;
+  }
+  __syncthreads();  // in_wave may still be read
+  if (lane == 63) in_wave[wave] = upto;
+  __syncthreads();
+  unsigned before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSelect / 64; ++w) {
+    before += w < wave ? in_wave[w] : 0;
+    total += in_wave[w];
+  }
+  return before + upto;
+}
+
+template <bool kInLds>
 __global__ __launch_bounds__(kSelect) void select_kernel(Evict a) {
-  __shared__ unsigned hist[256], in_wave[2][kSelect / 64], state[2];
+  extern __shared__ __attribute__((aligned(16))) unsigned keys[];
+  __shared__ unsigned hist[4096], in_wave[kSelect / 64], state[2];
   const int b = blockIdx.x / a.c.kv_heads, head = blockIdx.x % a.c.kv_heads, tid = threadIdx.x;
   const int n = min(max(a.c.len[b], 0), a.c.cap), stay = min(n, a.budget);
   int* kept = a.kept + (size_t)blockIdx.x * a.budget;
@@ -185,103 +229,85 @@ __global__ __launch_bounds__(kSelect) void select_kernel(Evict a) {
     return;
   }
   const int lo = a.first, hi = n - a.recent;
-  unsigned want = a.budget - a.first - a.recent, prefix = 0;  // of those in [lo, hi), of which there are more
-  uint32_t mask = 0;
-  if (want) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+  unsigned want = a.budget - a.first - a.recent;  // of those in [lo, hi), of which there are more
+  uint32_t prefix = 0;
+  auto key_at = [&](int t) { return kInLds ? keys[t] : key_of(weight_at(a.c, b, head, t)); };
+  const bool any = want != 0;
+  if (any) {
+    if (kInLds) {
+#pragma unroll 8
+      for (int t = lo + tid; t < hi; t += kSelect) keys[t] = key_of(weight_at(a.c, b, head, t));
+    }
+    int shift = 20;
+    uint32_t mask = 0;
+    for (int bits = 12;; bits = 10, shift -= 10) {
+      const int each = (1 << bits) / kSelect;  // digits of a thread: 4, then 1
+      for (int i = 0; i < each; ++i) hist[tid * each + i] = 0;
       __syncthreads();
       for (int t = lo + tid; t < hi; t += kSelect) {
-        const uint32_t k = key_of(weight_at(a.c, b, head, t));
-        if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & 255], 1u);
+        const uint32_t k = key_at(t);
+        if ((k & mask) == prefix) atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
       }
       __syncthreads();
-      if (tid < 64) {  // lane l: digits 255 - 4 l down to 252 - 4 l
-        unsigned sum = 0, h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum += h[i] = hist[255 - 4 * tid - i];
-        unsigned upto = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const unsigned y = __shfl_up(upto, o);
-          if (tid >= o) upto += y;
-        }
-        unsigned above = upto - sum;
-        if (above < want && upto >= want) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (above < want && above + h[i] >= want) {
-              state[0] = 255 - 4 * tid - i;
-              state[1] = want - above;
-            }
-            above += h[i];
+      // thread i: the i-th `each` digits from the largest on
+      const int top = (1 << bits) - 1 - tid * each;
+      unsigned sum = 0, all;
+      for (int i = 0; i < each; ++i) sum += hist[top - i];
+      const unsigned upto = block_scan(sum, in_wave, all);
+      unsigned above = upto - sum;
+      if (above < want && upto >= want) {
+        for (int i = 0; i < each; ++i) {
+          const unsigned h = hist[top - i];
+          if (above < want && above + h >= want) {
+            state[0] = top - i;
+            state[1] = want - above;
           }
+          above += h;
         }
       }
       __syncthreads();
       prefix |= state[0] << shift;
       want = state[1];
-      mask |= 255u << shift;
-      __syncthreads();
+      mask |= ((1u << bits) - 1) << shift;
+      if (shift == 0) break;
     }
   }
-  // those above the key stay, and of those that have it the first `want`
-  const bool any = a.budget > a.first + a.recent;
-  unsigned at = 0, equal = 0;
-  const int lane = tid & 63, wave = tid >> 6;
-  for (int t0 = 0; t0 < n; t0 += kSelect) {
-    const int t = t0 + tid;
-    bool sure = t < n && (t < lo || t >= hi), tie = false;
-    if (any && t >= lo && t < hi) {
-      const uint32_t k = key_of(weight_at(a.c, b, head, t));
-      sure = k > prefix;
-      tie = k == prefix;
-    }
-    const unsigned long long ties = __ballot(tie);
-    if (lane == 0) in_wave[0][wave] = __popcll(ties);
-    __syncthreads();
-    unsigned rank = equal + __popcll(ties & ((1ull << lane) - 1));
-    for (int w = 0; w < kSelect / 64; ++w) {
-      rank += w < wave ? in_wave[0][w] : 0;
-      equal += in_wave[0][w];
-    }
-    const bool stays = sure || (tie && rank < want);
-    const unsigned long long all = __ballot(stays);
-    if (lane == 0) in_wave[1][wave] = __popcll(all);
-    __syncthreads();
-    unsigned to = at + __popcll(all & ((1ull << lane) - 1));
-    for (int w = 0; w < kSelect / 64; ++w) {
-      to += w < wave ? in_wave[1][w] : 0;
-      at += in_wave[1][w];
-    }
-    if (stays && to < (unsigned)a.budget) kept[to] = t;
-    __syncthreads();
+  // Those above the key stay, and of those that have it the first `want`. A thread has tokens in a row.
+  const int per = ((n + kSelect - 1) / kSelect) | 1;  // odd: the threads' keys lie in different banks
+  const int t0 = min(tid * per, n), t1 = min(t0 + per, n);
+  unsigned ties = 0, sure = 0, all;
+  for (int t = t0; t < t1; ++t) {
+    const bool inner = any && t >= lo && t < hi;
+    const uint32_t k = inner ? key_at(t) : 0;
+    ties += inner && k == prefix;
+    sure += t < lo || t >= hi || (inner && k > prefix);
+  }
+  unsigned rank = block_scan(ties, in_wave, all) - ties;
+  const unsigned stays = sure + min(ties, want - min(want, rank));
+  unsigned to = block_scan(stays, in_wave, all) - stays;
+  for (int t = t0; t < t1; ++t) {
+    const bool inner = any && t >= lo && t < hi;
+    const uint32_t k = inner ? key_at(t) : 0;
+    const bool tie = inner && k == prefix;
+    if (t < lo || t >= hi || (inner && k > prefix) || (tie && rank < want)) kept[to++] = t;
+    rank += tie;
   }
 }
 
-// A thread copies 16 bytes of a token's key and of its value.
-constexpr int kCopies = 4;
 __global__ __launch_bounds__(256) void copy_kernel(Evict a, int units, int blocks_per_head) {
   const int bh = blockIdx.x / blocks_per_head, b = bh / a.c.kv_heads, head = bh % a.c.kv_heads;
   const int per = 256 / units, u = threadIdx.x % units;
   if ((int)threadIdx.x >= per * units) return;
   const int first = (blockIdx.x % blocks_per_head) * per * kCopies + threadIdx.x / units;
+  int t[kCopies];
 #pragma unroll
   for (int x = 0; x < kCopies; ++x) {
     const int i = first + x * per;
-    const int t = i < a.budget ? a.kept[(size_t)bh * a.budget + i] : -1;
-    if (t < 0) continue;
-    const int from = a.c.table[(size_t)b * a.c.table_ld + (t >> a.c.shift)];
-    const int dst = a.to.table[(size_t)b * a.to.table_ld + (i >> a.to.shift)];
-    if (!page_there(a.to, dst)) continue;
-    const bool there = page_there(a.c, from);
-    const size_t src = slot_row(a.c, there ? from : 0, head, t), out = slot_row(a.to, dst, head, i);
-    const u32x4 zero = {0, 0, 0, 0};
-    u32x4 k = load_global<u32x4>((const u32x4*)a.c.k + src * units + u), v = load_global<u32x4>((const u32x4*)a.c.v + src * units + u);
-    *(W4_GLOBAL u32x4*)((u32x4*)a.to.k + out * units + u) = there ? k : zero;
-    *(W4_GLOBAL u32x4*)((u32x4*)a.to.v + out * units + u) = there ? v : zero;
-    if (u == 0) a.to.weight[out] = there ? a.c.weight[src] : 0.0f;
+    t[x] = i < a.budget ? a.kept[(size_t)bh * a.budget + i] : -1;
   }
+#pragma unroll
+  for (int x = 0; x < kCopies; ++x)
+    if (t[x] >= 0) copy_token(a, b, head, t[x], first + x * per, units, u);
 }
 
 }  // namespace paged
@@ -337,12 +363,20 @@ int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache
   if (!d_kept && (!d_scratch || !aligned(d_scratch, 16) || scratch_bytes < need)) return W4A32_EINVAL;
   const Evict a{view(cache), view(to), budget, first, recent, d_kept ? d_kept : static_cast<int*>(d_scratch), to->d_len};
   const long long heads = (long long)cache->n_seqs * cache->kv_heads;
-  const int units = cache->dim * (cache->dtype == W4A32_CACHE_F32 ? 4 : 2) / 16, per = 256 / units * kCopies;
-  const long long blocks = (budget + per - 1) / per;
+  const int units = cache->dim * (cache->dtype == W4A32_CACHE_F32 ? 4 : 2) / 16, per = kCopies * (256 / units);
+  const long long blocks = ((long long)budget + per - 1) / per;
   if (heads * blocks >= (1ll << 31)) return W4A32_ESHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(select_kernel, dim3((unsigned)heads), dim3(kSelect), 0, s, a);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return W4A32_ELAUNCH;
+  // the table says how long a sequence can be
+  const size_t held = (size_t)cache->table_ld * cache->page;
+  if (held <= kHeld) {
+    static w4::LdsLimitOnce limit;
+    if (limit.raise((const void*)select_kernel<true>, kHeld * sizeof(unsigned)) != hipSuccess) return W4A32_ELAUNCH;
+    hipLaunchKernelGGL((select_kernel<true>), dim3((unsigned)heads), dim3(kSelect), held * sizeof(unsigned), s, a);
+  } else {
+    hipLaunchKernelGGL((select_kernel<false>), dim3((unsigned)heads), dim3(kSelect), 0, s, a);
+  }
+  if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   hipLaunchKernelGGL(copy_kernel, dim3((unsigned)(heads * blocks)), dim3(256), 0, s, a, units, (int)blocks);
   return from_hip(hipGetLastError());
 }

@@ -387,6 +387,12 @@ def test_evict(pkg, kind, kv, dim, page, lens, budget, first, recent):
     check_evict(pkg, pm.Batch(14, lens, [0] * len(lens), kv, dim, page, weights=True), kind, budget, first, recent)
 
 
+def test_evict_from_a_table_for_very_long_sequences(pkg):
+    """More slots than the selection holds in LDS"""
+    B = pm.Batch(29, [3000, 700], [0, 0], 1, 8, 64, weights=True, table_ld=600)
+    check_evict(pkg, B, "bf16", 900, 5, 100)
+
+
 def test_evict_equal_weights_and_odd_ones(pkg):
     B = pm.Batch(15, [500, 400, 300, 2500], [0] * 4, 1, 64, 16, weights=True)
     pick = np.array([0.0, -0.0, 1.0, 1.0, 2.0, -3.0, np.inf, -np.inf, 1e-40, np.nan])
