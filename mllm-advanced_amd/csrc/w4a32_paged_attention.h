@@ -10,8 +10,6 @@ namespace paged {
 
 constexpr int kRows = 16;         // query rows of a wavefront
 constexpr int kWaves = 4;         // wavefronts of a workgroup
-constexpr int kPromptLog2 = 7;    // log2 of the query rows of a workgroup of the prompts' kernel
-
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
@@ -31,6 +29,7 @@ struct Attend {
   int ldq, ldo, rows, max_rows, heads, group;
   int window, first;
   int prompt_rows;      // (token, head of the group) pairs from which on a sequence is the prompts' kernel's; 0: none is
+  int prompt_log2;      // log2 of the rows of a workgroup of that kernel: 7, or 5 where there are few
   int wide;             // log2 of the wavefronts with rows of their own (1, 2 or 4): an item has 16 << wide rows
   int slot_rows;        // rows of an item that can be there: what a slot of scratch memory holds
   unsigned most_items, most_tiles;  // what the scratch memory holds: row starts that overlap could ask for more, and get nothing
@@ -51,7 +50,7 @@ struct Seq {
   int items;       // per kv head
 };
 
-// kPrompt: the sequences of the prompts' kernel, in items of 1 << kPromptLog2 rows; else the others
+// kPrompt: the sequences of the prompts' kernel, in items of 1 << prompt_log2 rows; else the others
 template <int KT, bool kPrompt>
 __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   Seq q;
@@ -59,7 +58,7 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   const long long pairs = (long long)q.s.n * a.group;
   if ((a.prompt_rows && pairs >= a.prompt_rows) != kPrompt) q.s.n = 0;
   q.keys = min(q.s.len + q.s.n, a.c.cap);
-  const int log2 = kPrompt ? kPromptLog2 : 4 + a.wide;
+  const int log2 = kPrompt ? a.prompt_log2 : 4 + a.wide;
   q.items = q.s.n ? (int)((pairs + (1 << log2) - 1) >> log2) : 0;
   q.w0 = 0;
   q.ft = 0;

@@ -29,8 +29,10 @@ inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_EL
 constexpr int kGrid = 512;        // workgroups that a batch is dealt to: two per CU, all there at once
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
 constexpr int kAlone = 8;         // tiles of an item that is not shared, where there are workgroups enough for all items
-constexpr int kPromptRows = 64;   // pairs of token and head from which on a sequence is the prompts' kernel's
-constexpr int kPromptBlocks = 128;  // ... where that has so many workgroups
+// The prompts' kernel takes sequences of at least kPromptRows pairs of token and head, where it has kPromptLeast workgroups or
+// more: it does not share a row's keys between workgroups, and few of them on a long context would leave the chip idle.
+constexpr int kPromptRows = 256, kPromptLeast = 128;
+constexpr int kPromptBlocks = 256;  // workgroups of 128 rows that are worth while; fewer are taken as four times as many of 32
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
 
 template <int KT>
@@ -559,7 +561,7 @@ struct Plan {
   long long items, tiles, grid, key_groups;
   int dt, wide, slot_rows;
   bool join, sliced, others;  // others: rows that are not the prompts' kernel's
-  int prompt_rows;
+  int prompt_rows, prompt_log2;
   long long prompts;          // its workgroups
   size_t item_off, part_off, state_off, lse_off, dump_off, total;
 };
@@ -572,11 +574,13 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   const long long group = r->heads / c->kv_heads, cap = (long long)c->table_ld * c->page;
   long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
   p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
-  p.prompts = ((long long)r->rows * group / (1 << kPromptLog2) + c->n_seqs) * c->kv_heads;
+  auto blocks = [&](int log2) { return ((long long)r->rows * group / (1 << log2) + c->n_seqs) * c->kv_heads; };
+  p.prompt_log2 = blocks(7) >= kPromptBlocks ? 7 : 5;
+  p.prompts = blocks(p.prompt_log2);
   p.prompt_rows = 0;
   p.others = true;
   if (p.prompts >= (1ll << 31)) return W4A32_ESHAPE;
-  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && p.prompts >= kPromptBlocks) {
+  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && p.prompts >= kPromptLeast) {
     // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then. Else the rows'
     // kernel has what is left, of so few rows.
     const bool ragged = r->rows < (long long)r->max_rows * c->n_seqs;
@@ -678,7 +682,7 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows, rows->max_rows, rows->heads,
-                 rows->heads / cache->kv_heads, window, first, p.prompt_rows, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
+                 rows->heads / cache->kv_heads, window, first, p.prompt_rows, p.prompt_log2, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
                  (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
   hipStream_t s = static_cast<hipStream_t>(stream);

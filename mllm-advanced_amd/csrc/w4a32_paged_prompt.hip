@@ -19,6 +19,8 @@
 // Rows of one kv head lie together, so that a group of heads reads a key once; workgroups of consecutive numbers have
 // consecutive kv heads, which the dispatcher deals to the XCDs in turn: an L2 sees few heads. Late rows, which see most keys,
 // come first.
+// Where there are few such workgroups, one has 32 rows instead, and each of its four wavefronts (two where the head has 256 dims)
+// takes every fourth tile by itself, with no barrier; their softmax states are joined through LDS at the end.
 #include "w4a32_paged_attention.h"
 
 namespace w4 {
@@ -26,19 +28,25 @@ namespace paged {
 
 namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-constexpr int kBlock = 1 << kPromptLog2;
 constexpr int kThreads = 256;
 constexpr int kSlack = 8;
 
 __device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
-template <typename Act, typename KV, int DT>
+// A team of kMembers wavefronts shares tiles and has 32 rows of each; with kSplit a workgroup has several teams, of one wavefront
+// each, on the same rows.
+template <typename Act, typename KV, int DT, bool kSplit>
 struct Shape {
   static constexpr int kTerms = Math<Act, KV>::kTerms;
-  static constexpr int kKeys = kTerms == 1 && DT <= 128 ? 64 : 32;
-  static constexpr int kTile = kKeys * DT;            // elements of a tile of K or V
-  static constexpr size_t kLds = (size_t)4 * kTile * 2 + 4 * sizeof(int);
+  static constexpr int kMembers = kSplit ? 1 : 4, kTeams = !kSplit ? 1 : DT == 256 ? 2 : 4;
+  static constexpr int kKeys = !kSplit && kTerms == 1 && DT <= 128 ? 64 : 32;
+  static constexpr int kTile = kKeys * DT;                // elements of a tile of K or V
+  static constexpr size_t kTeam = (size_t)4 * kTile * 2;  // bytes of a team's tiles: K and V, twice
+  static constexpr int kSums = DT + 4;                    // floats of a row of sums, where teams are joined
+  static constexpr int kStates = kSplit ? kTeams * 32 * 2 : 0;
+  static constexpr size_t kLds = kTeams * kTeam + 4 * sizeof(int) + kStates * sizeof(float);
+  static_assert(!kSplit || (size_t)32 * kSums * 4 <= kTeam, "a team's sums lie where its tiles were");
   // by which the pieces of row r are exchanged: 16 bytes of K, 32 bytes of V
   static __device__ __forceinline__ int k_turn(int r) { return DT == 64 ? r >> 1 & 7 : r & 15; }
   static __device__ __forceinline__ int v_turn(int r) { return DT == 64 ? r >> 1 & 3 : r & 7; }
@@ -55,17 +63,19 @@ __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
 }
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
-template <typename Act, typename KV, int DT>
-__global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Attend a) {
+template <typename Act, typename KV, int DT, bool kSplit>
+__global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_kernel(Attend a) {
   using M = Math<Act, KV>;
-  using Sh = Shape<Act, KV, DT>;
+  using Sh = Shape<Act, KV, DT, kSplit>;
+  constexpr int kTeams = Sh::kTeams, kTeamThreads = 64 * Sh::kMembers, kBlock = 32 * Sh::kMembers;
   constexpr int NT = Sh::kTerms, KB = Sh::kKeys, kSub = KB / 32, kSteps = DT / 16, kDims = DT / 32;
   constexpr int kWeight = M::kScale ? M::kScale - kSlack : 0;  // exponent that weights carry
   constexpr int kPerKey = DT / 8;                      // 16-byte loads of a key
-  constexpr int kLoads = KB * kPerKey / kThreads;      // of a thread, for K and for V
+  constexpr int kLoads = KB * kPerKey / kTeamThreads;  // of a thread, for K and for V
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int* odd_flags = (int*)(lds + (size_t)4 * Sh::kTile * 2);
+  int* odd_flags = (int*)(lds + kTeams * Sh::kTeam);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 31, half = lane >> 5, dim = a.c.dim;
+  const int team = wave / Sh::kMembers, member = wave % Sh::kMembers, team_tid = member * 64 + lane;
 
   // ---- which rows ----
   Seqs<KB, true> seqs;
@@ -87,7 +97,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
     auto from = [&](int end) {  // this lane's blocks whose last row stands at `end` or behind
       if (!q.items || end > q.s.len + q.s.n - 1) return 0u;
       const long long need = (long long)(end - q.s.len) * a.group + 1;  // pairs up to the first that stands there
-      return (unsigned)(q.items - (need <= 0 ? 0 : (int)((need + kBlock - 1) >> kPromptLog2) - 1));
+      return (unsigned)(q.items - (need <= 0 ? 0 : (int)((need + kBlock - 1) / kBlock) - 1));
     };
     int lo = 0, hi = a.c.cap + a.max_rows;  // from(lo) counts more than `order`, from(hi) does not
     while (hi - lo > 1) {
@@ -113,7 +123,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
     block = (int)(p.inner / kv);
   }
   const Span s = p.q.s;
-  const int all_rows = s.n * (int)group, of0 = block * kBlock, row0 = of0 + 32 * wave, in_seq = row0 + row;
+  const int all_rows = s.n * (int)group, of0 = block * kBlock, row0 = of0 + 32 * member, in_seq = row0 + row;
   const bool real = in_seq < all_rows;
   auto slot_of = [&](int r) { return min(s.len + (int)((unsigned)min(r, all_rows - 1) / group), a.c.cap - 1); };
   const int j = (int)((unsigned)min(in_seq, all_rows - 1) / group), head = hk * a.group + (real ? in_seq - j * a.group : 0);
@@ -175,23 +185,24 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
     pages = t < nt && at < a.c.table_ld ? table[at] : -1;
   };
   // Where this lane's 16 bytes of a wavefront's load come from, in a row of the load
-  const int lane_row = lane / kPerKey, piece = lane % kPerKey, wave_row = 64 * wave / kPerKey;
-  unsigned k_at[2], v_at;  // the turn of K's rows in a load of odd number differs where a load has 8 rows
-  bool k_in[2], v_in;
+  const int lane_row = lane / kPerKey, piece = lane % kPerKey, wave_row = 64 * member / kPerKey;
+  // The turn of a row differs from load to load where a load of the team has fewer rows than the turns repeat after
+  constexpr int kRowsAtOnce = kTeamThreads / kPerKey, kKinds = kRowsAtOnce < 16 ? 16 / kRowsAtOnce : 1;
+  unsigned k_at[kKinds], v_at[kKinds];
+  bool k_in[kKinds], v_in[kKinds];
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int r = x * kThreads / kPerKey + wave_row + lane_row, from = piece ^ Sh::k_turn(r);
+  for (int x = 0; x < kKinds; ++x) {
+    const int r = x * kTeamThreads / kPerKey + wave_row + lane_row, from = piece ^ Sh::k_turn(r);
     k_in[x] = 8 * from < dim;
     k_at[x] = (unsigned)(lane_row * dim + 8 * from) * 2;
+    const int v_from = ((piece >> 1) ^ Sh::v_turn(r)) << 1 | (piece & 1);
+    v_in[x] = 8 * v_from < dim;
+    v_at[x] = (unsigned)(lane_row * dim + 8 * v_from) * 2;
   }
-  {
-    const int from = ((piece >> 1) ^ Sh::v_turn(wave_row + lane_row)) << 1 | (piece & 1);
-    v_in = 8 * from < dim;
-    v_at = (unsigned)(lane_row * dim + 8 * from) * 2;
-  }
-  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-  // Tile t to buffer t & 1; returns the sixteens of keys whose page is not there.
-  auto load = [&](int t) {
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + __builtin_amdgcn_readfirstlane(team) * (unsigned)Sh::kTeam;
+  uint16_t* tiles = (uint16_t*)(lds + team * Sh::kTeam);
+  // The team's n-th tile, t, to its buffer n & 1; returns the sixteens of keys whose page is not there.
+  auto load = [&](int t, int n) {
     int page[kBlocks], gone = 0;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
@@ -201,22 +212,23 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
         page[b] = 0;
       }
     }
-    find(t + 1);
-    const unsigned to = lds0 + (t & 1) * (4 * Sh::kTile) + __builtin_amdgcn_readfirstlane(wave) * 1024;
+    find(t + kTeams);
+    const unsigned to = lds0 + (n & 1) * (4 * Sh::kTile) + __builtin_amdgcn_readfirstlane(member) * 1024;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = i * kThreads / kPerKey + __builtin_amdgcn_readfirstlane(wave_row);
+      const int r = i * kTeamThreads / kPerKey + __builtin_amdgcn_readfirstlane(wave_row);
       int pg = page[0];
 #pragma unroll
       for (int b = 1; b < kBlocks; ++b) pg = r / 16 == b ? page[b] : pg;
       const size_t at = slot_row(a.c, pg, hk, key_of(t) + r) * dim;
       const uint16_t *k = (const uint16_t*)a.c.k + at, *v = (const uint16_t*)a.c.v + at;
+      constexpr int kStep = 1024 * Sh::kMembers;
       if (DT == dim) {
-        load_lds(k, k_at[i & 1], to + 4096 * i);
-        load_lds(v, v_at, to + 4096 * i + 2 * Sh::kTile);
+        load_lds(k, k_at[i % kKinds], to + kStep * i);
+        load_lds(v, v_at[i % kKinds], to + kStep * i + 2 * Sh::kTile);
       } else {  // zeros past the head's size
-        load_lds(k_in[i & 1] ? (const uint8_t*)k + k_at[i & 1] : (const uint8_t*)&kZeros, to + 4096 * i);
-        load_lds(v_in ? (const uint8_t*)v + v_at : (const uint8_t*)&kZeros, to + 4096 * i + 2 * Sh::kTile);
+        load_lds(k_in[i % kKinds] ? (const uint8_t*)k + k_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i);
+        load_lds(v_in[i % kKinds] ? (const uint8_t*)v + v_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i + 2 * Sh::kTile);
       }
     }
     return gone;
@@ -227,16 +239,22 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
   };
   // The tile has arrived, for all wavefronts. Where not all rows see all of it: zeros for what no row sees, and for values that
   // are not finite; whether there were any of those is noted.
-  if (tid < 4) odd_flags[tid] = 0;
-  auto arrive = [&](int t, int gone) {
+  if (lane == 0) odd_flags[wave] = 0;
+  auto team_sync = [&]() {  // a team of one wavefront runs in step with itself
+    if constexpr (kSplit)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else
+      __syncthreads();
+  };
+  auto arrive = [&](int t, int n, int gone) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+    team_sync();
     const int k0 = key_of(t);
     if (gone == 0 && all_seen(k0, block_min, block_max)) return;
-    u32x4* vs = (u32x4*)((uint16_t*)lds + (t & 1) * (2 * Sh::kTile) + Sh::kTile);
+    u32x4* vs = (u32x4*)(tiles + (n & 1) * (2 * Sh::kTile) + Sh::kTile);
     bool odd = false;
 #pragma unroll 1
-    for (int i = tid; i < KB * kPerKey; i += kThreads) {
+    for (int i = team_tid; i < KB * kPerKey; i += kTeamThreads) {
       const int key = i / kPerKey, at = k0 + key;
       const bool none = (gone >> key / 16 & 1) | (at > block_max) | ((a.window != 0) & (at <= block_min - a.window) & (at >= a.first));
       u32x4 x = vs[i];
@@ -249,7 +267,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
       vs[i] = x;
     }
     if (__any(odd) && lane == 0) odd_flags[wave] = 1;
-    __syncthreads();
+    team_sync();
   };
 
   f32x16 o[kDims];
@@ -259,12 +277,15 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  find(0);
-  int gone = load(0);
-  arrive(0, gone);
-  for (int t = 0; t < nt; ++t) {
-    const int next_gone = t + 1 < nt ? load(t + 1) : 0;
-    const uint16_t* ks = (const uint16_t*)lds + (t & 1) * (2 * Sh::kTile);
+  int t = __builtin_amdgcn_readfirstlane(team), n = 0, gone = 0;
+  find(t);
+  if (t < nt) {
+    gone = load(t, 0);
+    arrive(t, 0, gone);
+  }
+  for (; t < nt; t += kTeams, ++n) {
+    const int next_gone = t + kTeams < nt ? load(t + kTeams, n + 1) : 0;
+    const uint16_t* ks = tiles + (n & 1) * (2 * Sh::kTile);
     const uint16_t* vs = ks + Sh::kTile;
     const int k0 = key_of(t);
     const bool whole = gone == 0 && all_seen(k0, pos_min, pos_max);
@@ -358,20 +379,19 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
       }
       __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 1);
     }
-    if (t + 1 < nt) arrive(t + 1, next_gone);
+    if (t + kTeams < nt) arrive(t + kTeams, n + 1, next_gone);
     gone = next_gone;
   }
 
-  // ---- results: lane = row, four dims at a time ----
-  l += __shfl_xor(l, 32);
-  if (!real) return;
-  if (odd_flags[0] | odd_flags[1] | odd_flags[2] | odd_flags[3]) {  // behind a barrier at the last tile's arrival
+  bool some_odd = odd_flags[wave] != 0;
+  if constexpr (!kSplit) some_odd = (odd_flags[0] | odd_flags[1] | odd_flags[2] | odd_flags[3]) != 0;  // behind the last arrival's barrier
+  if (some_odd) {
 #pragma unroll 1
-    for (int t = 0; t < nt; ++t) {
+    for (t = team; t < nt; t += kTeams) {
 #pragma unroll 1
       for (int k = 0; k < KB; ++k) {
         const int key = key_of(t) + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
-        if (!page_there(a.c, pg) || key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
+        if (!real || !page_there(a.c, pg) || key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
         bool all_there = true;  // then its values were in the product as they are
         for (int b = 0; b < kBlocks; ++b) {
           const int i = (key_of(t) + 16 * b) >> a.c.shift;
@@ -390,6 +410,40 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
       }
     }
   }
+  // ---- results: lane = row, four dims at a time ----
+  l += __shfl_xor(l, 32);
+  if constexpr (kSplit) {
+    float* sums = (float*)(lds + team * Sh::kTeam);
+    float* states = (float*)(odd_flags + 4);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        *(f32x4*)(sums + row * Sh::kSums + 32 * d + 8 * b + 4 * half) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+    if (half == 0) {
+      states[(team * 32 + row) * 2] = m;
+      states[(team * 32 + row) * 2 + 1] = l;
+    }
+    __syncthreads();
+    const int rows = min(all_rows - of0, 32);
+    for (int i = tid; i < rows * (DT / 4); i += 64 * kTeams) {
+      const int r = i / (DT / 4), d = i % (DT / 4) * 4;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kTeams; ++w) top = fmaxf(top, states[(w * 32 + r) * 2]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kTeams; ++w) {
+        const float f = pow2(states[(w * 32 + r) * 2] - base);
+        sum += f * states[(w * 32 + r) * 2 + 1];
+        acc += f * *(const f32x4*)((const float*)(lds + w * Sh::kTeam) + r * Sh::kSums + d);
+      }
+      finish<Act, false>(a, s.r0, of0 + r, hk, 0, d, acc, base, sum);
+    }
+    return;
+  }
+  if (!real) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const size_t at = (size_t)(s.r0 + j) * a.ldo + (size_t)head * dim;
 #pragma unroll
@@ -401,28 +455,32 @@ __global__ __launch_bounds__(kThreads, DT == 256 ? 1 : 2) void prompt_kernel(Att
     }
 }
 
-template <typename Act, typename KV, int DT>
+template <typename Act, typename KV, int DT, bool kSplit>
 hipError_t launch(const Attend& a, unsigned items, hipStream_t s) {
-  constexpr size_t lds = Shape<Act, KV, DT>::kLds;
-  if constexpr (lds > 64 * 1024) {
+  using Sh = Shape<Act, KV, DT, kSplit>;
+  if constexpr (Sh::kLds > 64 * 1024) {
     static LdsLimitOnce limit;
-    if (hipError_t e = limit.raise((const void*)prompt_kernel<Act, KV, DT>, lds); e != hipSuccess) return e;
+    if (hipError_t e = limit.raise((const void*)prompt_kernel<Act, KV, DT, kSplit>, Sh::kLds); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT>), dim3(items), dim3(kThreads), lds, s, a);
+  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT, kSplit>), dim3(items), dim3(64 * Sh::kMembers * Sh::kTeams), Sh::kLds, s, a);
   return hipGetLastError();
 }
-template <typename Act, typename KV>
+template <typename Act, typename KV, bool kSplit>
 hipError_t launch_dim(const Attend& a, int dt, unsigned items, hipStream_t s) {
-  if (dt == 64) return launch<Act, KV, 64>(a, items, s);
-  if (dt == 128) return launch<Act, KV, 128>(a, items, s);
-  return launch<Act, KV, 256>(a, items, s);
+  if (dt == 64) return launch<Act, KV, 64, kSplit>(a, items, s);
+  if (dt == 128) return launch<Act, KV, 128, kSplit>(a, items, s);
+  return launch<Act, KV, 256, kSplit>(a, items, s);
+}
+template <typename Act, typename KV>
+hipError_t launch_shape(const Attend& a, int dt, unsigned items, hipStream_t s) {
+  return a.prompt_log2 == 5 ? launch_dim<Act, KV, true>(a, dt, items, s) : launch_dim<Act, KV, false>(a, dt, items, s);
 }
 }  // namespace
 
 hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s) {
-  if (act_bf16) return launch_dim<__bf16, __bf16>(a, dt, items, s);
-  if (dtype == W4A32_CACHE_F16) return launch_dim<float, _Float16>(a, dt, items, s);
-  return launch_dim<float, __bf16>(a, dt, items, s);
+  if (act_bf16) return launch_shape<__bf16, __bf16>(a, dt, items, s);
+  if (dtype == W4A32_CACHE_F16) return launch_shape<float, _Float16>(a, dt, items, s);
+  return launch_shape<float, __bf16>(a, dt, items, s);
 }
 
 }  // namespace paged

@@ -101,12 +101,20 @@ def test_attention(pkg, act, kind, heads, kv, dim, page, lens, rows):
 
 @pytest.mark.parametrize("act,kind", TYPES)
 @pytest.mark.parametrize("heads,kv,dim,page,lens,rows,window,first", [
-    (8, 8, 128, 32, [0, 70], [600, 601], 0, 0),              # enough workgroups for the prompts' kernel, all sequences alike
-    (14, 2, 64, 16, [33, 200, 5, 0], [300, 3, 1, 250], 0, 0),  # beside sequences that are not its own
+    # 32 rows of a workgroup: all sequences alike; beside sequences that are not the prompts' kernel's; odd sizes, windows
+    (8, 8, 128, 32, [0, 70], [600, 601], 0, 0),
+    (14, 2, 64, 16, [33, 200, 5, 0], [700, 3, 1, 450], 0, 0),
     (16, 8, 80, 64, [100, 0], [257, 333], 50, 5),
     (8, 8, 256, 16, [31], [700], 200, 40),
     (12, 12, 8, 128, [0], [1100], 0, 0),
     (7, 7, 96, 16, [130, 0], [450, 449], 1, 0),
+    # 128 rows of a workgroup (sequences without rows count among its workgroups)
+    (8, 8, 128, 32, [0, 70] + [9] * 40, [300, 401] + [0] * 40, 0, 0),
+    (14, 2, 64, 16, [33, 200, 5, 0] + [3] * 140, [300, 3, 1, 250] + [0] * 140, 0, 0),
+    (16, 8, 80, 64, [100, 0] + [3] * 40, [257, 333] + [1] * 20 + [0] * 20, 50, 5),
+    (8, 8, 256, 16, [31] + [0] * 40, [400] + [0] * 40, 200, 40),
+    (8, 8, 8, 128, [0] + [0] * 70, [500] + [2] * 70, 0, 0),   # more sequences than a wavefront has lanes
+    (7, 7, 96, 16, [130, 0] + [40] * 40, [350, 449] + [0] * 40, 1, 0),
 ])
 def test_prompts(pkg, act, kind, heads, kv, dim, page, lens, rows, window, first):
     B = pm.Batch(25, lens, rows, kv, dim, page)
@@ -115,14 +123,16 @@ def test_prompts(pkg, act, kind, heads, kv, dim, page, lens, rows, window, first
 
 
 @pytest.mark.parametrize("act,kind", TYPES)
-def test_prompts_with_missing_pages_and_odd_values(pkg, act, kind):
-    B = pm.Batch(26, [90, 40], [500, 400], 16, 64, 16)
+@pytest.mark.parametrize("many", [0, 20])
+def test_prompts_with_missing_pages_and_odd_values(pkg, act, kind, many):
+    many = many * [3]
+    B = pm.Batch(26, [90, 40] + many, [500, 400] + [0] * len(many), 16, 64, 16)
     fill_new(B)
     B.table[0, 3], B.table[0, 20], B.table[1, 0] = -1, B.n_pages + 7, -2 ** 31
     run_attention(pkg, B, act, kind, 16)
     run_attention(pkg, B, act, kind, 16, window=100, first=70)
     for bad, t in ((np.inf, 200), (np.nan, 89), (-np.inf, 10)):
-        B = pm.Batch(27, [90], [600], 16, 64, 16)
+        B = pm.Batch(27, [90] + many, [600] + [0] * len(many), 16, 64, 16)
         fill_new(B)
         p, i = B.slot(0, t)
         B.v[p, 5, i, 7] = bad
