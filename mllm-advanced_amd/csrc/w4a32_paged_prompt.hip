@@ -186,49 +186,50 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
   };
   // Where this lane's 16 bytes of a wavefront's load come from, in a row of the load
   const int lane_row = lane / kPerKey, piece = lane % kPerKey, wave_row = 64 * member / kPerKey;
-  // The turn of a row differs from load to load where a load of the team has fewer rows than the turns repeat after
+  // A load of the team has kRowsAtOnce rows. Load i's lie in the page of the tile's block block_of(i) of 16 keys, at place
+  // i % kKinds * kRowsAtOnce + wave_row (mod 16) + lane_row of it; both turns repeat after 16 rows.
   constexpr int kRowsAtOnce = kTeamThreads / kPerKey, kKinds = kRowsAtOnce < 16 ? 16 / kRowsAtOnce : 1;
   unsigned k_at[kKinds], v_at[kKinds];
   bool k_in[kKinds], v_in[kKinds];
 #pragma unroll
   for (int x = 0; x < kKinds; ++x) {
-    const int r = x * kTeamThreads / kPerKey + wave_row + lane_row, from = piece ^ Sh::k_turn(r);
+    const int r = (x * kRowsAtOnce + wave_row) % 16 + lane_row, from = piece ^ Sh::k_turn(r);
     k_in[x] = 8 * from < dim;
-    k_at[x] = (unsigned)(lane_row * dim + 8 * from) * 2;
+    k_at[x] = (unsigned)(r * dim + 8 * from) * 2;
     const int v_from = ((piece >> 1) ^ Sh::v_turn(r)) << 1 | (piece & 1);
     v_in[x] = 8 * v_from < dim;
-    v_at[x] = (unsigned)(lane_row * dim + 8 * v_from) * 2;
+    v_at[x] = (unsigned)(r * dim + 8 * v_from) * 2;
   }
+  auto block_of = [&](int i) { return i * kRowsAtOnce / 16 + (kRowsAtOnce > 16 ? __builtin_amdgcn_readfirstlane(wave_row) / 16 : 0); };
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + __builtin_amdgcn_readfirstlane(team) * (unsigned)Sh::kTeam;
   uint16_t* tiles = (uint16_t*)(lds + team * Sh::kTeam);
   // The team's n-th tile, t, to its buffer n & 1; returns the sixteens of keys whose page is not there.
   auto load = [&](int t, int n) {
-    int page[kBlocks], gone = 0;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b) {
-      page[b] = __builtin_amdgcn_readlane(pages, b);
-      if (!page_there(a.c, page[b])) {
-        gone |= 1 << b;
-        page[b] = 0;
-      }
-    }
+    // every lane works its block's place in the pools out, and the loads take them from there
+    const bool there = page_there(a.c, pages);
+    const int gone = (int)(__ballot(!there) & ((1u << kBlocks) - 1));
+    const u64 at = slot_row(a.c, there ? pages : 0, hk, key_of(t) + 16 * min(lane, kBlocks - 1)) * (unsigned)(2 * dim);
+    const unsigned at_lo = (unsigned)at, at_hi = (unsigned)(at >> 32);
     find(t + kTeams);
     const unsigned to = lds0 + (n & 1) * (4 * Sh::kTile) + __builtin_amdgcn_readfirstlane(member) * 1024;
+    constexpr int kStep = 1024 * Sh::kMembers;
+    auto base_of = [&](int i) {
+      const int b = block_of(i);
+      return (u64)(unsigned)__builtin_amdgcn_readlane((int)at_hi, b) << 32 | (unsigned)__builtin_amdgcn_readlane((int)at_lo, b);
+    };
+    if (DT == dim) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = i * kTeamThreads / kPerKey + __builtin_amdgcn_readfirstlane(wave_row);
-      int pg = page[0];
+      for (int i = 0; i < kLoads; ++i) {
+        const u64 base = base_of(i);
+        load_lds((const uint8_t*)a.c.k + base, k_at[i % kKinds], to + kStep * i);
+        load_lds((const uint8_t*)a.c.v + base, v_at[i % kKinds], to + kStep * i + 2 * Sh::kTile);
+      }
+    } else {  // zeros past the head's size
 #pragma unroll
-      for (int b = 1; b < kBlocks; ++b) pg = r / 16 == b ? page[b] : pg;
-      const size_t at = slot_row(a.c, pg, hk, key_of(t) + r) * dim;
-      const uint16_t *k = (const uint16_t*)a.c.k + at, *v = (const uint16_t*)a.c.v + at;
-      constexpr int kStep = 1024 * Sh::kMembers;
-      if (DT == dim) {
-        load_lds(k, k_at[i % kKinds], to + kStep * i);
-        load_lds(v, v_at[i % kKinds], to + kStep * i + 2 * Sh::kTile);
-      } else {  // zeros past the head's size
-        load_lds(k_in[i % kKinds] ? (const uint8_t*)k + k_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i);
-        load_lds(v_in[i % kKinds] ? (const uint8_t*)v + v_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i + 2 * Sh::kTile);
+      for (int i = 0; i < kLoads; ++i) {
+        const u64 base = base_of(i);
+        load_lds(k_in[i % kKinds] ? (const uint8_t*)a.c.k + base + k_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i);
+        load_lds(v_in[i % kKinds] ? (const uint8_t*)a.c.v + base + v_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i + 2 * Sh::kTile);
       }
     }
     return gone;
