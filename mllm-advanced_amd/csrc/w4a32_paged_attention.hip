@@ -29,10 +29,12 @@ inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_EL
 constexpr int kGrid = 512;        // workgroups that a batch is dealt to: two per CU, all there at once
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
 constexpr int kAlone = 8;         // tiles of an item that is not shared, where there are workgroups enough for all items
-// The prompts' kernel takes sequences of at least kPromptRows pairs of token and head, where it has kPromptLeast workgroups or
-// more: it does not share a row's keys between workgroups, and few of them on a long context would leave the chip idle.
-constexpr int kPromptRows = 256, kPromptLeast = 128;
-constexpr int kPromptBlocks = 256;  // workgroups of 128 rows that are worth while; fewer are taken as four times as many of 32
+// The prompts' kernel takes sequences of at least kPromptRows pairs of token and head, where it has kPromptLeast workgroups of 32
+// rows or more: it does not share a row's keys between workgroups, and few of them on a long context would leave the chip idle.
+// From kPromptWide workgroups of eight times as many rows on it has those (28 heads on 4, bf16: 512 rows 22 us with either, 2048
+// rows 72 us against 131; f32 rows, two or three terms of each operand, 1024 rows 64 us against 76 in favour of 32 and 2048 rows 164
+// against 147).
+constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideTerms = 160;
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
 
 template <int KT>
@@ -575,12 +577,13 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
   p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
   auto blocks = [&](int log2) { return ((long long)r->rows * group / (1 << log2) + c->n_seqs) * c->kv_heads; };
-  p.prompt_log2 = blocks(7) >= kPromptBlocks ? 7 : 5;
+  const int wide = p.dt == 256 ? 7 : 8;
+  p.prompt_log2 = blocks(wide) >= (r->act_bf16 ? kPromptWide : kPromptWideTerms) ? wide : 5;
   p.prompts = blocks(p.prompt_log2);
   p.prompt_rows = 0;
   p.others = true;
   if (p.prompts >= (1ll << 31)) return W4A32_ESHAPE;
-  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && p.prompts >= kPromptLeast) {
+  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && blocks(5) >= kPromptLeast) {
     // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then. Else the rows'
     // kernel has what is left, of so few rows.
     const bool ragged = r->rows < (long long)r->max_rows * c->n_seqs;

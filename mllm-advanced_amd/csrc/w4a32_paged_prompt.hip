@@ -28,7 +28,6 @@ namespace paged {
 
 namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-constexpr int kThreads = 256;
 constexpr int kSlack = 8;
 
 __device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
@@ -39,13 +38,15 @@ __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builti
 template <typename Act, typename KV, int DT, bool kSplit>
 struct Shape {
   static constexpr int kTerms = Math<Act, KV>::kTerms;
-  static constexpr int kMembers = kSplit ? 1 : 4, kTeams = !kSplit ? 1 : DT == 256 ? 2 : 4;
-  static constexpr int kKeys = !kSplit && kTerms == 1 && DT <= 128 ? 64 : 32;
+  static constexpr int kMembers = kSplit ? 1 : DT == 256 ? 4 : 8, kTeams = !kSplit ? 1 : DT == 256 ? 2 : 4;
+  static constexpr int kThreads = 64 * kMembers * kTeams;
+  static constexpr int kKeys = kSplit ? 32 : DT == 256 ? 64 : 128;         // of a tile
+  static constexpr int kStep = !kSplit && kTerms == 1 && DT <= 128 ? 64 : 32;  // of a step of the softmax
   static constexpr int kTile = kKeys * DT;                // elements of a tile of K or V
   static constexpr size_t kTeam = (size_t)4 * kTile * 2;  // bytes of a team's tiles: K and V, twice
   static constexpr int kSums = DT + 4;                    // floats of a row of sums, where teams are joined
   static constexpr int kStates = kSplit ? kTeams * 32 * 2 : 0;
-  static constexpr size_t kLds = kTeams * kTeam + 4 * sizeof(int) + kStates * sizeof(float);
+  static constexpr size_t kLds = kTeams * kTeam + 8 * sizeof(int) + kStates * sizeof(float);
   static_assert(!kSplit || (size_t)32 * kSums * 4 <= kTeam, "a team's sums lie where its tiles were");
   // by which the pieces of row r are exchanged: 16 bytes of K, 32 bytes of V
   static __device__ __forceinline__ int k_turn(int r) { return DT == 64 ? r >> 1 & 7 : r & 15; }
@@ -64,11 +65,11 @@ __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 template <typename Act, typename KV, int DT, bool kSplit>
-__global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_kernel(Attend a) {
+__global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 || kSplit ? 1 : 2) void prompt_kernel(Attend a) {
   using M = Math<Act, KV>;
   using Sh = Shape<Act, KV, DT, kSplit>;
   constexpr int kTeams = Sh::kTeams, kTeamThreads = 64 * Sh::kMembers, kBlock = 32 * Sh::kMembers;
-  constexpr int NT = Sh::kTerms, KB = Sh::kKeys, kSub = KB / 32, kSteps = DT / 16, kDims = DT / 32;
+  constexpr int NT = Sh::kTerms, KB = Sh::kKeys, KS = Sh::kStep, kSub = KS / 32, kSteps = DT / 16, kDims = DT / 32;
   constexpr int kWeight = M::kScale ? M::kScale - kSlack : 0;  // exponent that weights carry
   constexpr int kPerKey = DT / 8;                      // 16-byte loads of a key
   constexpr int kLoads = KB * kPerKey / kTeamThreads;  // of a thread, for K and for V
@@ -234,10 +235,11 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
     }
     return gone;
   };
-  // Whether rows that stand from lo to hi all see all keys from k0 on
-  auto all_seen = [&](int k0, int lo, int hi) {
-    return k0 + KB - 1 <= lo && (a.window == 0 || k0 > hi - a.window || k0 + KB - 1 < a.first);
+  // Whether rows that stand from lo to hi all see all `keys` keys from k0 on
+  auto seen_by = [&](int k0, int keys, int lo, int hi) {
+    return k0 + keys - 1 <= lo && (a.window == 0 || k0 > hi - a.window || k0 + keys - 1 < a.first);
   };
+  auto all_seen = [&](int k0, int lo, int hi) { return seen_by(k0, KB, lo, hi); };
   // The tile has arrived, for all wavefronts. Where not all rows see all of it: zeros for what no row sees, and for values that
   // are not finite; whether there were any of those is noted.
   if (lane == 0) odd_flags[wave] = 0;
@@ -288,10 +290,13 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
     const int next_gone = t + kTeams < nt ? load(t + kTeams, n + 1) : 0;
     const uint16_t* ks = tiles + (n & 1) * (2 * Sh::kTile);
     const uint16_t* vs = ks + Sh::kTile;
-    const int k0 = key_of(t);
-    const bool whole = gone == 0 && all_seen(k0, pos_min, pos_max);
-    const bool none = row0 >= all_rows || k0 > pos_max;  // of this wavefront
-    if (!none) {
+    const int tile0 = key_of(t);
+#pragma unroll 1
+    for (int k0 = tile0; k0 < tile0 + KB; k0 += KS, ks += KS * DT, vs += KS * DT) {
+    const int gone_here = gone >> (k0 - tile0) / 16;
+    const bool whole = gone == 0 && seen_by(k0, KS, pos_min, pos_max);
+    if (row0 >= all_rows || k0 > pos_max) break;  // nothing for this wavefront
+    {
       // ---- scores ----
       const int k_turn = 8 * Sh::k_turn(row);  // of rows 32 u + row
       f32x16 sc[kSub];
@@ -323,7 +328,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int key = first_key + 32 * u + 8 * (i / 4) + i % 4;
-            const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !(gone >> (2 * u + i / 8) & 1);
+            const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !(gone_here >> (2 * u + i / 8) & 1);
             sc[u][i] = sees ? sc[u][i] : -INFINITY;
           }
       }
@@ -342,6 +347,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
         for (int d = 0; d < kDims; ++d) o[d] *= down;
       }
       const float off = m == -INFINITY ? 0.0f : (float)kWeight - m;  // nothing seen yet: 2^-infinity is 0
+      __builtin_amdgcn_s_setprio(1);
       float pr[kSub][16];
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
@@ -380,12 +386,14 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
       }
       __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 1);
     }
+    __builtin_amdgcn_s_setprio(0);}
     if (t + kTeams < nt) arrive(t + kTeams, n + 1, next_gone);
     gone = next_gone;
   }
 
   bool some_odd = odd_flags[wave] != 0;
-  if constexpr (!kSplit) some_odd = (odd_flags[0] | odd_flags[1] | odd_flags[2] | odd_flags[3]) != 0;  // behind the last arrival's barrier
+  if constexpr (!kSplit)  // behind the last arrival's barrier
+    for (int w = 0; w < Sh::kMembers; ++w) some_odd = some_odd || odd_flags[w] != 0;
   if (some_odd) {
 #pragma unroll 1
     for (t = team; t < nt; t += kTeams) {
@@ -415,7 +423,7 @@ __global__ __launch_bounds__(kThreads, DT == 256 || kSplit ? 1 : 2) void prompt_
   l += __shfl_xor(l, 32);
   if constexpr (kSplit) {
     float* sums = (float*)(lds + team * Sh::kTeam);
-    float* states = (float*)(odd_flags + 4);
+    float* states = (float*)(odd_flags + 8);
 #pragma unroll
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
@@ -463,7 +471,7 @@ hipError_t launch(const Attend& a, unsigned items, hipStream_t s) {
     static LdsLimitOnce limit;
     if (hipError_t e = limit.raise((const void*)prompt_kernel<Act, KV, DT, kSplit>, Sh::kLds); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT, kSplit>), dim3(items), dim3(64 * Sh::kMembers * Sh::kTeams), Sh::kLds, s, a);
+  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT, kSplit>), dim3(items), dim3(Sh::kThreads), Sh::kLds, s, a);
   return hipGetLastError();
 }
 template <typename Act, typename KV, bool kSplit>
