@@ -1,15 +1,18 @@
 // Attention of prompts over a paged cache of 16-bit elements: the sequences of a batch that have so many rows that products bound
 // them and not the cache.
 //
-// A workgroup has 128 query rows of one kv head (pairs of token and head of the group, 32 to a wavefront) and takes the keys that
-// they can see, 64 (32 where an f32 operand is two or three terms, or the head has 256 dims) at a time through LDS: the next
-// tile goes from memory straight to the other half of it (global_load_lds_dwordx4) while this one is multiplied. Both products are transposed as in the rows' kernel, on
-// v_mfma_f32_32x32x16: a lane stands for query row lane % 32, and lanes l and l + 32 share it.
+// A workgroup has 256 query rows of one kv head (pairs of token and head of the group, 32 to a wavefront; 128 where a head has 256
+// dims) and takes the keys that they can see through LDS, in tiles of 128 (64 of 256 dims): the next tile goes from memory
+// straight to the other half of it (global_load_lds_dwordx4) while this one is multiplied. A tile's keys are worked through 64 at
+// a time, or 32 where an f32 operand is two or three terms, so that a step's scores stay in registers. Against 128 rows and tiles
+// of 64 a key is read half as often and waited for half as often (two prompts: 163 -> 154 us). Both products are transposed as in
+// the rows' kernel, on v_mfma_f32_32x32x16: a lane stands for query row lane % 32, and lanes l and l + 32 share it.
 //   S^T = K Q^T     A = K from LDS: lane = key l % 32, dims 16 c + 8 (l / 32) ..; B = Q in registers
 //   O^T += V^T P^T  B = the softmaxed S^T registers: half h of the wavefront has keys 8 b + 4 h .. + 3 of a block of 32;
 //                   A = V^T: ds_read_b64_tr_b16 of the same keys
-// What bounds it: a tile of 64 keys and 128 dims costs a SIMD 32 x 32 = 1024 clocks of bf16 products per wavefront, and about as
-// many of maxima, exponentials and sums, which run under the other wavefront's products (two per SIMD). So the sums' reference
+// What bounds it: 64 keys and 128 dims cost a SIMD 32 x 32 = 1024 clocks of bf16 products per wavefront, and about as many of
+// maxima, exponentials and sums, of which the other wavefront of the SIMD covers only a part: the matrix units are busy for 38% of
+// the time (2048 + 1024 rows, 28 heads on 4 of 128 dims, bf16: 150 us, 765 TFLOP/s where all workgroups run). So the sums' reference
 // follows a row's maximum only when that has grown by more than 2^kSlack: the 64 products that bring the sums to a new reference
 // are then rare, and weights of up to 2^kSlack are as exact as those up to 1 (f16 has its weights' scale lowered for them).
 // A wavefront's load fills 1024 bytes of LDS in lane order, so rows have no padding between them; instead the 16-byte pieces of a
@@ -293,10 +296,9 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     const int tile0 = key_of(t);
 #pragma unroll 1
     for (int k0 = tile0; k0 < tile0 + KB; k0 += KS, ks += KS * DT, vs += KS * DT) {
-    const int gone_here = gone >> (k0 - tile0) / 16;
-    const bool whole = gone == 0 && seen_by(k0, KS, pos_min, pos_max);
-    if (row0 >= all_rows || k0 > pos_max) break;  // nothing for this wavefront
-    {
+      const int gone_here = gone >> (k0 - tile0) / 16;
+      const bool whole = gone == 0 && seen_by(k0, KS, pos_min, pos_max);
+      if (row0 >= all_rows || k0 > pos_max) break;  // nothing for this wavefront
       // ---- scores ----
       const int k_turn = 8 * Sh::k_turn(row);  // of rows 32 u + row
       f32x16 sc[kSub];
@@ -347,7 +349,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
         for (int d = 0; d < kDims; ++d) o[d] *= down;
       }
       const float off = m == -INFINITY ? 0.0f : (float)kWeight - m;  // nothing seen yet: 2^-infinity is 0
-      __builtin_amdgcn_s_setprio(1);
+      __builtin_amdgcn_s_setprio(1);  // over the other wavefront's scores, whose turn comes: 154 -> 150 us for two prompts
       float pr[kSub][16];
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
@@ -385,8 +387,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
       }
       __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 1);
+      __builtin_amdgcn_s_setprio(0);
     }
-    __builtin_amdgcn_s_setprio(0);}
     if (t + kTeams < nt) arrive(t + kTeams, n + 1, next_gone);
     gone = next_gone;
   }

@@ -101,14 +101,14 @@ def test_attention(pkg, act, kind, heads, kv, dim, page, lens, rows):
 
 @pytest.mark.parametrize("act,kind", TYPES)
 @pytest.mark.parametrize("heads,kv,dim,page,lens,rows,window,first", [
-    # 32 rows of a workgroup: all sequences alike; beside sequences that are not the prompts' kernel's; odd sizes, windows
+    # few workgroups, so of 32 rows: all sequences alike; beside sequences that are not the prompts' kernel's; odd sizes, windows
     (8, 8, 128, 32, [0, 70], [600, 601], 0, 0),
     (14, 2, 64, 16, [33, 200, 5, 0], [700, 3, 1, 450], 0, 0),
     (16, 8, 80, 64, [100, 0], [257, 333], 50, 5),
     (8, 8, 256, 16, [31], [700], 200, 40),
     (12, 12, 8, 128, [0], [1100], 0, 0),
     (7, 7, 96, 16, [130, 0], [450, 449], 1, 0),
-    # 128 rows of a workgroup (sequences without rows count among its workgroups)
+    # workgroups of 256 or 128 rows (sequences without rows count among its workgroups)
     (8, 8, 128, 32, [0, 70] + [9] * 40, [300, 401] + [0] * 40, 0, 0),
     (14, 2, 64, 16, [33, 200, 5, 0] + [3] * 140, [300, 3, 1, 250] + [0] * 140, 0, 0),
     (16, 8, 80, 64, [100, 0] + [3] * 40, [257, 333] + [1] * 20 + [0] * 20, 50, 5),
