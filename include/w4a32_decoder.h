@@ -261,7 +261,10 @@ int w4a32_op_f16_to_f32(const void* d_in, float* d_out, size_t n, void* stream);
  *
  * What a device array may say wrongly is kept inside the pools: a page number outside [0, n_pages) stands for a page
  * that is not there (its tokens are not seen and not written; pages that a window has left may be given back so), a
- * negative length is 0, tokens behind the table's end are not there, and a sequence has at most max_rows rows.
+ * negative length is 0, tokens behind the table's end are not there, and a sequence has at most max_rows rows. Row starts
+ * do not decrease; where they do, what the rows get is unspecified.
+ *   Sequences may name the same page (a prompt that they share) as long as no call writes it: tokens are appended, and weights
+ * added up, only in pages that one sequence names once.
  *
  * The reference has one sequence per model and caches of a fixed length (mllm/Backends/Arm/Ops/KVCacheOp.cpp:44-72). */
 #define W4A32_CACHE_F32 1
@@ -270,7 +273,7 @@ int w4a32_op_f16_to_f32(const void* d_in, float* d_out, size_t n, void* stream);
 #define W4A32_PAGED_MAX_DIM 256
 
 /* Rows are f32 with any cache, or bf16 with a bf16 cache (`act_bf16`). dim % 8 == 0, dim <= 256; page is a power of two
- * from 16 on; table_ld * page and the rows of a step stay below 2^30. Pools and rows on 16 bytes; row strides (ld*, in
+ * from 16 on; table_ld * page and rows * heads stay below 2^30. Pools and rows on 16 bytes; row strides (ld*, in
  * elements) are multiples of 8 that hold a row. Zero-initialise the structs before filling them. */
 typedef struct {
   void *d_k, *d_v;        /* [n_pages][kv_heads][page][dim] of `dtype` */
@@ -288,7 +291,7 @@ typedef struct {
   int heads;                /* query heads, a multiple of kv_heads: head h reads kv head h / (heads / kv_heads) */
   int act_bf16;
   const void* d_q;          /* [rows][heads][dim] */
-  void* d_out;              /* [rows][heads][dim]: rotated q (append; may be d_q), attention's output */
+  void* d_out;              /* [rows][heads][dim]: rotated q (append; may be d_q), attention's output (apart from d_q) */
   int ldq, ldo;
 } w4a32_paged_rows;
 
@@ -305,12 +308,12 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
 
 /* out = softmax(scale q K^T) V per head over what a row sees: row j of sequence b, which stands at slot s = d_len[b] + j
  * (appended before the call), sees slots t <= s with t > s - window or t < first (window 0: all). A row that sees nothing
- * gets zeros; values that are not finite reach only the rows that see them. With `accumulate` the weights are added to
- * cache->d_weight: for every cached token the sum over the rows and over the heads of its kv head, in a fixed order
- * (the same call gives the same bits).
+ * gets zeros; what is not finite reaches only the rows that see it (a value as in the formula; an infinity in q or in a key
+ * makes a row NaN). With `accumulate` the weights are added to cache->d_weight: for every cached token the sum over the rows
+ * and over the heads of its kv head, in a fixed order (the same call gives the same bits).
  *   Sums, maxima and products are f32 at f32 accuracy for f32 rows (a 16-bit cache's elements are exact operands of the
  * 16-bit matrix instructions, q and the weights enter as two f16 or three bf16 terms); for bf16 rows the weights enter
- * the second product as bf16, as the output is rounded.
+ * the second product as bf16, as the output is rounded. `scale` is finite.
  *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time (calls that
  * overlap in time, on two streams or in two graphs, need one each). That is 0 for a call that w4a32_op_paged_attention refuses.
  * QWenAttention::forward, modeling_ds_qwen2.hpp:133-151, per sequence. */
@@ -338,12 +341,12 @@ int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache
  * drafted token alone has q = 1), token t is accepted while uniform[r] q(t) < p(t). Behind the last
  * accepted one the next token is drawn: where a token was refused from max(p - q, 0), else from p, as the least index whose
  * running sum exceeds choice[b] times the whole sum. uniform [rows] and choice [n_seqs] are the caller's numbers from
- * [0, 1). temperature 0: a token is accepted where it is the first maximum, and the next token is the first maximum (no
- * draft logits or numbers are read; they may be NULL).
+ * [0, 1). temperature 0: a token is accepted where it is the first maximum (which a NaN is not), and the next token is the
+ * first maximum, -1 where all are -infinity or NaN (no draft logits or numbers are read; they may be NULL).
  *   d_count[b] = accepted tokens + 1, the rows that stay; d_next[b] = the next token; d_len (may be NULL) += d_count.
  * A sequence without rows gets count 0 and token -1, and a token that has no distribution to come from (no finite
  * logit, a NaN, +infinity) is -1; -infinity is a probability of 0, and a drafted token outside [0, vocab) is refused.
- * Exponentials and sums are held in 64 bits: the choice depends on neither the order of sums nor the sizes of the parts.
+ * Exponentials and sums are held in 64 bits, 1e-11 relative: the choice depends on neither the order of sums nor the sizes of the parts.
  * Per sequence what AutoLLM.hpp:70-88 does for one token, with the test that keeps the target's distribution.
  *   d_scratch: w4a32_op_verify_drafts_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time. */
 typedef struct {

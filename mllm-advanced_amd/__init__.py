@@ -830,6 +830,13 @@ def _row_ld(t, what, dtype, device):
     return ld if t.shape[0] > 1 else t.shape[1]
 
 
+def _scratch_of(t, device):
+    """Refuses scratch memory that is not one piece of the device whose stream the call goes to."""
+    if t.get_device() != device or not t.is_contiguous():
+        raise W4A32Error(f"scratch: contiguous memory on device {device} is wanted: got strides {t.stride()} on {t.device}")
+    return t.data_ptr(), t.nbytes
+
+
 class PagedCache:
     """A paged key / value cache that several sequences share: k and v [pages][kv_heads][page][dim] (f32, f16 or bf16), table
     int32 [sequences][most pages of one] (a number outside the pool: no page), length int32 [sequences], and, where weights are
@@ -905,13 +912,16 @@ def op_paged_attention_scratch(cache, rows, max_rows, heads, accumulate=False):
 def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, first=0, accumulate=False, scratch=None, out=None):
     """Attention of rows q [rows][heads * dim] over their sequences' pages, the rows' own tokens included (appended before):
     row j of sequence b sees slots t <= s = cache.length[b] + j with t > s - window or t < first (window 0: all). max_rows: most
-    rows of one sequence. accumulate: the weights that the cached tokens receive are added to cache.weight."""
+    rows of one sequence. accumulate: the weights that the cached tokens receive are added to cache.weight (sequences may share
+    pages to be read, but then not with this). out is not q."""
     if out is None:
         out = _torch.empty_like(q)
     if scratch is None:
         scratch = op_paged_attention_scratch(cache, q.shape[0], max_rows, heads, accumulate)
     r = _paged_rows(cache, q, row_start, max_rows, heads, out)
-    _check(lib().w4a32_op_paged_attention(cache._ref, r, scale, window, first, accumulate, scratch.data_ptr(), scratch.nbytes, _stream()),
+    if window >> 31 or first >> 31:
+        raise W4A32Error(f"window {window} and first {first}: from 0 to 2^31 - 1")
+    _check(lib().w4a32_op_paged_attention(cache._ref, r, scale, window, first, accumulate, *_scratch_of(scratch, cache.device), _stream()),
            "w4a32_op_paged_attention")
     return out
 
@@ -926,14 +936,16 @@ def op_paged_evict_scratch(cache, budget):
 
 def op_paged_evict(cache, to, budget, first=0, recent=0, scratch=None):
     """Of every sequence's tokens the first, the most recent and those with the largest added-up weight, `budget` in all per kv
-    head, go in order to the pages of `to`, whose lengths are set. Returns the slots that stayed, int32
+    head, go in order to the pages of `to` (other ones, of the same pools or not), whose lengths are set. Returns the slots that stayed, int32
     [sequences][kv_heads][budget], -1 behind them."""
     if cache.device != _device() or to.device != cache.device:
         raise W4A32Error("the caches are not on the current device")
+    if budget >> 31 or first >> 31 or recent >> 31:
+        raise W4A32Error(f"budget {budget}, first {first} and recent {recent}: from 0 to 2^31 - 1")
     if scratch is None:
         scratch = op_paged_evict_scratch(cache, budget)
     kept = cache.table.new_empty((cache.n_seqs, cache.kv_heads, budget))
-    _check(lib().w4a32_op_paged_evict(cache._ref, to._ref, budget, first, recent, kept.data_ptr(), scratch.data_ptr(), scratch.nbytes,
+    _check(lib().w4a32_op_paged_evict(cache._ref, to._ref, budget, first, recent, kept.data_ptr(), *_scratch_of(scratch, cache.device),
                                       _stream()), "w4a32_op_paged_evict")
     return kept
 
@@ -973,7 +985,7 @@ def op_verify_drafts(logits, row_start, max_rows, tokens, uniform, choice, tempe
     a = _VERIFY_STRUCT.pack(logits.data_ptr(), _ptr(draft) or 0, row_start.data_ptr(), tokens.data_ptr(), _ptr(uniform) or 0,
                             _ptr(choice) or 0, count.data_ptr(), token.data_ptr(), _ptr(length) or 0, rows, max_rows, n, vocab, ldl, ldd,
                             temperature)
-    _check(lib().w4a32_op_verify_drafts(a, scratch.data_ptr(), scratch.nbytes, _stream()), "w4a32_op_verify_drafts")
+    _check(lib().w4a32_op_verify_drafts(a, *_scratch_of(scratch, device), _stream()), "w4a32_op_verify_drafts")
     return count, token
 
 

@@ -18,6 +18,10 @@ struct Cache {
   int cap;                                              // table_ld pages in tokens
 };
 
+// Most workgroups of a launch of `threads` each: a launch has less than 2^32 threads. What would need more is refused.
+constexpr long long most_groups(int threads) { return (1ll << 32) / threads - 1; }
+constexpr int kMost = 1 << 30;  // rows of a step, tokens of a sequence, pairs of row and head
+
 inline int log2_of(int page) { return __builtin_ctz((unsigned)page); }
 
 // Host: whether the cache's sizes are what the kernels assume. W4A32_OK or the code to return.

@@ -7,7 +7,6 @@ namespace paged {
 namespace {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_ELAUNCH; }
-constexpr int kMost = 1 << 30;
 }  // namespace
 
 int check_cache(const w4a32_paged_cache* c) {
@@ -27,7 +26,7 @@ int check_rows(const w4a32_paged_cache* c, const w4a32_paged_rows* r) {
   if (int e = check_cache(c)) return e;
   if (!r || !r->d_row_start || r->rows < 1 || r->max_rows < 1 || r->heads < 1) return W4A32_EINVAL;
   if (!aligned(r->d_row_start, 4) || !aligned(r->d_q, 16) || !aligned(r->d_out, 16)) return W4A32_EINVAL;
-  if (r->rows >= kMost || r->heads >= kMost / c->dim || r->heads % c->kv_heads) return W4A32_ESHAPE;
+  if (r->rows >= kMost || r->heads >= kMost / c->dim || (long long)r->rows * r->heads >= kMost || r->heads % c->kv_heads) return W4A32_ESHAPE;
   if (r->act_bf16 && c->dtype != W4A32_CACHE_BF16) return W4A32_ENOTSUP;
   if (r->d_q && (!r->d_out || r->ldq < r->heads * c->dim || r->ldo < r->heads * c->dim || r->ldq % 8 || r->ldo % 8)) return W4A32_EINVAL;
   return W4A32_OK;
@@ -327,11 +326,11 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
   if (ldk < width || ldv < width || ldk % 8 || ldv % 8) return W4A32_EINVAL;
   if (rot_dims < 0 || rot_dims > cache->dim || rot_dims % 8) return W4A32_ESHAPE;
   if (rot_dims && (!d_sin || !d_cos || table_rows < 1 || !aligned(d_sin, 16) || !aligned(d_cos, 16))) return W4A32_EINVAL;
-  const Append a{view(cache),   rows->d_row_start, d_pos,    rows->d_q, d_k, d_v, rows->d_out, d_sin, d_cos, rows->rows, rows->max_rows,
-                 rows->heads, rows->ldq, rows->ldo, ldk, ldv, rot_dims, table_rows};
+  const Append a{view(cache), rows->d_row_start, d_pos,       rows->d_q, d_k, d_v, rows->d_out, d_sin,      d_cos, rows->rows,
+                 rows->max_rows, rows->heads,   rows->ldq, rows->ldo, ldk, ldv, rot_dims,    table_rows};
   const long long units = (long long)((rows->d_q ? rows->heads : 0) + 2 * cache->kv_heads) * (cache->dim / 8);
   const long long per_row = (units + 255) / 256;
-  if (per_row * rows->rows >= (1ll << 31)) return W4A32_ESHAPE;
+  if (per_row * rows->rows > most_groups(256)) return W4A32_ESHAPE;
   const dim3 grid((unsigned)(per_row * rows->rows)), block(256);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows->act_bf16)
@@ -359,13 +358,15 @@ int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache
     return W4A32_ESHAPE;
   if ((long long)first + recent > budget || budget > (long long)to->table_ld * to->page) return W4A32_ESHAPE;
   if (cache->d_len == to->d_len) return W4A32_EINVAL;
+  if (cache->d_table == to->d_table && (cache->d_k == to->d_k || cache->d_v == to->d_v || cache->d_weight == to->d_weight))
+    return W4A32_EINVAL;  // the same pages
   const size_t need = w4a32_op_paged_evict_scratch_bytes(cache, budget);
   if (!d_kept && (!d_scratch || !aligned(d_scratch, 16) || scratch_bytes < need)) return W4A32_EINVAL;
   const Evict a{view(cache), view(to), budget, first, recent, d_kept ? d_kept : static_cast<int*>(d_scratch), to->d_len};
   const long long heads = (long long)cache->n_seqs * cache->kv_heads;
   const int units = cache->dim * (cache->dtype == W4A32_CACHE_F32 ? 4 : 2) / 16, per = kCopies * (256 / units);
   const long long blocks = ((long long)budget + per - 1) / per;
-  if (heads * blocks >= (1ll << 31)) return W4A32_ESHAPE;
+  if (heads > most_groups(kSelect) || heads * blocks > most_groups(256)) return W4A32_ESHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
   // the table says how long a sequence can be
   const size_t held = (size_t)cache->table_ld * cache->page;

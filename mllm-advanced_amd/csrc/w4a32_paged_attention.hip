@@ -35,6 +35,8 @@ constexpr int kAlone = 8;         // tiles of an item that is not shared, where 
 // rows 72 us against 131; f32 rows, two or three terms of each operand, 1024 rows 64 us against 76 in favour of 32 and 2048 rows 164
 // against 147).
 constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideTerms = 160;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kJoins = 1 << 20;   // workgroups of the joining launch, beyond which they take several rows each
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
 
 template <int KT>
@@ -449,12 +451,12 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 // Joins the shares of an item: a workgroup per query row and kSlice of its values, its threads four values of every 256 /
 // (kSlice / 4)th share each.
 template <typename Act, int DT, int kSlice, bool kDump>
-__global__ __launch_bounds__(256) void join_kernel(Attend a) {
+__device__ __forceinline__ void join(const Attend& a, unsigned unit) {
   constexpr int kPer = kSlice / 4, kAtOnce = 256 / kPer;
   __shared__ __attribute__((aligned(16))) float sums[kAtOnce][kSlice];
   __shared__ float tops[kAtOnce], totals[kAtOnce];
-  const int slice = blockIdx.x % (DT / kSlice), r = blockIdx.x / (DT / kSlice) % a.slot_rows;
-  const unsigned item = blockIdx.x / (DT / kSlice) / a.slot_rows;
+  const int slice = unit % (DT / kSlice), r = unit / (DT / kSlice) % a.slot_rows;
+  const unsigned item = unit / (DT / kSlice) / a.slot_rows;
   const unsigned count = *a.count;
   const Item it = a.item[item];
   if (item >= count || it.shares == 1 || r >= it.rows) return;
@@ -510,6 +512,13 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a) {
     sum += f * totals[i];
   }
   finish<Act, kDump>(a, it.r0, it.row0 + r, it.head, (size_t)item * a.slot_rows + r, d, acc, base, sum);
+}
+template <typename Act, int DT, int kSlice, bool kDump>
+__global__ __launch_bounds__(256) void join_kernel(Attend a, unsigned units) {
+  for (unsigned u = blockIdx.x; u < units; u += gridDim.x) {
+    join<Act, DT, kSlice, kDump>(a, u);
+    if (units > gridDim.x) __syncthreads();
+  }
 }
 
 // Adds the weights of a tile's keys up: a wavefront per tile of a kv head, over its items in order.
@@ -582,7 +591,6 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   p.prompts = blocks(p.prompt_log2);
   p.prompt_rows = 0;
   p.others = true;
-  if (p.prompts >= (1ll << 31)) return W4A32_ESHAPE;
   if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && blocks(5) >= kPromptLeast) {
     // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then. Else the rows'
     // kernel has what is left, of so few rows.
@@ -591,6 +599,7 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
     most = (kPromptRows - 1) / group;
     p.others = ragged && most > 0;
     if (!p.others) most = 1;
+    if (p.prompts > most_groups(512)) return W4A32_ESHAPE;
   }
   // 32 or 64 rows of an item are two or four wavefronts' that ask for the same keys at about the same time: the caches serve
   // all but the first, where as items of their own each would have the keys from memory again
@@ -607,7 +616,7 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   p.tiles = p.items * tiles;
   p.grid = p.tiles < kGrid ? p.tiles : kGrid;
   p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
-  if (p.tiles >= (1ll << 31) || p.items * p.slot_rows * (p.dt / 32) >= (1ll << 31) || p.key_groups >= (1ll << 31)) return W4A32_ESHAPE;
+  if (p.tiles >= (1ll << 31) || p.items * p.slot_rows >= kMost || (accumulate && p.key_groups > most_groups(64 * kWaves))) return W4A32_ESHAPE;
   // Nothing is shared where every item is short and has a workgroup. Where a join of one workgroup per row leaves most CUs
   // without work, a row's values are dealt to several.
   p.join = tiles > kAlone || p.items > p.grid;
@@ -641,7 +650,8 @@ hipError_t launch(const Attend& a, const Plan& p, bool accumulate, hipStream_t s
   if (p.join) {
     auto join = p.sliced ? (accumulate ? join_kernel<Act, DT, 32, true> : join_kernel<Act, DT, 32, false>)
                          : (accumulate ? join_kernel<Act, DT, DT, true> : join_kernel<Act, DT, DT, false>);
-    hipLaunchKernelGGL(join, dim3((unsigned)(p.items * p.slot_rows * (p.sliced ? DT / 32 : 1))), dim3(256), 0, s, a);
+    const long long units = p.items * p.slot_rows * (p.sliced ? DT / 32 : 1);
+    hipLaunchKernelGGL(join, dim3((unsigned)(units < kJoins ? units : kJoins)), dim3(256), 0, s, a, (unsigned)units);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (!accumulate) return hipSuccess;
@@ -679,13 +689,14 @@ size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, co
 int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale, int window, int first,
                              int accumulate, void* d_scratch, size_t scratch_bytes, void* stream) {
   if (int e = check(cache, rows, accumulate)) return e;
-  if (window < 0 || first < 0 || !(scale == scale) || !d_scratch || !aligned(d_scratch, 16)) return W4A32_EINVAL;
+  if (window < 0 || first < 0 || !(scale * kLog2e - scale * kLog2e == 0.0f) || !d_scratch || !aligned(d_scratch, 16)) return W4A32_EINVAL;
   Plan p;
   if (int e = plan_of(cache, rows, window, first, accumulate != 0, p)) return e;
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
-  const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows, rows->max_rows, rows->heads,
-                 rows->heads / cache->kv_heads, window, first, p.prompt_rows, p.prompt_log2, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * 1.44269504088896340736f,
+  const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
+                 rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, window, first,
+                 p.prompt_rows, p.prompt_log2, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * kLog2e,
                  (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -63,11 +63,12 @@ __device__ __forceinline__ double exp_neg(double x) {
   return __builtin_amdgcn_ldexp(y, (int)k);
 }
 
-// The same for sums alone, 7e-12 relative: k from the low bits of a sum that has no bits behind the point, 2^f by the Taylor
-// polynomial of degree 9 on |f| <= 1/2, and k added to the exponent. At least 2^-1000 where x is less (-infinity, NaN).
-__device__ __forceinline__ double exp_sum(float l, double c, double offset) {
+// e^((l - top) / t) with c = log2(e) / t, for sums alone, 7e-12 relative: k from the low bits of a sum that has no bits behind the
+// point, 2^f by the Taylor polynomial of degree 9 on |f| <= 1/2, and k added to the exponent. At least 2^-1000 where it is less
+// (-infinity, NaN). The difference first: c l - c top would be off by the rounding of c top, which a low temperature makes large.
+__device__ __forceinline__ double exp_sum(float l, double c, double top) {
   constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52
-  const double y = fmax(__builtin_fma((double)l, c, offset), -1000.0);
+  const double y = fmax(((double)l - top) * c, -1000.0);
   const double t = y + kMagic, f = y - (t - kMagic);
   constexpr double L = 0.69314718055994530942;
   constexpr double c1 = L, c2 = c1 * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6, c7 = c6 * L / 7,
@@ -200,9 +201,9 @@ __global__ __launch_bounds__(256) void stats_kernel(Verify a) {
   }
   double sum = 0.0;
   const double c = a.inv_t * 1.4426950408889634074;
-  const double offset = all == -INFINITY ? 0.0 : -(double)all * c;
+  const double from = all == -INFINITY ? 0.0 : (double)all;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sum += exp_sum(v[i], c, offset);
+  for (int i = 0; i < kEach; ++i) sum += exp_sum(v[i], c, from);
   if (nan || all == INFINITY) sum = (double)NAN;  // no distribution
   sum = all == -INFINITY ? 0.0 : wave_add(sum);
   if (lane == 0) sums[wave] = sum;
@@ -465,7 +466,8 @@ struct Layout {
 bool layout_of(int rows, int vocab, int n_seqs, Layout& l) {
   if (rows < 1 || vocab < 1 || n_seqs < 1 || rows >= 1 << 30 || vocab >= 1 << 30 || n_seqs >= 1 << 30) return false;
   l.segs = (vocab + kSegment - 1) / kSegment;
-  if ((long long)rows * l.segs >= 1ll << 31 || (long long)n_seqs * l.segs >= 1ll << 31) return false;
+  // a launch has less than 2^32 threads: 256 of a row's segment, 512 of a sequence's
+  if ((long long)rows * l.segs >= 1ll << 24 || (long long)n_seqs * l.segs >= 1ll << 23) return false;
   l.q = (size_t)rows * l.segs * sizeof(Part);
   l.left = 2 * l.q;
   l.found = l.left + (size_t)n_seqs * l.segs * sizeof(double);

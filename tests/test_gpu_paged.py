@@ -502,6 +502,20 @@ def test_verify_odd_logits(pkg):
     check_verify(pkg, starts, same, same, tokens, uniform, choice, 1.0)
 
 
+@pytest.mark.parametrize("temperature", [1e-2, 1e-6, 1e-12, 1e-20, 1e-38])
+def test_verify_low_temperatures(pkg, temperature):
+    """All that is left are the largest logits, each as likely as the other"""
+    rng = np.random.default_rng(23)
+    starts, logits, other, tokens, uniform, choice = drafted(rng, [2, 3] * 12, 5000, False)
+    for r in range(len(logits)):
+        at = rng.choice(5000, int(rng.integers(1, 5)), replace=False)
+        logits[r, at] = np.float32(37.3) + r
+        if r + 1 < len(tokens):
+            tokens[r + 1] = rng.choice(at)
+    check_verify(pkg, starts, logits, None, tokens, uniform, choice, temperature)
+    check_verify(pkg, starts, logits, np.roll(logits, 1, 0), tokens, uniform, choice, temperature)
+
+
 def test_verify_of_rows_in_wider_tensors(pkg):
     rng = np.random.default_rng(21)
     starts, logits, other, tokens, uniform, choice = drafted(rng, [3, 1, 4], 1001, True)
@@ -625,3 +639,132 @@ def test_other_streams_and_graphs_at_other_lengths(pkg):
         torch.cuda.synchronize()
         for a, b in zip([*held_out, weight, length, to.k, to.length], want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("act,kind", [("bf16", "bf16"), ("f32", "f16")])
+def test_a_captured_portion_of_prompts(pkg, act, kind):
+    """Buffers for 700 rows of three sequences, of which every replay finds other numbers; the graph and eager calls share their
+    scratch memory in turn."""
+    heads, kv, dim, page = 8, 4, 128, 32
+    B = pm.Batch(29, [700, 700, 700], [0, 0, 0], kv, dim, page)
+    cache, _, _ = on_gpu(pkg, B, kind)
+    q = torch.randn(700, heads * dim, device="cuda").to(torch.bfloat16 if act == "bf16" else torch.float32)
+    starts, out = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    scratch = pkg.op_paged_attention_scratch(cache, 700, 600, heads)
+
+    def step(out):
+        return pkg.op_paged_attention(cache, q, starts, 600, heads, 0.1, scratch=scratch, out=out)
+
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step(out)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(out)
+    for lens, rows in (([100, 0, 30], [600, 99, 1]), ([0, 5, 0], [2, 0, 1]), ([690, 0, 10], [4, 590, 50]), ([0, 0, 0], [0, 0, 0]),
+                       ([100, 0, 30], [600, 99, 1])):
+        starts.copy_(torch.tensor(np.concatenate([[0], np.cumsum(rows)]), dtype=torch.int32))
+        cache.length.copy_(torch.tensor(lens, dtype=torch.int32))
+        want = step(torch.full_like(q, 3.0)).clone()
+        out.fill_(3.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert bool((want[sum(rows):] == 3.0).all()) and not bool((want[:sum(rows)] == 3.0).all(1).any())
+
+
+@pytest.mark.parametrize("rows", [[2, 3], [600, 300]])
+def test_most_rows_of_any_number(pkg, rows):
+    B = pm.Batch(30, [40, 70], rows, 4, 64, 16)
+    fill_new(B)
+    q64, q = held(B.rng.standard_normal((B.total, 8 * 64)), "f32")
+    cache, k64, v64 = on_gpu(pkg, B, "bf16")
+    outs = [pkg.op_paged_attention(cache, q, dev(B.row_start), most, 8, 0.125) for most in (max(rows), 2 ** 31 - 1)]
+    want = pm.attend(B, q64.reshape(-1, 8, 64), k64, v64, 8, 0.125)[0].reshape(B.total, -1)
+    for out in outs:
+        assert np.all(np.abs(out.double().cpu().numpy() - want) <= 1e-5)
+
+
+def test_sequences_that_share_a_prompts_pages(pkg):
+    """Two sequences read the same pages and append to pages of their own, on two streams at once with the same step alone"""
+    heads, kv, dim, page = 8, 2, 64, 16
+    B = pm.Batch(31, [64, 64, 64], [3, 2, 0], kv, dim, page)
+    B.table[1, :4] = B.table[0, :4]
+    fill_new(B)
+    q64, q = held(B.rng.standard_normal((B.total, heads * dim)), "f32")
+    cache, k64, v64 = on_gpu(pkg, B, "f16")
+    want = pm.attend(B, q64.reshape(-1, heads, dim), k64, v64, heads, 0.125)[0].reshape(B.total, -1)
+    starts, outs = dev(B.row_start), [torch.empty_like(q) for _ in range(2)]
+    scratch = [pkg.op_paged_attention_scratch(cache, B.total, 3, heads) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, o, w in zip(streams, outs, scratch):
+            with torch.cuda.stream(s):
+                pkg.op_paged_attention(cache, q, starts, 3, heads, 0.125, scratch=w, out=o)
+    torch.cuda.synchronize()
+    for o in outs:
+        assert np.all(np.abs(o.double().cpu().numpy() - want) <= 1e-5)
+    assert torch.equal(*outs)
+
+
+def test_more_rows_than_the_join_has_workgroups(pkg):
+    """5000 sequences of 4 rows and 64 heads: 1.3 million rows of heads, each shared by several workgroups or not"""
+    n, rows, heads, dim, length = 5000, 4, 64, 8, 150
+    g = torch.Generator(device="cuda").manual_seed(5)
+    pages = (length + rows + 15) // 16
+    k, v = (torch.randn(n * pages, 1, 16, dim, device="cuda", generator=g) for _ in range(2))
+    q = torch.randn(n * rows, heads * dim, device="cuda", generator=g)
+    table = torch.arange(n * pages, dtype=torch.int32, device="cuda").reshape(n, pages)
+    cache = pkg.PagedCache(k, v, table, torch.full((n,), length, dtype=torch.int32, device="cuda"))
+    starts = torch.arange(n + 1, dtype=torch.int32, device="cuda") * rows
+    got = pkg.op_paged_attention(cache, q, starts, rows, heads, 0.3).reshape(n, rows * heads, dim)
+    seen = torch.arange(pages * 16, device="cuda")[None] <= length + torch.arange(rows, device="cuda")[:, None].repeat_interleave(heads, 0)
+    for b in range(0, n, 500):
+        kk, vv, qq = (x.double() for x in (k.reshape(n, -1, dim)[b:b + 500], v.reshape(n, -1, dim)[b:b + 500],
+                                           q.reshape(n, rows * heads, dim)[b:b + 500]))
+        s = torch.matmul(qq, kk.transpose(1, 2).contiguous()) * 0.3
+        want = torch.matmul(torch.softmax(s.masked_fill(~seen, float("-inf")), -1), vv)
+        assert bool(((got[b:b + 500] - want).abs() <= 1e-5).all())
+
+
+def test_refused_tensors(pkg):
+    B = pm.Batch(32, [40], [2], 2, 64, 16)
+    fill_new(B)
+    cache, _, _ = on_gpu(pkg, B, "f32")
+    q, starts = torch.randn(2, 256, device="cuda"), dev(B.row_start)
+    scratch = pkg.op_paged_attention_scratch(cache, 2, 2, 4)
+    good = dict(q=q, row_start=starts, max_rows=2, heads=4, scale=0.1, scratch=scratch)
+    for bad in (dict(q=q.cpu()), dict(q=q.half()), dict(q=q[:, ::2]), dict(q=q[0]), dict(q=q[:, :128]), dict(row_start=starts.long()),
+                dict(row_start=starts.cpu()), dict(row_start=starts[:1]), dict(scratch=scratch.cpu()), dict(scratch=scratch[:64]),
+                dict(window=2 ** 31), dict(first=2 ** 32), dict(window=-1), dict(scale=float("inf")), dict(out=q[:1].clone()),
+                dict(out=torch.empty_like(q).bfloat16()), dict(heads=3), dict(heads=0), dict(max_rows=0)):
+        with pytest.raises((pkg.W4A32Error, IndexError)):
+            pkg.op_paged_attention(cache, **{**good, **bad})
+    pkg.op_paged_attention(cache, **good)
+    k, v, table, length = cache.k, cache.v, cache.table, cache.length
+    for bad in ((k.cpu(), v, table, length), (k, v[:-1], table, length), (k, v.half(), table, length), (k, v, table.long(), length),
+                (k, v, table, length.cpu()), (k, v, table[0], length), (k.double(), v.double(), table, length),
+                (k.transpose(1, 2), v, table, length), (k, v, table, length, torch.zeros(3, device="cuda"))):
+        with pytest.raises(pkg.W4A32Error):
+            pkg.PagedCache(*bad)
+    weight = torch.zeros(k.shape[:3], device="cuda")
+    one = pkg.PagedCache(k, v, table, length, weight)
+    two = pkg.PagedCache(k.clone(), v.clone(), table, length.clone(), weight.clone())
+    for bad in (dict(to=one), dict(to=cache), dict(budget=0), dict(budget=2 ** 31), dict(first=2 ** 32), dict(recent=9),
+                dict(scratch=torch.empty(10 ** 4)), dict(to=pkg.PagedCache(k, v, table, length.clone(), weight.clone()))):
+        with pytest.raises(pkg.W4A32Error):
+            pkg.op_paged_evict(one, **{**dict(to=two, budget=8), **bad})
+    logits, tokens = torch.randn(2, 50, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    u, c = torch.rand(2, device="cuda"), torch.rand(1, device="cuda")
+    good = dict(logits=logits, row_start=starts, max_rows=2, tokens=tokens, uniform=u, choice=c, temperature=1.0)
+    for bad in (dict(logits=logits.half()), dict(logits=logits.t()), dict(tokens=tokens.int()), dict(tokens=tokens[:1]), dict(uniform=None),
+                dict(choice=None), dict(uniform=u.double()), dict(choice=c.cpu()), dict(temperature=-0.5), dict(draft=logits[:, :49]),
+                dict(scratch=torch.empty(10 ** 5)), dict(length=torch.zeros(2, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(pkg.W4A32Error):
+            pkg.op_verify_drafts(**{**good, **bad})
+    count, token = pkg.op_verify_drafts(**{**good, "uniform": None, "choice": None, "temperature": 0.0})
+    assert count.tolist()[0] in (1, 2) and int(token) == int(logits[int(count) - 1].argmax())

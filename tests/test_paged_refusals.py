@@ -28,7 +28,7 @@ BAD_CACHES = [
 BAD_ROWS = [
     (dict(d_row_start=None), EINVAL), (dict(rows=0), EINVAL), (dict(max_rows=0), EINVAL), (dict(heads=0), EINVAL), (dict(heads=3), ESHAPE),
     (dict(ldq=248), EINVAL), (dict(ldo=255), EINVAL), (dict(ldq=260), EINVAL), (dict(d_q=P + 4), EINVAL), (dict(d_out=None), EINVAL),
-    (dict(rows=1 << 30), ESHAPE),
+    (dict(rows=1 << 30), ESHAPE), (dict(rows=1 << 28, max_rows=1), ESHAPE),   # rows * heads
 ]
 
 
@@ -76,7 +76,7 @@ def test_append(pkg, bad, code):
     assert append(pkg, cache(pkg), rows(pkg), **bad) == code
 
 
-@pytest.mark.parametrize("bad", [dict(scale=float("nan")), dict(window=-1), dict(first=-1), dict(scratch=None), dict(scratch=P + 8),
+@pytest.mark.parametrize("bad", [dict(scale=float("nan")), dict(scale=float("-inf")), dict(scale=3e38), dict(window=-1), dict(first=-1), dict(scratch=None), dict(scratch=P + 8),
                                  dict(size=0)])
 def test_attention(pkg, bad):
     assert attend(pkg, cache(pkg), rows(pkg), **bad) == EINVAL
@@ -93,7 +93,7 @@ def test_attention_without_queries_weights_or_room(pkg):
 
 
 def test_evict(pkg):
-    L, c, to = pkg.lib(), cache(pkg), cache(pkg, d_len=P + 64)
+    L, c, to = pkg.lib(), cache(pkg), cache(pkg, d_len=P + 64, d_table=P + 64)
 
     def call(c=c, to=to, budget=16, first=0, recent=0, kept=None, scratch=P, size=1 << 40):
         return L.w4a32_op_paged_evict(ctypes.byref(c), ctypes.byref(to), budget, first, recent, kept, scratch, size, None)
@@ -101,10 +101,16 @@ def test_evict(pkg):
     assert call(budget=0) == EINVAL and call(first=-1) == EINVAL and call(recent=-1) == EINVAL
     assert call(first=10, recent=7) == ESHAPE and call(budget=65) == ESHAPE and call(first=2 ** 31 - 1, recent=2 ** 31 - 1) == ESHAPE
     assert call(scratch=None) == EINVAL and call(size=3 * 2 * 16 * 4 - 1) == EINVAL and call(kept=P + 2) == EINVAL
-    assert call(c=cache(pkg, d_weight=None)) == EINVAL and call(to=cache(pkg, d_len=P + 64, d_weight=None)) == EINVAL
+    assert call(c=cache(pkg, d_weight=None)) == EINVAL and call(to=cache(pkg, d_len=P + 64, d_table=P + 64, d_weight=None)) == EINVAL
     assert call(to=c) == EINVAL   # the lengths of both
+    assert call(to=cache(pkg, d_len=P + 64)) == EINVAL   # the pages of both, one pool of three among them
+    for pool in ("d_k", "d_v", "d_weight"):
+        others = {name: P + 4096 for name in ("d_k", "d_v", "d_weight") if name != pool}
+        assert call(to=cache(pkg, d_len=P + 64, **others)) == EINVAL
+    many = dict(n_seqs=1 << 21, kv_heads=2, table_ld=1)
+    assert call(c=cache(pkg, **many), to=cache(pkg, d_len=P + 64, d_table=P + 64, **many)) == ESHAPE
     for other in (dict(dtype=pkg.CACHE_F16), dict(dim=128), dict(kv_heads=1), dict(n_seqs=2)):
-        assert call(to=cache(pkg, **{"d_len": P + 64, **other})) == ESHAPE
+        assert call(to=cache(pkg, **{"d_len": P + 64, "d_table": P + 64, **other})) == ESHAPE
 
 
 def test_verify(pkg):
@@ -122,5 +128,6 @@ def test_verify(pkg):
                 dict(size=L.w4a32_op_verify_drafts_scratch_bytes(6, 1000, 2) - 1)):
         assert call(**bad) == EINVAL, bad
     assert call(rows=1 << 30) == ESHAPE and call(vocab=1 << 30, ldl=1 << 30, ldd=1 << 30) == ESHAPE
-    for sizes in ((0, 10, 1), (1, 0, 1), (1, 10, 0), (1 << 30, 10, 1), (1 << 20, 1 << 29, 1)):
+    for sizes in ((0, 10, 1), (1, 0, 1), (1, 10, 0), (1 << 30, 10, 1), (1 << 20, 1 << 29, 1), (1 << 20, 4096 * 16, 1),
+                  (1, 4096 * 8, 1 << 20)):
         assert L.w4a32_op_verify_drafts_scratch_bytes(*sizes) == 0
