@@ -34,7 +34,7 @@ constexpr int kAlone = 8;         // tiles of an item that is not shared, where 
 // From kPromptWide workgroups of eight times as many rows on it has those (28 heads on 4, bf16: 512 rows 22 us with either, 2048
 // rows 72 us against 131; f32 rows, two or three terms of each operand, 1024 rows 64 us against 76 in favour of 32 and 2048 rows 164
 // against 147).
-constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideTerms = 160;
+constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideSlow = 160;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kJoins = 1 << 20;   // workgroups of the joining launch, beyond which they take several rows each
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
@@ -453,8 +453,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 template <typename Act, int DT, int kSlice, bool kDump>
 __device__ __forceinline__ void join(const Attend& a, unsigned unit) {
   constexpr int kPer = kSlice / 4, kAtOnce = 256 / kPer;
-  __shared__ __attribute__((aligned(16))) float sums[kAtOnce][kSlice];
-  __shared__ float tops[kAtOnce], totals[kAtOnce];
+  __shared__ __attribute__((aligned(16))) float sums[4][kSlice];
+  __shared__ float tops[4], totals[4];
   const int slice = unit % (DT / kSlice), r = unit / (DT / kSlice) % a.slot_rows;
   const unsigned item = unit / (DT / kSlice) / a.slot_rows;
   const unsigned count = *a.count;
@@ -493,23 +493,36 @@ __device__ __forceinline__ void join(const Attend& a, unsigned unit) {
       acc += f * v[x];
     }
   }
-  *(f32x4*)&sums[mine][threadIdx.x % kPer * 4] = acc;
-  if (threadIdx.x % kPer == 0) {
-    tops[mine] = top;
-    totals[mine] = sum;
+  // the threads of a wavefront that have the same values, by moves, then the wavefronts
+  float most = top;
+#pragma unroll
+  for (int x = kPer; x < 64; x <<= 1) most = fmaxf(most, __shfl_xor(most, x));
+  const float in_wave = pow2(top - (most == -INFINITY ? 0.0f : most));
+  sum *= in_wave;
+  acc *= in_wave;
+#pragma unroll
+  for (int x = kPer; x < 64; x <<= 1) {
+    sum += __shfl_xor(sum, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], x);
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane < kPer) *(f32x4*)&sums[wave][4 * lane] = acc;
+  if (lane == 0) {
+    tops[wave] = most;
+    totals[wave] = sum;
   }
   __syncthreads();
-  if (mine != 0) return;
-  const int n = min(it.shares, kAtOnce);
-  for (int i = 1; i < n; ++i) top = fmaxf(top, tops[i]);
+  if (threadIdx.x >= kPer) return;
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   const float base = top == -INFINITY ? 0.0f : top;
-  float f = pow2(tops[0] - base);
-  acc *= f;
-  sum *= f;
-  for (int i = 1; i < n; ++i) {
-    f = pow2(tops[i] - base);
-    acc += f * *(const f32x4*)&sums[i][threadIdx.x % kPer * 4];
-    sum += f * totals[i];
+  sum = 0.0f;
+  acc = f32x4{0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = pow2(tops[w] - base);
+    acc += f * *(const f32x4*)&sums[w][4 * lane];
+    sum += f * totals[w];
   }
   finish<Act, kDump>(a, it.r0, it.row0 + r, it.head, (size_t)item * a.slot_rows + r, d, acc, base, sum);
 }
@@ -587,7 +600,7 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
   auto blocks = [&](int log2) { return ((long long)r->rows * group / (1 << log2) + c->n_seqs) * c->kv_heads; };
   const int wide = p.dt == 256 ? 7 : 8;
-  p.prompt_log2 = blocks(wide) >= (r->act_bf16 ? kPromptWide : kPromptWideTerms) ? wide : 5;
+  p.prompt_log2 = blocks(wide) >= (r->act_bf16 && p.dt <= 128 ? kPromptWide : kPromptWideSlow) ? wide : 5;
   p.prompts = blocks(p.prompt_log2);
   p.prompt_rows = 0;
   p.others = true;
