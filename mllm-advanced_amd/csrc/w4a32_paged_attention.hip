@@ -35,6 +35,10 @@ constexpr int kAlone = 8;         // tiles of an item that is not shared, where 
 // rows 72 us against 131; f32 rows, two or three terms of each operand, 1024 rows 64 us against 76 in favour of 32 and 2048 rows 164
 // against 147).
 constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideSlow = 160;
+// Sequences of fewer rows are its too where a row has at most kPromptKeys keys: it goes through 2560 of them in 33 us with 32 rows
+// of a workgroup and in 50 with more (4096: 54 and 80), beside the others, where the rows' two launches take 9 us for nothing and 17
+// for a row of 4096 (256 + 1 rows, the latter on 4096 keys: 48 us against 30; 1024 + 1: 88 against 56).
+constexpr int kPromptKeys = 2560;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kJoins = 1 << 20;   // workgroups of the joining launch, beyond which they take several rows each
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
@@ -602,16 +606,19 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   const int wide = p.dt == 256 ? 7 : 8;
   p.prompt_log2 = blocks(wide) >= (r->act_bf16 && p.dt <= 128 ? kPromptWide : kPromptWideSlow) ? wide : 5;
   p.prompts = blocks(p.prompt_log2);
+  long long keys = cap;  // that a row can see
+  if (window) {
+    const long long near = (long long)first + window;
+    keys = near < cap ? near : cap;
+  }
   p.prompt_rows = 0;
   p.others = true;
   if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && blocks(5) >= kPromptLeast) {
-    // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then. Else the rows'
-    // kernel has what is left, of so few rows.
-    const bool ragged = r->rows < (long long)r->max_rows * c->n_seqs;
-    p.prompt_rows = ragged ? kPromptRows : 1;
-    most = (kPromptRows - 1) / group;
-    p.others = ragged && most > 0;
-    if (!p.others) most = 1;
+    // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then, as where few
+    // keys are what a row has to go through. Else the rows' kernel has what is left, of so few rows.
+    p.others = r->rows < (long long)r->max_rows * c->n_seqs && keys > kPromptKeys && (kPromptRows - 1) / group > 0;
+    p.prompt_rows = p.others ? kPromptRows : 1;
+    most = p.others ? (kPromptRows - 1) / group : 1;
     if (p.prompts > most_groups(512)) return W4A32_ESHAPE;
   }
   // 32 or 64 rows of an item are two or four wavefronts' that ask for the same keys at about the same time: the caches serve

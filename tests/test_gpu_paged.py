@@ -123,6 +123,20 @@ def test_prompts(pkg, act, kind, heads, kv, dim, page, lens, rows, window, first
 
 
 @pytest.mark.parametrize("act,kind", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,page,lens,rows,window,first", [
+    # rows of one token and prompts where the table has room for so many tokens that they are two kernels'
+    (14, 2, 64, 16, [33, 2600, 5, 0], [700, 3, 1, 450], 0, 0),
+    (8, 8, 128, 32, [0, 70] + [9] * 40, [300, 401] + [2] * 40, 0, 0),
+    (16, 8, 80, 64, [100, 0, 2800], [257, 333, 1], 2700, 5),
+    (8, 8, 256, 16, [31, 200], [700, 5], 0, 0),
+])
+def test_prompts_beside_few_rows_on_long_tables(pkg, act, kind, heads, kv, dim, page, lens, rows, window, first):
+    B = pm.Batch(33, lens, rows, kv, dim, page, table_ld=3200 // page)
+    fill_new(B)
+    run_attention(pkg, B, act, kind, heads, window, first, pad_rows=3, stride=16)
+
+
+@pytest.mark.parametrize("act,kind", TYPES)
 @pytest.mark.parametrize("many", [0, 20])
 def test_prompts_with_missing_pages_and_odd_values(pkg, act, kind, many):
     many = many * [3]
