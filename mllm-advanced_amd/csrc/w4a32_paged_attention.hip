@@ -622,13 +622,17 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
     if (p.prompts > most_groups(512)) return W4A32_ESHAPE;
   }
   // 32 or 64 rows of an item are two or four wavefronts' that ask for the same keys at about the same time: the caches serve
-  // all but the first, where as items of their own each would have the keys from memory again
-  p.wide = most * group <= kRows ? 1 : most * group <= 2 * kRows ? 2 : 4;
-  const long long of_item = kRows * p.wide;
-  p.slot_rows = (int)(most * group < of_item ? most * group : of_item);
-  const long long by_seq = (most * group + of_item - 1) / of_item * c->n_seqs, by_rows = (long long)r->rows * group / of_item + c->n_seqs;
-  p.items = (by_seq < by_rows ? by_seq : by_rows) * c->kv_heads;
+  // all but the first, where as items of their own each would have the keys from memory again. But then fewer of a workgroup's
+  // wavefronts share its tiles, so not where there are too few tiles to give every workgroup kMinTiles (16 + 5 rows of 11 heads on
+  // 160 tokens: 18 us with 64 rows of an item, 10 with 16).
   long long tiles = (cap + kt - 1) / kt;
+  for (p.wide = most * group <= kRows ? 1 : most * group <= 2 * kRows ? 2 : 4;; p.wide /= 2) {
+    const long long of_item = kRows * p.wide, by_seq = (most * group + of_item - 1) / of_item * c->n_seqs,
+                    by_rows = (long long)r->rows * group / of_item + c->n_seqs;
+    p.items = (by_seq < by_rows ? by_seq : by_rows) * c->kv_heads;
+    p.slot_rows = (int)(most * group < of_item ? most * group : of_item);
+    if (p.wide == 1 || p.items * tiles >= kGrid * kMinTiles) break;
+  }
   if (window) {
     const long long near = ((long long)first + kt - 1) / kt + (window + most) / kt + 2;
     tiles = near < tiles ? near : tiles;

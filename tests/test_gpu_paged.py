@@ -100,6 +100,21 @@ def test_attention(pkg, act, kind, heads, kv, dim, page, lens, rows):
 
 
 @pytest.mark.parametrize("act,kind", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,page,lens,rows", [
+    (14, 2, 128, 32, [5, 31, 300, 33, 0, 64], [1, 4, 3, 1, 2, 0]),   # up to 28 rows of a kv head: two wavefronts'
+    (12, 2, 64, 16, [70, 9, 400], [9, 2, 17]),                      # four
+    (34, 2, 72, 32, [70, 9], [2, 1]),
+    (4, 2, 256, 128, [130, 17, 255], [1, 14, 1]),
+])
+def test_attention_on_a_long_table(pkg, act, kind, heads, kv, dim, page, lens, rows):
+    """Room for so many tokens that a workgroup has 32 or 64 rows"""
+    B = pm.Batch(34, lens, rows, kv, dim, page, table_ld=65536 // page, weights=True)
+    fill_new(B)
+    run_attention(pkg, B, act, kind, heads)
+    run_attention(pkg, B, act, kind, heads, window=60, first=3, accumulate=True)
+
+
+@pytest.mark.parametrize("act,kind", TYPES)
 @pytest.mark.parametrize("heads,kv,dim,page,lens,rows,window,first", [
     # few workgroups, so of 32 rows: all sequences alike; beside sequences that are not the prompts' kernel's; odd sizes, windows
     (8, 8, 128, 32, [0, 70], [600, 601], 0, 0),
