@@ -27,6 +27,8 @@ struct Attend {
   void* out;
   const int* row_start;
   int ldq, ldo, rows, max_rows, heads, group;
+  unsigned group_mul;   // by_group()
+  int group_shift;
   int window, first;
   int prompt_rows;      // (token, head of the group) pairs from which on a sequence is the prompts' kernel's; 0: none is
   int prompt_log2;      // log2 of the rows of a workgroup of that kernel: 8 (7 of 256 dims), or 5 where there are few
@@ -41,6 +43,16 @@ struct Attend {
   float* lse;           // [item][slot_rows] (accumulate)
   float* dump;          // [tile of an item][wide][lane][keys of the tile / 4]: scores (accumulate)
 };
+
+// x / group for x below 2^30, as x m / 2^(30 + l) with 2^l >= group > 2^(l - 1) and m the next whole number from 2^(30 + l) / group:
+// m is off by less than 1, the quotient by less than 2^-l, and group is at most 2^l. A division takes the compiler 30 instructions.
+inline void set_group(Attend& a) {
+  int l = 0;
+  while ((1ll << l) < a.group) ++l;
+  a.group_shift = 30 + l;
+  a.group_mul = (unsigned)(((1ull << (30 + l)) + a.group - 1) / a.group);
+}
+__device__ __forceinline__ int by_group(const Attend& a, int x) { return (int)((u64)(unsigned)x * a.group_mul >> a.group_shift); }
 
 // The keys that a sequence's rows can see, in tiles: [0, ft) of the first tokens, then [w0, w0 + nt - ft).
 struct Seq {
@@ -281,7 +293,7 @@ template <typename Act, bool kDump>
 __device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, size_t lse_at, int d, f32x4 acc, float base, float sum) {
   if (d < a.c.dim) {
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int j = (int)((unsigned)of / (unsigned)a.group);
+    const int j = by_group(a, of);
     const size_t at = (size_t)(r0 + j) * a.ldo + (size_t)(hk * a.group + of - j * a.group) * a.c.dim;
     store4<Act>(a.out, at + d, acc * inv);
   }

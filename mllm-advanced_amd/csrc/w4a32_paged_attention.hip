@@ -114,7 +114,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     const Span s = p.q.s;
     // the item (of the sequence), the tiles of this share, the workgroups that share the item
     int item, t_lo, t_hi, w_first, shares;
-    if (deal.apart) {
+    if (deal.apart && p.q.nt <= (int)deal.per) {
+      shares = 1;
+      item = (int)p.inner;
+      t_lo = 0;
+      t_hi = p.q.nt;
+      w_first = (int)blockIdx.x;
+    } else if (deal.apart) {
       shares = (int)((p.q.nt + deal.per - 1) / deal.per);
       item = (int)(p.inner / (unsigned)shares);
       const int mine = (int)p.inner - item * shares;
@@ -129,14 +135,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       w_first = (int)(begin / deal.per);
       shares = (int)((begin + p.q.nt - 1) / deal.per) - w_first + 1;
     }
-    const unsigned group = a.group;
-    const int hk = (int)((unsigned)item / (unsigned)p.q.items), of0 = (item - hk * p.q.items) * (kRows << a.wide);
+    const int hk = p.q.items == 1 ? item : (int)((unsigned)item / (unsigned)p.q.items), of0 = (item - hk * p.q.items) * (kRows << a.wide);
     // this lane's query row, and the rows of its wavefront
     const int all_rows = s.n * a.group, row0 = of0 + (wave & (wide - 1)) * kRows;
     const int in_seq = row0 + row;
     const bool real = in_seq < all_rows, busy = row0 < all_rows;
-    const int j = (int)((unsigned)min(in_seq, all_rows - 1) / group), head = hk * a.group + (real ? in_seq - j * a.group : 0);
-    const int j_min = (int)((unsigned)min(row0, all_rows - 1) / group), j_max = (int)((unsigned)min(row0 + kRows - 1, all_rows - 1) / group);
+    const int j = by_group(a, min(in_seq, all_rows - 1)), head = hk * a.group + (real ? in_seq - j * a.group : 0);
+    const int j_min = by_group(a, min(row0, all_rows - 1)), j_max = by_group(a, min(row0 + kRows - 1, all_rows - 1));
     const int pos = min(s.len + j, a.c.cap - 1);
     const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
 
@@ -718,11 +723,12 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
   if (int e = plan_of(cache, rows, window, first, accumulate != 0, p)) return e;
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
-  const Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
-                 rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, window, first,
+  Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
+                 rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, window, first,
                  p.prompt_rows, p.prompt_log2, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * kLog2e,
                  (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
+  set_group(a);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool acc = accumulate != 0;
   if (p.prompt_rows)

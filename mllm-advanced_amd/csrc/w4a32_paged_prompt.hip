@@ -129,8 +129,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
   const Span s = p.q.s;
   const int all_rows = s.n * (int)group, of0 = block * kBlock, row0 = of0 + 32 * member, in_seq = row0 + row;
   const bool real = in_seq < all_rows;
-  auto slot_of = [&](int r) { return min(s.len + (int)((unsigned)min(r, all_rows - 1) / group), a.c.cap - 1); };
-  const int j = (int)((unsigned)min(in_seq, all_rows - 1) / group), head = hk * a.group + (real ? in_seq - j * a.group : 0);
+  auto slot_of = [&](int r) { return min(s.len + by_group(a, min(r, all_rows - 1)), a.c.cap - 1); };
+  const int j = by_group(a, min(in_seq, all_rows - 1)), head = hk * a.group + (real ? in_seq - j * a.group : 0);
   const int pos = min(s.len + j, a.c.cap - 1), pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
   const int block_min = slot_of(of0), block_max = slot_of(of0 + kBlock - 1);
   // tiles that the workgroup's rows can see: [0, ft) and [w0, ..)
