@@ -72,6 +72,19 @@ __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
 }
 
 
+// Of a sequence's tiles those that a wavefront's rows, which stand from lo to hi, can see: [0, firsts), which have the first tokens, and
+// [from, to). The others are dealt like these but passed over (256 dims in f32, 850 rows that see 94 tokens each: 101 us against 253
+// with all of them gone through).
+struct Sight {
+  int firsts, from, to;
+  __device__ __forceinline__ bool skips(int t) const { return t >= firsts && t < from; }
+};
+template <int KT>
+__device__ __forceinline__ Sight sight_of(const Attend& a, const Seq& q, int lo, int hi) {
+  if (a.window == 0) return {0, 0, hi / KT + 1};
+  return {(min(a.first, a.c.cap) + KT - 1) / KT, q.ft + max(0, lo - a.window + 1) / KT - q.w0, q.ft + hi / KT - q.w0 + 1};
+}
+
 template <typename KV>
 constexpr int tile_keys() { return sizeof(KV) == 2 ? 32 : 16; }
 template <typename KV, int DT>
@@ -196,9 +209,12 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     // Lane h has the page of half h of a tile (-1: not there). It is asked for a tile ahead of the loads that need it, and in front
     // of the loads of the tile between: loads return in order, and behind these it would take as long as all of them.
     int pages = -1;
+    const Sight sight = sight_of<KT>(a, p.q, pos_min, pos_max);
+    const int t_end = busy ? min(t_hi, sight.to) : 0;
+    auto seen_from = [&](int t) { return sight.skips(t) ? t + ((sight.from - t + streams - 1) & -streams) : t; };
     auto find = [&](int t) {
       const int i = (key_of(t) + 16 * min(lane, kHalves - 1)) >> a.c.shift;
-      pages = t < t_hi && i < a.c.table_ld ? table[i] : -1;
+      pages = t < t_end && i < a.c.table_ld ? table[i] : -1;
     };
 
     Raw kr[kHalves][kSteps], vr[kVLoads];
@@ -209,7 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         const int pg = __builtin_amdgcn_readlane(pages, h);
         page[h] = page_there(a.c, pg) ? pg : -1;
       }
-      find(t + streams);
+      find(seen_from(t + streams));
     };
     auto load_k = [&](int t) {
 #pragma unroll
@@ -240,14 +256,15 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     float m = -INFINITY, l = 0.0f;
     bool odd = false;  // values that are not finite, in a tile that not every row sees whole
 
-    int t = busy ? t_lo + stream : t_hi;
+    int t = seen_from(t_lo + stream);
     find(t);
-    if (t < t_hi) {
+    if (t < t_end) {
       turn(t);
       load_k(t);
       load_v(t);
     }
-    for (; t < t_hi; t += streams) {
+    for (int next; t < t_end; t = next) {
+      next = seen_from(t + streams);
       const int k0 = key_of(t);
       bool there = true;
       int cur[kHalves];
@@ -308,10 +325,10 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
           }
         }
       }
-      if (t + streams < t_hi) {
-        turn(t + streams);
-        load_k(t + streams);
-        load_v(t + streams);
+      if (next < t_end) {
+        turn(next);
+        load_k(next);
+        load_v(next);
       }
       uint32_t seen = 0xff;  // bit 4 h + i: key 16 h + 4 grp + i
       if (!whole) {
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 
     if (odd) {
 #pragma unroll 1
-      for (t = t_lo + stream; t < t_hi; t += streams) {
+      for (t = seen_from(t_lo + stream); t < t_end; t = seen_from(t + streams)) {
 #pragma unroll 1
         for (int k = 0; k < KT; ++k) {
           const int k0 = key_of(t), key = k0 + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
@@ -559,8 +576,12 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   for (int i = 0; i < p.q.items << a.wide; ++i) {
     const int item = hk * p.q.items + (i >> a.wide), rt = i & ((1 << a.wide) - 1), r = rt * kRows + row;
     const u64 tile = (u64)p.tile0 + (u64)item * p.q.nt + t;
-    if (i * kRows >= p.q.s.n * a.group) break;
-    const bool real = i * kRows + row < p.q.s.n * a.group;
+    const int all_rows = p.q.s.n * a.group, row0 = i * kRows;
+    if (row0 >= all_rows) break;
+    const int lo = min(p.q.s.len + by_group(a, row0), a.c.cap - 1), hi = min(p.q.s.len + by_group(a, min(row0 + kRows, all_rows) - 1), a.c.cap - 1);
+    const Sight sight = sight_of<KT>(a, p.q, lo, hi);
+    if (t >= sight.to || sight.skips(t)) continue;
+    const bool real = row0 + row < all_rows;
     const float lse = real ? a.lse[((size_t)p.item0 + item) * a.slot_rows + r] : INFINITY;
     const float* from = a.dump + (((tile << a.wide) + rt) * 64 + lane) * (4 * kHalves);
 #pragma unroll
