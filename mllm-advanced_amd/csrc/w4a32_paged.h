@@ -49,11 +49,5 @@ __device__ __forceinline__ size_t slot_row(const Cache& c, int page, int head, i
 }
 __device__ __forceinline__ bool page_there(const Cache& c, int page) { return (unsigned)page < (unsigned)c.n_pages; }
 
-__device__ __forceinline__ float bf16_round(float x, uint32_t& bits) {  // to nearest even; NaN stays NaN
-  const __bf16 h = (__bf16)x;
-  bits = __builtin_bit_cast(unsigned short, h);
-  return (float)h;
-}
-
 }  // namespace paged
 }  // namespace w4

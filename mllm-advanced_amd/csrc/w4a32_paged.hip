@@ -26,7 +26,8 @@ int check_rows(const w4a32_paged_cache* c, const w4a32_paged_rows* r) {
   if (int e = check_cache(c)) return e;
   if (!r || !r->d_row_start || r->rows < 1 || r->max_rows < 1 || r->heads < 1) return W4A32_EINVAL;
   if (!aligned(r->d_row_start, 4) || !aligned(r->d_q, 16) || !aligned(r->d_out, 16)) return W4A32_EINVAL;
-  if (r->rows >= kMost || r->heads >= kMost / c->dim || (long long)r->rows * r->heads >= kMost || r->heads % c->kv_heads) return W4A32_ESHAPE;
+  if (r->rows >= kMost || r->heads >= kMost / c->dim || (long long)r->rows * r->heads >= kMost) return W4A32_ESHAPE;
+  if (r->heads % c->kv_heads) return W4A32_ESHAPE;
   if (r->act_bf16 && c->dtype != W4A32_CACHE_BF16) return W4A32_ENOTSUP;
   if (r->d_q && (!r->d_out || r->ldq < r->heads * c->dim || r->ldo < r->heads * c->dim || r->ldq % 8 || r->ldo % 8)) return W4A32_EINVAL;
   return W4A32_OK;
@@ -40,7 +41,8 @@ Cache view(const w4a32_paged_cache* c) {
 // ---------------------------------------------------------------------------------------------
 // Append. A thread takes eight elements of one head of one row: four pairs (i, i + rot / 2) to be turned, or eight
 // elements that stay. Everything is read and written once; a step of few rows is bound by its chain of dependent loads
-// (row starts, length, page number) and prompts by memory.
+// (row starts, length, page number) and prompts by memory. 64 rows of 28 + 4 + 4 heads of 128 dims in bf16: 3.3 us; 3000 rows of
+// 12 + 2 + 2 heads, f32 kept as f16 (75 MB): 13 us, 5.8 TB/s of the memory and the cache in front of it.
 // ---------------------------------------------------------------------------------------------
 struct Append {
   Cache c;
@@ -153,8 +155,10 @@ __global__ __launch_bounds__(256) void append_kernel(Append a, int blocks_per_ro
 // Eviction. One workgroup per (sequence, kv head) finds the weight of the last token that stays, 12, 10 and 10 bits of its
 // order-preserving key at a time (a histogram in LDS each: 12 first, so that weights of similar size, which have few exponents,
 // do not all count in the same place), and lists the slots that stay in order; a second launch copies. Up to kHeld keys lie in
-// LDS; beyond them every pass has the weights from memory. The selection is all latency, the copy all memory. (The first and the
-// last tokens copied by other workgroups of the first launch took as much longer there as the second took less.)
+// LDS; beyond them every pass has the weights from memory. The selection is all latency, the copy all memory: 32 sequences of 1500
+// to 9000 tokens, 4 heads of 128 dims in bf16, to 2048 each: 17 and 50 us, the latter 268 MB at 5.4 TB/s; one of 4099, 2 heads in f32,
+// to 1024: 9.9 and 4.4 us. (The first and the last tokens copied by other workgroups of the first launch took as much longer
+// there as the second took less.)
 // ---------------------------------------------------------------------------------------------
 struct Evict {
   Cache c, to;

@@ -17,6 +17,11 @@
 //                   B = the softmaxed S^T as it lies in the registers: lane group g holds keys 4 g .. 4 g + 3 of a half
 // The matrix instruction's 16 columns are what a group of 6 or 7 heads needs; a kv head with one query head uses one of 16,
 // which costs no time: a 16-bit tile of head size 128 is 16 kilobytes for 16 to 48 instructions of 16 clocks.
+//
+// What bounds it: memory where contexts are long: one row each of 64 sequences of 500 to 8000 tokens, 28 heads on 4 of 128 dims in
+// bf16 (559 MB): 108 us, 5.2 TB/s, and 5 for the join; one row on 131001 tokens, 12 heads on 2, f32 on f16 (134 MB): 27 us, 4.9 TB/s,
+// and 6. Below that a chain of waits: one row on 60 tokens takes 7.3 us, of which 1.4 are the launch, 0.6 the deal, 1.6 the
+// place and q, 0.6 the keys and values, 1.9 the tile and 1.5 the wavefronts' join and the store.
 #include "w4a32_paged_attention.h"
 
 namespace w4 {
@@ -26,7 +31,9 @@ namespace {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_ELAUNCH; }
 
-constexpr int kGrid = 512;        // workgroups that a batch is dealt to: two per CU, all there at once
+// Workgroups that a batch is dealt to: two per CU, all there at once. (256 of eight wavefronts: one row on 200 tokens 14.2 us against
+// 12.3, one on 131001 34.9 against 32.9, 64 sequences 116 against 114, 16 of drafted tokens 30.8 against 31.7.)
+constexpr int kGrid = 512;
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
 constexpr int kAlone = 8;         // tiles of an item that is not shared, where there are workgroups enough for all items
 // The prompts' kernel takes sequences of at least kPromptRows pairs of token and head, where it has kPromptLeast workgroups of 32
@@ -110,7 +117,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   float* states = (float*)(lds + kWaves * wave_lds<KV, DT>());
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, grp = lane >> 4, dim = a.c.dim;
-  const int streams = kWaves >> a.wide, stream = wave >> a.wide, wide = 1 << a.wide;  // wavefronts that share rows, and which of them this one is
+  // wavefronts that share rows, and which of them this one is
+  const int streams = kWaves >> a.wide, stream = wave >> a.wide, wide = 1 << a.wide;
 
   Seqs<KT> seqs;
   const Deal deal = deal_of<KT>(a, seqs);
@@ -560,7 +568,9 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a, unsigned units) {
   }
 }
 
-// Adds the weights of a tile's keys up: a wavefront per tile of a kv head, over its items in order.
+// Adds the weights of a tile's keys up: a wavefront per tile of a kv head, over its items in order. It reads the scores that the
+// rows' kernel left, 64 bytes a key and 16 rows: an eighth of the key itself with 128 dims of 16 bits (16 sequences of 300 to
+// 4100 tokens, 2 to 5 rows of 12 heads on 2: 7 us of 32).
 template <typename KV>
 __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
@@ -578,8 +588,8 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
     const u64 tile = (u64)p.tile0 + (u64)item * p.q.nt + t;
     const int all_rows = p.q.s.n * a.group, row0 = i * kRows;
     if (row0 >= all_rows) break;
-    const int lo = min(p.q.s.len + by_group(a, row0), a.c.cap - 1), hi = min(p.q.s.len + by_group(a, min(row0 + kRows, all_rows) - 1), a.c.cap - 1);
-    const Sight sight = sight_of<KT>(a, p.q, lo, hi);
+    auto slot_of = [&](int r) { return min(p.q.s.len + by_group(a, r), a.c.cap - 1); };
+    const Sight sight = sight_of<KT>(a, p.q, slot_of(row0), slot_of(min(row0 + kRows, all_rows) - 1));
     if (t >= sight.to || sight.skips(t)) continue;
     const bool real = row0 + row < all_rows;
     const float lse = real ? a.lse[((size_t)p.item0 + item) * a.slot_rows + r] : INFINITY;
@@ -666,7 +676,8 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   p.tiles = p.items * tiles;
   p.grid = p.tiles < kGrid ? p.tiles : kGrid;
   p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
-  if (p.tiles >= (1ll << 31) || p.items * p.slot_rows >= kMost || (accumulate && p.key_groups > most_groups(64 * kWaves))) return W4A32_ESHAPE;
+  if (p.tiles >= (1ll << 31) || p.items * p.slot_rows >= kMost) return W4A32_ESHAPE;
+  if (accumulate && p.key_groups > most_groups(64 * kWaves)) return W4A32_ESHAPE;
   // Nothing is shared where every item is short and has a workgroup. Where a join of one workgroup per row leaves most CUs
   // without work, a row's values are dealt to several.
   p.join = tiles > kAlone || p.items > p.grid;

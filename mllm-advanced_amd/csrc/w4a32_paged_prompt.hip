@@ -205,7 +205,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     v_at[x] = (unsigned)(r * dim + 8 * v_from) * 2;
   }
   auto block_of = [&](int i) { return i * kRowsAtOnce / 16 + (kRowsAtOnce > 16 ? __builtin_amdgcn_readfirstlane(wave_row) / 16 : 0); };
-  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + __builtin_amdgcn_readfirstlane(team) * (unsigned)Sh::kTeam;
+  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds +
+                        __builtin_amdgcn_readfirstlane(team) * (unsigned)Sh::kTeam;
   uint16_t* tiles = (uint16_t*)(lds + team * Sh::kTeam);
   // The team's n-th tile, t, to its buffer n & 1; returns the sixteens of keys whose page is not there.
   auto load = [&](int t, int n) {
@@ -330,7 +331,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int key = first_key + 32 * u + 8 * (i / 4) + i % 4;
-            const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !(gone_here >> (2 * u + i / 8) & 1);
+            const bool gone_key = gone_here >> (2 * u + i / 8) & 1;
+            const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !gone_key;
             sc[u][i] = sees ? sc[u][i] : -INFINITY;
           }
       }
@@ -430,7 +432,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     for (int d = 0; d < kDims; ++d)
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        *(f32x4*)(sums + row * Sh::kSums + 32 * d + 8 * b + 4 * half) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+        *(f32x4*)(sums + row * Sh::kSums + 32 * d + 8 * b + 4 * half) =
+            f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
     if (half == 0) {
       states[(team * 32 + row) * 2] = m;
       states[(team * 32 + row) * 2 + 1] = l;
