@@ -12,6 +12,7 @@ constexpr int kRows = 16;         // query rows of a wavefront
 constexpr int kWaves = 4;         // wavefronts of a workgroup
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef unsigned long long u64;
 
@@ -257,6 +258,11 @@ template <>
 struct Math<float, float> {
   static constexpr int kTerms = 1;
   static constexpr int kScale = 0;
+  typedef f8 V8;
+  static __device__ __forceinline__ void split(const float (&x)[8], V8 (&t)[kTerms]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[0][i] = x[i];
+  }
   static __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
   static constexpr uint32_t kSize = 0x7fffffffu, kStep = 0x00800000u;
   static __device__ __forceinline__ uint32_t finite(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u ? 0u : w; }

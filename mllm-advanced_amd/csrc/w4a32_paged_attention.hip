@@ -39,13 +39,15 @@ constexpr int kAlone = 8;         // tiles of an item that is not shared, where 
 // The prompts' kernel takes sequences of at least kPromptRows pairs of token and head, where it has kPromptLeast workgroups of 32
 // rows or more: it does not share a row's keys between workgroups, and few of them on a long context would leave the chip idle.
 // From kPromptWide workgroups of eight times as many rows on it has those (28 heads on 4, bf16: 512 rows 22 us with either, 2048
-// rows 72 us against 131; f32 rows, two or three terms of each operand, 1024 rows 64 us against 76 in favour of 32 and 2048 rows 164
-// against 147).
+// rows 72 us against 131); from kPromptWideSlow on with f32 rows, two or three terms of each operand (1024 rows 64 us against 76 in favour of
+// 32, 2048 rows 164 against 147), and with 256 dims (16 heads on 4, bf16: 1024 rows 57 against 63, 2048 rows 167 against 115).
+// With an f32 cache and 128 or 256 dims it takes none below that (12 heads on 2: 1000 rows 148 us against 116 of the rows' kernel and its
+// join, 2000 rows 287 against 358).
 constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideSlow = 160;
 // Sequences of fewer rows are its too where a row has at most kPromptKeys keys: it goes through 2560 of them in 33 us with 32 rows
 // of a workgroup and in 50 with more (4096: 54 and 80), beside the others, where the rows' two launches take 9 us for nothing and 17
 // for a row of 4096 (256 + 1 rows, the latter on 4096 keys: 48 us against 30; 1024 + 1: 88 against 56).
-constexpr int kPromptKeys = 2560;
+constexpr int kPromptKeys = 2560, kPromptKeysF32 = 512;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kJoins = 1 << 20;   // workgroups of the joining launch, beyond which they take several rows each
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
@@ -639,8 +641,10 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
   p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
   auto blocks = [&](int log2) { return ((long long)r->rows * group / (1 << log2) + c->n_seqs) * c->kv_heads; };
-  const int wide = p.dt == 256 ? 7 : 8;
-  p.prompt_log2 = blocks(wide) >= (r->act_bf16 && p.dt <= 128 ? kPromptWide : kPromptWideSlow) ? wide : 5;
+  const bool f32 = c->dtype == W4A32_CACHE_F32;
+  const int wide = p.dt == 256 || f32 ? 7 : 8;
+  const int from = r->act_bf16 && p.dt <= 128 ? kPromptWide : kPromptWideSlow;
+  p.prompt_log2 = (f32 ? p.dt != 64 : blocks(wide) >= from) ? wide : 5;
   p.prompts = blocks(p.prompt_log2);
   long long keys = cap;  // that a row can see
   if (window) {
@@ -649,10 +653,10 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   }
   p.prompt_rows = 0;
   p.others = true;
-  if (!accumulate && c->dtype != W4A32_CACHE_F32 && most * group >= kPromptRows && blocks(5) >= kPromptLeast) {
+  if (!accumulate && most * group >= kPromptRows && (f32 && p.dt != 64 ? blocks(wide) >= from : blocks(5) >= kPromptLeast)) {
     // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then, as where few
     // keys are what a row has to go through. Else the rows' kernel has what is left, of so few rows.
-    p.others = r->rows < (long long)r->max_rows * c->n_seqs && keys > kPromptKeys && (kPromptRows - 1) / group > 0;
+    p.others = r->rows < (long long)r->max_rows * c->n_seqs && keys > (f32 ? kPromptKeysF32 : kPromptKeys) && (kPromptRows - 1) / group > 0;
     p.prompt_rows = p.others ? kPromptRows : 1;
     most = p.others ? (kPromptRows - 1) / group : 1;
     if (p.prompts > most_groups(512)) return W4A32_ESHAPE;

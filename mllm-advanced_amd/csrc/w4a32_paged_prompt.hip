@@ -1,5 +1,5 @@
-// Attention of prompts over a paged cache of 16-bit elements: the sequences of a batch that have so many rows that products bound
-// them and not the cache.
+// Attention of prompts over a paged cache: the sequences of a batch that have so many rows that products bound them and not the
+// cache.
 //
 // A workgroup has 256 query rows of one kv head (pairs of token and head of the group, 32 to a wavefront; 128 where a head has 256
 // dims) and takes the keys that they can see through LDS, in tiles of 128 (64 of 256 dims): the next tile goes from memory
@@ -24,6 +24,10 @@
 // come first.
 // Where there are few such workgroups, one has 32 rows instead, and each of its four wavefronts (two where the head has 256 dims)
 // takes every fourth tile by itself, with no barrier; their softmax states are joined through LDS at the end.
+// An f32 cache has tiles of 32 keys and v_mfma_f32_32x32x2, to which a lane gives one element of K or V: a tile of 128 dims
+// costs a SIMD 128 x 64 = 8192 clocks per wavefront, beside which the rest is small (4096 rows, 28 heads on 4: 0.97 ms, 124 TFLOP/s, where
+// the rows' kernel takes 3.15). 64 dims are always taken in the second way (2600 rows of 14 heads: 179 us against 237), 128 and 256, for
+// which LDS has not the room, always in the first, with 128 rows of a workgroup.
 #include "w4a32_paged_attention.h"
 
 namespace w4 {
@@ -35,25 +39,32 @@ constexpr int kSlack = 8;
 
 __device__ __forceinline__ f32x16 mfma32(bf8 a, bf8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma32(h8 a, h8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 mfma32(f8 a, f8 b, f32x16 c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = mfma32(a[i], b[i], c);
+  return c;
+}
 
 // A team of kMembers wavefronts shares tiles and has 32 rows of each; with kSplit a workgroup has several teams, of one wavefront
 // each, on the same rows.
 template <typename Act, typename KV, int DT, bool kSplit>
 struct Shape {
   static constexpr int kTerms = Math<Act, KV>::kTerms;
-  static constexpr int kMembers = kSplit ? 1 : DT == 256 ? 4 : 8, kTeams = !kSplit ? 1 : DT == 256 ? 2 : 4;
+  static constexpr bool k32 = sizeof(KV) == 4;
+  static constexpr int kMembers = kSplit ? 1 : DT == 256 || k32 ? 4 : 8, kTeams = !kSplit ? 1 : DT == 256 ? 2 : 4;
   static constexpr int kThreads = 64 * kMembers * kTeams;
-  static constexpr int kKeys = kSplit ? 32 : DT == 256 ? 64 : 128;         // of a tile
-  static constexpr int kStep = !kSplit && kTerms == 1 && DT <= 128 ? 64 : 32;  // of a step of the softmax
-  static constexpr int kTile = kKeys * DT;                // elements of a tile of K or V
-  static constexpr size_t kTeam = (size_t)4 * kTile * 2;  // bytes of a team's tiles: K and V, twice
+  static constexpr int kKeys = kSplit || k32 ? 32 : DT == 256 ? 64 : 128;              // of a tile
+  static constexpr int kStep = !kSplit && !k32 && kTerms == 1 && DT <= 128 ? 64 : 32;  // of a step of the softmax
+  static constexpr int kTile = kKeys * DT;                          // elements of a tile of K or V
+  static constexpr size_t kTeam = (size_t)4 * kTile * sizeof(KV);   // bytes of a team's tiles: K and V, twice
   static constexpr int kSums = DT + 4;                    // floats of a row of sums, where teams are joined
   static constexpr int kStates = kSplit ? kTeams * 32 * 2 : 0;
   static constexpr size_t kLds = kTeams * kTeam + 8 * sizeof(int) + kStates * sizeof(float);
   static_assert(!kSplit || (size_t)32 * kSums * 4 <= kTeam, "a team's sums lie where its tiles were");
-  // by which the pieces of row r are exchanged: 16 bytes of K, 32 bytes of V
-  static __device__ __forceinline__ int k_turn(int r) { return DT == 64 ? r >> 1 & 7 : r & 15; }
-  static __device__ __forceinline__ int v_turn(int r) { return DT == 64 ? r >> 1 & 3 : r & 7; }
+  // by which the pieces of row r are exchanged: 16 bytes of K, 32 bytes of V, 128 bytes of V in f32
+  static __device__ __forceinline__ int k_turn(int r) { return DT == 64 && !k32 ? r >> 1 & 7 : r & 15; }
+  static __device__ __forceinline__ int v_turn(int r) { return k32 ? r >> 2 & 1 : DT == 64 ? r >> 1 & 3 : r & 7; }
 };
 
 // 16 bytes of every lane, from `base` + `at` (or, second form, from `from`) to LDS from `to` on. The wait for it is the caller's:
@@ -74,7 +85,11 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
   constexpr int kTeams = Sh::kTeams, kTeamThreads = 64 * Sh::kMembers, kBlock = 32 * Sh::kMembers;
   constexpr int NT = Sh::kTerms, KB = Sh::kKeys, KS = Sh::kStep, kSub = KS / 32, kSteps = DT / 16, kDims = DT / 32;
   constexpr int kWeight = M::kScale ? M::kScale - kSlack : 0;  // exponent that weights carry
-  constexpr int kPerKey = DT / 8;                      // 16-byte loads of a key
+  constexpr bool k32 = Sh::k32;
+  typedef typename std::conditional<k32, float, uint16_t>::type E;
+  constexpr int kE = 16 / (int)sizeof(E);              // elements of a load
+  constexpr int kPerKey = DT / kE;                     // 16-byte loads of a key
+  constexpr unsigned kTileBytes = Sh::kTile * sizeof(E);
   constexpr int kLoads = KB * kPerKey / kTeamThreads;  // of a thread, for K and for V
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int* odd_flags = (int*)(lds + kTeams * Sh::kTeam);
@@ -198,25 +213,25 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
 #pragma unroll
   for (int x = 0; x < kKinds; ++x) {
     const int r = (x * kRowsAtOnce + wave_row) % 16 + lane_row, from = piece ^ Sh::k_turn(r);
-    k_in[x] = 8 * from < dim;
-    k_at[x] = (unsigned)(r * dim + 8 * from) * 2;
-    const int v_from = ((piece >> 1) ^ Sh::v_turn(r)) << 1 | (piece & 1);
-    v_in[x] = 8 * v_from < dim;
-    v_at[x] = (unsigned)(r * dim + 8 * v_from) * 2;
+    k_in[x] = kE * from < dim;
+    k_at[x] = (unsigned)((r * dim + kE * from) * sizeof(E));
+    const int v_from = piece ^ Sh::v_turn(r) * (k32 ? 8 : 2);
+    v_in[x] = kE * v_from < dim;
+    v_at[x] = (unsigned)((r * dim + kE * v_from) * sizeof(E));
   }
   auto block_of = [&](int i) { return i * kRowsAtOnce / 16 + (kRowsAtOnce > 16 ? __builtin_amdgcn_readfirstlane(wave_row) / 16 : 0); };
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds +
                         __builtin_amdgcn_readfirstlane(team) * (unsigned)Sh::kTeam;
-  uint16_t* tiles = (uint16_t*)(lds + team * Sh::kTeam);
+  E* tiles = (E*)(lds + team * Sh::kTeam);
   // The team's n-th tile, t, to its buffer n & 1; returns the sixteens of keys whose page is not there.
   auto load = [&](int t, int n) {
     // every lane works its block's place in the pools out, and the loads take them from there
     const bool there = page_there(a.c, pages);
     const int gone = (int)(__ballot(!there) & ((1u << kBlocks) - 1));
-    const u64 at = slot_row(a.c, there ? pages : 0, hk, key_of(t) + 16 * min(lane, kBlocks - 1)) * (unsigned)(2 * dim);
+    const u64 at = slot_row(a.c, there ? pages : 0, hk, key_of(t) + 16 * min(lane, kBlocks - 1)) * (unsigned)(sizeof(E) * dim);
     const unsigned at_lo = (unsigned)at, at_hi = (unsigned)(at >> 32);
     find(t + kTeams);
-    const unsigned to = lds0 + (n & 1) * (4 * Sh::kTile) + __builtin_amdgcn_readfirstlane(member) * 1024;
+    const unsigned to = lds0 + (n & 1) * (2 * kTileBytes) + __builtin_amdgcn_readfirstlane(member) * 1024;
     constexpr int kStep = 1024 * Sh::kMembers;
     auto base_of = [&](int i) {
       const int b = block_of(i);
@@ -227,14 +242,14 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       for (int i = 0; i < kLoads; ++i) {
         const u64 base = base_of(i);
         load_lds((const uint8_t*)a.c.k + base, k_at[i % kKinds], to + kStep * i);
-        load_lds((const uint8_t*)a.c.v + base, v_at[i % kKinds], to + kStep * i + 2 * Sh::kTile);
+        load_lds((const uint8_t*)a.c.v + base, v_at[i % kKinds], to + kStep * i + kTileBytes);
       }
     } else {  // zeros past the head's size
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const u64 base = base_of(i);
         load_lds(k_in[i % kKinds] ? (const uint8_t*)a.c.k + base + k_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i);
-        load_lds(v_in[i % kKinds] ? (const uint8_t*)a.c.v + base + v_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i + 2 * Sh::kTile);
+        load_lds(v_in[i % kKinds] ? (const uint8_t*)a.c.v + base + v_at[i % kKinds] : (const uint8_t*)&kZeros, to + kStep * i + kTileBytes);
       }
     }
     return gone;
@@ -292,8 +307,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
   }
   for (; t < nt; t += kTeams, ++n) {
     const int next_gone = t + kTeams < nt ? load(t + kTeams, n + 1) : 0;
-    const uint16_t* ks = tiles + (n & 1) * (2 * Sh::kTile);
-    const uint16_t* vs = ks + Sh::kTile;
+    const E* ks = tiles + (n & 1) * (2 * Sh::kTile);
+    const E* vs = ks + Sh::kTile;
     const int tile0 = key_of(t);
 #pragma unroll 1
     for (int k0 = tile0; k0 < tile0 + KB; k0 += KS, ks += KS * DT, vs += KS * DT) {
@@ -301,7 +316,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       const bool whole = gone == 0 && seen_by(k0, KS, pos_min, pos_max);
       if (row0 >= all_rows || k0 > pos_max) break;  // nothing for this wavefront
       // ---- scores ----
-      const int k_turn = 8 * Sh::k_turn(row);  // of rows 32 u + row
+      const int k_turn = kE * Sh::k_turn(row);  // of rows 32 u + row
       f32x16 sc[kSub];
 #pragma unroll
       for (int u = 0; u < kSub; ++u)
@@ -311,18 +326,27 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       for (int c = 0; c < kSteps; ++c)
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
-          const typename M::V8 kf = *(const typename M::V8*)(ks + (32 * u + row) * DT + (8 * (2 * c + half) ^ k_turn));
+          const E* at = ks + (32 * u + row) * DT;
+          const int d = 8 * (2 * c + half);
+          typename M::V8 kf;
+          if constexpr (k32) {
+            const f32x4 lo = *(const f32x4*)(at + (d ^ k_turn)), hi = *(const f32x4*)(at + ((d + 4) ^ k_turn));
+            kf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          } else {
+            kf = *(const typename M::V8*)(at + (d ^ k_turn));
+          }
 #pragma unroll
           for (int k = NT - 1; k >= 0; --k) sc[u] = mfma32(kf, q[k][c], sc[u]);
         }
       // four reads ahead of the products
-      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      constexpr int kReads = k32 ? 2 : 1, kProducts = k32 ? 8 : NT;
+      __builtin_amdgcn_sched_group_barrier(0x100, 4 * kReads, 0);
 #pragma unroll
       for (int i = 0; i < kSteps * kSub - 4; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 4 * kProducts, 0);
       if (!whole) {
         int first_key = k0 + 4 * half;
         asm volatile("" : "+v"(first_key));  // here, not in front of the loop in a register for each key
@@ -365,30 +389,39 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
         float p8[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) p8[i] = pr[c / 2][8 * (c % 2) + i];
-        typename M::V8 pt[NT];
-        M::split(p8, pt);
-        const int r0 = 4 * half + ((lane & 15) >> 2);  // of rows 16 c + 8 x + r0
+        if constexpr (k32) {
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) {
-          union {
-            s4 part[2];
-            typename M::V8 v8;
-          } vt;
+          for (int i = 0; i < 8; ++i)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            vt.part[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(
-                vs + (16 * c + 8 * x + r0) * DT + ((2 * d + (lane >> 4 & 1)) ^ Sh::v_turn(8 * x + r0)) * 16 + 4 * (lane & 3)));
+            for (int d = 0; d < kDims; ++d)
+              o[d] = mfma32(vs[(16 * c + 8 * (i / 4) + 4 * half + i % 4) * DT + 32 * (d ^ half) + row], p8[i], o[d]);
+        } else {
+          typename M::V8 pt[NT];
+          M::split(p8, pt);
+          const int r0 = 4 * half + ((lane & 15) >> 2);  // of rows 16 c + 8 x + r0
 #pragma unroll
-          for (int k = NT - 1; k >= 0; --k) o[d] = mfma32(vt.v8, pt[k], o[d]);
+          for (int d = 0; d < kDims; ++d) {
+            union {
+              s4 part[2];
+              typename M::V8 v8;
+            } vt;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              vt.part[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(
+                  vs + (16 * c + 8 * x + r0) * DT + ((2 * d + (lane >> 4 & 1)) ^ Sh::v_turn(8 * x + r0)) * 16 + 4 * (lane & 3)));
+#pragma unroll
+            for (int k = NT - 1; k >= 0; --k) o[d] = mfma32(vt.v8, pt[k], o[d]);
+          }
         }
       }
-      __builtin_amdgcn_sched_group_barrier(0x100, 8, 1);
+      constexpr int kVReads = k32 ? 4 : 2, kVProducts = k32 ? 4 : NT;
+      __builtin_amdgcn_sched_group_barrier(0x100, 4 * kVReads, 1);
 #pragma unroll
-      for (int i = 0; i < 2 * kSub * kDims - 4; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NT, 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+      for (int i = 0; i < (k32 ? 4 : 2) * kSub * kDims - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, kVProducts, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, kVReads, 1);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, 4 * NT, 1);
+      __builtin_amdgcn_sched_group_barrier(0x008, 4 * kVProducts, 1);
       __builtin_amdgcn_s_setprio(0);
     }
     if (t + kTeams < nt) arrive(t + kTeams, n + 1, next_gone);
@@ -411,14 +444,19 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
           all_there = all_there && i < a.c.table_ld && page_there(a.c, table[i]);
         }
         if (all_there && all_seen(key_of(t), block_min, block_max)) continue;
-        const uint16_t* v = (const uint16_t*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
+        const KV* v = (const KV*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
 #pragma unroll
         for (int d = 0; d < kDims; ++d)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int x = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-            const uint32_t bits = x < dim ? v[x] : 0u;
-            if (M::finite(bits) != bits) o[d][i] += M::widen((uint16_t)bits);
+            if constexpr (k32) {
+              const uint32_t bits = x < dim ? ((const uint32_t*)v)[x] : 0u;
+              if (M::finite(bits) != bits) o[d][i] += __uint_as_float(bits);
+            } else {
+              const uint32_t bits = x < dim ? ((const uint16_t*)v)[x] : 0u;
+              if (M::finite(bits) != bits) o[d][i] += M::widen((uint16_t)bits);
+            }
           }
       }
     }
@@ -492,6 +530,10 @@ hipError_t launch_shape(const Attend& a, int dt, unsigned items, hipStream_t s) 
 }  // namespace
 
 hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s) {
+  if (dtype == W4A32_CACHE_F32) {
+    if (dt == 64) return launch<float, float, 64, true>(a, items, s);
+    return dt == 128 ? launch<float, float, 128, false>(a, items, s) : launch<float, float, 256, false>(a, items, s);
+  }
   if (act_bf16) return launch_shape<__bf16, __bf16>(a, dt, items, s);
   if (dtype == W4A32_CACHE_F16) return launch_shape<float, _Float16>(a, dt, items, s);
   return launch_shape<float, __bf16>(a, dt, items, s);
