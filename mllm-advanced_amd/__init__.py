@@ -813,15 +813,16 @@ def _setup():
 
 def _need(t, what, dtype, device, shape=None):
     """Refuses a tensor that is not contiguous, of the type and shape, and on the device whose stream the call goes to."""
-    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or (shape is not None and t.shape != shape):
+    if t.dtype is not dtype or t.get_device() != device or (shape is not None and t.shape != shape) or not t.is_contiguous():
         raise W4A32Error(f"{what}: {dtype}{'' if shape is None else ' ' + str(tuple(shape))}, contiguous, on device {device} is wanted: "
                          f"got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
-def _row_ld(t, what, dtype, device):
-    """Elements from one row to the next of a tensor [rows][width] whose rows are contiguous."""
-    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2:
-        raise W4A32Error(f"{what}: rows of {dtype} on device {device} are wanted: got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _row_ld(t, what, dtype, device, shape=None):
+    """Elements from one row to the next of a tensor [rows][width] (`shape`, if given) whose rows are contiguous."""
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2 or (shape is not None and t.shape != shape):
+        raise W4A32Error(f"{what}: rows of {dtype}{'' if shape is None else ' ' + str(tuple(shape))} on device {device} are wanted: "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     if t.is_contiguous():
         return t.shape[1]
     ld, one = t.stride()
@@ -858,6 +859,7 @@ class PagedCache:
         self.dtype, self.device, self.kv_heads, self.dim, self.n_seqs = k.dtype, device, kv, dim, table.shape[0]
         self.args = PagedCacheArgs(k.data_ptr(), v.data_ptr(), _ptr(weight), table.data_ptr(), length.data_ptr(), _kinds[k.dtype],
                                    pages, page, kv, dim, table.shape[0], table.shape[1])
+        self.starts = (table.shape[0] + 1,)   # shape of the row starts
         self._ref = ctypes.byref(self.args)
 
 
@@ -867,26 +869,28 @@ def _paged_rows(cache, q, row_start, max_rows, heads, out):
         raise W4A32Error(f"the cache is on device {cache.device}, the current one is {device}")
     if dtype is not _torch.float32 and dtype is not _torch.bfloat16:
         raise W4A32Error(f"rows are f32 or bf16, not {dtype}")
-    ldq, ldo = _row_ld(q, "q", dtype, device), _row_ld(out, "out", dtype, device)
+    ldq = _row_ld(q, "q", dtype, device)
     rows, width = q.shape
-    if heads < 1 or width != heads * cache.dim or out.shape != q.shape:
-        raise W4A32Error(f"rows of {heads} heads of {cache.dim}: got q {tuple(q.shape)} and out {tuple(out.shape)}")
-    _need(row_start, "row_start", _torch.int32, device, (cache.n_seqs + 1,))
-    return _ROWS_STRUCT.pack(row_start.data_ptr(), rows, max_rows, heads, dtype is _torch.bfloat16, q.data_ptr(), out.data_ptr(), ldq, ldo)
+    if heads < 1 or width != heads * cache.dim:
+        raise W4A32Error(f"rows of {heads} heads of {cache.dim}: got q {tuple(q.shape)}")
+    if out is None:
+        out = _torch.empty_like(q)
+        ldo = width if out.is_contiguous() else out.stride(0)
+    else:
+        ldo = _row_ld(out, "out", dtype, device, q.shape)
+    _need(row_start, "row_start", _torch.int32, device, cache.starts)
+    return out, _ROWS_STRUCT.pack(row_start.data_ptr(), rows, max_rows, heads, dtype is _torch.bfloat16, q.data_ptr(), out.data_ptr(), ldq, ldo)
 
 
 def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max_rows=None, out=None):
     """Rows q [rows][heads * dim], k and v [rows][kv_heads * dim] of all sequences (sequence b: row_start[b] .. row_start[b + 1]):
     returns the rotated q and writes the rotated k, and v, behind the sequences' tokens. sin, cos [positions][rotated / 2]: none,
     no rotation. pos int32 [sequences]: position of a sequence's first row where it is not cache.length."""
-    if out is None:
-        out = _torch.empty_like(q)
-    rows, dtype, device = q.shape[0], q.dtype, cache.device
-    r = _paged_rows(cache, q, row_start, max_rows or rows, q.shape[1] // cache.dim, out)
-    ldk, ldv = _row_ld(k, "k", dtype, device), _row_ld(v, "v", dtype, device)
-    width = (rows, cache.kv_heads * cache.dim)
-    if k.shape != width or v.shape != width:
-        raise W4A32Error(f"k and v are {width}: got {tuple(k.shape)} and {tuple(v.shape)}")
+    rows, width = q.shape
+    dtype, device = q.dtype, cache.device
+    out, r = _paged_rows(cache, q, row_start, max_rows or rows, width // cache.dim, out)
+    shape = (rows, cache.kv_heads * cache.dim)
+    ldk, ldv = _row_ld(k, "k", dtype, device, shape), _row_ld(v, "v", dtype, device, shape)
     rot = positions = d_sin = d_cos = 0
     if sin is not None:
         _need(sin, "sin", _torch.float32, device), _need(cos, "cos", _torch.float32, device, sin.shape)
@@ -914,11 +918,9 @@ def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, fi
     row j of sequence b sees slots t <= s = cache.length[b] + j with t > s - window or t < first (window 0: all). max_rows: most
     rows of one sequence. accumulate: the weights that the cached tokens receive are added to cache.weight (sequences may share
     pages to be read, but then not with this). out is not q."""
-    if out is None:
-        out = _torch.empty_like(q)
     if scratch is None:
         scratch = op_paged_attention_scratch(cache, q.shape[0], max_rows, heads, accumulate)
-    r = _paged_rows(cache, q, row_start, max_rows, heads, out)
+    out, r = _paged_rows(cache, q, row_start, max_rows, heads, out)
     if window >> 31 or first >> 31:
         raise W4A32Error(f"window {window} and first {first}: from 0 to 2^31 - 1")
     _check(lib().w4a32_op_paged_attention(cache._ref, r, scale, window, first, accumulate, *_scratch_of(scratch, cache.device), _stream()),

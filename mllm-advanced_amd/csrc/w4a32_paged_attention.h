@@ -32,7 +32,7 @@ struct Attend {
   int group_shift;
   int window, first;
   int prompt_rows;      // (token, head of the group) pairs from which on a sequence is the prompts' kernel's; 0: none is
-  int prompt_log2;      // log2 of the rows of a workgroup of that kernel: 8 (7 of 256 dims), or 5 where there are few
+  int prompt_log2;      // log2 of the rows of a workgroup of that kernel: 8 (7 with 256 dims or in f32), or 5
   int wide;             // log2 of the wavefronts with rows of their own (1, 2 or 4): an item has 16 << wide rows
   int slot_rows;        // rows of an item that can be there: what a slot of scratch memory holds
   unsigned most_items, most_tiles;  // what the scratch memory holds: row starts that overlap could ask for more, and get nothing

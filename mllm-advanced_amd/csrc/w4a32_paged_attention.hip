@@ -697,7 +697,7 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   if (accumulate) at = up256(at + (size_t)p.items * p.slot_rows * 4);
   p.dump_off = at;
   if (accumulate) at = up256(at + (size_t)p.tiles * p.wide * kRows * kt * 4);
-  p.total = at;
+  p.total = p.others ? at : 256;  // the prompts' kernel needs none
   return W4A32_OK;
 }
 
