@@ -797,3 +797,37 @@ def test_refused_tensors(pkg):
             pkg.op_verify_drafts(**{**good, **bad})
     count, token = pkg.op_verify_drafts(**{**good, "uniform": None, "choice": None, "temperature": 0.0})
     assert count.tolist()[0] in (1, 2) and int(token) == int(logits[int(count) - 1].argmax())
+
+
+def test_pages_beyond_32_bits_of_the_pools(pkg):
+    """Pools of 4.5 thousand million elements, of which the last pages are used: the same bits as from small ones"""
+    heads, kv, dim, page, far, few = 16, 8, 256, 128, 17100, 12
+    assert (far - few) * kv * page * dim > 2 ** 32
+    small = [torch.randn(few, kv, page, dim, device="cuda").bfloat16() for _ in range(2)]
+    large = [torch.empty(far, kv, page, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    weight = torch.rand(few, kv, page, device="cuda")
+    far_weight = torch.empty(far, kv, page, device="cuda")
+    for a, b in zip((*small, weight), (*large, far_weight)):
+        b[far - few:] = a
+    table = torch.tensor([[3, 0, 7, 5], [1, 6, 2, 4]], dtype=torch.int32, device="cuda")
+    length = torch.tensor([300, 30], dtype=torch.int32, device="cuda")
+    caches = [pkg.PagedCache(*small, table, length, weight), pkg.PagedCache(*large, table + (far - few), length, far_weight)]
+    others = torch.tensor([[8, 9], [10, 11]], dtype=torch.int32, device="cuda")
+    sin, cos = pkg.op_rope_table(600, dim, 1e4)
+    for rows in ([2, 1], [200, 300]):
+        starts = torch.tensor([0, rows[0], sum(rows)], dtype=torch.int32, device="cuda")
+        q, k, v = (torch.randn(sum(rows), n * dim, device="cuda").bfloat16() for n in (heads, kv, kv))
+        outs = []
+        for cache in caches:
+            turned = pkg.op_paged_append(cache, q, k, v, starts, sin, cos)
+            outs.append([turned, pkg.op_paged_attention(cache, turned, starts, max(rows), heads, dim ** -0.5),
+                         pkg.op_paged_attention(cache, turned, starts, max(rows), heads, dim ** -0.5, window=40, first=2, accumulate=True)])
+        for a, b in zip(*outs):
+            assert torch.equal(a, b) and bool(a.isfinite().all())
+        for a, b in zip((*small, weight), (*large, far_weight)):
+            assert torch.equal(a, b[far - few:])
+    tos = [pkg.PagedCache(c.k, c.v, others + shift, torch.zeros_like(length), c.weight) for c, shift in zip(caches, (0, far - few))]
+    kept = [pkg.op_paged_evict(c, to, 100, 4, 20) for c, to in zip(caches, tos)]
+    assert torch.equal(*kept) and torch.equal(tos[0].length, tos[1].length)
+    for a, b in zip((*small, weight), (*large, far_weight)):
+        assert torch.equal(a, b[far - few:])
