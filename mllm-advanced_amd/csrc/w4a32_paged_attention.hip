@@ -168,52 +168,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     const int pos = min(s.len + j, a.c.cap - 1);
     const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
 
-    // ---- q ----
+    // The page numbers of the first tile are asked for, then q, then its keys and values: q is made ready while those are on their way.
     typedef typename std::conditional<k16, u32x4, f32x4>::type Raw;
-    float row_scale = a.scale;
-    u32x4 qt[k16 ? NT : 1][k16 ? kSteps : 1];
-    f32x4 qf[k16 ? 1 : kSteps];
-    {
-      const size_t at = (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
-      if constexpr (k16) {
-        float x[kSteps][8], most = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          const int d = 32 * c + 8 * grp;
-          load8<Act>(a.q, at + (DT == dim || d < dim ? d : 0), x[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          const int d = 32 * c + 8 * grp;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[c][i] = DT == dim || d < dim ? x[c][i] : 0.0f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(x[c][i]));
-        }
-        if constexpr (M::kScale != 0) {
-          const float up = M::row_scale(group_max(most), row_scale);
-#pragma unroll
-          for (int c = 0; c < kSteps; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[c][i] *= up;
-        }
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          typename M::V8 t[NT];
-          M::split(x[c], t);
-#pragma unroll
-          for (int k = 0; k < NT; ++k) qt[k][c] = __builtin_bit_cast(u32x4, t[k]);
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c) {
-          const int d = 16 * c + 4 * grp;
-          qf[c] = load_global<f32x4>((const float*)a.q + at + (DT == dim || d < dim ? d : 0));
-          if (DT != dim && d >= dim) qf[c] = f32x4{0, 0, 0, 0};
-        }
-      }
-    }
-
     const int* table = a.c.table + (size_t)p.b * a.c.table_ld;
     auto key_of = [&](int t) { return (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT; };
     // Lane h has the page of half h of a tile (-1: not there). It is asked for a tile ahead of the loads that need it, and in front
@@ -258,6 +214,59 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         vr[i] = DT == dim || d < dim ? load_global<Raw>(base + (key - 16 * h) * dim + d) : Raw{0, 0, 0, 0};
       }
     };
+    int t = seen_from(t_lo + stream);
+    find(t);
+
+    // ---- q ----
+    constexpr int kQ = k16 && sizeof(Act) == 4 ? 2 : 1;  // 16-byte loads of a step
+    float row_scale = a.scale;
+    u32x4 qr[kSteps][kQ], qt[k16 ? NT : 1][k16 ? kSteps : 1];
+    f32x4 qf[k16 ? 1 : kSteps];
+    const int q_step = k16 ? 32 : 16, q_first = (k16 ? 8 : 4) * grp;
+    {
+      const Act* from = (const Act*)a.q + (size_t)(s.r0 + j) * a.ldq + (size_t)head * dim;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const int d = q_step * c + q_first;
+#pragma unroll
+        for (int h = 0; h < kQ; ++h) qr[c][h] = load_global<u32x4>(from + (DT == dim || d < dim ? d : 0) + 4 * h);
+      }
+    }
+    if (t < t_end) {
+      turn(t);
+      load_k(t);
+      load_v(t);
+    }
+    if constexpr (k16) {
+      float x[kSteps][8], most = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t w = qr[c][kQ == 2 ? i / 4 : 0][kQ == 2 ? i % 4 : i / 2];
+          const float f = __uint_as_float(kQ == 2 ? w : i & 1 ? w & 0xffff0000u : w << 16);
+          x[c][i] = DT == dim || 32 * c + 8 * grp < dim ? f : 0.0f;
+          most = fmaxf(most, fabsf(x[c][i]));
+        }
+      if constexpr (M::kScale != 0) {
+        const float up = M::row_scale(group_max(most), row_scale);
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[c][i] *= up;
+      }
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        typename M::V8 terms[NT];
+        M::split(x[c], terms);
+#pragma unroll
+        for (int k = 0; k < NT; ++k) qt[k][c] = __builtin_bit_cast(u32x4, terms[k]);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+        qf[c] = DT == dim || q_step * c + q_first < dim ? __builtin_bit_cast(f32x4, qr[c][0]) : f32x4{0, 0, 0, 0};
+    }
 
     KV* vs = (KV*)(lds + wave * wave_lds<KV, DT>());
     f32x4 o[DT / 16];
@@ -265,14 +274,6 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     for (int d = 0; d < DT / 16; ++d) o[d] = f32x4{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
     bool odd = false;  // values that are not finite, in a tile that not every row sees whole
-
-    int t = seen_from(t_lo + stream);
-    find(t);
-    if (t < t_end) {
-      turn(t);
-      load_k(t);
-      load_v(t);
-    }
     for (int next; t < t_end; t = next) {
       next = seen_from(t + streams);
       const int k0 = key_of(t);
