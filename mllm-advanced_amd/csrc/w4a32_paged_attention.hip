@@ -35,7 +35,7 @@ inline int from_hip(hipError_t e) { return e == hipSuccess ? W4A32_OK : W4A32_EL
 // 12.3, one on 131001 34.9 against 32.9, 64 sequences 116 against 114, 16 of drafted tokens 30.8 against 31.7.)
 constexpr int kGrid = 512;
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
-constexpr int kAlone = 8;         // tiles of an item that is not shared, where there are workgroups enough for all items
+constexpr int kAlone = 8;         // tiles up to which items are not shared, where all are so short
 // The prompts' kernel takes sequences of at least kPromptRows pairs of token and head, where it has kPromptLeast workgroups of 32
 // rows or more: it does not share a row's keys between workgroups, and few of them on a long context would leave the chip idle.
 // From kPromptWide workgroups of eight times as many rows on it has those (28 heads on 4, bf16: 512 rows 22 us with either, 2048
@@ -70,7 +70,7 @@ __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
   if (d.total == 0 || d.total > a.most_tiles || d.items > a.most_items) return d;
   d.per = max((d.total + kGrid - 1) / kGrid, (unsigned)kMinTiles);
   const unsigned more = gridDim.x - min(gridDim.x, d.items);  // workgroups beyond one per item
-  if (all_short && d.items <= gridDim.x) {
+  if (all_short) {  // a workgroup takes every gridDim.x-th
     d.per = kAlone;
     d.apart = true;
   } else if (more && (d.total + more - 1) / more <= kFew) {
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
   const Deal deal = deal_of<KT>(a, seqs);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = deal.per ? deal.items : 0;
   if (deal.per == 0) return;
-  unsigned u = blockIdx.x, u_end = u + 1;
+  unsigned u = blockIdx.x, u_end = max(deal.items, gridDim.x);
   if (!deal.apart) {
     u *= deal.per;
     u_end = min(deal.total, u + deal.per);
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         finish<Act, kDump>(a, s.r0, of0 + r, hk, (size_t)(p.item0 + item) * a.slot_rows + r, d, acc, base, sum);
       }
     }
-    u += deal.apart ? 1 : t_hi - t_lo;
+    u += deal.apart ? gridDim.x : t_hi - t_lo;
     if (u < u_end) __syncthreads();  // the next item's tiles go where these sums were read
   }
 }
@@ -683,9 +683,9 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   p.key_groups = (long long)c->n_seqs * c->kv_heads * ((tiles + kWaves - 1) / kWaves);
   if (p.tiles >= (1ll << 31) || p.items * p.slot_rows >= kMost) return W4A32_ESHAPE;
   if (accumulate && p.key_groups > most_groups(64 * kWaves)) return W4A32_ESHAPE;
-  // Nothing is shared where every item is short and has a workgroup. Where a join of one workgroup per row leaves most CUs
+  // Nothing is shared where every item is short. Where a join of one workgroup per row leaves most CUs
   // without work, a row's values are dealt to several.
-  p.join = tiles > kAlone || p.items > p.grid;
+  p.join = tiles > kAlone;
   p.sliced = p.items * p.slot_rows <= 128;
   size_t at = 256;
   p.item_off = at;

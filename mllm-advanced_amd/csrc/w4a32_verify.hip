@@ -19,6 +19,7 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 
 constexpr int kSegment = 4096;  // logits of a segment: 16 of each thread, all requested at once
 constexpr int kEach = kSegment / 256;
+constexpr int kChoose = 1024;   // threads of the third launch: what takes time there is the f64 arithmetic of four logits each
 constexpr int kTestWaves = 8;   // wavefronts of the second launch: rows of a sequence that are tested at once
 
 struct Part {
@@ -318,9 +319,10 @@ __global__ __launch_bounds__(64 * kTestWaves) void test_kernel(Verify a) {
 }
 
 // A workgroup per sequence
-__global__ __launch_bounds__(256) void choose_kernel(Verify a) {
-  __shared__ double in_wave[4], before, target;
-  __shared__ int seg, last[4], hit[4];
+__global__ __launch_bounds__(kChoose) void choose_kernel(Verify a) {
+  constexpr int kEach = kSegment / kChoose, kWaves = kChoose / 64;
+  __shared__ double in_wave[kWaves], before, target;
+  __shared__ int seg, refused, last[kWaves], hit[kWaves];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Found f = a.found[b];
   const float choice = a.choice[b];
@@ -372,12 +374,11 @@ __global__ __launch_bounds__(256) void choose_kernel(Verify a) {
       seg = at;
       before = in_front;
       target = mark;
-      last[0] = f.refused;
+      refused = f.refused;
     }
   }
   __syncthreads();
-  f.refused = last[0];
-  __syncthreads();
+  f.refused = refused;
   int64_t token = -1;
   if (seg >= 0) {
     const float *p = a.logits + (size_t)r * a.ldl, *q = a.draft && f.refused ? a.draft + (size_t)r * a.ldd : nullptr;
@@ -420,8 +421,13 @@ __global__ __launch_bounds__(256) void choose_kernel(Verify a) {
       last[wave] = positive;
     }
     __syncthreads();
-    const int first = min(min(hit[0], hit[1]), min(hit[2], hit[3]));
-    token = first != 0x7fffffff ? first : max(max(last[0], last[1]), max(last[2], last[3]));
+    int first = 0x7fffffff, end = -1;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      first = min(first, hit[w]);
+      end = max(end, last[w]);
+    }
+    token = first != 0x7fffffff ? first : end;
   }
   if (threadIdx.x == 0) {
     a.count[b] = f.count;
@@ -468,8 +474,8 @@ struct Layout {
 bool layout_of(int rows, int vocab, int n_seqs, Layout& l) {
   if (rows < 1 || vocab < 1 || n_seqs < 1 || rows >= 1 << 30 || vocab >= 1 << 30 || n_seqs >= 1 << 30) return false;
   l.segs = (vocab + kSegment - 1) / kSegment;
-  // a launch has less than 2^32 threads: 256 of a row's segment, 512 of a sequence's
-  if ((long long)rows * l.segs >= 1ll << 24 || (long long)n_seqs * l.segs >= 1ll << 23) return false;
+  // a launch has less than 2^32 threads: 256 of a row's segment, 512 of a sequence's, 1024 of a sequence
+  if ((long long)rows * l.segs >= 1ll << 24 || (long long)n_seqs * l.segs >= 1ll << 23 || n_seqs >= 1 << 22) return false;
   l.q = (size_t)rows * l.segs * sizeof(Part);
   l.left = 2 * l.q;
   l.found = l.left + (size_t)n_seqs * l.segs * sizeof(double);
@@ -517,7 +523,7 @@ int w4a32_op_verify_drafts(const w4a32_verify_args* v, void* d_scratch, size_t s
     if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
     hipLaunchKernelGGL(test_kernel, dim3((unsigned)(v->n_seqs * (long long)l.segs)), dim3(64 * kTestWaves), 0, s, a);
     if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
-    hipLaunchKernelGGL(choose_kernel, dim3((unsigned)v->n_seqs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(choose_kernel, dim3((unsigned)v->n_seqs), dim3(kChoose), 0, s, a);
   }
   return hipGetLastError() == hipSuccess ? W4A32_OK : W4A32_ELAUNCH;
 }

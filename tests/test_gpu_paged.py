@@ -760,6 +760,17 @@ def test_more_rows_than_the_join_has_workgroups(pkg):
         assert bool(((got[b:b + 500] - want).abs() <= 1e-5).all())
 
 
+@pytest.mark.parametrize("act,kind", TYPES)
+def test_many_short_sequences(pkg, act, kind):
+    """More sequences than workgroups, of up to eight tiles each: none is shared"""
+    rng = np.random.default_rng(6)
+    n = 650
+    B = pm.Batch(35, rng.integers(0, 60, n).tolist(), rng.integers(0, 4, n).tolist(), 2, 16, 16, table_ld=4, weights=True)
+    fill_new(B)
+    run_attention(pkg, B, act, kind, 6)
+    run_attention(pkg, B, act, kind, 6, accumulate=True)
+
+
 def test_refused_tensors(pkg):
     B = pm.Batch(32, [40], [2], 2, 64, 16)
     fill_new(B)
