@@ -7,8 +7,8 @@
 //
 // Exponentials and sums are f64: an f64 sum or product takes as long as an f32 one here, an exponential 16 of them, and so the
 // first launch stays near what memory gives: 48 sequences of 2 to 8 rows of 152064 logits, target and draft (270 MB): 57 us, 4.7 TB/s.
-// The second, which reads the refused rows again, takes 22 there and the third 11; for one sequence of five rows the three
-// take 4, 6 and 6 us, all of it latency. In f32 the sums' rounding would decide which token a number falls on whenever it
+// The second, which reads the refused rows again, takes 22 there and the third 8; for one sequence of five rows the three
+// take 4, 6 and 5 us, all of it latency. In f32 the sums' rounding would decide which token a number falls on whenever it
 // lies within 1e-7 of a border, as one of 150000 tokens' borders often does.
 #include "w4a32_internal.h"
 #include "w4a32_decoder.h"
@@ -19,7 +19,7 @@ inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_
 
 constexpr int kSegment = 4096;  // logits of a segment: 16 of each thread, all requested at once
 constexpr int kEach = kSegment / 256;
-constexpr int kChoose = 1024;   // threads of the third launch: what takes time there is the f64 arithmetic of four logits each
+constexpr int kChoose = 1024;   // threads of the third launch: what takes time is their f64 arithmetic (with 256: 11 us for 48 sequences, not 8)
 constexpr int kTestWaves = 8;   // wavefronts of the second launch: rows of a sequence that are tested at once
 
 struct Part {
