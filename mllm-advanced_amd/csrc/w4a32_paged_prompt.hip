@@ -68,13 +68,16 @@ struct Shape {
 };
 
 // 16 bytes of every lane, from `base` + `at` (or, second form, from `from`) to LDS from `to` on. The wait for it is the caller's:
-// the compiler does not see these loads, whose arrival it would otherwise wait for at the next read of any LDS. (M0 holds their
-// place in LDS and is the compiler's to set in front of each of its own uses.)
+// the compiler does not see these loads, whose arrival it would otherwise wait for at the next read of any LDS. Nor does it see to
+// what has to lie in front of one: a wait state behind the scalar write of M0, which holds the place in LDS, and five between a
+// vector instruction that writes a scalar register (a lane's value, a register brought back from its spill) and the load that
+// reads it. The move of the base to scalar registers of the load's own is the first, and ends the second.
 __device__ __forceinline__ void load_lds(const void* base, unsigned at, unsigned to) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(base), "s"(to) : "memory");
+  u64 own;
+  asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(own) : "v"(at), "s"(base), "s"(to) : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
