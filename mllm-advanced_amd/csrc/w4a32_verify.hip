@@ -207,8 +207,10 @@ __global__ __launch_bounds__(256) void stats_kernel(Verify a) {
   const double from = all == -INFINITY ? 0.0 : (double)all;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) sum += exp_sum(v[i], c, from);
-  if (nan || all == INFINITY) sum = (double)NAN;  // no distribution
-  sum = all == -INFINITY ? 0.0 : wave_add(sum);
+  // A NaN or +infinity leaves no distribution, and its sum stays NaN whatever else the segment has: its maximum may be -infinity.
+  if (all == -INFINITY) sum = 0.0;
+  if (nan || all == INFINITY) sum = (double)NAN;
+  sum = wave_add(sum);
   if (lane == 0) sums[wave] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
