@@ -72,6 +72,8 @@ struct Shape {
 // what has to lie in front of one: a wait state behind the scalar write of M0, which holds the place in LDS, and five between a
 // vector instruction that writes a scalar register (a lane's value, a register brought back from its spill) and the load that
 // reads it. The move of the base to scalar registers of the load's own is the first, and ends the second.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 is a register that the compiler keeps to itself, and that is what is said here
 __device__ __forceinline__ void load_lds(const void* base, unsigned at, unsigned to) {
   u64 own;
   asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0" : "=&s"(own) : "v"(at), "s"(base), "s"(to) : "memory", "m0");
@@ -79,6 +81,7 @@ __device__ __forceinline__ void load_lds(const void* base, unsigned at, unsigned
 __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 template <typename Act, typename KV, int DT, bool kSplit>
