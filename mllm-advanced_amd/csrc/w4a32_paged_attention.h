@@ -189,7 +189,14 @@ __device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x
 
 // ---- element types ---------------------------------------------------------------------------------------------------------
 // Values that are not finite must reach only rows that see their key, and 0 times one would reach all. In a tile that not every
-// row sees whole they are zeros to the product; where there were some, they are added behind the last tile, key by key.
+// row sees whole they are zeros to the product; where there were some, or where a row's sums are not finite, they are added behind
+// the last tile, key by key.
+
+// What brings a share's sums to a common reference is at least this for the values: an infinity stays one where the share's
+// weight underflows, and finite ones add next to nothing.
+constexpr float kLeast = 0x1p-126f;
+template <typename KV>
+using Bits = typename std::conditional<sizeof(KV) == 2, uint16_t, uint32_t>::type;  // an element as it lies in the pools
 
 // kTerms operands stand for one f32 operand of the 16-bit matrix instruction. kScale: exponent that the softmaxed scores
 // carry until the sums are divided (they cancel there).
@@ -266,7 +273,7 @@ struct Math<float, float> {
   static __device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
   static constexpr uint32_t kSize = 0x7fffffffu, kStep = 0x00800000u;
   static __device__ __forceinline__ uint32_t finite(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u ? 0u : w; }
-  static __device__ __forceinline__ float widen(float x) { return x; }
+  static __device__ __forceinline__ float widen(uint32_t x) { return __uint_as_float(x); }
 };
 
 template <typename Act>
@@ -291,6 +298,32 @@ __device__ __forceinline__ void store4(void* p, size_t at, f32x4 x) {
   } else {
     typedef __bf16 b4 __attribute__((ext_vector_type(4)));
     *(W4_GLOBAL b4*)((uint16_t*)p + at) = b4{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3]};
+  }
+}
+
+// A wavefront's rows' sums lie in LDS ([kRows], `stride` apart; its first row is row0 of the sequence's all_rows, whose tokens follow
+// len cached ones). Of the keys [k0, k0 + keys), the values that are not finite go to the sums of the rows that see them: zeros in
+// their place first, then (`add`) the values. Lanes have dims; all is rare and short but the look at every value.
+template <typename M, typename KV, int kRows>
+__device__ __forceinline__ void put_odd(const Attend& a, const int* table, int hk, int k0, int keys, bool add, float* sums, int stride, int len,
+                                        int row0, int all_rows) {
+#pragma unroll 1
+  for (int key = k0; key < k0 + keys; ++key) {
+    const int at = key >> a.c.shift, page = at < a.c.table_ld ? table[at] : -1;
+    if (!page_there(a.c, page)) continue;
+    const Bits<KV>* v = (const Bits<KV>*)a.c.v + slot_row(a.c, page, hk, key) * a.c.dim;
+#pragma unroll 1
+    for (int d = threadIdx.x & 63; d - (int)(threadIdx.x & 63) < a.c.dim; d += 64) {
+      const uint32_t bits = d < a.c.dim ? v[d] : 0u;
+      const bool odd = M::finite(bits) != bits;
+      if (!__any(odd)) continue;
+#pragma unroll 1
+      for (int r = 0; r < min(kRows, all_rows - row0); ++r) {
+        const int pos = min(len + by_group(a, row0 + r), a.c.cap - 1);
+        if (key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
+        if (odd) sums[r * stride + d] = add ? sums[r * stride + d] + M::widen((Bits<KV>)bits) : 0.0f;
+      }
+    }
   }
 }
 

@@ -410,42 +410,28 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       }
     }
 
-    if (odd) {
-#pragma unroll 1
-      for (t = seen_from(t_lo + stream); t < t_end; t = seen_from(t + streams)) {
-#pragma unroll 1
-        for (int k = 0; k < KT; ++k) {
-          const int k0 = key_of(t), key = k0 + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
-          const bool sees = real & page_there(a.c, pg) & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first));
-          bool whole = k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
-          for (int h = 0; h < kHalves; ++h) {
-            const int i = (k0 + 16 * h) >> a.c.shift;
-            whole = whole && i < a.c.table_ld && page_there(a.c, table[i]);
-          }
-          if (whole || !sees) continue;  // whole: they were in the product as they are
-          const KV* v = (const KV*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
-#pragma unroll
-          for (int d = 0; d < DT / 16; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int x = 16 * d + 4 * grp + e;
-              if constexpr (k16) {
-                const uint32_t bits = x < dim ? ((const uint16_t*)v)[x] : 0u;
-                if (M::finite(bits) != bits) o[d][e] += M::widen((uint16_t)bits);
-              } else {
-                const uint32_t bits = x < dim ? ((const uint32_t*)v)[x] : 0u;
-                if (M::finite(bits) != bits) o[d][e] += __uint_as_float(bits);
-              }
-            }
-        }
-      }
-    }
-
     // ---- join the wavefronts ----
     l = group_sum(l) * ldexpf(1.0f, -M::kScale);
     float* sums = (float*)(lds + wave * wave_lds<KV, DT>());
+    float probe[4] = {};
 #pragma unroll
-    for (int d = 0; d < DT / 16; ++d) *(f32x4*)(sums + row * (DT + 4) + 16 * d + 4 * grp) = o[d] * ldexpf(1.0f, -M::kScale);
+    for (int d = 0; d < DT / 16; ++d) {
+      *(f32x4*)(sums + row * (DT + 4) + 16 * d + 4 * grp) = o[d] * ldexpf(1.0f, -M::kScale);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) probe[e] = __fmaf_rn(o[d][e], 0.0f, probe[e]);
+    }
+    // Values that are not finite were zeros in the tiles that not every row sees whole; in the others they met weights of several
+    // terms, of which one may be 0 or negative and make them NaN. So a row whose sums are not finite, though its weights are
+    // numbers, has those values added up instead.
+    const float strange = (probe[0] + probe[1]) + (probe[2] + probe[3]);
+    if (__builtin_expect(odd || __any(real & (l == l) & (strange != strange)), 0)) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+      for (int add = 0; add < 2; ++add)
+#pragma unroll 1
+        for (t = seen_from(t_lo + stream); t < t_end; t = seen_from(t + streams))
+          put_odd<M, KV, kRows>(a, table, hk, key_of(t), KT, add != 0, sums, DT + 4, s.len, row0, all_rows);
+    }
     if (grp == 0) {
       states[(wave * kRows + row) * 2] = m;
       states[(wave * kRows + row) * 2 + 1] = l;
@@ -467,7 +453,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       for (int w = w0; w < kWaves; w += wide) {
         const float f = pow2(states[(w * kRows + r % kRows) * 2] - base);
         sum += f * states[(w * kRows + r % kRows) * 2 + 1];
-        acc += f * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + (r % kRows) * (DT + 4) + d);
+        acc += fmaxf(f, kLeast) * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + (r % kRows) * (DT + 4) + d);
       }
       if (shares > 1) {
         const size_t at = (size_t)slot * a.slot_rows + r;
@@ -521,13 +507,13 @@ __device__ __forceinline__ void join(const Attend& a, unsigned unit) {
     for (int x = 0; x < 8; ++x) most = fmaxf(most, m[x]);
     const float base = most == -INFINITY ? 0.0f : most, down = pow2(top - base);
     sum *= down;
-    acc *= down;
+    acc *= fmaxf(down, kLeast);
     top = most;
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const float f = pow2(m[x] - base);
       sum += f * l[x];
-      acc += f * v[x];
+      acc += fmaxf(f, kLeast) * v[x];
     }
   }
   // the threads of a wavefront that have the same values, by moves, then the wavefronts
@@ -536,7 +522,7 @@ __device__ __forceinline__ void join(const Attend& a, unsigned unit) {
   for (int x = kPer; x < 64; x <<= 1) most = fmaxf(most, __shfl_xor(most, x));
   const float in_wave = pow2(top - (most == -INFINITY ? 0.0f : most));
   sum *= in_wave;
-  acc *= in_wave;
+  acc *= fmaxf(in_wave, kLeast);
 #pragma unroll
   for (int x = kPer; x < 64; x <<= 1) {
     sum += __shfl_xor(sum, x);
@@ -558,7 +544,7 @@ __device__ __forceinline__ void join(const Attend& a, unsigned unit) {
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
     const float f = pow2(tops[w] - base);
-    acc += f * *(const f32x4*)&sums[w][4 * lane];
+    acc += fmaxf(f, kLeast) * *(const f32x4*)&sums[w][4 * lane];
     sum += f * totals[w];
   }
   finish<Act, kDump>(a, it.r0, it.row0 + r, it.head, (size_t)item * a.slot_rows + r, d, acc, base, sum);

@@ -434,41 +434,42 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     gone = next_gone;
   }
 
+  // ---- values that are not finite: as in the rows' kernel, in LDS where the sums go there ----
+  l += __shfl_xor(l, 32);
   bool some_odd = odd_flags[wave] != 0;
   if constexpr (!kSplit)  // behind the last arrival's barrier
     for (int w = 0; w < Sh::kMembers; ++w) some_odd = some_odd || odd_flags[w] != 0;
-  if (some_odd) {
-#pragma unroll 1
-    for (t = team; t < nt; t += kTeams) {
-#pragma unroll 1
-      for (int k = 0; k < KB; ++k) {
-        const int key = key_of(t) + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
-        if (!real || !page_there(a.c, pg) || key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
-        bool all_there = true;  // then its values were in the product as they are
-        for (int b = 0; b < kBlocks; ++b) {
-          const int i = (key_of(t) + 16 * b) >> a.c.shift;
-          all_there = all_there && i < a.c.table_ld && page_there(a.c, table[i]);
-        }
-        if (all_there && all_seen(key_of(t), block_min, block_max)) continue;
-        const KV* v = (const KV*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
+  float probe[4] = {};
 #pragma unroll
-        for (int d = 0; d < kDims; ++d)
+  for (int d = 0; d < kDims; ++d)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int x = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-            if constexpr (k32) {
-              const uint32_t bits = x < dim ? ((const uint32_t*)v)[x] : 0u;
-              if (M::finite(bits) != bits) o[d][i] += __uint_as_float(bits);
-            } else {
-              const uint32_t bits = x < dim ? ((const uint16_t*)v)[x] : 0u;
-              if (M::finite(bits) != bits) o[d][i] += M::widen((uint16_t)bits);
-            }
+    for (int i = 0; i < 16; ++i) probe[i % 4] = __fmaf_rn(o[d][i], 0.0f, probe[i % 4]);
+  const float strange = (probe[0] + probe[1]) + (probe[2] + probe[3]);
+  some_odd = some_odd || __any(real & (l == l) & (strange != strange));
+  if constexpr (!kSplit) {
+    if (__builtin_expect(some_odd, 0)) {
+#pragma unroll 1
+      for (int add = 0; add < 2; ++add)
+#pragma unroll 1
+        for (t = team; t < nt; t += kTeams) {
+#pragma unroll 1
+          for (int k = 0; k < KB; ++k) {
+            const int key = key_of(t) + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
+            if (!real || !page_there(a.c, pg) || key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
+            const Bits<KV>* v = (const Bits<KV>*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int x = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
+                const uint32_t bits = x < dim ? v[x] : 0u;
+                o[d][i] = M::finite(bits) == bits ? o[d][i] : add ? o[d][i] + M::widen((Bits<KV>)bits) : 0.0f;
+              }
           }
-      }
+        }
     }
   }
   // ---- results: lane = row, four dims at a time ----
-  l += __shfl_xor(l, 32);
   if constexpr (kSplit) {
     float* sums = (float*)(lds + team * Sh::kTeam);
     float* states = (float*)(odd_flags + 8);
@@ -478,6 +479,14 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       for (int b = 0; b < 4; ++b)
         *(f32x4*)(sums + row * Sh::kSums + 32 * d + 8 * b + 4 * half) =
             f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+    if (__builtin_expect(some_odd, 0)) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+      for (int add = 0; add < 2; ++add)
+#pragma unroll 1
+        for (t = team; t < nt; t += kTeams)
+          put_odd<M, KV, 32>(a, table, hk, key_of(t), KB, add != 0, sums, Sh::kSums, s.len, row0, all_rows);
+    }
     if (half == 0) {
       states[(team * 32 + row) * 2] = m;
       states[(team * 32 + row) * 2 + 1] = l;
@@ -495,7 +504,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       for (int w = 0; w < kTeams; ++w) {
         const float f = pow2(states[(w * 32 + r) * 2] - base);
         sum += f * states[(w * 32 + r) * 2 + 1];
-        acc += f * *(const f32x4*)((const float*)(lds + w * Sh::kTeam) + r * Sh::kSums + d);
+        acc += fmaxf(f, kLeast) * *(const f32x4*)((const float*)(lds + w * Sh::kTeam) + r * Sh::kSums + d);
       }
       finish<Act, false>(a, s.r0, of0 + r, hk, 0, d, acc, base, sum);
     }
