@@ -571,6 +571,7 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   const int t = (int)p.inner % per_head * kWaves + (threadIdx.x >> 6);
   if (t >= p.q.nt) return;
   const int lane = threadIdx.x & 63, row = lane & 15, grp = lane >> 4;
+  const int k0 = (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT;
   float w[4 * kHalves] = {};
   for (int i = 0; i < p.q.items << a.wide; ++i) {
     const int item = hk * p.q.items + (i >> a.wide), rt = i & ((1 << a.wide) - 1), r = rt * kRows + row;
@@ -583,19 +584,31 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
     const bool real = row0 + row < all_rows;
     const float lse = real ? a.lse[((size_t)p.item0 + item) * a.slot_rows + r] : INFINITY;
     const float* from = a.dump + (((tile << a.wide) + rt) * 64 + lane) * (4 * kHalves);
+    f32x4 x[kHalves];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const f32x4 x = load_global<f32x4>(from + 4 * h);
+    for (int h = 0; h < kHalves; ++h) x[h] = load_global<f32x4>(from + 4 * h);
+    if (__builtin_expect(__any(lse != lse), 0)) {  // a row of NaN: it has no weight, not NaN, for the keys that it does not see
+      const int pos = slot_of(row0 + row);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[4 * h + e] += real ? pow2(x[e] - lse) : 0.0f;
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + 16 * h + 4 * grp + e;
+          const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first));
+          w[4 * h + e] += sees ? pow2(x[h][e] - lse) : 0.0f;
+        }
+      continue;
     }
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * h + e] += real ? pow2(x[h][e] - lse) : 0.0f;
   }
 #pragma unroll
   for (int i = 0; i < 4 * kHalves; ++i)
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) w[i] += __shfl_xor(w[i], x);
   if (row != 0) return;
-  const int k0 = (t < p.q.ft ? t : t - p.q.ft + p.q.w0) * KT;
 #pragma unroll
   for (int h = 0; h < kHalves; ++h) {
     const int key = k0 + 16 * h + 4 * grp;
