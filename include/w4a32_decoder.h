@@ -261,7 +261,8 @@ int w4a32_op_f16_to_f32(const void* d_in, float* d_out, size_t n, void* stream);
  *
  * What a device array may say wrongly is kept inside the pools: a page number outside [0, n_pages) stands for a page
  * that is not there (its tokens are not seen and not written; pages that a window has left may be given back so), a
- * negative length is 0, tokens behind the table's end are not there, and a sequence has at most max_rows rows. Row starts
+ * negative length is 0 and one past 2^30 is that, tokens behind the table's end are not there (rows that stand behind it see what
+ * their windows leave them), and a sequence has at most max_rows rows. Row starts
  * do not decrease; where they do, what the rows get is unspecified.
  *   Sequences may name the same page (a prompt that they share) as long as no call writes it: tokens are appended, and weights
  * added up, only in pages that one sequence names once.

@@ -30,14 +30,14 @@ int check_rows(const w4a32_paged_cache* c, const w4a32_paged_rows* r);
 Cache view(const w4a32_paged_cache* c);
 
 // The rows of sequence b and the tokens in front of them, with everything a device array may say wrongly brought back
-// into range.
+// into range. A length may pass the table: row j stands at len + j all the same, of which neither that nor a window's start is moved.
 struct Span {
-  int r0, n, len;  // first row, rows, tokens in the cache
+  int r0, n, len;  // first row, rows, tokens in front (kMost at most, so that no row's place passes 31 bits)
 };
 __device__ __forceinline__ Span span_of(const Cache& c, const int* row_start, int rows, int max_rows, int b) {
   Span s;
   const int lo = row_start[b], hi = row_start[b + 1];
-  s.len = min(max(c.len[b], 0), c.cap);
+  s.len = min(max(c.len[b], 0), kMost);
   s.r0 = min(max(lo, 0), rows);
   s.n = min(min(max(hi, s.r0), rows) - s.r0, max_rows);
   return s;

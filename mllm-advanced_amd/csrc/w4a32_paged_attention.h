@@ -319,7 +319,7 @@ __device__ __forceinline__ void put_odd(const Attend& a, const int* table, int h
       if (!__any(odd)) continue;
 #pragma unroll 1
       for (int r = 0; r < min(kRows, all_rows - row0); ++r) {
-        const int pos = min(len + by_group(a, row0 + r), a.c.cap - 1);
+        const int pos = len + by_group(a, row0 + r);
         if (key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
         if (odd) sums[r * stride + d] = add ? sums[r * stride + d] + M::widen((Bits<KV>)bits) : 0.0f;
       }

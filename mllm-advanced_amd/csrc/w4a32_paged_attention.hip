@@ -165,8 +165,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     const bool real = in_seq < all_rows, busy = row0 < all_rows;
     const int j = by_group(a, min(in_seq, all_rows - 1)), head = hk * a.group + (real ? in_seq - j * a.group : 0);
     const int j_min = by_group(a, min(row0, all_rows - 1)), j_max = by_group(a, min(row0 + kRows - 1, all_rows - 1));
-    const int pos = min(s.len + j, a.c.cap - 1);
-    const int pos_min = min(s.len + j_min, a.c.cap - 1), pos_max = min(s.len + j_max, a.c.cap - 1);
+    const int pos = s.len + j, pos_min = s.len + j_min, pos_max = s.len + j_max;
 
     // The page numbers of the first tile are asked for, then q, then its keys and values: q is made ready while those are on their way.
     typedef typename std::conditional<k16, u32x4, f32x4>::type Raw;
@@ -578,7 +577,7 @@ __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
     const u64 tile = (u64)p.tile0 + (u64)item * p.q.nt + t;
     const int all_rows = p.q.s.n * a.group, row0 = i * kRows;
     if (row0 >= all_rows) break;
-    auto slot_of = [&](int r) { return min(p.q.s.len + by_group(a, r), a.c.cap - 1); };
+    auto slot_of = [&](int r) { return p.q.s.len + by_group(a, r); };
     const Sight sight = sight_of<KT>(a, p.q, slot_of(row0), slot_of(min(row0 + kRows, all_rows) - 1));
     if (t >= sight.to || sight.skips(t)) continue;
     const bool real = row0 + row < all_rows;

@@ -119,9 +119,10 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     // The blocks of all sequences by the last key that they see, most keys first: the position from which on `order` blocks
     // or fewer are left is searched for, all sequences counting at once.
     const Seq& q = seqs.q;
+    const int len = min(q.s.len, a.c.cap);
     auto from = [&](int end) {  // this lane's blocks whose last row stands at `end` or behind
-      if (!q.items || end > q.s.len + q.s.n - 1) return 0u;
-      const long long need = (long long)(end - q.s.len) * a.group + 1;  // pairs up to the first that stands there
+      if (!q.items || end > len + q.s.n - 1) return 0u;
+      const long long need = (long long)(end - len) * a.group + 1;  // pairs up to the first that stands there
       return (unsigned)(q.items - (need <= 0 ? 0 : (int)((need + kBlock - 1) / kBlock) - 1));
     };
     int lo = 0, hi = a.c.cap + a.max_rows;  // from(lo) counts more than `order`, from(hi) does not
@@ -150,14 +151,14 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
   const Span s = p.q.s;
   const int all_rows = s.n * (int)group, of0 = block * kBlock, row0 = of0 + 32 * member, in_seq = row0 + row;
   const bool real = in_seq < all_rows;
-  auto slot_of = [&](int r) { return min(s.len + by_group(a, min(r, all_rows - 1)), a.c.cap - 1); };
+  auto slot_of = [&](int r) { return s.len + by_group(a, min(r, all_rows - 1)); };
   const int j = by_group(a, min(in_seq, all_rows - 1)), head = hk * a.group + (real ? in_seq - j * a.group : 0);
-  const int pos = min(s.len + j, a.c.cap - 1), pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
+  const int pos = s.len + j, pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
   const int block_min = slot_of(of0), block_max = slot_of(of0 + kBlock - 1);
-  // tiles that the workgroup's rows can see: [0, ft) and [w0, ..)
-  const int w0 = a.window ? max(0, block_min - a.window + 1) / KB : 0;
+  // tiles that the workgroup's rows can see: [0, ft) and [w0, ..), of those that the table has
+  const int w0 = a.window ? max(0, min(block_min, a.c.cap - 1) - a.window + 1) / KB : 0;
   const int ft = a.window ? min((min(a.first, a.c.cap) + KB - 1) / KB, w0) : 0;
-  const int nt = ft + block_max / KB + 1 - w0;
+  const int nt = ft + min(block_max, a.c.cap - 1) / KB + 1 - w0;
   auto key_of = [&](int t) { return (t < ft ? t : t - ft + w0) * KB; };
 
   // ---- q ----
