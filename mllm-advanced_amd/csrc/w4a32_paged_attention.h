@@ -239,11 +239,12 @@ struct Math<Act, _Float16> {
   static constexpr int kTerms = 2;
   static constexpr int kScale = 15;
   typedef h8 V8;
-  // the power of two that brings a row of q, of which `most` is the largest, to 2^14 .. 2^15; its inverse joins the row's scale
+  // the power of two (2^127 at most) that brings a row of q, of which `most` is the largest, to 2^14 .. 2^15; its inverse joins the
+  // row's scale, which stays finite: what it is the scale of may be 0
   static __device__ __forceinline__ float row_scale(float most, float& scale) {
     int e = 0;
-    if (most > 0.0f && most < INFINITY) e = min(max(14 - ilogbf(most), -100), 100);
-    scale *= ldexpf(1.0f, -e);
+    if (most > 0.0f && most < INFINITY) e = min(14 - ilogbf(most), 127);
+    scale = __builtin_amdgcn_fmed3f(scale * ldexpf(1.0f, -e), -3.40282347e38f, 3.40282347e38f);
     return ldexpf(1.0f, e);
   }
   static __device__ __forceinline__ f32x4 mfma(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }

@@ -185,7 +185,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       most = fmaxf(most, __shfl_xor(most, 32));
       up *= M::row_scale(most, row_scale);
     }
-    if (a.scale == 0.0f) {  // all alike: scores of 0, not infinity times 0 where a key is not seen
+    if (row_scale == 0.0f) {  // all alike (a scale of 0, or next to it): scores of 0, not infinity times 0 where a key is not seen
       up = 0.0f;
       row_scale = 1.0f;
     }
