@@ -317,6 +317,9 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
  * the second product as bf16, as the output is rounded. `scale` is finite.
  *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time (calls that
  * overlap in time, on two streams or in two graphs, need one each). That is 0 for a call that w4a32_op_paged_attention refuses.
+ * With `accumulate` it holds the scores, 4 bytes for each row of a head (rounded up to 16 or
+ * 64 of a kv head) and token that the table has room for: a step of more than 1 GiB of them is gone through in passes of 128 rows or
+ * more, and with scratch memory for fewer rows at once in more passes (each adds its sums to cache->d_weight).
  * QWenAttention::forward, modeling_ds_qwen2.hpp:133-151, per sequence. */
 size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows,
                                               int accumulate);

@@ -30,6 +30,7 @@ struct Attend {
   int ldq, ldo, rows, max_rows, heads, group;
   unsigned group_mul;   // by_group()
   int group_shift;
+  int row_lo, row_hi;   // of the step's rows those that the launch is about
   int window, first;
   int prompt_rows;      // (token, head of the group) pairs from which on a sequence is the prompts' kernel's; 0: none is
   int prompt_log2;      // log2 of the rows of a workgroup of that kernel: 8 (7 with 256 dims or in f32), or 5
@@ -68,6 +69,10 @@ template <int KT, bool kPrompt>
 __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   Seq q;
   q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
+  const int before = max(a.row_lo - q.s.r0, 0);  // rows of an earlier launch: tokens to these
+  q.s.n = max(min(q.s.n, a.row_hi - q.s.r0) - before, 0);
+  q.s.r0 += before;
+  q.s.len += before;
   const long long pairs = (long long)q.s.n * a.group;
   if ((a.prompt_rows && pairs >= a.prompt_rows) != kPrompt) q.s.n = 0;
   q.keys = min(q.s.len + q.s.n, a.c.cap);

@@ -51,6 +51,12 @@ constexpr int kPromptKeys = 2560, kPromptKeysF32 = 512;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kJoins = 1 << 20;   // workgroups of the joining launch, beyond which they take several rows each
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
+// Where weights are added up the scores of a pass lie in scratch memory, 4 bytes for each row of a head and each token that the table
+// has room for: a step of more rows than fit into kMostScores is gone through in passes of kLeastPass rows or more (28 heads on 4 of
+// 128 dims, bf16: 8192 rows 5.7 ms with 0.97 GB against 7.5 ms with 7.6 GB at once; 2048 rows on a table for 131072 tokens 1.13 ms with
+// 1.9 GB against 1.00 with 30).
+constexpr size_t kMostScores = (size_t)1 << 30;
+constexpr int kLeastPass = 128;
 
 template <int KT>
 __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
@@ -626,6 +632,7 @@ struct Plan {
   long long items, tiles, grid, key_groups;
   int dt, wide, slot_rows;
   bool join, sliced, others;  // others: rows that are not the prompts' kernel's
+  int pass_rows;              // rows of the step that are gone through at a time
   int prompt_rows, prompt_log2;
   long long prompts;          // its workgroups
   size_t item_off, part_off, state_off, lse_off, dump_off, total;
@@ -633,41 +640,17 @@ struct Plan {
 
 inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// W4A32_OK and what a call takes at most, whatever the device arrays say
-int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, int first, bool accumulate, Plan& p) {
+// The rows' launches over `rows` rows of the step, `most` of a sequence at most
+int plan_rows(const w4a32_paged_cache* c, long long group, long long rows, long long most, long long seqs, int window, int first, bool accumulate, Plan& p) {
   const int kt = c->dtype == W4A32_CACHE_F32 ? 16 : 32;
-  const long long group = r->heads / c->kv_heads, cap = (long long)c->table_ld * c->page;
-  long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
-  p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
-  auto blocks = [&](int log2) { return ((long long)r->rows * group / (1 << log2) + c->n_seqs) * c->kv_heads; };
-  const bool f32 = c->dtype == W4A32_CACHE_F32;
-  const int wide = p.dt == 256 || f32 ? 7 : 8;
-  const int from = r->act_bf16 && p.dt <= 128 ? kPromptWide : kPromptWideSlow;
-  p.prompt_log2 = (f32 ? p.dt != 64 : blocks(wide) >= from) ? wide : 5;
-  p.prompts = blocks(p.prompt_log2);
-  long long keys = cap;  // that a row can see
-  if (window) {
-    const long long near = (long long)first + window;
-    keys = near < cap ? near : cap;
-  }
-  p.prompt_rows = 0;
-  p.others = true;
-  if (!accumulate && most * group >= kPromptRows && (f32 && p.dt != 64 ? blocks(wide) >= from : blocks(5) >= kPromptLeast)) {
-    // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then, as where few
-    // keys are what a row has to go through. Else the rows' kernel has what is left, of so few rows.
-    p.others = r->rows < (long long)r->max_rows * c->n_seqs && keys > (f32 ? kPromptKeysF32 : kPromptKeys) && (kPromptRows - 1) / group > 0;
-    p.prompt_rows = p.others ? kPromptRows : 1;
-    most = p.others ? (kPromptRows - 1) / group : 1;
-    if (p.prompts > most_groups(512)) return W4A32_ESHAPE;
-  }
   // 32 or 64 rows of an item are two or four wavefronts' that ask for the same keys at about the same time: the caches serve
   // all but the first, where as items of their own each would have the keys from memory again. But then fewer of a workgroup's
   // wavefronts share its tiles, so not where there are too few tiles to give every workgroup kMinTiles (16 + 5 rows of 11 heads on
   // 160 tokens: 18 us with 64 rows of an item, 10 with 16).
-  long long tiles = (cap + kt - 1) / kt;
+  long long tiles = ((long long)c->table_ld * c->page + kt - 1) / kt;
   for (p.wide = most * group <= kRows ? 1 : most * group <= 2 * kRows ? 2 : 4;; p.wide /= 2) {
-    const long long of_item = kRows * p.wide, by_seq = (most * group + of_item - 1) / of_item * c->n_seqs,
-                    by_rows = (long long)r->rows * group / of_item + c->n_seqs;
+    const long long of_item = kRows * p.wide, by_seq = (most * group + of_item - 1) / of_item * seqs,
+                    by_rows = rows * group / of_item + seqs;
     p.items = (by_seq < by_rows ? by_seq : by_rows) * c->kv_heads;
     p.slot_rows = (int)(most * group < of_item ? most * group : of_item);
     if (p.wide == 1 || p.items * tiles >= kGrid * kMinTiles) break;
@@ -700,8 +683,42 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   return W4A32_OK;
 }
 
+// W4A32_OK and what a call takes at most, whatever the device arrays say; `room`: scratch memory that there is
+int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, int first, bool accumulate, size_t room, Plan& p) {
+  const long long group = r->heads / c->kv_heads, cap = (long long)c->table_ld * c->page;
+  long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
+  p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
+  auto blocks = [&](int log2) { return ((long long)r->rows * group / (1 << log2) + c->n_seqs) * c->kv_heads; };
+  const bool f32 = c->dtype == W4A32_CACHE_F32;
+  const int wide = p.dt == 256 || f32 ? 7 : 8;
+  const int from = r->act_bf16 && p.dt <= 128 ? kPromptWide : kPromptWideSlow;
+  p.prompt_log2 = (f32 ? p.dt != 64 : blocks(wide) >= from) ? wide : 5;
+  p.prompts = blocks(p.prompt_log2);
+  long long keys = cap;  // that a row can see
+  if (window) {
+    const long long near = (long long)first + window;
+    keys = near < cap ? near : cap;
+  }
+  p.prompt_rows = 0;
+  p.others = true;
+  if (!accumulate && most * group >= kPromptRows && (f32 && p.dt != 64 ? blocks(wide) >= from : blocks(5) >= kPromptLeast)) {
+    // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then, as where few
+    // keys are what a row has to go through. Else the rows' kernel has what is left, of so few rows.
+    p.others = r->rows < (long long)r->max_rows * c->n_seqs && keys > (f32 ? kPromptKeysF32 : kPromptKeys) && (kPromptRows - 1) / group > 0;
+    p.prompt_rows = p.others ? kPromptRows : 1;
+    most = p.others ? (kPromptRows - 1) / group : 1;
+    if (p.prompts > most_groups(512)) return W4A32_ESHAPE;
+  }
+  for (p.pass_rows = r->rows;; p.pass_rows = p.pass_rows > 2 * kLeastPass ? (p.pass_rows / 2 + 63) & -64 : kLeastPass) {
+    const bool whole = p.pass_rows == r->rows;
+    const int e = plan_rows(c, group, p.pass_rows, whole || most < p.pass_rows ? most : p.pass_rows,
+                            whole || c->n_seqs < p.pass_rows ? c->n_seqs : p.pass_rows, window, first, accumulate, p);
+    if (!accumulate || p.pass_rows <= kLeastPass || (e == W4A32_OK && p.total - p.dump_off <= kMostScores && p.total <= room)) return e;
+  }
+}
+
 template <typename Act, typename KV, int DT>
-hipError_t launch(const Attend& a, const Plan& p, bool accumulate, hipStream_t s) {
+hipError_t launch(Attend a, const Plan& p, bool accumulate, hipStream_t s) {
   constexpr size_t lds = lds_bytes<KV, DT>();
   auto kernel = accumulate ? rows_kernel<Act, KV, DT, true> : rows_kernel<Act, KV, DT, false>;
   if constexpr (lds > 64 * 1024) {
@@ -709,18 +726,22 @@ hipError_t launch(const Attend& a, const Plan& p, bool accumulate, hipStream_t s
     if (hipError_t e = limit[accumulate].raise((const void*)kernel, lds); e != hipSuccess) return e;
   }
   if (!p.others) return hipSuccess;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)p.grid), dim3(64 * kWaves), lds, s, a);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (p.join) {
-    auto join = p.sliced ? (accumulate ? join_kernel<Act, DT, 32, true> : join_kernel<Act, DT, 32, false>)
-                         : (accumulate ? join_kernel<Act, DT, DT, true> : join_kernel<Act, DT, DT, false>);
-    const long long units = p.items * p.slot_rows * (p.sliced ? DT / 32 : 1);
-    hipLaunchKernelGGL(join, dim3((unsigned)(units < kJoins ? units : kJoins)), dim3(256), 0, s, a, (unsigned)units);
+  for (a.row_lo = 0; a.row_lo < a.rows; a.row_lo = a.row_hi) {
+    a.row_hi = a.rows - a.row_lo > p.pass_rows ? a.row_lo + p.pass_rows : a.rows;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)p.grid), dim3(64 * kWaves), lds, s, a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    if (p.join) {
+      auto join = p.sliced ? (accumulate ? join_kernel<Act, DT, 32, true> : join_kernel<Act, DT, 32, false>)
+                           : (accumulate ? join_kernel<Act, DT, DT, true> : join_kernel<Act, DT, DT, false>);
+      const long long units = p.items * p.slot_rows * (p.sliced ? DT / 32 : 1);
+      hipLaunchKernelGGL(join, dim3((unsigned)(units < kJoins ? units : kJoins)), dim3(256), 0, s, a, (unsigned)units);
+      if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    }
+    if (!accumulate) continue;
+    hipLaunchKernelGGL((weights_kernel<KV>), dim3((unsigned)p.key_groups), dim3(64 * kWaves), 0, s, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  if (!accumulate) return hipSuccess;
-  hipLaunchKernelGGL((weights_kernel<KV>), dim3((unsigned)p.key_groups), dim3(64 * kWaves), 0, s, a);
-  return hipGetLastError();
+  return hipSuccess;
 }
 template <typename Act, typename KV>
 hipError_t launch_dim(const Attend& a, const Plan& p, bool accumulate, hipStream_t s) {
@@ -746,7 +767,7 @@ extern "C" {
 
 size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accumulate) {
   Plan p;
-  if (check(cache, rows, accumulate) || plan_of(cache, rows, 0, 0, accumulate != 0, p)) return 0;
+  if (check(cache, rows, accumulate) || plan_of(cache, rows, 0, 0, accumulate != 0, SIZE_MAX, p)) return 0;
   return p.total;
 }
 
@@ -755,11 +776,11 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
   if (int e = check(cache, rows, accumulate)) return e;
   if (window < 0 || first < 0 || !(scale * kLog2e - scale * kLog2e == 0.0f) || !d_scratch || !aligned(d_scratch, 16)) return W4A32_EINVAL;
   Plan p;
-  if (int e = plan_of(cache, rows, window, first, accumulate != 0, p)) return e;
+  if (int e = plan_of(cache, rows, window, first, accumulate != 0, scratch_bytes, p)) return e;
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
-                 rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, window, first,
+                 rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, 0, rows->rows, window, first,
                  p.prompt_rows, p.prompt_log2, p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, (unsigned)p.items, (unsigned)p.tiles, scale * kLog2e,
                  (Item*)(scratch + p.item_off), (unsigned*)scratch, (float*)(scratch + p.part_off),
                  (float*)(scratch + p.state_off), (float*)(scratch + p.lse_off), (float*)(scratch + p.dump_off)};
