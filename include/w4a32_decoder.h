@@ -316,13 +316,16 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
  * 16-bit matrix instructions, q and the weights enter as two f16 or three bf16 terms); for bf16 rows the weights enter
  * the second product as bf16, as the output is rounded. `scale` is finite.
  *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time (calls that
- * overlap in time, on two streams or in two graphs, need one each). That is 0 for a call that w4a32_op_paged_attention refuses.
- * With `accumulate` it holds the scores, 4 bytes for each row of a head (rounded up to 16 or
+ * overlap in time, on two streams or in two graphs, need one each). That serves every window; for one window and first, for which
+ * less does, ask w4a32_op_paged_attention_window_scratch_bytes(). Both are 0 for a call that w4a32_op_paged_attention refuses (one
+ * without a window, the former). With `accumulate` it holds the scores, 4 bytes for each row of a head (rounded up to 16 or
  * 64 of a kv head) and token that the table has room for: a step of more than 1 GiB of them is gone through in passes of 128 rows or
  * more, and with scratch memory for fewer rows at once in more passes (each adds its sums to cache->d_weight).
  * QWenAttention::forward, modeling_ds_qwen2.hpp:133-151, per sequence. */
 size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows,
                                               int accumulate);
+size_t w4a32_op_paged_attention_window_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int window,
+                                                     int first, int accumulate);
 int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale, int window,
                              int first, int accumulate, void* d_scratch, size_t scratch_bytes, void* stream);
 

@@ -95,6 +95,7 @@ ABI = {
     "w4a32_decoder_step": (_ci, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "w4a32_op_paged_append": (_ci, [_vp, _vp, _vp, _ci, _vp, _ci, _vp, _vp, _vp, _ci, _ci, _vp]),
     "w4a32_op_paged_attention_scratch_bytes": (_sz, [_vp, _vp, _ci]),
+    "w4a32_op_paged_attention_window_scratch_bytes": (_sz, [_vp, _vp, _ci, _ci, _ci]),
     "w4a32_op_paged_attention": (_ci, [_vp, _vp, ctypes.c_float, _ci, _ci, _ci, _vp, _sz, _vp]),
     "w4a32_op_paged_evict_scratch_bytes": (_sz, [_vp, _ci]),
     "w4a32_op_paged_evict": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _vp, _sz, _vp]),
@@ -903,13 +904,14 @@ def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max
     return out
 
 
-def op_paged_attention_scratch(cache, rows, max_rows, heads, accumulate=False):
-    """Scratch memory of op_paged_attention() for so many rows: kept between calls, not shared by calls that overlap in time."""
+def op_paged_attention_scratch(cache, rows, max_rows, heads, accumulate=False, window=0, first=0):
+    """Scratch memory of op_paged_attention() for so many rows, of any window or of one: kept between calls, not shared by calls that
+    overlap in time."""
     some = cache.args.d_k   # the sizes alone are asked about
     r = PagedRowsArgs(some, rows, max_rows, heads, 0, some, some, heads * cache.dim, heads * cache.dim)
-    need = int(lib().w4a32_op_paged_attention_scratch_bytes(cache._ref, ctypes.byref(r), int(accumulate)))
+    need = int(lib().w4a32_op_paged_attention_window_scratch_bytes(cache._ref, ctypes.byref(r), window, first, int(accumulate)))
     if need == 0:
-        raise W4A32Error("w4a32_op_paged_attention_scratch_bytes: sizes that w4a32_op_paged_attention refuses")
+        raise W4A32Error("w4a32_op_paged_attention_window_scratch_bytes: sizes that w4a32_op_paged_attention refuses")
     return _dev_empty(need)
 
 
@@ -918,11 +920,11 @@ def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, fi
     row j of sequence b sees slots t <= s = cache.length[b] + j with t > s - window or t < first (window 0: all). max_rows: most
     rows of one sequence. accumulate: the weights that the cached tokens receive are added to cache.weight (sequences may share
     pages to be read, but then not with this). out is not q."""
-    if scratch is None:
-        scratch = op_paged_attention_scratch(cache, q.shape[0], max_rows, heads, accumulate)
-    out, r = _paged_rows(cache, q, row_start, max_rows, heads, out)
     if window >> 31 or first >> 31:
         raise W4A32Error(f"window {window} and first {first}: from 0 to 2^31 - 1")
+    if scratch is None:
+        scratch = op_paged_attention_scratch(cache, q.shape[0], max_rows, heads, accumulate, window, first)
+    out, r = _paged_rows(cache, q, row_start, max_rows, heads, out)
     _check(lib().w4a32_op_paged_attention(cache._ref, r, scale, window, first, accumulate, *_scratch_of(scratch, cache.device), _stream()),
            "w4a32_op_paged_attention")
     return out

@@ -765,10 +765,15 @@ using namespace w4::paged;
 
 extern "C" {
 
-size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accumulate) {
+size_t w4a32_op_paged_attention_window_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int window, int first,
+                                                     int accumulate) {
   Plan p;
-  if (check(cache, rows, accumulate) || plan_of(cache, rows, 0, 0, accumulate != 0, SIZE_MAX, p)) return 0;
-  return p.total;
+  if (check(cache, rows, accumulate) || window < 0 || first < 0) return 0;
+  return plan_of(cache, rows, window, first, accumulate != 0, SIZE_MAX, p) ? 0 : p.total;
+}
+
+size_t w4a32_op_paged_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accumulate) {
+  return w4a32_op_paged_attention_window_scratch_bytes(cache, rows, 0, 0, accumulate);
 }
 
 int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale, int window, int first,

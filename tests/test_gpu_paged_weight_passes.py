@@ -46,6 +46,19 @@ def test_passes_follow_the_scratch_memory(pkg):
         assert bool(((weight - got[0][1]).abs()[there] <= 2.0 ** -24 * 2 * (rows * heads // kv) ** 0.5 * (1 + weight[there])).all())
 
 
+def test_a_window_and_its_own_scratch_memory(pkg):
+    """512 rows on a table for 131072 tokens"""
+    B = pm.Batch(50, [2000], [512], 2, 64, 64, table_ld=2048, weights=True)
+    fill_new(B)
+    cache, _, _ = on_gpu(pkg, B, "bf16")
+    own = pkg.op_paged_attention_scratch(cache, 512, 512, 12, True, 1024, 4)
+    every = pkg.op_paged_attention_scratch(cache, 512, 512, 12, True)
+    assert own.numel() < every.numel() // 4
+    run_attention(pkg, B, "f32", "bf16", 12, 1024, 4, accumulate=True, scratch=own)
+    run_attention(pkg, B, "f32", "bf16", 12, 1024, 4, accumulate=True, scratch=every)
+    run_attention(pkg, B, "f32", "bf16", 12, 1024, 4, accumulate=True)
+
+
 def test_a_captured_step_of_passes(pkg):
     heads, kv, dim, rows = 12, 2, 64, 500
     B = pm.Batch(51, [50, 9], [300, 200], kv, dim, 16, table_ld=100, weights=True)
