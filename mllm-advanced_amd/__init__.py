@@ -812,6 +812,20 @@ def _setup():
     _torch = torch
 
 
+def _sizes(*values):
+    """Refuses what an int of the C interface would hold as another number."""
+    for v in values:
+        if v >> 31:
+            raise W4A32Error(f"{v}: sizes go from 0 to 2^31 - 1")
+
+
+def _packed(layout, *values):
+    try:
+        return layout.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise W4A32Error(f"sizes go to 2^31 - 1, numbers are f32: got {values}") from e
+
+
 def _need(t, what, dtype, device, shape=None):
     """Refuses a tensor that is not contiguous, of the type and shape, and on the device whose stream the call goes to."""
     if t.dtype is not dtype or t.get_device() != device or (shape is not None and t.shape != shape) or not t.is_contiguous():
@@ -829,6 +843,8 @@ def _row_ld(t, what, dtype, device, shape=None):
     ld, one = t.stride()
     if one != 1 and t.shape[1] > 1:
         raise W4A32Error(f"{what}: rows of contiguous elements are wanted, got {tuple(t.shape)} with strides {t.stride()}")
+    if ld >> 31:
+        raise W4A32Error(f"{what}: rows less than 2^31 elements apart are wanted, got strides {t.stride()}")
     return ld if t.shape[0] > 1 else t.shape[1]
 
 
@@ -854,6 +870,7 @@ class PagedCache:
         pages, kv, page, dim = k.shape
         _need(k, "k", k.dtype, device), _need(v, "v", k.dtype, device, k.shape), _need(table, "table", _torch.int32, device)
         _need(length, "length", _torch.int32, device, table.shape[:1])
+        _sizes(*k.shape, *table.shape)
         if weight is not None:
             _need(weight, "weight", _torch.float32, device, k.shape[:3])
         self.k, self.v, self.table, self.length, self.weight = k, v, table, length, weight
@@ -880,7 +897,7 @@ def _paged_rows(cache, q, row_start, max_rows, heads, out):
     else:
         ldo = _row_ld(out, "out", dtype, device, q.shape)
     _need(row_start, "row_start", _torch.int32, device, cache.starts)
-    return out, _ROWS_STRUCT.pack(row_start.data_ptr(), rows, max_rows, heads, dtype is _torch.bfloat16, q.data_ptr(), out.data_ptr(), ldq, ldo)
+    return out, _packed(_ROWS_STRUCT, row_start.data_ptr(), rows, max_rows, heads, dtype is _torch.bfloat16, q.data_ptr(), out.data_ptr(), ldq, ldo)
 
 
 def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max_rows=None, out=None):
@@ -896,6 +913,8 @@ def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max
     if sin is not None:
         _need(sin, "sin", _torch.float32, device), _need(cos, "cos", _torch.float32, device, sin.shape)
         positions, rot = sin.shape
+        if positions >> 31 or rot >> 30:
+            raise W4A32Error(f"sin {tuple(sin.shape)}: sizes go to 2^31 - 1")
         d_sin, d_cos, rot = sin.data_ptr(), cos.data_ptr(), 2 * rot
     if pos is not None:
         _need(pos, "pos", _torch.int32, device, (cache.n_seqs,))
@@ -907,6 +926,7 @@ def op_paged_append(cache, q, k, v, row_start, sin=None, cos=None, pos=None, max
 def op_paged_attention_scratch(cache, rows, max_rows, heads, accumulate=False, window=0, first=0):
     """Scratch memory of op_paged_attention() for so many rows, of any window or of one: kept between calls, not shared by calls that
     overlap in time."""
+    _sizes(rows, max_rows, heads, window, first)
     some = cache.args.d_k   # the sizes alone are asked about
     r = PagedRowsArgs(some, rows, max_rows, heads, 0, some, some, heads * cache.dim, heads * cache.dim)
     need = int(lib().w4a32_op_paged_attention_window_scratch_bytes(cache._ref, ctypes.byref(r), window, first, int(accumulate)))
@@ -932,6 +952,7 @@ def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, fi
 
 def op_paged_evict_scratch(cache, budget):
     """Scratch memory of op_paged_evict(), as op_paged_attention_scratch()."""
+    _sizes(budget)
     need = int(lib().w4a32_op_paged_evict_scratch_bytes(cache._ref, budget))
     if need == 0:
         raise W4A32Error("w4a32_op_paged_evict_scratch_bytes: sizes that w4a32_op_paged_evict refuses")
@@ -956,6 +977,7 @@ def op_paged_evict(cache, to, budget, first=0, recent=0, scratch=None):
 
 def op_verify_drafts_scratch(rows, vocab, n_seqs):
     """Scratch memory of op_verify_drafts(), as op_paged_attention_scratch()."""
+    _sizes(rows, vocab, n_seqs)
     need = int(lib().w4a32_op_verify_drafts_scratch_bytes(rows, vocab, n_seqs))
     if need == 0:
         raise W4A32Error("w4a32_op_verify_drafts_scratch_bytes: sizes that w4a32_op_verify_drafts refuses")
@@ -986,9 +1008,8 @@ def op_verify_drafts(logits, row_start, max_rows, tokens, uniform, choice, tempe
     if scratch is None:
         scratch = op_verify_drafts_scratch(rows, vocab, n)
     count, token = row_start.new_empty(n), tokens.new_empty(n)
-    a = _VERIFY_STRUCT.pack(logits.data_ptr(), _ptr(draft) or 0, row_start.data_ptr(), tokens.data_ptr(), _ptr(uniform) or 0,
-                            _ptr(choice) or 0, count.data_ptr(), token.data_ptr(), _ptr(length) or 0, rows, max_rows, n, vocab, ldl, ldd,
-                            temperature)
+    a = _packed(_VERIFY_STRUCT, logits.data_ptr(), _ptr(draft) or 0, row_start.data_ptr(), tokens.data_ptr(), _ptr(uniform) or 0,
+                _ptr(choice) or 0, count.data_ptr(), token.data_ptr(), _ptr(length) or 0, rows, max_rows, n, vocab, ldl, ldd, temperature)
     _check(lib().w4a32_op_verify_drafts(a, *_scratch_of(scratch, device), _stream()), "w4a32_op_verify_drafts")
     return count, token
 
