@@ -42,12 +42,17 @@ constexpr int kAlone = 8;         // tiles up to which items are not shared, whe
 // rows 72 us against 131); from kPromptWideSlow on with f32 rows, two or three terms of each operand (1024 rows 64 us against 76 in favour of
 // 32, 2048 rows 164 against 147), and with 256 dims (16 heads on 4, bf16: 1024 rows 57 against 63, 2048 rows 167 against 115).
 // With an f32 cache and 128 or 256 dims it takes none below that (12 heads on 2: 1000 rows 148 us against 116 of the rows' kernel and its
-// join, 2000 rows 287 against 358).
+// join, 2000 rows 287 against 358). Nor does it with f32 rows on a bf16 cache of 256 dims where a row has over kPromptKeysSpilt keys more
+// than its sequence has rows: three terms of q and 128 sums of a lane do not fit into its registers (98 are spilled with 32 rows of a
+// workgroup, 61 with 128; two terms, on an f16 cache, spill 15 and none). 16 heads on 4, 32 rows of a workgroup against the rows'
+// kernel: 512 rows alone 65 us against 82, behind 256 tokens 95 against 98, behind 4096 544 against 276, of those with a window of 500
+// 68 against 114; 1024 rows alone 140 against 159, behind 256 tokens 179 against 186, behind 4096 1087 against 544. (On an f16
+// cache behind 4096: 512 rows 209 against 250, 1024 421 against 486.)
 constexpr int kPromptRows = 256, kPromptLeast = 128, kPromptWide = 64, kPromptWideSlow = 160;
 // Sequences of fewer rows are its too where a row has at most kPromptKeys keys: it goes through 2560 of them in 33 us with 32 rows
 // of a workgroup and in 50 with more (4096: 54 and 80), beside the others, where the rows' two launches take 9 us for nothing and 17
 // for a row of 4096 (256 + 1 rows, the latter on 4096 keys: 48 us against 30; 1024 + 1: 88 against 56).
-constexpr int kPromptKeys = 2560, kPromptKeysF32 = 512;
+constexpr int kPromptKeys = 2560, kPromptKeysF32 = 512, kPromptKeysSpilt = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kJoins = 1 << 20;   // workgroups of the joining launch, beyond which they take several rows each
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
@@ -701,7 +706,9 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
   }
   p.prompt_rows = 0;
   p.others = true;
-  if (!accumulate && most * group >= kPromptRows && (f32 && p.dt != 64 ? blocks(wide) >= from : blocks(5) >= kPromptLeast)) {
+  const bool spilt = !r->act_bf16 && c->dtype == W4A32_CACHE_BF16 && p.dt == 256 && keys > most + kPromptKeysSpilt;
+  const bool wide_only = (f32 && p.dt != 64) || spilt;
+  if (!accumulate && most * group >= kPromptRows && (wide_only ? blocks(wide) >= from : blocks(5) >= kPromptLeast)) {
     // Where every sequence can have max_rows rows they all do, or the batch is padded: one kernel for all then, as where few
     // keys are what a row has to go through. Else the rows' kernel has what is left, of so few rows.
     p.others = r->rows < (long long)r->max_rows * c->n_seqs && keys > (f32 ? kPromptKeysF32 : kPromptKeys) && (kPromptRows - 1) / group > 0;

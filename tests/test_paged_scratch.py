@@ -49,3 +49,15 @@ def test_a_window_is_enough_where_all_tokens_are_too_many(pkg):
     assert 0 < need(pkg, c, r, 1024, 4, accumulate=0) < GIB
     for bad in ((-1, 0), (0, -1)):
         assert need(pkg, c, r, *bad) == 0
+
+
+def test_which_prompts_share_their_keys(pkg):
+    """The prompts' kernel takes next to no scratch memory, the rows' kernel room for the shares' sums. 256 dims of f32 rows on a bf16 cache,
+    16 heads on 4: the former for a prompt alone, through a small window, or of many rows; the latter on a long context"""
+    def size(tokens, n, window=0, act=0, dtype=None):
+        c, r = batch(pkg, tokens, 1, n, n, heads=16, kv=4, dim=256, dtype=dtype)
+        r.act_bf16 = act
+        return need(pkg, c, r, window, 4, accumulate=0)
+    assert size(512, 512) == size(832, 800) == size(1280, 1024) == size(4608, 512, 500) == size(6144, 2048) == 256
+    assert size(4608, 512) > 1 << 20 and size(5120, 1024) > 1 << 20 and size(4608, 512, 1000) > 1 << 20
+    assert size(4608, 512, act=1) == size(4608, 512, dtype=pkg.CACHE_F16) == 256
