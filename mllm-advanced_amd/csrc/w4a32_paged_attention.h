@@ -307,12 +307,11 @@ __device__ __forceinline__ void store4(void* p, size_t at, f32x4 x) {
   }
 }
 
-// A wavefront's rows' sums lie in LDS ([kRows], `stride` apart; its first row is row0 of the sequence's all_rows, whose tokens follow
-// len cached ones). Of the keys [k0, k0 + keys), the values that are not finite go to the sums of the rows that see them: zeros in
-// their place first, then (`add`) the values. Lanes have dims; all is rare and short but the look at every value.
-template <typename M, typename KV, int kRows>
-__device__ __forceinline__ void put_odd(const Attend& a, const int* table, int hk, int k0, int keys, bool add, float* sums, int stride, int len,
-                                        int row0, int all_rows) {
+// Of the keys [k0, k0 + keys), the values that are not finite to a wavefront's kRows rows that see them, by put(row, dim, value); the
+// first is row0 of the sequence's all_rows, whose tokens follow len cached ones. Lanes have dims; all is rare and short but the look
+// at every value.
+template <typename M, typename KV, int kRows, typename Put>
+__device__ __forceinline__ void put_odd(const Attend& a, const int* table, int hk, int k0, int keys, int len, int row0, int all_rows, Put put) {
 #pragma unroll 1
   for (int key = k0; key < k0 + keys; ++key) {
     const int at = key >> a.c.shift, page = at < a.c.table_ld ? table[at] : -1;
@@ -327,7 +326,7 @@ __device__ __forceinline__ void put_odd(const Attend& a, const int* table, int h
       for (int r = 0; r < min(kRows, all_rows - row0); ++r) {
         const int pos = len + by_group(a, row0 + r);
         if (key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
-        if (odd) sums[r * stride + d] = add ? sums[r * stride + d] + M::widen((Bits<KV>)bits) : 0.0f;
+        if (odd) put(r, d, M::widen((Bits<KV>)bits));
       }
     }
   }

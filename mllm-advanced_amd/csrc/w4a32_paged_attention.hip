@@ -43,8 +43,8 @@ constexpr int kAlone = 8;         // tiles up to which items are not shared, whe
 // 32, 2048 rows 164 against 147), and with 256 dims (16 heads on 4, bf16: 1024 rows 57 against 63, 2048 rows 167 against 115).
 // With an f32 cache and 128 or 256 dims it takes none below that (12 heads on 2: 1000 rows 148 us against 116 of the rows' kernel and its
 // join, 2000 rows 287 against 358). Nor does it with f32 rows on a bf16 cache of 256 dims where a row has over kPromptKeysSpilt keys more
-// than its sequence has rows: three terms of q and 128 sums of a lane do not fit into its registers (98 are spilled with 32 rows of a
-// workgroup, 61 with 128; two terms, on an f16 cache, spill 15 and none). 16 heads on 4, 32 rows of a workgroup against the rows'
+// than its sequence has rows: three terms of q and 128 sums of a lane do not fit into its registers (97 are spilled with 32 rows of a
+// workgroup, 92 with 128; two terms, on an f16 cache, spill 15 and none). 16 heads on 4, 32 rows of a workgroup against the rows'
 // kernel: 512 rows alone 65 us against 82, behind 256 tokens 95 against 98, behind 4096 544 against 276, of those with a window of 500
 // 68 against 114; 1024 rows alone 140 against 159, behind 256 tokens 179 against 186, behind 4096 1087 against 544. (On an f16
 // cache behind 4096: 512 rows 209 against 250, 1024 421 against 486.)
@@ -432,7 +432,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     }
     // Values that are not finite were zeros in the tiles that not every row sees whole; in the others they met weights of several
     // terms, of which one may be 0 or negative and make them NaN. So a row whose sums are not finite, though its weights are
-    // numbers, has those values added up instead.
+    // numbers, has those values added up instead: first zeros in their place, then the values.
     const float strange = (probe[0] + probe[1]) + (probe[2] + probe[3]);
     if (__builtin_expect(odd || __any(real & (l == l) & (strange != strange)), 0)) {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -440,7 +440,10 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
       for (int add = 0; add < 2; ++add)
 #pragma unroll 1
         for (t = seen_from(t_lo + stream); t < t_end; t = seen_from(t + streams))
-          put_odd<M, KV, kRows>(a, table, hk, key_of(t), KT, add != 0, sums, DT + 4, s.len, row0, all_rows);
+          put_odd<M, KV, kRows>(a, table, hk, key_of(t), KT, s.len, row0, all_rows, [&](int r, int d, float v) {
+            float& sum = sums[r * (DT + 4) + d];
+            sum = add ? sum + v : 0.0f;
+          });
     }
     if (grp == 0) {
       states[(wave * kRows + row) * 2] = m;

@@ -435,7 +435,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     gone = next_gone;
   }
 
-  // ---- values that are not finite: as in the rows' kernel, in LDS where the sums go there ----
+  // ---- values that are not finite: as in the rows' kernel, where the results are ----
   l += __shfl_xor(l, 32);
   bool some_odd = odd_flags[wave] != 0;
   if constexpr (!kSplit)  // behind the last arrival's barrier
@@ -447,29 +447,6 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     for (int i = 0; i < 16; ++i) probe[i % 4] = __fmaf_rn(o[d][i], 0.0f, probe[i % 4]);
   const float strange = (probe[0] + probe[1]) + (probe[2] + probe[3]);
   some_odd = some_odd || __any(real & (l == l) & (strange != strange));
-  if constexpr (!kSplit) {
-    if (__builtin_expect(some_odd, 0)) {
-#pragma unroll 1
-      for (int add = 0; add < 2; ++add)
-#pragma unroll 1
-        for (t = team; t < nt; t += kTeams) {
-#pragma unroll 1
-          for (int k = 0; k < KB; ++k) {
-            const int key = key_of(t) + k, at = key >> a.c.shift, pg = at < a.c.table_ld ? table[at] : -1;
-            if (!real || !page_there(a.c, pg) || key > pos || !(a.window == 0 || key > pos - a.window || key < a.first)) continue;
-            const Bits<KV>* v = (const Bits<KV>*)a.c.v + slot_row(a.c, pg, hk, key) * dim;
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int x = 32 * d + 8 * (i / 4) + 4 * half + i % 4;
-                const uint32_t bits = x < dim ? v[x] : 0u;
-                o[d][i] = M::finite(bits) == bits ? o[d][i] : add ? o[d][i] + M::widen((Bits<KV>)bits) : 0.0f;
-              }
-          }
-        }
-    }
-  }
   // ---- results: lane = row, four dims at a time ----
   if constexpr (kSplit) {
     float* sums = (float*)(lds + team * Sh::kTeam);
@@ -486,7 +463,10 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
       for (int add = 0; add < 2; ++add)
 #pragma unroll 1
         for (t = team; t < nt; t += kTeams)
-          put_odd<M, KV, 32>(a, table, hk, key_of(t), KB, add != 0, sums, Sh::kSums, s.len, row0, all_rows);
+          put_odd<M, KV, 32>(a, table, hk, key_of(t), KB, s.len, row0, all_rows, [&](int r, int d, float v) {
+            float& sum = sums[r * Sh::kSums + d];
+            sum = add ? sum + v : 0.0f;
+          });
     }
     if (half == 0) {
       states[(team * 32 + row) * 2] = m;
@@ -511,16 +491,31 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     }
     return;
   }
-  if (!real) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const size_t at = (size_t)(s.r0 + j) * a.ldo + (size_t)head * dim;
+  if (real) {
 #pragma unroll
-  for (int d = 0; d < kDims; ++d)
+    for (int d = 0; d < kDims; ++d)
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int to = 32 * d + 8 * b + 4 * half;
-      if (DT == dim || to < dim) store4<Act>(a.out, at + to, f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]} * inv);
-    }
+      for (int b = 0; b < 4; ++b) {
+        const int to = 32 * d + 8 * b + 4 * half;
+        if (DT == dim || to < dim) store4<Act>(a.out, at + to, f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]} * inv);
+      }
+  }
+  if (__builtin_expect(some_odd, 0)) {
+    const u64 numbers = __ballot(l == l);  // the other rows are NaN
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+#pragma unroll 1
+    for (int add = 0; add < 2; ++add)
+#pragma unroll 1
+      for (t = team; t < nt; t += kTeams)
+        put_odd<M, KV, 32>(a, table, hk, key_of(t), KB, s.len, row0, all_rows, [&](int r, int d, float v) {
+          if (!(numbers >> r & 1)) return;
+          const int of = row0 + r, token = by_group(a, of);
+          Act* to = (Act*)a.out + (size_t)(s.r0 + token) * a.ldo + (size_t)(hk * (int)group + of - token * (int)group) * dim + d;
+          *to = add ? (Act)((float)*to + v) : (Act)0.0f;
+        });
+  }
 }
 
 template <typename Act, typename KV, int DT, bool kSplit>
