@@ -314,7 +314,8 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
  * and over the heads of its kv head, in a fixed order (the same call gives the same bits).
  *   Sums, maxima and products are f32 at f32 accuracy for f32 rows (a 16-bit cache's elements are exact operands of the
  * 16-bit matrix instructions, q and the weights enter as two f16 or three bf16 terms); for bf16 rows the weights enter
- * the second product as bf16, as the output is rounded. `scale` is finite.
+ * the second product as bf16, as the output is rounded. `scale` is finite. Scores are within f32's range, and so are a row's sums of
+ * values, which weigh up to 2^8 each before they are divided: values below 2^100 are safe on any cache.
  *   d_scratch: w4a32_op_paged_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time (calls that
  * overlap in time, on two streams or in two graphs, need one each). That serves every window; for one window and first, for which
  * less does, ask w4a32_op_paged_attention_window_scratch_bytes(). Both are 0 for a call that w4a32_op_paged_attention refuses (one

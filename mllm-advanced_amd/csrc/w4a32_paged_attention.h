@@ -208,7 +208,9 @@ using Bits = typename std::conditional<sizeof(KV) == 2, uint16_t, uint32_t>::typ
 template <typename Act, typename KV>
 struct Math;
 
-// bf16: three truncations hold the 24 bits of an f32 whatever its exponent
+// bf16: three truncations hold the 24 bits of an f32 whatever its exponent. Rows of bf16 are operands as they are, and their weights,
+// whose sum is f32, are rounded to one bf16 (half a step, 2^-8 at most, of signs that cancel): less than the rounding of the result, which is
+// bf16 too (against 64 bits 1.8e-3 for one row on a long context and 2.3e-3 for a prompt, 1.7e-3 with exact weights), for a third of the products.
 template <typename Act>
 struct Math<Act, __bf16> {
   static constexpr int kTerms = sizeof(Act) == 4 ? 3 : 1;

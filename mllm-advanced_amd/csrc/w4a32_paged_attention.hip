@@ -19,7 +19,7 @@
 // which costs no time: a 16-bit tile of head size 128 is 16 kilobytes for 16 to 48 instructions of 16 clocks.
 //
 // What bounds it: memory where contexts are long: one row each of 64 sequences of 500 to 8000 tokens, 28 heads on 4 of 128 dims in
-// bf16 (559 MB): 108 us, 5.2 TB/s, and 5 for the join; one row on 131001 tokens, 12 heads on 2, f32 on f16 (134 MB): 27 us, 4.9 TB/s,
+// bf16 (559 MB): 109 us, 5.1 TB/s, and 5 for the join; one row on 131001 tokens, 12 heads on 2, f32 on f16 (134 MB): 25 us, 5.3 TB/s,
 // and 6. Below that a chain of waits: one row on 60 tokens takes 7.3 us, of which 1.4 are the launch, 0.6 the deal, 1.6 the
 // place and q, 0.6 the keys and values, 1.9 the tile and 1.5 the wavefronts' join and the store.
 #include "w4a32_paged_attention.h"

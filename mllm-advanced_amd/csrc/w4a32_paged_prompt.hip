@@ -25,7 +25,7 @@
 // Where there are few such workgroups, one has 32 rows instead, and each of its four wavefronts (two where the head has 256 dims)
 // takes every fourth tile by itself, with no barrier; their softmax states are joined through LDS at the end.
 // An f32 cache has tiles of 32 keys and v_mfma_f32_32x32x2, to which a lane gives one element of K or V: a tile of 128 dims
-// costs a SIMD 128 x 64 = 8192 clocks per wavefront, beside which the rest is small (4096 rows, 28 heads on 4: 0.97 ms, 124 TFLOP/s, where
+// costs a SIMD 128 x 64 = 8192 clocks per wavefront, beside which the rest is small (4096 rows, 28 heads on 4: 0.95 ms, 126 TFLOP/s, where
 // the rows' kernel takes 3.15). 64 dims are always taken in the second way (2600 rows of 14 heads: 179 us against 237), 128 and 256, for
 // which LDS has not the room, always in the first, with 128 rows of a workgroup.
 #include "w4a32_paged_attention.h"
