@@ -719,12 +719,19 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int window, i
     most = p.others ? (kPromptRows - 1) / group : 1;
     if (p.prompts > most_groups(512)) return W4A32_ESHAPE;
   }
-  for (p.pass_rows = r->rows;; p.pass_rows = p.pass_rows > 2 * kLeastPass ? (p.pass_rows / 2 + 63) & -64 : kLeastPass) {
-    const bool whole = p.pass_rows == r->rows;
-    const int e = plan_rows(c, group, p.pass_rows, whole || most < p.pass_rows ? most : p.pass_rows,
-                            whole || c->n_seqs < p.pass_rows ? c->n_seqs : p.pass_rows, window, first, accumulate, p);
-    if (!accumulate || p.pass_rows <= kLeastPass || (e == W4A32_OK && p.total - p.dump_off <= kMostScores && p.total <= room)) return e;
-  }
+  auto pass_of = [&](int rows) {
+    const bool whole = rows == r->rows;
+    p.pass_rows = rows;
+    return plan_rows(c, group, rows, whole || most < rows ? most : rows, whole || c->n_seqs < rows ? c->n_seqs : rows, window, first, accumulate, p);
+  };
+  if (!accumulate || r->rows <= kLeastPass) return pass_of(r->rows);
+  // The longest passes whose scores fit, or take no more than those of the shortest: many sequences' rows do not get fewer
+  const int least = pass_of(kLeastPass);
+  if (least) return least;
+  const size_t scores = p.total - p.dump_off > kMostScores ? p.total - p.dump_off : kMostScores;
+  for (int rows = r->rows; rows > kLeastPass; rows = rows > 2 * kLeastPass ? (rows / 2 + 63) & -64 : kLeastPass)
+    if (pass_of(rows) == W4A32_OK && p.total - p.dump_off <= scores && p.total <= room) return W4A32_OK;
+  return pass_of(kLeastPass);
 }
 
 template <typename Act, typename KV, int DT>
