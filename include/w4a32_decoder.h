@@ -310,8 +310,9 @@ int w4a32_op_paged_append(const w4a32_paged_cache* cache, const w4a32_paged_rows
 /* out = softmax(scale q K^T) V per head over what a row sees: row j of sequence b, which stands at slot s = d_len[b] + j
  * (appended before the call), sees slots t <= s with t > s - window or t < first (window 0: all). A row that sees nothing
  * gets zeros; what is not finite reaches only the rows that see it (a value as in the formula, an infinity of a token with next to no
- * weight too; an infinity in q or in a key may make a row NaN where a score of -infinity would leave the token out). With `accumulate` the weights are added to cache->d_weight: for every cached token the sum over the rows
- * and over the heads of its kv head, in a fixed order (the same call gives the same bits).
+ * weight too; an infinity in q or in a key may make a row NaN where a score of -infinity would leave the token out). With
+ * `accumulate` the weights are added to cache->d_weight: for every cached token the sum over the rows and over the heads of its kv
+ * head, in a fixed order (the same call gives the same bits).
  *   Sums, maxima and products are f32 at f32 accuracy for f32 rows (a 16-bit cache's elements are exact operands of the
  * 16-bit matrix instructions, q and the weights enter as two f16 or three bf16 terms); for bf16 rows the weights enter
  * the second product as bf16, as the output is rounded. `scale` is finite. Scores are within f32's range, and so are a row's sums of
