@@ -344,6 +344,53 @@ size_t w4a32_op_paged_evict_scratch_bytes(const w4a32_paged_cache* cache, int bu
 int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache* to, int budget, int first, int recent,
                          int* d_kept, void* d_scratch, size_t scratch_bytes, void* stream);
 
+/* Pages handed out, shared and taken back. Of every page of the pool d_refs [n_pages] says how many places of the table name it:
+ * 0 is a free page, and a page with a negative number is someone else's, never handed out, moved or counted (tables may name it: rows
+ * that would be written to it get a copy). A fresh pool has zeros there, -1 in the table and lengths 0; these two operators keep
+ * all of it true. Layers have pools of their own and one table: they are called once, and w4a32_op_paged_copy for all layers.
+ *
+ * Fork. Sequence b becomes the first min(length, d_keep[b]) tokens of sequence d_parent[b], as all of them were before the call,
+ * with room for its rows of the coming step (d_row_start, as the step will have them):
+ *   - places with its tokens name the parent's pages, which it shares from then on;
+ *   - a page that its rows will write is its own: where others name it too (or it is someone else's) it is replaced, and what it
+ *     holds of the sequence's tokens is to be copied. Of sequences that all leave a page the last one keeps it;
+ *   - places behind its tokens that its rows need get free pages, places behind those are -1, and pages that nobody names any
+ *     more are free. Pages are handed out in the order of the places, the lowest free number first.
+ * d_parent NULL: each goes on from itself. A parent outside [0, n_seqs): an empty sequence (a sequence that has ended; a new one, if it has
+ * rows). d_keep NULL: all tokens; fewer take back what a step wrote too much. d_row_start NULL: no rows (rows and max_rows unused).
+ * A place whose page is not there stays so where the sequence has tokens; what the table has no place for gets none.
+ *   d_table and d_len are written, d_moves gets the pages to be copied, (from, to), -1 behind them, and d_counts their number
+ * and how many pages were missing. Where that is not 0 nothing else has changed, and the rows must not be appended.
+ * n_seqs * table_ld and n_pages are at most 2^26.
+ *   d_scratch: w4a32_op_paged_fork_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time.
+ * The reference frees a model's cache as a whole (KVCacheOp.cpp:44-72). */
+typedef struct {
+  const int* d_parent;      /* [n_seqs], or NULL */
+  const int* d_keep;        /* [n_seqs], or NULL */
+  const int* d_row_start;   /* [n_seqs + 1], or NULL */
+  int* d_refs;              /* [n_pages] */
+  int* d_moves;             /* [n_seqs][2] */
+  int* d_counts;            /* [2] */
+  int rows, max_rows;       /* as in w4a32_paged_rows */
+} w4a32_paged_fork_args;
+size_t w4a32_op_paged_fork_scratch_bytes(const w4a32_paged_cache* cache, int rows);
+int w4a32_op_paged_fork(const w4a32_paged_cache* cache, const w4a32_paged_fork_args* args, void* d_scratch,
+                        size_t scratch_bytes, void* stream);
+
+/* In each of n_caches caches of the same sizes (the layers') page d_moves[i][1] becomes a copy of page d_moves[i][0], keys,
+ * values and weights (which all have, or none), for i < d_count[0] <= most; pairs of which one is outside the pool are left out. No page is copied to twice, nor
+ * from and to: so are the lists of the other two operators. `caches` is host memory, read during the call. */
+int w4a32_op_paged_copy(const w4a32_paged_cache* const* caches, int n_caches, const int* d_moves, const int* d_count,
+                        int most, void* stream);
+
+/* Compaction: with U pages in use, those with numbers from U on move, in order, to the free numbers below U, in order; pages of
+ * someone else stay. Tables and d_refs are renamed, d_moves [n_pages / 2][2] gets the pages to be copied, (from, to), -1 behind them,
+ * and d_counts [2] their number and the number behind the last page in use: the pool can end there.
+ *   d_scratch: w4a32_op_paged_compact_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time. */
+size_t w4a32_op_paged_compact_scratch_bytes(const w4a32_paged_cache* cache);
+int w4a32_op_paged_compact(const w4a32_paged_cache* cache, int* d_refs, int* d_moves, int* d_counts, void* d_scratch,
+                           size_t scratch_bytes, void* stream);
+
 /* Verification of drafted tokens. Sequence b's rows are its last token and then the tokens drafted behind it (d_tokens
  * [rows]); row r's logits (f32 [rows][ldl]) judge token r + 1. With p = softmax(logits / temperature) and q the draft
  * model's distribution, softmax(d_draft[r] / temperature) (f32 [rows][ldd], a sequence's last row is not read; NULL: the
@@ -372,6 +419,28 @@ typedef struct {
 } w4a32_verify_args;
 size_t w4a32_op_verify_drafts_scratch_bytes(int rows, int vocab, int n_seqs);
 int w4a32_op_verify_drafts(const w4a32_verify_args* args, void* d_scratch, size_t scratch_bytes, void* stream);
+
+/* Of rows of logits z (f32, f16 or bf16), with p = softmax(z / temperature): the given token's log probability and its rank (how many
+ * tokens are more probable, or as probable with a lower index), the row's entropy - sum p ln p, and the `top` most probable tokens in
+ * order (equal ones by index) with their log probabilities. d_tokens NULL: no token is given; d_logprob, d_rank and d_entropy may be NULL,
+ * d_top_* where top is 0. A token outside the vocabulary has log probability -infinity and rank -1, as have, with token -1, places
+ * behind the last token of a probability above 0 (top may pass the vocabulary). Where a logit is NaN or +infinity, or all are
+ * -infinity, there is no distribution: NaN, rank -1 and tokens -1. Natural logarithms; off by 1e-6 and the rounding of the result.
+ * temperature: 1e-30 .. 1e30; top <= 1024. Per row what AutoLLM.hpp:70-88 does without saying how sure it was.
+ *   d_scratch: w4a32_op_token_logprobs_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time. */
+typedef struct {
+  const void* d_logits;       /* [rows][ldl] of `dtype` */
+  const int64_t* d_tokens;    /* [rows], or NULL */
+  float* d_logprob;           /* [rows], or NULL */
+  int* d_rank;                /* [rows], or NULL */
+  float* d_entropy;           /* [rows], or NULL */
+  int64_t* d_top_token;       /* [rows][top] */
+  float* d_top_logprob;       /* [rows][top] */
+  int rows, vocab, ldl, dtype, top;   /* dtype: W4A32_CACHE_* */
+  double temperature;
+} w4a32_logprobs_args;
+size_t w4a32_op_token_logprobs_scratch_bytes(int rows, int vocab, int top);
+int w4a32_op_token_logprobs(const w4a32_logprobs_args* args, void* d_scratch, size_t scratch_bytes, void* stream);
 
 /* ---- decoder runner -------------------------------------------------------------------- */
 

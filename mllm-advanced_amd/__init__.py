@@ -99,6 +99,13 @@ ABI = {
     "w4a32_op_paged_attention": (_ci, [_vp, _vp, ctypes.c_float, _ci, _ci, _ci, _vp, _sz, _vp]),
     "w4a32_op_paged_evict_scratch_bytes": (_sz, [_vp, _ci]),
     "w4a32_op_paged_evict": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _vp, _sz, _vp]),
+    "w4a32_op_paged_fork_scratch_bytes": (_sz, [_vp, _ci]),
+    "w4a32_op_paged_fork": (_ci, [_vp, _vp, _vp, _sz, _vp]),
+    "w4a32_op_paged_copy": (_ci, [_vp, _ci, _vp, _vp, _ci, _vp]),
+    "w4a32_op_paged_compact_scratch_bytes": (_sz, [_vp]),
+    "w4a32_op_paged_compact": (_ci, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "w4a32_op_token_logprobs_scratch_bytes": (_sz, [_ci, _ci, _ci]),
+    "w4a32_op_token_logprobs": (_ci, [_vp, _vp, _sz, _vp]),
     "w4a32_op_verify_drafts_scratch_bytes": (_sz, [_ci, _ci, _ci]),
     "w4a32_op_verify_drafts": (_ci, [_vp, _vp, _sz, _vp]),
     # include/w4a32_layered.h
@@ -157,6 +164,18 @@ class VerifyArgs(ctypes.Structure):
                                                "d_next", "d_len")] + \
                [(n, ctypes.c_int) for n in ("rows", "max_rows", "n_seqs", "vocab", "ldl", "ldd")] + \
                [("temperature", ctypes.c_float)]
+
+
+class ForkArgs(ctypes.Structure):
+    """w4a32_paged_fork_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_parent", "d_keep", "d_row_start", "d_refs", "d_moves", "d_counts")] + \
+               [(n, ctypes.c_int) for n in ("rows", "max_rows")]
+
+
+class LogprobsArgs(ctypes.Structure):
+    """w4a32_logprobs_args"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_logits", "d_tokens", "d_logprob", "d_rank", "d_entropy", "d_top_token", "d_top_logprob")] + \
+               [(n, ctypes.c_int) for n in ("rows", "vocab", "ldl", "dtype", "top")] + [("temperature", ctypes.c_double)]
 
 
 class DecoderConfig(ctypes.Structure):
@@ -800,6 +819,8 @@ def decode_linear(x, packed_list, n_list, norm_weight=None, eps=1e-6, delta=None
 _torch = _device = _kinds = None
 _ROWS_STRUCT = struct.Struct("@P4iPP2i")                # w4a32_paged_rows
 _VERIFY_STRUCT = struct.Struct("@9P6if4x")              # w4a32_verify_args
+_FORK_STRUCT = struct.Struct("@6P2i")                   # w4a32_paged_fork_args
+_LOGPROBS_STRUCT = struct.Struct("@7P5id")              # w4a32_logprobs_args
 
 
 def _setup():
@@ -878,7 +899,7 @@ class PagedCache:
         self.args = PagedCacheArgs(k.data_ptr(), v.data_ptr(), _ptr(weight), table.data_ptr(), length.data_ptr(), _kinds[k.dtype],
                                    pages, page, kv, dim, table.shape[0], table.shape[1])
         self.starts = (table.shape[0] + 1,)   # shape of the row starts
-        self._ref = ctypes.byref(self.args)
+        self._ref, self._address = ctypes.byref(self.args), ctypes.addressof(self.args)
 
 
 def _paged_rows(cache, q, row_start, max_rows, heads, out):
@@ -975,6 +996,80 @@ def op_paged_evict(cache, to, budget, first=0, recent=0, scratch=None):
     return kept
 
 
+def op_paged_fork_scratch(cache, rows=0):
+    """Scratch memory of op_paged_fork() for so many rows, as op_paged_attention_scratch()."""
+    _sizes(rows)
+    need = int(lib().w4a32_op_paged_fork_scratch_bytes(cache._ref, rows))
+    if need == 0:
+        raise W4A32Error("w4a32_op_paged_fork_scratch_bytes: sizes that w4a32_op_paged_fork refuses")
+    return _dev_empty(need)
+
+
+def op_paged_fork(cache, refs, parent=None, keep=None, row_start=None, rows=0, max_rows=None, scratch=None):
+    """Every sequence b becomes the first keep[b] tokens (None: all) of sequence parent[b] (None: itself; outside the batch: empty), with room
+    for its rows row_start[b] .. row_start[b + 1] of the coming step (`rows` in all, max_rows of one) in pages of its own. refs int32 [pages]:
+    how many places of the table name a page (0: free, negative: never touched). Writes cache.table, cache.length and refs; returns
+    (moves, counts): moves int32 [sequences][2], the pages to be copied with op_paged_copy() in all layers, -1 behind them, and counts int32 [2],
+    their number and how many pages were missing (where that is not 0, nothing has changed)."""
+    device, i32, n = _device(), _torch.int32, cache.n_seqs
+    if cache.device != device:
+        raise W4A32Error(f"the cache is on device {cache.device}, the current one is {device}")
+    _need(refs, "refs", i32, device, cache.k.shape[:1])
+    if parent is not None:
+        _need(parent, "parent", i32, device, (n,))
+    if keep is not None:
+        _need(keep, "keep", i32, device, (n,))
+    if row_start is not None:
+        _need(row_start, "row_start", i32, device, cache.starts)
+    if scratch is None:
+        scratch = op_paged_fork_scratch(cache, rows if row_start is not None else 0)
+    moves, counts = cache.table.new_empty((n, 2)), cache.table.new_empty(2)
+    a = _packed(_FORK_STRUCT, _ptr(parent) or 0, _ptr(keep) or 0, _ptr(row_start) or 0, refs.data_ptr(), moves.data_ptr(), counts.data_ptr(), rows,
+                rows if max_rows is None else max_rows)
+    _check(lib().w4a32_op_paged_fork(cache._ref, a, *_scratch_of(scratch, device), _stream()), "w4a32_op_paged_fork")
+    return moves, counts
+
+
+def op_paged_copy(caches, moves, counts):
+    """In every one of `caches` (the layers', of the same sizes) page moves[i][1] becomes a copy of page moves[i][0], weights included, for
+    i < counts[0]: what op_paged_fork() and op_paged_compact() return."""
+    device, many = _device(), (caches,) if isinstance(caches, PagedCache) else tuple(caches)
+    if not many or any(c.device != device for c in many):
+        raise W4A32Error(f"caches on device {device}, the current one, are wanted")
+    if moves.ndim != 2 or moves.shape[1] != 2 or counts.numel() < 1:
+        raise W4A32Error(f"moves is [pairs][2] and counts has their number first: got {tuple(moves.shape)}, {tuple(counts.shape)}")
+    _need(moves, "moves", _torch.int32, device), _need(counts, "counts", _torch.int32, device)
+    if moves.shape[0] == 0:
+        return
+    _sizes(*moves.shape)
+    refs = (ctypes.c_void_p * len(many))(*[c._address for c in many])
+    _check(lib().w4a32_op_paged_copy(refs, len(many), moves.data_ptr(), counts.data_ptr(), moves.shape[0], _stream()), "w4a32_op_paged_copy")
+
+
+def op_paged_compact_scratch(cache):
+    """Scratch memory of op_paged_compact(), as op_paged_attention_scratch()."""
+    need = int(lib().w4a32_op_paged_compact_scratch_bytes(cache._ref))
+    if need == 0:
+        raise W4A32Error("w4a32_op_paged_compact_scratch_bytes: sizes that w4a32_op_paged_compact refuses")
+    return _dev_empty(need)
+
+
+def op_paged_compact(cache, refs, scratch=None):
+    """The pages in use move to the lowest numbers: cache.table and refs (as op_paged_fork() has them) are renamed. Returns (moves, counts): moves
+    int32 [pages / 2][2], the pages to be copied with op_paged_copy() in all layers, -1 behind them, and counts int32 [2], their number and the
+    number behind the last page in use."""
+    device = _device()
+    if cache.device != device:
+        raise W4A32Error(f"the cache is on device {cache.device}, the current one is {device}")
+    _need(refs, "refs", _torch.int32, device, cache.k.shape[:1])
+    if scratch is None:
+        scratch = op_paged_compact_scratch(cache)
+    moves, counts = cache.table.new_empty((cache.k.shape[0] // 2, 2)), cache.table.new_empty(2)
+    _check(lib().w4a32_op_paged_compact(cache._ref, refs.data_ptr(), moves.data_ptr() or None, counts.data_ptr(), *_scratch_of(scratch, device),
+                                        _stream()), "w4a32_op_paged_compact")
+    return moves, counts
+
+
 def op_verify_drafts_scratch(rows, vocab, n_seqs):
     """Scratch memory of op_verify_drafts(), as op_paged_attention_scratch()."""
     _sizes(rows, vocab, n_seqs)
@@ -1012,6 +1107,41 @@ def op_verify_drafts(logits, row_start, max_rows, tokens, uniform, choice, tempe
                 _ptr(choice) or 0, count.data_ptr(), token.data_ptr(), _ptr(length) or 0, rows, max_rows, n, vocab, ldl, ldd, temperature)
     _check(lib().w4a32_op_verify_drafts(a, *_scratch_of(scratch, device), _stream()), "w4a32_op_verify_drafts")
     return count, token
+
+
+def op_token_logprobs_scratch(rows, vocab, top=0):
+    """Scratch memory of op_token_logprobs(), as op_paged_attention_scratch()."""
+    _sizes(rows, vocab, top)
+    need = int(lib().w4a32_op_token_logprobs_scratch_bytes(rows, vocab, top))
+    if need == 0:
+        raise W4A32Error("w4a32_op_token_logprobs_scratch_bytes: sizes that w4a32_op_token_logprobs refuses")
+    return _dev_empty(need)
+
+
+def op_token_logprobs(logits, tokens=None, top=0, temperature=1.0, scratch=None):
+    """logits [rows][vocab] (f32, f16 or bf16), tokens int64 [rows] -> (logprob f32 [rows], rank int32 [rows], entropy f32 [rows], top_tokens
+    int64 [rows][top], top_logprobs f32 [rows][top]) of softmax(logits / temperature): the tokens' log probabilities and how many tokens come
+    before them (None without tokens), the rows' entropies, and the most probable tokens in order, equal ones by index (None with top 0)."""
+    if _torch is None:
+        _setup()
+    device, kind, f32 = _device(), _kinds.get(logits.dtype), _torch.float32
+    if kind is None:
+        raise W4A32Error(f"logits are f32, f16 or bf16, not {logits.dtype}")
+    ldl = _row_ld(logits, "logits", logits.dtype, device)
+    rows, vocab = logits.shape
+    logprob = rank = top_tokens = top_logprobs = None
+    if scratch is None:
+        scratch = op_token_logprobs_scratch(rows, vocab, top)
+    entropy = logits.new_empty(rows, dtype=f32)
+    if tokens is not None:
+        _need(tokens, "tokens", _torch.int64, device, (rows,))
+        logprob, rank = logits.new_empty(rows, dtype=f32), logits.new_empty(rows, dtype=_torch.int32)
+    if top:
+        top_tokens, top_logprobs = logits.new_empty((rows, top), dtype=_torch.int64), logits.new_empty((rows, top), dtype=f32)
+    a = _packed(_LOGPROBS_STRUCT, logits.data_ptr(), _ptr(tokens) or 0, _ptr(logprob) or 0, _ptr(rank) or 0, entropy.data_ptr(),
+                _ptr(top_tokens) or 0, _ptr(top_logprobs) or 0, rows, vocab, ldl, kind, top, temperature)
+    _check(lib().w4a32_op_token_logprobs(a, *_scratch_of(scratch, device), _stream()), "w4a32_op_token_logprobs")
+    return logprob, rank, entropy, top_tokens, top_logprobs
 
 
 class Decoder:

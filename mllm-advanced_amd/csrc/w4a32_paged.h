@@ -49,5 +49,28 @@ __device__ __forceinline__ size_t slot_row(const Cache& c, int page, int head, i
 }
 __device__ __forceinline__ bool page_there(const Cache& c, int page) { return (unsigned)page < (unsigned)c.n_pages; }
 
+// Sums of a workgroup's threads up to this one, and of all
+template <int kThreads>
+__device__ __forceinline__ unsigned block_scan(unsigned x, unsigned* in_wave, unsigned& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned upto = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned y = __shfl_up(upto, o);
+    if (lane >= o) upto += y;
+  }
+  __syncthreads();  // in_wave may still be read
+  if (lane == 63) in_wave[wave] = upto;
+  __syncthreads();
+  unsigned before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    before += w < wave ? in_wave[w] : 0;
+    total += in_wave[w];
+  }
+  return before + upto;
+}
+
 }  // namespace paged
 }  // namespace w4

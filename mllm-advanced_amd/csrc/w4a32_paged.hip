@@ -196,28 +196,6 @@ constexpr int kCopies = 4;  // tokens of a thread
 constexpr int kSelect = 1024;
 constexpr int kHeld = 32 * 1024;
 
-// Sums of all threads up to this one, and of all
-__device__ __forceinline__ unsigned block_scan(unsigned x, unsigned* in_wave, unsigned& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned upto = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned y = __shfl_up(upto, o);
-    if (lane >= o) upto += y;
-  }
-  __syncthreads();  // in_wave may still be read
-  if (lane == 63) in_wave[wave] = upto;
-  __syncthreads();
-  unsigned before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kSelect / 64; ++w) {
-    before += w < wave ? in_wave[w] : 0;
-    total += in_wave[w];
-  }
-  return before + upto;
-}
-
 template <bool kInLds>
 __global__ __launch_bounds__(kSelect) void select_kernel(Evict a) {
   extern __shared__ __attribute__((aligned(16))) unsigned keys[];
@@ -256,7 +234,7 @@ __global__ __launch_bounds__(kSelect) void select_kernel(Evict a) {
       const int top = (1 << bits) - 1 - tid * each;
       unsigned sum = 0, all;
       for (int i = 0; i < each; ++i) sum += hist[top - i];
-      const unsigned upto = block_scan(sum, in_wave, all);
+      const unsigned upto = block_scan<kSelect>(sum, in_wave, all);
       unsigned above = upto - sum;
       if (above < want && upto >= want) {
         for (int i = 0; i < each; ++i) {
@@ -285,9 +263,9 @@ __global__ __launch_bounds__(kSelect) void select_kernel(Evict a) {
     ties += inner && k == prefix;
     sure += t < lo || t >= hi || (inner && k > prefix);
   }
-  unsigned rank = block_scan(ties, in_wave, all) - ties;
+  unsigned rank = block_scan<kSelect>(ties, in_wave, all) - ties;
   const unsigned stays = sure + min(ties, want - min(want, rank));
-  unsigned to = block_scan(stays, in_wave, all) - stays;
+  unsigned to = block_scan<kSelect>(stays, in_wave, all) - stays;
   for (int t = t0; t < t1; ++t) {
     const bool inner = any && t >= lo && t < hi;
     const uint32_t k = inner ? key_at(t) : 0;
