@@ -331,6 +331,22 @@ size_t w4a32_op_paged_attention_window_scratch_bytes(const w4a32_paged_cache* ca
 int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale, int window,
                              int first, int accumulate, void* d_scratch, size_t scratch_bytes, void* stream);
 
+/* w4a32_op_paged_attention (without window and added-up weights) for a batch whose sequences share prefixes: group g is sequences
+ * d_group_start[g] .. d_group_start[g + 1] (n_groups of them, at most n_seqs; sequences outside all groups share nothing), and its first
+ * d_prefix[g] tokens are read once for all of its rows, from the pages of the group's first sequence; each sequence has its own tokens
+ * from there on, the rest of the page in which the prefix ends among them. As a fork of one sequence leaves it, the prefix being what they all had
+ * then, or less. A prefix beyond the length of one of the group's sequences with rows is cut to that, so that a row sees what
+ * it would see alone, as long as the tables name the same tokens. Same results as w4a32_op_paged_attention up to the order of sums: maxima and sums are
+ * f32, and each of the two parts is divided by nothing until they are joined. Group starts do not decrease; where they do, what the
+ * rows get is unspecified.
+ *   d_scratch: w4a32_op_paged_prefix_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time; 0 for a call that is
+ * refused. It holds the sums, dim (rounded up to 64, 128 or 256) * 4 bytes for each row of a head and, below 256 workgroups, for each
+ * share of a prefix that the chip is filled with. */
+size_t w4a32_op_paged_prefix_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int n_groups);
+int w4a32_op_paged_prefix_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale,
+                                    const int* d_group_start, const int* d_prefix, int n_groups, void* d_scratch,
+                                    size_t scratch_bytes, void* stream);
+
 /* Of every sequence's tokens `budget` stay, per kv head: the first `first` ones, the last `recent` ones and of the others
  * those with the largest added-up weight (of equal ones the earlier; NaN counts as +infinity). Their keys, values and
  * weights go in order to slots 0, 1, .. of the sequence in `to` (same sizes; pages that no table of `cache` names: what is

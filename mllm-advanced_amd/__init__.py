@@ -97,6 +97,8 @@ ABI = {
     "w4a32_op_paged_attention_scratch_bytes": (_sz, [_vp, _vp, _ci]),
     "w4a32_op_paged_attention_window_scratch_bytes": (_sz, [_vp, _vp, _ci, _ci, _ci]),
     "w4a32_op_paged_attention": (_ci, [_vp, _vp, ctypes.c_float, _ci, _ci, _ci, _vp, _sz, _vp]),
+    "w4a32_op_paged_prefix_attention_scratch_bytes": (_sz, [_vp, _vp, _ci]),
+    "w4a32_op_paged_prefix_attention": (_ci, [_vp, _vp, ctypes.c_float, _vp, _vp, _ci, _vp, _sz, _vp]),
     "w4a32_op_paged_evict_scratch_bytes": (_sz, [_vp, _ci]),
     "w4a32_op_paged_evict": (_ci, [_vp, _vp, _ci, _ci, _ci, _vp, _vp, _sz, _vp]),
     "w4a32_op_paged_fork_scratch_bytes": (_sz, [_vp, _ci]),
@@ -968,6 +970,32 @@ def op_paged_attention(cache, q, row_start, max_rows, heads, scale, window=0, fi
     out, r = _paged_rows(cache, q, row_start, max_rows, heads, out)
     _check(lib().w4a32_op_paged_attention(cache._ref, r, scale, window, first, accumulate, *_scratch_of(scratch, cache.device), _stream()),
            "w4a32_op_paged_attention")
+    return out
+
+
+def op_paged_prefix_attention_scratch(cache, rows, max_rows, heads, n_groups):
+    """Scratch memory of op_paged_prefix_attention(), as op_paged_attention_scratch()."""
+    _sizes(rows, max_rows, heads, n_groups)
+    some = cache.args.d_k   # the sizes alone are asked about
+    r = PagedRowsArgs(some, rows, max_rows, heads, 0, some, some, heads * cache.dim, heads * cache.dim)
+    need = int(lib().w4a32_op_paged_prefix_attention_scratch_bytes(cache._ref, ctypes.byref(r), n_groups))
+    if need == 0:
+        raise W4A32Error("w4a32_op_paged_prefix_attention_scratch_bytes: sizes that w4a32_op_paged_prefix_attention refuses")
+    return _dev_empty(need)
+
+
+def op_paged_prefix_attention(cache, q, row_start, max_rows, heads, scale, group_start, prefix, scratch=None, out=None):
+    """op_paged_attention() of a batch whose sequences share prefixes: group_start int32 [groups + 1], sequences group_start[g] ..
+    group_start[g + 1] have their first prefix[g] tokens (prefix int32 [groups]) in common. Those are read once for all of the group's rows, from the
+    pages of its first sequence, and the others from each sequence's own."""
+    device, n = cache.device, prefix.numel()
+    if scratch is None:
+        scratch = op_paged_prefix_attention_scratch(cache, q.shape[0], max_rows, heads, n)
+    out, r = _paged_rows(cache, q, row_start, max_rows, heads, out)
+    _need(prefix, "prefix", _torch.int32, device, (n,)), _need(group_start, "group_start", _torch.int32, device, (n + 1,))
+    _sizes(n)
+    _check(lib().w4a32_op_paged_prefix_attention(cache._ref, r, scale, group_start.data_ptr(), prefix.data_ptr(), n,
+                                                 *_scratch_of(scratch, device), _stream()), "w4a32_op_paged_prefix_attention")
     return out
 
 

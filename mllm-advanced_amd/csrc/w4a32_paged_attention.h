@@ -22,6 +22,22 @@ struct Item {
   int r0, row0, rows, head;  // first row of the sequence, first of the item among (token, head of the group), their number, kv head
 };
 
+// Groups of sequences with a prefix in common: what the first of their launches leaves to the others
+struct PrefixGroup {
+  int b, r0, n, tokens;       // the sequence whose pages have it, the group's rows, the prefix
+  int first, shares, blocks;  // workgroup of its first share, shares of an item, items of a kv head
+  int pad;
+};
+struct Prefix {
+  int* total;           // workgroups that have a share
+  PrefixGroup* group;   // [n_groups]
+  int* from;            // [n_seqs]: the first token that a sequence reads by itself
+  int* group_of;        // [n_seqs]: -1 where that is 0
+  int* item_seq;        // [items of the sequences' own tokens]: whose they are
+  float *part, *state;  // [workgroups][rows of an item][dt], [..][2]: as those of a share
+  int n_groups;
+};
+
 struct Attend {
   Cache c;
   const void* q;
@@ -44,6 +60,7 @@ struct Attend {
   float* state;         // [2 grid][slot_rows][2]: maxima (log2) and sums of weights
   float* lse;           // [item][slot_rows] (accumulate)
   float* dump;          // [tile of an item][wide][lane][keys of the tile / 4]: scores (accumulate)
+  Prefix prefix;        // of groups of sequences
 };
 
 // x / group for x below 2^30, as x m / 2^(30 + l) with 2^l >= group > 2^(l - 1) and m the next whole number from 2^(30 + l) / group:
@@ -62,10 +79,13 @@ struct Seq {
   int keys;        // tokens there are once the rows are appended
   int ft, w0, nt;  // tiles; at least one where there are rows
   int items;       // per kv head
+  int from;        // kOwn: the first token
 };
 
-// kPrompt: the sequences of the prompts' kernel, in items of 1 << prompt_log2 rows; else the others
-template <int KT, bool kPrompt>
+// kPrompt: the sequences of the prompts' kernel, in items of 1 << prompt_log2 rows; kRest: the others; kOwn: all, and of their tokens those
+// behind a prefix
+enum Which { kRest, kPrompt, kOwn };
+template <int KT, Which kWhich>
 __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   Seq q;
   q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
@@ -74,15 +94,19 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
   q.s.r0 += before;
   q.s.len += before;
   const long long pairs = (long long)q.s.n * a.group;
-  if ((a.prompt_rows && pairs >= a.prompt_rows) != kPrompt) q.s.n = 0;
+  if (kWhich != kOwn && (a.prompt_rows && pairs >= a.prompt_rows) != (kWhich == kPrompt)) q.s.n = 0;
   q.keys = min(q.s.len + q.s.n, a.c.cap);
-  const int log2 = kPrompt ? a.prompt_log2 : 4 + a.wide;
+  const int log2 = kWhich == kPrompt ? a.prompt_log2 : 4 + a.wide;
   q.items = q.s.n ? (int)((pairs + (1 << log2) - 1) >> log2) : 0;
   q.w0 = 0;
   q.ft = 0;
   if (a.window) {
     q.w0 = max(0, min(q.s.len, a.c.cap - 1) - a.window + 1) / KT;
     q.ft = min((min(a.first, a.c.cap) + KT - 1) / KT, q.w0);
+  }
+  if constexpr (kWhich == kOwn) {
+    q.from = a.prefix.from[b];
+    q.w0 = min(q.from, a.c.cap - 1) / KT;
   }
   q.nt = q.s.n ? q.ft + (q.keys + KT - 1) / KT - q.w0 : 0;
   return q;
@@ -118,7 +142,7 @@ struct Place {
 };
 
 // The sequences of a block of 64, one of each lane: kept where there is one block only.
-template <int KT, bool kPrompt = false>
+template <int KT, Which kWhich = kRest>
 struct Seqs {
   Seq q;
   unsigned tiles, items;
@@ -127,7 +151,7 @@ struct Seqs {
     q = {};
     tiles = items = 0;
     if (b < a.c.n_seqs) {
-      q = seq_of<KT, kPrompt>(a, b);
+      q = seq_of<KT, kWhich>(a, b);
       const u64 n = (u64)q.items * a.c.kv_heads;
       items = (unsigned)min(n, (u64)0xffffffffu);
       tiles = (unsigned)min(n * q.nt, (u64)0xffffffffu);
@@ -135,8 +159,8 @@ struct Seqs {
   }
 };
 
-template <int KT, bool kPrompt>
-__device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT, kPrompt>& s, unsigned u, Unit unit, unsigned per) {
+template <int KT, Which kWhich>
+__device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT, kWhich>& s, unsigned u, Unit unit, unsigned per) {
   Place p;
   p.there = false;
   p.tile0 = p.item0 = 0;
@@ -144,7 +168,8 @@ __device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT, kPrompt>& s,
     auto from = [&](int x) { return __builtin_amdgcn_readfirstlane(x); };
     p.b = 0;
     p.inner = u;
-    p.q = {{from(s.q.s.r0), from(s.q.s.n), from(s.q.s.len)}, from(s.q.keys), from(s.q.ft), from(s.q.w0), from(s.q.nt), from(s.q.items)};
+    p.q = {{from(s.q.s.r0), from(s.q.s.n), from(s.q.s.len)}, from(s.q.keys), from(s.q.ft), from(s.q.w0), from(s.q.nt), from(s.q.items), 0};
+    if constexpr (kWhich == kOwn) p.q.from = from(s.q.from);
     const unsigned each = unit == kTiles ? p.q.nt : unit == kShares ? (p.q.nt + per - 1) / per : unit == kItems ? 1 : (p.q.nt + kWaves - 1) / kWaves;
     p.there = u < each * (unsigned)a.c.kv_heads * (unit == kKeyTiles ? 1 : p.q.items);
     return p;
@@ -173,6 +198,7 @@ __device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT, kPrompt>& s,
       p.q.w0 = from(s.q.w0);
       p.q.nt = from(s.q.nt);
       p.q.items = from(s.q.items);
+      if constexpr (kWhich == kOwn) p.q.from = from(s.q.from);
       return p;
     }
     before = add_sat(before, last_lane(upto));
@@ -348,6 +374,19 @@ __device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, 
 
 // The prompts' kernel over the sequences of at least a.prompt_rows pairs (w4a32_paged_prompt.hip); items: its most workgroups
 hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s);
+// The same kernel over the prefixes of a.prefix
+hipError_t launch_prefixes(const Attend& a, int dtype, bool act_bf16, int dt, unsigned groups, hipStream_t s);
+inline int prefix_keys(int dtype, int dt, int log2) { return log2 == 5 || dtype == W4A32_CACHE_F32 ? 32 : dt == 256 ? 64 : 128; }  // of its tiles
+
+// The rows' kernel over what sequences have behind their prefixes, all of whose sums go to scratch memory
+struct OwnPlan {
+  long long items, tiles;
+  unsigned grid, slots;  // slots: rooms for an item's sums; the first are those of shares, then one for each item that is not shared
+  int wide, slot_rows, dt;
+};
+int plan_own(const w4a32_paged_cache* c, const w4a32_paged_rows* r, OwnPlan& o);
+hipError_t launch_own(const Attend& a, const OwnPlan& o, int dtype, bool act_bf16, hipStream_t s);
+constexpr int kOwnSlots = 1024;  // of shares: two of a workgroup
 
 }  // namespace paged
 }  // namespace w4

@@ -63,8 +63,8 @@ constexpr int kFew = 16;          // tiles of a share up to which it has tiles o
 constexpr size_t kMostScores = (size_t)1 << 30;
 constexpr int kLeastPass = 128;
 
-template <int KT>
-__device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT>& s) {
+template <int KT, Which kWhich>
+__device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT, kWhich>& s) {
   Deal d = {0, 0, 0, false};
   bool all_short = true;
   if (a.c.n_seqs == 1) {  // nothing to add up: a decode step of one sequence is all latency
@@ -101,7 +101,7 @@ struct Sight {
 };
 template <int KT>
 __device__ __forceinline__ Sight sight_of(const Attend& a, const Seq& q, int lo, int hi) {
-  if (a.window == 0) return {0, 0, hi / KT + 1};
+  if (a.window == 0) return {0, 0, hi / KT + 1 - q.w0};
   return {(min(a.first, a.c.cap) + KT - 1) / KT, q.ft + max(0, lo - a.window + 1) / KT - q.w0, q.ft + hi / KT - q.w0 + 1};
 }
 
@@ -117,8 +117,9 @@ constexpr size_t wave_lds() {  // a wavefront's tile of V; at the end its 16 row
 template <typename KV, int DT>
 constexpr size_t lds_bytes() { return kWaves * (wave_lds<KV, DT>() + kRows * 2 * sizeof(float)); }
 
-// DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up.
-template <typename Act, typename KV, int DT, bool kDump>
+// DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up. kWhich == kOwn: the tokens
+// behind a prefix, whose sums another launch joins with the prefix's.
+template <typename Act, typename KV, int DT, bool kDump, Which kWhich = kRest>
 __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(Attend a) {
   using M = Math<Act, KV>;
   constexpr int KT = tile_keys<KV>(), NT = M::kTerms, kHalves = KT / 16;
@@ -133,8 +134,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
   // wavefronts that share rows, and which of them this one is
   const int streams = kWaves >> a.wide, stream = wave >> a.wide, wide = 1 << a.wide;
 
-  Seqs<KT> seqs;
-  const Deal deal = deal_of<KT>(a, seqs);
+  Seqs<KT, kWhich> seqs;
+  const Deal deal = deal_of(a, seqs);
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.count = deal.per ? deal.items : 0;
   if (deal.per == 0) return;
   unsigned u = blockIdx.x, u_end = max(deal.items, gridDim.x);
@@ -295,7 +296,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         there = there && cur[h] >= 0;
       }
       // every key seen by every row, or each looked at
-      const bool whole = there && k0 + KT - 1 <= pos_min && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
+      auto in_front = [&](int key) { return kWhich == kOwn && key < p.q.from; };  // in the prefix
+      const bool whole = there && k0 + KT - 1 <= pos_min && !in_front(k0) && (a.window == 0 || k0 > pos_max - a.window || k0 + KT - 1 < a.first);
       if (!whole) {
         asm volatile("");
         uint32_t top = 0;  // the signs' places: whether a value is not finite
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i) {
           const int in = (64 * i + lane) / kPerKey, key = k0 + in;
-          const bool none = ((kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0) | (key > pos_max) |
+          const bool none = ((kHalves == 1 ? cur[0] : in < 16 ? cur[0] : cur[kHalves - 1]) < 0) | (key > pos_max) | in_front(key) |
                             ((a.window != 0) & (key <= pos_min - a.window) & (key >= a.first));
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -360,7 +362,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int key = k0 + 16 * h + 4 * grp + i;
-            const bool sees = real & (cur[h] >= 0) & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first));
+            const bool sees = real & (cur[h] >= 0) & (key <= pos) & !in_front(key) & ((a.window == 0) | (key > pos - a.window) | (key < a.first));
             seen |= sees ? 1u << (4 * h + i) : 0u;
           }
       }
@@ -439,11 +441,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
 #pragma unroll 1
       for (int add = 0; add < 2; ++add)
 #pragma unroll 1
-        for (t = seen_from(t_lo + stream); t < t_end; t = seen_from(t + streams))
-          put_odd<M, KV, kRows>(a, table, hk, key_of(t), KT, s.len, row0, all_rows, [&](int r, int d, float v) {
+        for (t = seen_from(t_lo + stream); t < t_end; t = seen_from(t + streams)) {
+          const int before = kWhich == kOwn ? max(p.q.from - key_of(t), 0) : 0;
+          put_odd<M, KV, kRows>(a, table, hk, key_of(t) + before, KT - before, s.len, row0, all_rows, [&](int r, int d, float v) {
             float& sum = sums[r * (DT + 4) + d];
             sum = add ? sum + v : 0.0f;
           });
+        }
     }
     if (grp == 0) {
       states[(wave * kRows + row) * 2] = m;
@@ -455,7 +459,10 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
     // workgroup one begins there and the other does not.
     const int rows = min(all_rows - of0, kRows << a.wide);
     const int slot = 2 * (int)blockIdx.x + (t_lo == 0);
-    if (t_lo == 0 && threadIdx.x == 0) a.item[p.item0 + item] = Item{w_first, shares, s.r0, of0, rows, hk};
+    if (t_lo == 0 && threadIdx.x == 0) {
+      a.item[p.item0 + item] = Item{w_first, shares, s.r0, of0, rows, hk};
+      if constexpr (kWhich == kOwn) a.prefix.item_seq[p.item0 + item] = p.b;
+    }
     constexpr int kPer = DT / 4;  // threads of a row
     for (int i = threadIdx.x; i < rows * kPer; i += 64 * kWaves) {
       const int r = i / kPer, d = i % kPer * 4, w0 = r / kRows;
@@ -468,8 +475,8 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(At
         sum += f * states[(w * kRows + r % kRows) * 2 + 1];
         acc += fmaxf(f, kLeast) * *(const f32x4*)((const float*)(lds + w * wave_lds<KV, DT>()) + (r % kRows) * (DT + 4) + d);
       }
-      if (shares > 1) {
-        const size_t at = (size_t)slot * a.slot_rows + r;
+      if (kWhich == kOwn || shares > 1) {
+        const size_t at = (size_t)(kWhich == kOwn && shares == 1 ? kOwnSlots + (int)(p.item0 + item) : slot) * a.slot_rows + r;
         *(W4_GLOBAL f32x4*)(a.part + at * DT + d) = acc;
         if (d == 0) {
           a.state[2 * at] = top;
@@ -577,7 +584,7 @@ template <typename KV>
 __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
   Seqs<KT> seqs;
-  if (deal_of<KT>(a, seqs).per == 0) return;
+  if (deal_of(a, seqs).per == 0) return;
   const Place p = place_of(a, seqs, blockIdx.x, kKeyTiles, 1);
   if (!p.there) return;
   const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = (int)p.inner / per_head;
@@ -767,6 +774,24 @@ hipError_t launch_dim(const Attend& a, const Plan& p, bool accumulate, hipStream
   return launch<Act, KV, 256>(a, p, accumulate, s);
 }
 
+template <typename Act, typename KV, int DT>
+hipError_t launch_rest(const Attend& a, const OwnPlan& o, hipStream_t s) {
+  constexpr size_t lds = lds_bytes<KV, DT>();
+  auto kernel = rows_kernel<Act, KV, DT, false, kOwn>;
+  if constexpr (lds > 64 * 1024) {
+    static LdsLimitOnce limit;
+    if (hipError_t e = limit.raise((const void*)kernel, lds); e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(kernel, dim3(o.grid), dim3(64 * kWaves), lds, s, a);
+  return hipGetLastError();
+}
+template <typename Act, typename KV>
+hipError_t launch_rest_dim(const Attend& a, const OwnPlan& o, hipStream_t s) {
+  if (o.dt == 64) return launch_rest<Act, KV, 64>(a, o, s);
+  if (o.dt == 128) return launch_rest<Act, KV, 128>(a, o, s);
+  return launch_rest<Act, KV, 256>(a, o, s);
+}
+
 int check(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accumulate) {
   if (int e = check_rows(cache, rows)) return e;
   if (!rows->d_q || !rows->d_out) return W4A32_EINVAL;
@@ -774,6 +799,24 @@ int check(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int accu
   return W4A32_OK;
 }
 }  // namespace
+
+int plan_own(const w4a32_paged_cache* c, const w4a32_paged_rows* r, OwnPlan& o) {
+  static_assert(kOwnSlots == 2 * kGrid, "two shares of a workgroup can lie in scratch memory");
+  Plan p;
+  p.dt = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
+  p.others = true;
+  const long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
+  if (int e = plan_rows(c, r->heads / c->kv_heads, r->rows, most, c->n_seqs, 0, 0, false, p)) return e;
+  o = {p.items, p.tiles, (unsigned)p.grid, (unsigned)(kOwnSlots + p.items), p.wide == 4 ? 2 : p.wide - 1, p.slot_rows, p.dt};
+  return W4A32_OK;
+}
+
+hipError_t launch_own(const Attend& a, const OwnPlan& o, int dtype, bool act_bf16, hipStream_t s) {
+  if (act_bf16) return launch_rest_dim<__bf16, __bf16>(a, o, s);
+  if (dtype == W4A32_CACHE_F32) return launch_rest_dim<float, float>(a, o, s);
+  if (dtype == W4A32_CACHE_F16) return launch_rest_dim<float, _Float16>(a, o, s);
+  return launch_rest_dim<float, __bf16>(a, o, s);
+}
 
 }  // namespace paged
 }  // namespace w4

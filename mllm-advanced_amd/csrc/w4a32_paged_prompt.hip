@@ -84,7 +84,8 @@ __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
 #pragma clang diagnostic pop
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
-template <typename Act, typename KV, int DT, bool kSplit>
+// kPrefix: a workgroup has a share of the keys of a prefix, for rows of all sequences of the group, and leaves its sums in scratch memory
+template <typename Act, typename KV, int DT, bool kSplit, bool kPrefix = false>
 __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 || kSplit ? 1 : 2) void prompt_kernel(Attend a) {
   using M = Math<Act, KV>;
   using Sh = Shape<Act, KV, DT, kSplit>;
@@ -103,62 +104,78 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
   const int team = wave / Sh::kMembers, member = wave % Sh::kMembers, team_tid = member * 64 + lane;
 
   // ---- which rows ----
-  Seqs<KB, true> seqs;
-  unsigned total = 0;
-  for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
-    seqs.load(a, b0);
-    total = add_sat(total, last_lane(wave_scan(seqs.items)));
-  }
-  if (blockIdx.x >= total) return;
   const unsigned group = a.group, kv = a.c.kv_heads;
-  const unsigned order = blockIdx.x / kv;
-  const int hk = (int)(blockIdx.x - order * kv);
   Place p;
-  int block;
-  if (a.c.n_seqs > 1 && a.c.n_seqs <= 64) {
-    // The blocks of all sequences by the last key that they see, most keys first: the position from which on `order` blocks
-    // or fewer are left is searched for, all sequences counting at once.
-    const Seq& q = seqs.q;
-    const int len = min(q.s.len, a.c.cap);
-    auto from = [&](int end) {  // this lane's blocks whose last row stands at `end` or behind
-      if (!q.items || end > len + q.s.n - 1) return 0u;
-      const long long need = (long long)(end - len) * a.group + 1;  // pairs up to the first that stands there
-      return (unsigned)(q.items - (need <= 0 ? 0 : (int)((need + kBlock - 1) / kBlock) - 1));
-    };
-    int lo = 0, hi = a.c.cap + a.max_rows;  // from(lo) counts more than `order`, from(hi) does not
-    while (hi - lo > 1) {
-      const int mid = lo + (hi - lo) / 2;
-      if (last_lane(wave_scan(from(mid))) > order)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    const unsigned more = from(hi), mine = from(lo) - more;
-    const unsigned before = last_lane(wave_scan(more)), upto = wave_scan(mine);
-    const u64 found = __ballot(before + upto > order);
-    if (!found) return;
-    const int at = __builtin_ctzll(found);
-    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-    p.b = at;
-    p.q.s = {of(q.s.r0), of(q.s.n), of(q.s.len)};
-    const unsigned nth = order - before - (unsigned)of((int)(upto - mine));
-    block = of(q.items) - 1 - of((int)more) - (int)nth;
+  int block, hk, first_tile = 0, end_tile = 0;
+  if constexpr (kPrefix) {
+    const Prefix& x = a.prefix;
+    if ((int)blockIdx.x >= *x.total) return;
+    int before = 0;  // the last group whose first workgroup is this one or stands in front of it; groups without any are passed over
+    for (int g0 = 0; g0 < x.n_groups; g0 += 64) before += __popcll(__ballot(g0 + lane < x.n_groups && x.group[g0 + lane].first <= (int)blockIdx.x));
+    const PrefixGroup g = x.group[before - 1];
+    const unsigned in = blockIdx.x - g.first, in_kv = in / kv, share = in_kv / g.blocks;
+    hk = (int)(in - in_kv * kv);
+    block = (int)(in_kv - share * g.blocks);
+    const int tiles = (g.tokens + KB - 1) / KB;
+    first_tile = (int)((long long)tiles * share / g.shares);
+    end_tile = (int)((long long)tiles * (share + 1) / g.shares);
+    p.b = g.b;
+    p.q.s = {g.r0, g.n, g.tokens - 1};
   } else {
-    p = place_of(a, seqs, (total / kv - 1 - order) * kv + hk, kItems, 1);
-    if (!p.there) return;
-    block = (int)(p.inner / kv);
+    Seqs<KB, kPrompt> seqs;
+    unsigned total = 0;
+    for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+      seqs.load(a, b0);
+      total = add_sat(total, last_lane(wave_scan(seqs.items)));
+    }
+    if (blockIdx.x >= total) return;
+    const unsigned order = blockIdx.x / kv;
+    hk = (int)(blockIdx.x - order * kv);
+    if (a.c.n_seqs > 1 && a.c.n_seqs <= 64) {
+      // The blocks of all sequences by the last key that they see, most keys first: the position from which on `order` blocks
+      // or fewer are left is searched for, all sequences counting at once.
+      const Seq& q = seqs.q;
+      const int len = min(q.s.len, a.c.cap);
+      auto from = [&](int end) {  // this lane's blocks whose last row stands at `end` or behind
+        if (!q.items || end > len + q.s.n - 1) return 0u;
+        const long long need = (long long)(end - len) * a.group + 1;  // pairs up to the first that stands there
+        return (unsigned)(q.items - (need <= 0 ? 0 : (int)((need + kBlock - 1) / kBlock) - 1));
+      };
+      int lo = 0, hi = a.c.cap + a.max_rows;  // from(lo) counts more than `order`, from(hi) does not
+      while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2;
+        if (last_lane(wave_scan(from(mid))) > order)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      const unsigned more = from(hi), mine = from(lo) - more;
+      const unsigned before = last_lane(wave_scan(more)), upto = wave_scan(mine);
+      const u64 found = __ballot(before + upto > order);
+      if (!found) return;
+      const int at = __builtin_ctzll(found);
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+      p.b = at;
+      p.q.s = {of(q.s.r0), of(q.s.n), of(q.s.len)};
+      const unsigned nth = order - before - (unsigned)of((int)(upto - mine));
+      block = of(q.items) - 1 - of((int)more) - (int)nth;
+    } else {
+      p = place_of(a, seqs, (total / kv - 1 - order) * kv + hk, kItems, 1);
+      if (!p.there) return;
+      block = (int)(p.inner / kv);
+    }
   }
   const Span s = p.q.s;
   const int all_rows = s.n * (int)group, of0 = block * kBlock, row0 = of0 + 32 * member, in_seq = row0 + row;
   const bool real = in_seq < all_rows;
-  auto slot_of = [&](int r) { return s.len + by_group(a, min(r, all_rows - 1)); };
+  auto slot_of = [&](int r) { return kPrefix ? s.len : s.len + by_group(a, min(r, all_rows - 1)); };  // a prefix is seen whole
   const int j = by_group(a, min(in_seq, all_rows - 1)), head = hk * a.group + (real ? in_seq - j * a.group : 0);
-  const int pos = s.len + j, pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
+  const int pos = kPrefix ? s.len : s.len + j, pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
   const int block_min = slot_of(of0), block_max = slot_of(of0 + kBlock - 1);
   // tiles that the workgroup's rows can see: [0, ft) and [w0, ..), of those that the table has
   const int w0 = a.window ? max(0, min(block_min, a.c.cap - 1) - a.window + 1) / KB : 0;
   const int ft = a.window ? min((min(a.first, a.c.cap) + KB - 1) / KB, w0) : 0;
-  const int nt = ft + min(block_max, a.c.cap - 1) / KB + 1 - w0;
+  const int nt = kPrefix ? end_tile : ft + min(block_max, a.c.cap - 1) / KB + 1 - w0;
   auto key_of = [&](int t) { return (t < ft ? t : t - ft + w0) * KB; };
 
   // ---- q ----
@@ -306,7 +323,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  int t = __builtin_amdgcn_readfirstlane(team), n = 0, gone = 0;
+  int t = first_tile + __builtin_amdgcn_readfirstlane(team), n = 0, gone = 0;
   find(t);
   if (t < nt) {
     gone = load(t, 0);
@@ -447,6 +464,7 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
     for (int i = 0; i < 16; ++i) probe[i % 4] = __fmaf_rn(o[d][i], 0.0f, probe[i % 4]);
   const float strange = (probe[0] + probe[1]) + (probe[2] + probe[3]);
   some_odd = some_odd || __any(real & (l == l) & (strange != strange));
+  auto odd_keys = [&](int t) { return kPrefix ? min(KB, s.len + 1 - key_of(t)) : KB; };
   // ---- results: lane = row, four dims at a time ----
   if constexpr (kSplit) {
     float* sums = (float*)(lds + team * Sh::kTeam);
@@ -462,8 +480,8 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
 #pragma unroll 1
       for (int add = 0; add < 2; ++add)
 #pragma unroll 1
-        for (t = team; t < nt; t += kTeams)
-          put_odd<M, KV, 32>(a, table, hk, key_of(t), KB, s.len, row0, all_rows, [&](int r, int d, float v) {
+        for (t = first_tile + team; t < nt; t += kTeams)
+          put_odd<M, KV, 32>(a, table, hk, key_of(t), odd_keys(t), s.len, row0, all_rows, [&](int r, int d, float v) {
             float& sum = sums[r * Sh::kSums + d];
             sum = add ? sum + v : 0.0f;
           });
@@ -487,7 +505,45 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
         sum += f * states[(w * 32 + r) * 2 + 1];
         acc += fmaxf(f, kLeast) * *(const f32x4*)((const float*)(lds + w * Sh::kTeam) + r * Sh::kSums + d);
       }
-      finish<Act, false>(a, s.r0, of0 + r, hk, 0, d, acc, base, sum);
+      if constexpr (kPrefix) {
+        const size_t at = (size_t)blockIdx.x * kBlock + r;
+        *(W4_GLOBAL f32x4*)(a.prefix.part + at * DT + d) = acc;
+        if (d == 0) {
+          a.prefix.state[2 * at] = top - (float)kWeight;
+          a.prefix.state[2 * at + 1] = sum;
+        }
+      } else {
+        finish<Act, false>(a, s.r0, of0 + r, hk, 0, d, acc, base, sum);
+      }
+    }
+    return;
+  }
+  if constexpr (kPrefix) {
+    const size_t at = (size_t)blockIdx.x * kBlock + 32 * member + row;
+    float* part = a.prefix.part + at * DT;
+    if (real) {
+#pragma unroll
+      for (int d = 0; d < kDims; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          *(W4_GLOBAL f32x4*)(part + 32 * d + 8 * b + 4 * half) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
+      if (half == 0) {
+        a.prefix.state[2 * at] = m - (float)kWeight;
+        a.prefix.state[2 * at + 1] = l;
+      }
+    }
+    if (__builtin_expect(some_odd, 0)) {
+      const u64 numbers = __ballot(l == l);  // the other rows are NaN
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+#pragma unroll 1
+      for (int add = 0; add < 2; ++add)
+#pragma unroll 1
+        for (t = first_tile; t < nt; ++t)
+          put_odd<M, KV, 32>(a, table, hk, key_of(t), odd_keys(t), s.len, row0, all_rows, [&](int r, int d, float v) {
+            if (!(numbers >> r & 1)) return;
+            float& sum = a.prefix.part[((size_t)blockIdx.x * kBlock + 32 * member + r) * DT + d];
+            sum = add ? sum + v : 0.0f;
+          });
     }
     return;
   }
@@ -518,36 +574,43 @@ __global__ __launch_bounds__((Shape<Act, KV, DT, kSplit>::kThreads), DT == 256 |
   }
 }
 
-template <typename Act, typename KV, int DT, bool kSplit>
+template <typename Act, typename KV, int DT, bool kSplit, bool kPrefix>
 hipError_t launch(const Attend& a, unsigned items, hipStream_t s) {
   using Sh = Shape<Act, KV, DT, kSplit>;
   if constexpr (Sh::kLds > 64 * 1024) {
     static LdsLimitOnce limit;
-    if (hipError_t e = limit.raise((const void*)prompt_kernel<Act, KV, DT, kSplit>, Sh::kLds); e != hipSuccess) return e;
+    if (hipError_t e = limit.raise((const void*)prompt_kernel<Act, KV, DT, kSplit, kPrefix>, Sh::kLds); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT, kSplit>), dim3(items), dim3(Sh::kThreads), Sh::kLds, s, a);
+  hipLaunchKernelGGL((prompt_kernel<Act, KV, DT, kSplit, kPrefix>), dim3(items), dim3(Sh::kThreads), Sh::kLds, s, a);
   return hipGetLastError();
 }
-template <typename Act, typename KV, bool kSplit>
+template <typename Act, typename KV, bool kSplit, bool kPrefix>
 hipError_t launch_dim(const Attend& a, int dt, unsigned items, hipStream_t s) {
-  if (dt == 64) return launch<Act, KV, 64, kSplit>(a, items, s);
-  if (dt == 128) return launch<Act, KV, 128, kSplit>(a, items, s);
-  return launch<Act, KV, 256, kSplit>(a, items, s);
+  if (dt == 64) return launch<Act, KV, 64, kSplit, kPrefix>(a, items, s);
+  if (dt == 128) return launch<Act, KV, 128, kSplit, kPrefix>(a, items, s);
+  return launch<Act, KV, 256, kSplit, kPrefix>(a, items, s);
 }
-template <typename Act, typename KV>
+template <typename Act, typename KV, bool kPrefix>
 hipError_t launch_shape(const Attend& a, int dt, unsigned items, hipStream_t s) {
-  return a.prompt_log2 == 5 ? launch_dim<Act, KV, true>(a, dt, items, s) : launch_dim<Act, KV, false>(a, dt, items, s);
+  return a.prompt_log2 == 5 ? launch_dim<Act, KV, true, kPrefix>(a, dt, items, s) : launch_dim<Act, KV, false, kPrefix>(a, dt, items, s);
+}
+template <bool kPrefix>
+hipError_t launch_types(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s) {
+  if (dtype == W4A32_CACHE_F32) {
+    if (dt == 64) return launch<float, float, 64, true, kPrefix>(a, items, s);
+    return dt == 128 ? launch<float, float, 128, false, kPrefix>(a, items, s) : launch<float, float, 256, false, kPrefix>(a, items, s);
+  }
+  if (act_bf16) return launch_shape<__bf16, __bf16, kPrefix>(a, dt, items, s);
+  if (dtype == W4A32_CACHE_F16) return launch_shape<float, _Float16, kPrefix>(a, dt, items, s);
+  return launch_shape<float, __bf16, kPrefix>(a, dt, items, s);
 }
 }  // namespace
 
 hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s) {
-  if (dtype == W4A32_CACHE_F32) {
-    if (dt == 64) return launch<float, float, 64, true>(a, items, s);
-    return dt == 128 ? launch<float, float, 128, false>(a, items, s) : launch<float, float, 256, false>(a, items, s);
-  }
-  if (act_bf16) return launch_shape<__bf16, __bf16>(a, dt, items, s);
-  if (dtype == W4A32_CACHE_F16) return launch_shape<float, _Float16>(a, dt, items, s);
-  return launch_shape<float, __bf16>(a, dt, items, s);
+  return launch_types<false>(a, dtype, act_bf16, dt, items, s);
+}
+hipError_t launch_prefixes(const Attend& a, int dtype, bool act_bf16, int dt, unsigned groups, hipStream_t s) {
+  return launch_types<true>(a, dtype, act_bf16, dt, groups, s);
 }
 
 }  // namespace paged
