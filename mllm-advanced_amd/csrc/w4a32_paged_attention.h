@@ -28,12 +28,17 @@ struct PrefixGroup {
   int first, shares, blocks;  // workgroup of its first share, shares of an item, items of a kv head
   int pad;
 };
+// What the join has to know of an item of own tokens: the shares of its own, and those of the prefix
+struct OwnItem {
+  Item own;
+  int pair, from, shares, step;  // its first pair among the group's, workgroup of the first share of its kv head, shares, workgroups between them
+};
 struct Prefix {
   int* total;           // workgroups that have a share
   PrefixGroup* group;   // [n_groups]
   int* from;            // [n_seqs]: the first token that a sequence reads by itself
   int* group_of;        // [n_seqs]: -1 where that is 0
-  int* item_seq;        // [items of the sequences' own tokens]: whose they are
+  OwnItem* item;        // [items of the sequences' own tokens]
   float *part, *state;  // [workgroups][rows of an item][dt], [..][2]: as those of a share
   int n_groups;
 };
@@ -374,19 +379,19 @@ __device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, 
 
 // The prompts' kernel over the sequences of at least a.prompt_rows pairs (w4a32_paged_prompt.hip); items: its most workgroups
 hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s);
-// The same kernel over the prefixes of a.prefix
-hipError_t launch_prefixes(const Attend& a, int dtype, bool act_bf16, int dt, unsigned groups, hipStream_t s);
-inline int prefix_keys(int dtype, int dt, int log2) { return log2 == 5 || dtype == W4A32_CACHE_F32 ? 32 : dt == 256 ? 64 : 128; }  // of its tiles
+inline int prefix_keys(int dtype, int dt) { return dtype == W4A32_CACHE_F32 || dt == 256 ? 32 : 64; }  // of its tiles over prefixes
 
 // The rows' kernel over what sequences have behind their prefixes, all of whose sums go to scratch memory
 struct OwnPlan {
   long long items, tiles;
-  unsigned grid, slots;  // slots: rooms for an item's sums; the first are those of shares, then one for each item that is not shared
+  unsigned slots;  // slots: rooms for an item's sums; the first are those of shares, then one for each item that is not shared
   int wide, slot_rows, dt;
 };
 int plan_own(const w4a32_paged_cache* c, const w4a32_paged_rows* r, OwnPlan& o);
-hipError_t launch_own(const Attend& a, const OwnPlan& o, int dtype, bool act_bf16, hipStream_t s);
-constexpr int kOwnSlots = 1024;  // of shares: two of a workgroup
+// Workgroups that own tokens are dealt to. More than are there at once, so that most of them have a share of one item and no more (64 sequences
+// of 16 to 1200 tokens behind 8003: 47 us with 768, 51 with 512, 57 with 320, of which most have the end of one item and the start of the next).
+constexpr int kOwnGrid = 768;
+constexpr int kOwnSlots = 2 * kOwnGrid;  // of shares: two of a workgroup
 
 }  // namespace paged
 }  // namespace w4
