@@ -34,13 +34,15 @@ struct OwnItem {
   int pair, from, shares, step;  // its first pair among the group's, workgroup of the first share of its kv head, shares, workgroups between them
 };
 struct Prefix {
+  const int *group_start, *tokens;  // as they are given
+  int n_groups, grid;   // grid: most workgroups that have a share
+  OwnItem* item;        // [items of the sequences' own tokens]
+  float *part, *state;  // [workgroups][rows of an item][dt], [..][2]: as those of a share
+  // Where a launch in front deals the batch; else every wavefront does
   int* total;           // workgroups that have a share
   PrefixGroup* group;   // [n_groups]
   int* from;            // [n_seqs]: the first token that a sequence reads by itself
   int* group_of;        // [n_seqs]: -1 where that is 0
-  OwnItem* item;        // [items of the sequences' own tokens]
-  float *part, *state;  // [workgroups][rows of an item][dt], [..][2]: as those of a share
-  int n_groups;
 };
 
 struct Attend {
@@ -91,7 +93,7 @@ struct Seq {
 // behind a prefix
 enum Which { kRest, kPrompt, kOwn };
 template <int KT, Which kWhich>
-__device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
+__device__ __forceinline__ Seq seq_of(const Attend& a, int b, int own_from) {
   Seq q;
   q.s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
   const int before = max(a.row_lo - q.s.r0, 0);  // rows of an earlier launch: tokens to these
@@ -110,7 +112,7 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b) {
     q.ft = min((min(a.first, a.c.cap) + KT - 1) / KT, q.w0);
   }
   if constexpr (kWhich == kOwn) {
-    q.from = a.prefix.from[b];
+    q.from = a.prefix.from ? a.prefix.from[b] : own_from;
     q.w0 = min(q.from, a.c.cap - 1) / KT;
   }
   q.nt = q.s.n ? q.ft + (q.keys + KT - 1) / KT - q.w0 : 0;
@@ -151,12 +153,13 @@ template <int KT, Which kWhich = kRest>
 struct Seqs {
   Seq q;
   unsigned tiles, items;
+  int own_from = 0;  // kOwn, at most 64 sequences: this lane's
   __device__ __forceinline__ void load(const Attend& a, int b0) {
     const int b = b0 + (int)(threadIdx.x & 63);
     q = {};
     tiles = items = 0;
     if (b < a.c.n_seqs) {
-      q = seq_of<KT, kWhich>(a, b);
+      q = seq_of<KT, kWhich>(a, b, own_from);
       const u64 n = (u64)q.items * a.c.kv_heads;
       items = (unsigned)min(n, (u64)0xffffffffu);
       tiles = (unsigned)min(n * q.nt, (u64)0xffffffffu);
@@ -379,8 +382,6 @@ __device__ __forceinline__ void finish(const Attend& a, int r0, int of, int hk, 
 
 // The prompts' kernel over the sequences of at least a.prompt_rows pairs (w4a32_paged_prompt.hip); items: its most workgroups
 hipError_t launch_prompts(const Attend& a, int dtype, bool act_bf16, int dt, unsigned items, hipStream_t s);
-inline int prefix_keys(int dtype, int dt) { return dtype == W4A32_CACHE_F32 || dt == 256 ? 32 : 64; }  // of its tiles over prefixes
-
 // The rows' kernel over what sequences have behind their prefixes, all of whose sums go to scratch memory
 struct OwnPlan {
   long long items, tiles;

@@ -59,7 +59,7 @@ constexpr int kLeastPass = 128;
 
 template <typename Act, typename KV, int DT, bool kDump>
 __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(Attend a) {
-  rows_body<Act, KV, DT, kDump, kRest>(a, blockIdx.x, gridDim.x);
+  rows_body<Act, KV, DT, kDump, kRest>(a, blockIdx.x, gridDim.x, 0, 0);
 }
 
 // Joins the shares of an item: a workgroup per query row and kSlice of its values, its threads four values of every 256 /

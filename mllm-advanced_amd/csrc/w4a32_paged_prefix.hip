@@ -23,148 +23,174 @@ constexpr int kLog2 = 7;         // log2 of the rows of a workgroup of a prefix
 constexpr int kManyRows = 8192;  // rows from which on a workgroup joins several of them
 constexpr int kJoins = 1 << 20;  // workgroups of the joining launch, beyond which they take more
 
-struct Groups {
-  const int *group_start, *tokens;
-  int keys, own_keys;  // of a tile of a prefix, and of one of own tokens
-  int grid;            // most workgroups that prefixes get
-};
+constexpr int kLanes = 64;        // sequences up to which every wavefront deals the batch by itself, one in each lane, where there are
+constexpr int kLaneGroups = 16;   // few groups, which it goes through one by one
 
-__device__ __forceinline__ unsigned long long wave_sum(unsigned long long v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ __forceinline__ unsigned wave_sum(unsigned v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
-  return v;
+__device__ __forceinline__ unsigned wave_sum(unsigned x) { return last_lane(wave_scan(x)); }  // sums that do not fit are the most
+__device__ __forceinline__ int wave_min(int x) {
+#define W4_MIN(ctrl, rows) x = min(x, __builtin_amdgcn_update_dpp(0x7fffffff, x, ctrl, rows, 0xf, false))
+  W4_MIN(0x111, 0xf);  // row_shr 1, 2, 4, 8
+  W4_MIN(0x112, 0xf);
+  W4_MIN(0x114, 0xf);
+  W4_MIN(0x118, 0xf);
+  W4_MIN(0x142, 0xa);  // row_bcast 15, 31
+  W4_MIN(0x143, 0xc);
+#undef W4_MIN
+  return __builtin_amdgcn_readlane(x, 63);
 }
 
-// Who has what. A wavefront per group finds how much of the prefix all of its sequences with rows have (a group with one such sequence has
-// none). The slots of the chip then go to the prefixes and to the own tokens as their work is estimated, and a prefix's tiles to as few
-// workgroups per item as keep to that. kLds: everything that is read lies in LDS, asked for at once; else (many sequences) it is read
-// where it is needed.
-template <bool kLds>
-__global__ __launch_bounds__(kPlan) void deal_kernel(Attend a, Groups d) {
-  constexpr int kIn = kLds ? kPlan : 1;
-  __shared__ int starts[kIn + 1], lens[kIn], group_starts[kIn + 1], wanted[kIn], froms[kIn];
-  __shared__ PrefixGroup groups[kIn];
-  __shared__ unsigned long long of_wave[kPlan / 64];
-  const Prefix& x = a.prefix;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n_seqs = a.c.n_seqs, n_groups = x.n_groups;
-  PrefixGroup* const group = kLds ? groups : x.group;
-  int* const from = kLds ? froms : x.from;
-  if constexpr (kLds) {
-    if (tid <= n_seqs) starts[tid] = a.row_start[tid];
-    if (tid == kPlan - 1 && n_seqs == kPlan) starts[kPlan] = a.row_start[kPlan];
-    if (tid < n_seqs) lens[tid] = a.c.len[tid];
-    if (tid <= n_groups) group_starts[tid] = d.group_start[tid];
-    if (tid == kPlan - 1 && n_groups == kPlan) group_starts[kPlan] = d.group_start[kPlan];
-    if (tid < n_groups) wanted[tid] = d.tokens[tid];
+// A group whose sequences with rows, `with_rows` of them, have `least` tokens or more, rows from r0 to before r1: one such sequence alone has no
+// prefix.
+__device__ __forceinline__ PrefixGroup group_of(const Attend& a, int b0, int with_rows, int least, int r0, int r1) {
+  PrefixGroup q = {b0, 0, 0, 0, 0, 0, 0, 0};
+  if (with_rows < 2 || least <= 0) return q;
+  q.tokens = least;
+  q.r0 = r0;
+  q.n = max(r1 - r0, 0);
+  q.blocks = (int)(((long long)q.n * a.group + (1 << kLog2) - 1) >> kLog2);
+  return q;
+}
+// Tiles of a wavefront each, of the tokens behind `from`
+template <int kKeys>
+__device__ __forceinline__ unsigned own_tiles(const Attend& a, const Span& s, int from) {
+  if (s.n == 0) return 0;
+  const int keys = min(s.len + s.n, a.c.cap), first = min(from, a.c.cap - 1);
+  const unsigned long long n = ((unsigned long long)s.n * a.group + 15) / 16 * (unsigned)((keys + kKeys - 1) / kKeys - first / kKeys);
+  return (unsigned)min(n, 0xffffffffull);
+}
+// Tiles of a prefix that a share of it has: the slots of the chip go to the prefixes and to the own tokens as their work is estimated (a workgroup
+// takes 3 units of time for a tile of a prefix, 8 for kWaves tiles of own tokens), and an item gets as few shares as keep to that. count(per): shares of
+// `per` tiles that all items have. Whole shares: ceil(tiles / (most - items)) tiles always leave no more than `most`.
+template <typename Count>
+__device__ __forceinline__ unsigned share_of(const Attend& a, unsigned tiles, unsigned items, unsigned own, Count count) {
+  const float work = (float)tiles * 3.0f, rest = (float)own * a.c.kv_heads * (8.0f / kWaves);
+  unsigned most = min(max((unsigned)(kSlots * (work / (work + rest + 1.0f)) + 0.5f), (unsigned)kSlots / 4), (unsigned)kSlots * 7 / 8);
+  if (2 * items > most) most *= 2;  // in two rounds, so that what one leaves over is small
+  most = min(most, (unsigned)a.prefix.grid);
+  if (most <= items) return 1u << 30;
+  unsigned lo = max((tiles + most - 1) / most, 1u), per = max((tiles + most - items - 1) / (most - items), 1u);
+  while (lo < per) {
+    const unsigned mid = (lo + per) / 2;
+    if (count(mid) <= most)
+      per = mid;
+    else
+      lo = mid + 1;
   }
+  return per;
+}
+template <int kKeys>
+__device__ __forceinline__ unsigned tiles_of(const PrefixGroup& q) { return (unsigned)(q.tokens + kKeys - 1) / kKeys; }
+
+// What this lane's group and this lane's sequence have, by each wavefront
+struct Mine {
+  int total;      // workgroups that have a share of a prefix
+  PrefixGroup q;  // of group `lane`
+  int from, of;   // of sequence `lane`
+};
+__device__ __forceinline__ PrefixGroup of_lane(const PrefixGroup& q, int at) {
+  auto from = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+  return {from(q.b), from(q.r0), from(q.n), from(q.tokens), from(q.first), from(q.shares), from(q.blocks), 0};
+}
+template <int kKeys, int kOwnKeys>
+__device__ __forceinline__ Mine deal_by_lanes(const Attend& a) {
+  const Prefix& x = a.prefix;
+  const int lane = threadIdx.x & 63, n_seqs = a.c.n_seqs;
+  Mine m = {0, {}, 0, -1};
+  Span s = {};
+  int end = 0, b0 = 0, b1 = 0, want = 0;
+  if (lane < n_seqs) {
+    s = span_of(a.c, a.row_start, a.rows, a.max_rows, lane);
+    end = min(a.row_start[lane + 1], a.rows);
+  }
+  if (lane < x.n_groups) {
+    b0 = min(max(x.group_start[lane], 0), n_seqs);
+    b1 = min(max(x.group_start[lane + 1], b0), n_seqs);
+    want = min(x.tokens[lane], a.c.cap);
+  }
+  for (int g = 0; g < x.n_groups; ++g) {
+    const int lo = __builtin_amdgcn_readlane(b0, g), hi = __builtin_amdgcn_readlane(b1, g);
+    if (lo == hi) continue;
+    const bool in = lane >= lo && lane < hi, has = in && s.n > 0;
+    const int least = wave_min(has ? s.len : __builtin_amdgcn_readlane(want, g));
+    const PrefixGroup q = group_of(a, lo, __popcll(__ballot(has)), min(least, __builtin_amdgcn_readlane(want, g)), __builtin_amdgcn_readlane(s.r0, lo),
+                                   __builtin_amdgcn_readlane(end, hi - 1));
+    if (lane == g) m.q = q;
+    if (in && q.tokens) {
+      m.from = q.tokens;
+      m.of = g;
+    }
+  }
+  const unsigned of_group = (unsigned)m.q.blocks * a.c.kv_heads, tiles = tiles_of<kKeys>(m.q);
+  const unsigned per = share_of(a, wave_sum(of_group * tiles), wave_sum(of_group), wave_sum(own_tiles<kOwnKeys>(a, s, m.from)),
+                                [&](unsigned n) { return wave_sum(of_group * ((tiles + n - 1) / n)); });
+  m.q.shares = (int)((tiles + per - 1) / per);
+  const unsigned n = of_group * m.q.shares, upto = wave_scan(n);
+  m.q.first = (int)(upto - n);
+  m.total = (int)last_lane(upto);
+  if ((unsigned)m.total > (unsigned)x.grid) m = {0, {}, 0, -1};  // row or group starts that decrease: all read everything by themselves
+  return m;
+}
+
+// The same for many sequences, by a launch of its own: a wavefront per group, then one for all groups
+template <int kKeys, int kOwnKeys>
+__global__ __launch_bounds__(kPlan) void deal_kernel(Attend a) {
+  __shared__ unsigned of_wave[kPlan / 64];
+  const Prefix& x = a.prefix;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n_seqs = a.c.n_seqs;
   for (int b = tid; b < n_seqs; b += kPlan) {
-    from[b] = 0;
+    x.from[b] = 0;
     x.group_of[b] = -1;
   }
   __syncthreads();
-  const int *row_start = kLds ? starts : a.row_start, *group_start = kLds ? group_starts : d.group_start, *tokens = kLds ? wanted : d.tokens;
-  Cache c = a.c;
-  if constexpr (kLds) c.len = lens;
-  auto bounds = [&](int g, int& b0, int& b1) {
-    b0 = min(max(group_start[g], 0), n_seqs);
-    b1 = min(max(group_start[g + 1], b0), n_seqs);
-  };
-  for (int g = wave; g < n_groups; g += kPlan / 64) {
-    int b0, b1;
-    bounds(g, b0, b1);
-    int least = min(max(tokens[g], 0), c.cap), with_rows = 0;
+  for (int g = wave; g < x.n_groups; g += kPlan / 64) {
+    const int b0 = min(max(x.group_start[g], 0), n_seqs), b1 = min(max(x.group_start[g + 1], b0), n_seqs);
+    int least = min(x.tokens[g], a.c.cap), with_rows = 0;
     for (int b = b0 + lane; b - lane < b1; b += 64) {
       Span s = {};
-      if (b < b1) s = span_of(c, row_start, a.rows, a.max_rows, b);
+      if (b < b1) s = span_of(a.c, a.row_start, a.rows, a.max_rows, b);
       with_rows += __popcll(__ballot(s.n > 0));
       if (s.n > 0) least = min(least, s.len);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) least = min(least, __shfl_xor(least, o));
-    if (with_rows < 2) least = 0;
-    if (lane == 0) {
-      PrefixGroup q = {b0, 0, 0, least, 0, 0, 0, 0};
-      if (least) {
-        q.r0 = min(max(row_start[b0], 0), a.rows);
-        q.n = min(max(row_start[b1], q.r0), a.rows) - q.r0;
-        q.blocks = (int)(((long long)q.n * a.group + (1 << kLog2) - 1) >> kLog2);
-      }
-      group[g] = q;
-    }
-    if (least)
+    const PrefixGroup q = group_of(a, b0, with_rows, wave_min(least), min(max(a.row_start[b0], 0), a.rows), min(a.row_start[b1], a.rows));
+    if (lane == 0) x.group[g] = q;
+    if (q.tokens)
       for (int b = b0 + lane; b < b1; b += 64) {
-        from[b] = least;
+        x.from[b] = q.tokens;
         x.group_of[b] = g;
       }
   }
   __syncthreads();
-  // ---- tiles of own tokens, of a wavefront each ----
-  unsigned long long own = 0;
-  for (int b = tid; b < n_seqs; b += kPlan) {
-    const Span s = span_of(c, row_start, a.rows, a.max_rows, b);
-    if (kLds) x.from[b] = from[b];
-    if (s.n == 0) continue;
-    const int keys = min(s.len + s.n, c.cap), first = min(from[b], c.cap - 1);
-    own += (((unsigned long long)s.n * a.group + 15) / 16) * ((keys + d.own_keys - 1) / d.own_keys - first / d.own_keys);
-  }
+  unsigned own = 0;
+  for (int b = tid; b < n_seqs; b += kPlan) own = add_sat(own, own_tiles<kOwnKeys>(a, span_of(a.c, a.row_start, a.rows, a.max_rows, b), x.from[b]));
   own = wave_sum(own);
   if (lane == 0) of_wave[wave] = own;
   __syncthreads();
   if (wave != 0) return;
   own = 0;
 #pragma unroll
-  for (int w = 0; w < kPlan / 64; ++w) own += of_wave[w];
-  // ---- and of prefixes ----
-  auto tiles_of = [&](int g) { return (unsigned)(group[g].tokens + d.keys - 1) / (unsigned)d.keys; };
-  unsigned long long tiles = 0;
-  unsigned items = 0;
-  for (int g = lane; g < n_groups; g += 64) {
-    items += (unsigned)group[g].blocks * a.c.kv_heads;
-    tiles += (unsigned long long)group[g].blocks * a.c.kv_heads * tiles_of(g);
-  }
-  items = wave_sum(items);
-  tiles = wave_sum(tiles);
-  // Times that a workgroup takes: 3 units for a tile of a prefix, 8 for kWaves tiles of own tokens
-  const float work = (float)tiles * 3.0f, rest = (float)own * a.c.kv_heads * (8.0f / kWaves);
-  unsigned most = min(max((unsigned)(kSlots * (work / (work + rest + 1.0f)) + 0.5f), (unsigned)kSlots / 4), (unsigned)kSlots * 7 / 8);
-  if (2 * items > most) most *= 2;  // in two rounds, so that what one leaves over is small
-  most = min(most, (unsigned)d.grid);
-  // Shares of `per` tiles, the fewest that leave no more than `most` of them: ceil(tiles / (most - items)) are enough
-  unsigned per = 1u << 30;
-  if (most > items) {
-    unsigned lo = (unsigned)max((tiles + most - 1) / most, 1ull);
-    per = (unsigned)max((tiles + most - items - 1) / (most - items), 1ull);
-    while (lo < per) {
-      const unsigned mid = (lo + per) / 2;
-      unsigned n = 0;
-      for (int g = lane; g < n_groups; g += 64) n += (unsigned)group[g].blocks * a.c.kv_heads * ((tiles_of(g) + mid - 1) / mid);
-      if (wave_sum(n) <= most)
-        per = mid;
-      else
-        lo = mid + 1;
+  for (int w = 0; w < kPlan / 64; ++w) own = add_sat(own, of_wave[w]);
+  auto all = [&](auto of) {  // of all groups together
+    unsigned sum = 0;
+    for (int g = lane; g < x.n_groups; g += 64) {
+      const PrefixGroup q = x.group[g];
+      sum = add_sat(sum, (unsigned)q.blocks * a.c.kv_heads * of(tiles_of<kKeys>(q)));
     }
-  }
+    return wave_sum(sum);
+  };
+  const unsigned per = share_of(a, all([](unsigned tiles) { return tiles; }), all([](unsigned) { return 1u; }), own,
+                                [&](unsigned n) { return all([&](unsigned tiles) { return (tiles + n - 1) / n; }); });
   unsigned total = 0;
-  for (int g0 = 0; g0 < n_groups; g0 += 64) {
+  for (int g0 = 0; g0 < x.n_groups; g0 += 64) {
     const int g = g0 + lane;
     PrefixGroup q = {};
-    unsigned n = 0;
-    if (g < n_groups) {
-      q = group[g];
-      q.shares = (int)((tiles_of(g) + per - 1) / per);
-      n = (unsigned)q.blocks * a.c.kv_heads * q.shares;
-    }
-    const unsigned upto = wave_scan(n);
+    if (g < x.n_groups) q = x.group[g];
+    q.shares = (int)((tiles_of<kKeys>(q) + per - 1) / per);
+    const unsigned n = (unsigned)q.blocks * a.c.kv_heads * q.shares, upto = wave_scan(n);
     q.first = (int)(total + upto - n);
-    if (g < n_groups) x.group[g] = q;
+    if (g < x.n_groups) x.group[g] = q;
     total = add_sat(total, last_lane(upto));
   }
-  const bool fits = total <= (unsigned)d.grid;  // else (row or group starts that decrease) all read everything by themselves
+  const bool fits = total <= (unsigned)x.grid;
   if (!fits)
     for (int b = lane; b < n_seqs; b += 64) {
       x.from[b] = 0;
@@ -229,12 +255,32 @@ __device__ __forceinline__ void add_shares(const Attend& a, const Shares& s, uns
 // Both parts in one launch: the first workgroups have the prefixes
 template <typename Act, typename KV, int DT>
 __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void both_kernel(Attend a) {
-  static_assert(Shape<Act, KV, DT, kHalfForm>::kThreads == 64 * kWaves, "workgroups of either kind");
-  const unsigned prefixes = (unsigned)*a.prefix.total;
-  if (blockIdx.x < prefixes)
-    prompt_body<Act, KV, DT, kHalfForm, true>(a, blockIdx.x);
-  else if (blockIdx.x - prefixes < kOwnGrid)
-    rows_body<Act, KV, DT, false, kOwn>(a, blockIdx.x - prefixes, kOwnGrid);
+  using Sh = Shape<Act, KV, DT, kHalfForm>;
+  static_assert(Sh::kThreads == 64 * kWaves && 32 * Sh::kMembers == 1 << kLog2, "workgroups of either kind");
+  const Prefix& x = a.prefix;
+  const int unit = blockIdx.x, lane = threadIdx.x & 63;
+  Mine m = {0, {}, 0, -1};
+  if (x.from)
+    m.total = *x.total;
+  else
+    m = deal_by_lanes<Sh::kKeys, tile_keys<KV>()>(a);
+  if (unit < m.total) {
+    // the last group whose first workgroup is this one or stands in front of it; groups without any are passed over
+    PrefixGroup g;
+    if (x.from) {
+      int before = 0;
+      for (int g0 = 0; g0 < x.n_groups; g0 += 64) before += __popcll(__ballot(g0 + lane < x.n_groups && x.group[g0 + lane].first <= unit));
+      g = x.group[before - 1];
+    } else {
+      g = of_lane(m.q, __popcll(__ballot(lane < x.n_groups && m.q.first <= unit)) - 1);
+    }
+    prompt_body<Act, KV, DT, kHalfForm, true>(a, (unsigned)unit, g);
+  } else if (unit - m.total < kOwnGrid) {
+    rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)(unit - m.total), kOwnGrid, m.from, [&](int b) {
+      const int of = x.from ? x.group_of[b] : __builtin_amdgcn_readlane(m.of, b);
+      return of < 0 ? PrefixGroup{} : x.from ? x.group[of] : of_lane(m.q, of);
+    });
+  }
 }
 
 // Where rows are few: a workgroup per row and kSlice of its values, its threads four values of every 256 / (kSlice / 4)th share each
@@ -304,7 +350,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(Attend a, unsigned rows)
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
   OwnPlan own;
-  int keys;
+  bool dealt;     // by a launch in front
   unsigned grid;  // workgroups of the prefixes
   size_t group_off, from_off, of_off, item_off, part_off, state_off, pre_part_off, pre_state_off, total;
 };
@@ -313,7 +359,7 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int n_groups,
   if (int e = plan_own(c, r, p.own)) return e;
   const long long group = r->heads / c->kv_heads;
   const int dt = p.own.dt;
-  p.keys = prefix_keys(c->dtype, dt);
+  p.dealt = c->n_seqs > kLanes || n_groups > kLaneGroups;
   const long long items = (((long long)r->rows * group >> kLog2) + n_groups) * c->kv_heads;
   const long long grid = items > 2 * kSlots ? items : 2 * kSlots;
   if (grid > most_groups(512)) return W4A32_ESHAPE;
@@ -364,6 +410,10 @@ hipError_t launch_both(const Attend& a, const Plan& p, hipStream_t s) {
     static LdsLimitOnce limit;
     if (hipError_t e = limit.raise((const void*)both_kernel<Act, KV, DT>, lds); e != hipSuccess) return e;
   }
+  if (p.dealt) {
+    hipLaunchKernelGGL((deal_kernel<Shape<Act, KV, DT, kHalfForm>::kKeys, tile_keys<KV>()>), dim3(1), dim3(kPlan), 0, s, a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(p.grid + kOwnGrid), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
@@ -404,8 +454,9 @@ int w4a32_op_paged_prefix_attention(const w4a32_paged_cache* cache, const w4a32_
   if (int e = plan_of(cache, rows, n_groups, p)) return e;
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
-  const Prefix x{(int*)(scratch + 128), (PrefixGroup*)(scratch + p.group_off), (int*)(scratch + p.from_off), (int*)(scratch + p.of_off),
-                 (OwnItem*)(scratch + p.item_off), (float*)(scratch + p.pre_part_off), (float*)(scratch + p.pre_state_off), n_groups};
+  auto at = [&](size_t off) { return p.dealt ? (int*)(scratch + off) : nullptr; };
+  const Prefix x{d_group_start, d_prefix, n_groups, (int)p.grid, (OwnItem*)(scratch + p.item_off), (float*)(scratch + p.pre_part_off),
+                 (float*)(scratch + p.pre_state_off), at(128), (PrefixGroup*)at(p.group_off), at(p.from_off), at(p.of_off)};
   Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
            rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, 0, rows->rows, 0, 0, 0, kLog2,
            p.own.wide, p.own.slot_rows, (unsigned)p.own.items, (unsigned)p.own.tiles, scale * kLog2e, nullptr,
@@ -414,12 +465,6 @@ int w4a32_op_paged_prefix_attention(const w4a32_paged_cache* cache, const w4a32_
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int dtype = cache->dtype;
   const bool bf16 = rows->act_bf16 != 0;
-  const Groups d{d_group_start, d_prefix, p.keys, dtype == W4A32_CACHE_F32 ? 16 : 32, (int)p.grid};
-  if (cache->n_seqs <= kPlan)
-    hipLaunchKernelGGL((deal_kernel<true>), dim3(1), dim3(kPlan), 0, s, a, d);
-  else
-    hipLaunchKernelGGL((deal_kernel<false>), dim3(1), dim3(kPlan), 0, s, a, d);
-  if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   const hipError_t e = bf16                        ? launch_both_dim<__bf16, __bf16>(a, p, s)
                        : dtype == W4A32_CACHE_F32 ? launch_both_dim<float, float>(a, p, s)
                        : dtype == W4A32_CACHE_F16 ? launch_both_dim<float, _Float16>(a, p, s)

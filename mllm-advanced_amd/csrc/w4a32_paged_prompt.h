@@ -59,7 +59,7 @@ static __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 // kPrefix: a workgroup has a share of the keys of a prefix, for rows of all sequences of the group, and leaves its sums in scratch memory
 template <typename Act, typename KV, int DT, Form kForm, bool kPrefix>
-__device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit) {
+__device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, const PrefixGroup& g) {
   using M = Math<Act, KV>;
   using Sh = Shape<Act, KV, DT, kForm>;
   constexpr bool kSplit = kForm == kTeamsForm;
@@ -82,11 +82,6 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit) {
   Place p;
   int block, hk, first_tile = 0, end_tile = 0;
   if constexpr (kPrefix) {
-    const Prefix& x = a.prefix;
-    if ((int)unit >= *x.total) return;
-    int before = 0;  // the last group whose first workgroup is this one or stands in front of it; groups without any are passed over
-    for (int g0 = 0; g0 < x.n_groups; g0 += 64) before += __popcll(__ballot(g0 + lane < x.n_groups && x.group[g0 + lane].first <= (int)unit));
-    const PrefixGroup g = x.group[before - 1];
     const unsigned in = unit - g.first, in_kv = in / kv, share = in_kv / g.blocks;
     hk = (int)(in - in_kv * kv);
     block = (int)(in_kv - share * g.blocks);

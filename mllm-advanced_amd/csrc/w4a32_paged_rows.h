@@ -69,8 +69,9 @@ constexpr size_t lds_bytes() { return kWaves * (wave_lds<KV, DT>() + kRows * 2 *
 
 // DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up. kWhich == kOwn: the tokens
 // behind a prefix, whose sums another launch joins with the prefix's.
-template <typename Act, typename KV, int DT, bool kDump, Which kWhich>
-__device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsigned grid) {
+// own_from: where this lane's sequence's own tokens begin; group_at: the group of a sequence, without rows where it has none.
+template <typename Act, typename KV, int DT, bool kDump, Which kWhich, typename GroupAt>
+__device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsigned grid, int own_from, GroupAt group_at) {
   using M = Math<Act, KV>;
   constexpr int KT = tile_keys<KV>(), NT = M::kTerms, kHalves = KT / 16;
   constexpr bool k16 = sizeof(KV) == 2;
@@ -85,6 +86,7 @@ __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsig
   const int streams = kWaves >> a.wide, stream = wave >> a.wide, wide = 1 << a.wide;
 
   Seqs<KT, kWhich> seqs;
+  seqs.own_from = own_from;
   const Deal deal = deal_of(a, seqs, grid);
   if (block == 0 && threadIdx.x == 0) *a.count = deal.per ? deal.items : 0;
   if (deal.per == 0) return;
@@ -410,20 +412,16 @@ __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsig
     // workgroup one begins there and the other does not.
     const int rows = min(all_rows - of0, kRows << a.wide);
     const int slot = 2 * (int)block + (t_lo == 0);
-    if (t_lo == 0 && threadIdx.x == 0) {
-      const Item it{w_first, shares, s.r0, of0, rows, hk};
-      if constexpr (kWhich == kOwn) {
-        OwnItem o{it, 0, 0, 0, 0};
-        const int g = a.prefix.group_of[p.b];
-        if (g >= 0) {
-          const PrefixGroup q = a.prefix.group[g];
-          const int row = s.r0 - q.r0;
-          if (row >= 0 && row + s.n <= q.n) o = {it, row * a.group + of0, q.first + hk, q.shares, q.blocks * a.c.kv_heads};  // always, where starts do not decrease
-        }
-        a.prefix.item[p.item0 + item] = o;
-      } else {
-        a.item[p.item0 + item] = it;
+    if constexpr (kWhich == kOwn) {
+      if (t_lo == 0 && wave == 0) {
+        const PrefixGroup q = group_at(p.b);
+        const int row = s.r0 - q.r0;
+        OwnItem o{{w_first, shares, s.r0, of0, rows, hk}, 0, 0, 0, 0};
+        if (row >= 0 && row + s.n <= q.n) o = {o.own, row * a.group + of0, q.first + hk, q.shares, q.blocks * a.c.kv_heads};
+        if (lane == 0) a.prefix.item[p.item0 + item] = o;
       }
+    } else {
+      if (t_lo == 0 && threadIdx.x == 0) a.item[p.item0 + item] = Item{w_first, shares, s.r0, of0, rows, hk};
     }
     constexpr int kPer = DT / 4;  // threads of a row
     for (int i = threadIdx.x; i < rows * kPer; i += 64 * kWaves) {
