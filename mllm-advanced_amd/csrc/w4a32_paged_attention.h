@@ -35,7 +35,7 @@ struct OwnItem {
 };
 struct Prefix {
   const int *group_start, *tokens;  // as they are given
-  int n_groups, grid;   // grid: most workgroups that have a share
+  int n_groups, grid, blocks;  // most workgroups that have a share of a prefix, or a block of own rows
   OwnItem* item;        // [items of the sequences' own tokens]
   float *part, *state;  // [workgroups][rows of an item][dt], [..][2]: as those of a share
   // Where a launch in front deals the batch; else every wavefront does
@@ -90,8 +90,9 @@ struct Seq {
 };
 
 // kPrompt: the sequences of the prompts' kernel, in items of 1 << prompt_log2 rows; kRest: the others; kOwn: all, and of their tokens those
-// behind a prefix
-enum Which { kRest, kPrompt, kOwn };
+// behind a prefix; kOwnPrompt: of these the sequences of at least prompt_rows pairs, in items of 1 << prompt_log2 rows, where kOwn
+// counts their items but has no tiles of them
+enum Which { kRest, kPrompt, kOwn, kOwnPrompt };
 template <int KT, Which kWhich>
 __device__ __forceinline__ Seq seq_of(const Attend& a, int b, int own_from) {
   Seq q;
@@ -101,9 +102,10 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b, int own_from) {
   q.s.r0 += before;
   q.s.len += before;
   const long long pairs = (long long)q.s.n * a.group;
-  if (kWhich != kOwn && (a.prompt_rows && pairs >= a.prompt_rows) != (kWhich == kPrompt)) q.s.n = 0;
+  const bool prompt = a.prompt_rows && pairs >= a.prompt_rows;
+  if (kWhich != kOwn && prompt != (kWhich != kRest)) q.s.n = 0;
   q.keys = min(q.s.len + q.s.n, a.c.cap);
-  const int log2 = kWhich == kPrompt ? a.prompt_log2 : 4 + a.wide;
+  const int log2 = kWhich == kPrompt || kWhich == kOwnPrompt ? a.prompt_log2 : 4 + a.wide;
   q.items = q.s.n ? (int)((pairs + (1 << log2) - 1) >> log2) : 0;
   q.w0 = 0;
   q.ft = 0;
@@ -111,11 +113,12 @@ __device__ __forceinline__ Seq seq_of(const Attend& a, int b, int own_from) {
     q.w0 = max(0, min(q.s.len, a.c.cap - 1) - a.window + 1) / KT;
     q.ft = min((min(a.first, a.c.cap) + KT - 1) / KT, q.w0);
   }
-  if constexpr (kWhich == kOwn) {
+  if constexpr (kWhich == kOwn || kWhich == kOwnPrompt) {
     q.from = a.prefix.from ? a.prefix.from[b] : own_from;
     q.w0 = min(q.from, a.c.cap - 1) / KT;
   }
   q.nt = q.s.n ? q.ft + (q.keys + KT - 1) / KT - q.w0 : 0;
+  if (kWhich == kOwn && prompt) q.nt = 0;
   return q;
 }
 
@@ -137,6 +140,7 @@ __device__ __forceinline__ unsigned last_lane(unsigned x) { return (unsigned)__b
 enum Unit { kTiles, kShares, kKeyTiles, kItems };
 struct Deal {
   unsigned total, items, per;  // tiles, items, tiles of a share; per = 0: nothing can be done
+  bool fits;                   // for want of scratch memory, or else there is nothing to do
   bool apart;                  // a share has tiles of one item only: ceil(nt / per) of them per item
 };
 struct Place {
@@ -153,7 +157,7 @@ template <int KT, Which kWhich = kRest>
 struct Seqs {
   Seq q;
   unsigned tiles, items;
-  int own_from = 0;  // kOwn, at most 64 sequences: this lane's
+  int own_from = 0;  // kOwn, kOwnPrompt, at most 64 sequences: this lane's
   __device__ __forceinline__ void load(const Attend& a, int b0) {
     const int b = b0 + (int)(threadIdx.x & 63);
     q = {};
@@ -177,7 +181,7 @@ __device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT, kWhich>& s, 
     p.b = 0;
     p.inner = u;
     p.q = {{from(s.q.s.r0), from(s.q.s.n), from(s.q.s.len)}, from(s.q.keys), from(s.q.ft), from(s.q.w0), from(s.q.nt), from(s.q.items), 0};
-    if constexpr (kWhich == kOwn) p.q.from = from(s.q.from);
+    if constexpr (kWhich == kOwn || kWhich == kOwnPrompt) p.q.from = from(s.q.from);
     const unsigned each = unit == kTiles ? p.q.nt : unit == kShares ? (p.q.nt + per - 1) / per : unit == kItems ? 1 : (p.q.nt + kWaves - 1) / kWaves;
     p.there = u < each * (unsigned)a.c.kv_heads * (unit == kKeyTiles ? 1 : p.q.items);
     return p;
@@ -206,7 +210,7 @@ __device__ __forceinline__ Place place_of(const Attend& a, Seqs<KT, kWhich>& s, 
       p.q.w0 = from(s.q.w0);
       p.q.nt = from(s.q.nt);
       p.q.items = from(s.q.items);
-      if constexpr (kWhich == kOwn) p.q.from = from(s.q.from);
+      if constexpr (kWhich == kOwn || kWhich == kOwnPrompt) p.q.from = from(s.q.from);
       return p;
     }
     before = add_sat(before, last_lane(upto));

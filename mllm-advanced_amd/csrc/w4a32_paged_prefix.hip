@@ -20,7 +20,10 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kPlan = 1024;      // threads of the workgroup that deals
 constexpr int kSlots = 512;      // workgroups that are there at once: two per CU
 constexpr int kLog2 = 7;         // log2 of the rows of a workgroup of a prefix
-constexpr int kManyRows = 8192;  // rows from which on a workgroup joins several of them
+// Pairs of row and head from which on a sequence's own tokens go by blocks of 128 rows as well, and not by 16 of a wavefront (eight prompts of 60 to
+// 300 rows, 28 heads on 4, bf16: behind 64 tokens 46 us against 68, behind 4099 141 against 148; 64, 256, 512: the same).
+constexpr int kOwnPromptRows = 128;
+constexpr int kManyRows = 1024;  // rows from which on a workgroup joins several of them
 constexpr int kJoins = 1 << 20;  // workgroups of the joining launch, beyond which they take more
 
 constexpr int kLanes = 64;        // sequences up to which every wavefront deals the batch by itself, one in each lane, where there are
@@ -59,16 +62,21 @@ __device__ __forceinline__ unsigned own_tiles(const Attend& a, const Span& s, in
   return (unsigned)min(n, 0xffffffffull);
 }
 // Tiles of a prefix that a share of it has: the slots of the chip go to the prefixes and to the own tokens as their work is estimated (a workgroup
-// takes 3 units of time for a tile of a prefix, 8 for kWaves tiles of own tokens), and an item gets as few shares as keep to that. count(per): shares of
-// `per` tiles that all items have. Whole shares: ceil(tiles / (most - items)) tiles always leave no more than `most`.
-template <typename Count>
-__device__ __forceinline__ unsigned share_of(const Attend& a, unsigned tiles, unsigned items, unsigned own, Count count) {
+// takes 3 units of time for a tile of a prefix, 8 for kWaves tiles of own tokens), and an item gets as few shares as keep to that. But a share
+// costs as well: its sums are written and read again, some 50 ns where all of a workgroup's rows are there, against 1 us for a tile (f32: 5), so
+// that sqrt(tiles * 50 / 1000) tiles of a share take the least time together (six groups of eight, 12 heads on 2, f32 on f16, behind 1000
+// tokens: 28 us against 36 with a tile of a share). count(per): shares of `per` tiles that all items have. Whole shares: ceil(tiles / (most - items))
+// tiles always leave no more than `most`.
+template <bool kF32, typename Count>
+__device__ __forceinline__ unsigned share_of(const Attend& a, unsigned tiles, unsigned items, unsigned pairs, unsigned own, Count count) {
   const float work = (float)tiles * 3.0f, rest = (float)own * a.c.kv_heads * (8.0f / kWaves);
   unsigned most = min(max((unsigned)(kSlots * (work / (work + rest + 1.0f)) + 0.5f), (unsigned)kSlots / 4), (unsigned)kSlots * 7 / 8);
   if (2 * items > most) most *= 2;  // in two rounds, so that what one leaves over is small
   most = min(most, (unsigned)a.prefix.grid);
   if (most <= items) return 1u << 30;
-  unsigned lo = max((tiles + most - 1) / most, 1u), per = max((tiles + most - items - 1) / (most - items), 1u);
+  const float rows = (float)pairs / ((float)max(items, 1u) * (1 << kLog2));  // of those that a workgroup has room for
+  const unsigned least = max((unsigned)(__builtin_sqrtf((float)tiles * rows * (kF32 ? 0.01f : 0.05f)) + 0.5f), 1u);
+  unsigned lo = max((tiles + most - 1) / most, least), per = max((tiles + most - items - 1) / (most - items), lo);
   while (lo < per) {
     const unsigned mid = (lo + per) / 2;
     if (count(mid) <= most)
@@ -91,7 +99,7 @@ __device__ __forceinline__ PrefixGroup of_lane(const PrefixGroup& q, int at) {
   auto from = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
   return {from(q.b), from(q.r0), from(q.n), from(q.tokens), from(q.first), from(q.shares), from(q.blocks), 0};
 }
-template <int kKeys, int kOwnKeys>
+template <int kKeys, int kOwnKeys, bool kF32>
 __device__ __forceinline__ Mine deal_by_lanes(const Attend& a) {
   const Prefix& x = a.prefix;
   const int lane = threadIdx.x & 63, n_seqs = a.c.n_seqs;
@@ -121,8 +129,9 @@ __device__ __forceinline__ Mine deal_by_lanes(const Attend& a) {
     }
   }
   const unsigned of_group = (unsigned)m.q.blocks * a.c.kv_heads, tiles = tiles_of<kKeys>(m.q);
-  const unsigned per = share_of(a, wave_sum(of_group * tiles), wave_sum(of_group), wave_sum(own_tiles<kOwnKeys>(a, s, m.from)),
-                                [&](unsigned n) { return wave_sum(of_group * ((tiles + n - 1) / n)); });
+  const unsigned pairs = (unsigned)(m.q.n * a.group) * a.c.kv_heads;
+  const unsigned per = share_of<kF32>(a, wave_sum(of_group * tiles), wave_sum(of_group), wave_sum(pairs), wave_sum(own_tiles<kOwnKeys>(a, s, m.from)),
+                                      [&](unsigned n) { return wave_sum(of_group * ((tiles + n - 1) / n)); });
   m.q.shares = (int)((tiles + per - 1) / per);
   const unsigned n = of_group * m.q.shares, upto = wave_scan(n);
   m.q.first = (int)(upto - n);
@@ -132,7 +141,7 @@ __device__ __forceinline__ Mine deal_by_lanes(const Attend& a) {
 }
 
 // The same for many sequences, by a launch of its own: a wavefront per group, then one for all groups
-template <int kKeys, int kOwnKeys>
+template <int kKeys, int kOwnKeys, bool kF32>
 __global__ __launch_bounds__(kPlan) void deal_kernel(Attend a) {
   __shared__ unsigned of_wave[kPlan / 64];
   const Prefix& x = a.prefix;
@@ -169,16 +178,15 @@ __global__ __launch_bounds__(kPlan) void deal_kernel(Attend a) {
   own = 0;
 #pragma unroll
   for (int w = 0; w < kPlan / 64; ++w) own = add_sat(own, of_wave[w]);
-  auto all = [&](auto of) {  // of all groups together
+  auto all = [&](auto of) {  // of all groups together, per kv head
     unsigned sum = 0;
-    for (int g = lane; g < x.n_groups; g += 64) {
-      const PrefixGroup q = x.group[g];
-      sum = add_sat(sum, (unsigned)q.blocks * a.c.kv_heads * of(tiles_of<kKeys>(q)));
-    }
+    for (int g = lane; g < x.n_groups; g += 64) sum = add_sat(sum, of(x.group[g]) * a.c.kv_heads);
     return wave_sum(sum);
   };
-  const unsigned per = share_of(a, all([](unsigned tiles) { return tiles; }), all([](unsigned) { return 1u; }), own,
-                                [&](unsigned n) { return all([&](unsigned tiles) { return (tiles + n - 1) / n; }); });
+  typedef const PrefixGroup& Q;
+  const unsigned per = share_of<kF32>(a, all([](Q q) { return q.blocks * tiles_of<kKeys>(q); }), all([](Q q) { return (unsigned)q.blocks; }),
+                                      all([&](Q q) { return (unsigned)(q.n * a.group); }), own,
+                                      [&](unsigned n) { return all([&](Q q) { return q.blocks * ((tiles_of<kKeys>(q) + n - 1) / n); }); });
   unsigned total = 0;
   for (int g0 = 0; g0 < x.n_groups; g0 += 64) {
     const int g = g0 + lane;
@@ -258,12 +266,13 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void both_kernel(At
   using Sh = Shape<Act, KV, DT, kHalfForm>;
   static_assert(Sh::kThreads == 64 * kWaves && 32 * Sh::kMembers == 1 << kLog2, "workgroups of either kind");
   const Prefix& x = a.prefix;
-  const int unit = blockIdx.x, lane = threadIdx.x & 63;
+  int unit = blockIdx.x;
+  const int lane = threadIdx.x & 63;
   Mine m = {0, {}, 0, -1};
   if (x.from)
     m.total = *x.total;
   else
-    m = deal_by_lanes<Sh::kKeys, tile_keys<KV>()>(a);
+    m = deal_by_lanes<Sh::kKeys, tile_keys<KV>(), sizeof(KV) == 4>(a);
   if (unit < m.total) {
     // the last group whose first workgroup is this one or stands in front of it; groups without any are passed over
     PrefixGroup g;
@@ -274,13 +283,59 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void both_kernel(At
     } else {
       g = of_lane(m.q, __popcll(__ballot(lane < x.n_groups && m.q.first <= unit)) - 1);
     }
-    prompt_body<Act, KV, DT, kHalfForm, true>(a, (unsigned)unit, g);
-  } else if (unit - m.total < kOwnGrid) {
-    rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)(unit - m.total), kOwnGrid, m.from, [&](int b) {
-      const int of = x.from ? x.group_of[b] : __builtin_amdgcn_readlane(m.of, b);
-      return of < 0 ? PrefixGroup{} : x.from ? x.group[of] : of_lane(m.q, of);
-    });
+    const unsigned kv = a.c.kv_heads, in = (unsigned)(unit - g.first), in_kv = in / kv, share = in_kv / g.blocks;
+    const int tiles = (int)tiles_of<Sh::kKeys>(g);
+    const size_t row = (size_t)unit << kLog2;
+    const Piece piece{g.b, {g.r0, g.n, g.tokens - 1}, (int)(in - in_kv * kv), (int)(in_kv - share * g.blocks), (int)((long long)tiles * share / g.shares),
+                      (int)((long long)tiles * (share + 1) / g.shares), 0, x.part + row * DT, x.state + 2 * row};
+    prompt_body<Act, KV, DT, kHalfForm, kPrefixTokens>(a, 0, piece);
+    return;
   }
+  unit -= m.total;
+  auto group_at = [&](int b) {
+    const int of = x.from ? x.group_of[b] : __builtin_amdgcn_readlane(m.of, b);
+    return of < 0 ? PrefixGroup{} : x.from ? x.group[of] : of_lane(m.q, of);
+  };
+  if (a.prompt_rows) {
+    Seqs<Sh::kKeys, kOwnPrompt> prompts;
+    Seqs<tile_keys<KV>(), kOwn> seqs;
+    prompts.own_from = seqs.own_from = m.from;
+    unsigned blocks = 0, items = 0;
+    for (int b0 = 0; b0 < a.c.n_seqs; b0 += 64) {
+      prompts.load(a, b0);
+      seqs.load(a, b0);
+      blocks = add_sat(blocks, last_lane(wave_scan(prompts.items)));
+      items = add_sat(items, last_lane(wave_scan(seqs.items)));
+    }
+    if (blocks > (unsigned)x.blocks || items > a.most_items) {  // row starts that overlap
+      if (unit == 0 && threadIdx.x == 0) *a.count = 0;
+      return;
+    }
+    if ((unsigned)unit < blocks) {
+      const Place p = place_of(a, prompts, blocks - 1 - unit, kItems, 1);  // late rows first, which see most keys
+      if (!p.there) return;
+      // the items of the rows' kernel that this block is, by the sequences in front
+      unsigned first = 0;
+      for (int b0 = 0; b0 <= p.b; b0 += 64) {
+        if (a.c.n_seqs > 64) seqs.load(a, b0);
+        const unsigned upto = wave_scan(seqs.items);
+        first += b0 + 64 <= p.b ? last_lane(upto) : (unsigned)__builtin_amdgcn_readlane((int)(upto - seqs.items), p.b - b0);
+      }
+      const int block = (int)(p.inner / (unsigned)a.c.kv_heads), hk = (int)p.inner - block * a.c.kv_heads, log2 = 4 + a.wide;
+      const int all_rows = p.q.s.n * a.group, of_seq = (all_rows + (1 << log2) - 1) >> log2, of_block = 1 << (kLog2 - log2);
+      first += (unsigned)(hk * of_seq + block * of_block);
+      const PrefixGroup g = group_at(p.b);
+      if ((int)threadIdx.x < min(of_block, of_seq - block * of_block)) {
+        const int row0 = (block << kLog2) + ((int)threadIdx.x << log2);
+        x.item[first + threadIdx.x] = own_item(a, {0, 1, p.q.s.r0, row0, min(all_rows - row0, 1 << log2), hk}, p.q.s.n, g);
+      }
+      const size_t row = (size_t)(kOwnSlots + first) * a.slot_rows;
+      prompt_body<Act, KV, DT, kHalfForm, kOwnTokens>(a, 0, {p.b, p.q.s, hk, block, 0, 0, p.q.from, a.part + row * DT, a.state + 2 * row});
+      return;
+    }
+    unit -= (int)blocks;
+  }
+  if (unit < kOwnGrid) rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)unit, kOwnGrid, m.from, group_at);
 }
 
 // Where rows are few: a workgroup per row and kSlice of its values, its threads four values of every 256 / (kSlice / 4)th share each
@@ -342,7 +397,7 @@ __global__ __launch_bounds__(256) void join_rows_kernel(Attend a, unsigned rows)
     if (r >= s.rows) continue;
     float top = -INFINITY, sum = 0.0f;
     f32x4 acc = {0, 0, 0, 0};
-    for (int i0 = 0; i0 < s.count; i0 += 4) add_shares<DT, 4, 1>(a, s, item, r, d, i0, top, sum, acc);
+    for (int i0 = 0; i0 < s.count; i0 += 8) add_shares<DT, 8, 1>(a, s, item, r, d, i0, top, sum, acc);
     finish<Act, false>(a, s.own.r0, s.own.row0 + r, s.own.head, 0, d, acc, top == -INFINITY ? 0.0f : top, sum);
   }
 }
@@ -350,7 +405,9 @@ __global__ __launch_bounds__(256) void join_rows_kernel(Attend a, unsigned rows)
 // ---- host ------------------------------------------------------------------------------------------------------------------
 struct Plan {
   OwnPlan own;
-  bool dealt;     // by a launch in front
+  bool dealt;       // by a launch in front
+  int prompt_rows;  // pairs of a sequence from which on it goes by blocks of them, of which there are `blocks`; 0: none does
+  unsigned blocks;
   unsigned grid;  // workgroups of the prefixes
   size_t group_off, from_off, of_off, item_off, part_off, state_off, pre_part_off, pre_state_off, total;
 };
@@ -362,7 +419,11 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int n_groups,
   p.dealt = c->n_seqs > kLanes || n_groups > kLaneGroups;
   const long long items = (((long long)r->rows * group >> kLog2) + n_groups) * c->kv_heads;
   const long long grid = items > 2 * kSlots ? items : 2 * kSlots;
-  if (grid > most_groups(512)) return W4A32_ESHAPE;
+  const long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
+  p.prompt_rows = most * group >= kOwnPromptRows ? kOwnPromptRows : 0;
+  const long long blocks = p.prompt_rows ? (((long long)r->rows * group >> kLog2) + c->n_seqs) * c->kv_heads : 0;
+  if (grid + blocks + kOwnGrid > most_groups(64 * kWaves)) return W4A32_ESHAPE;
+  p.blocks = (unsigned)blocks;
   p.grid = (unsigned)grid;
   size_t at = 256;
   auto take = [&](size_t bytes) {
@@ -411,10 +472,10 @@ hipError_t launch_both(const Attend& a, const Plan& p, hipStream_t s) {
     if (hipError_t e = limit.raise((const void*)both_kernel<Act, KV, DT>, lds); e != hipSuccess) return e;
   }
   if (p.dealt) {
-    hipLaunchKernelGGL((deal_kernel<Shape<Act, KV, DT, kHalfForm>::kKeys, tile_keys<KV>()>), dim3(1), dim3(kPlan), 0, s, a);
+    hipLaunchKernelGGL((deal_kernel<Shape<Act, KV, DT, kHalfForm>::kKeys, tile_keys<KV>(), sizeof(KV) == 4>), dim3(1), dim3(kPlan), 0, s, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(p.grid + kOwnGrid), dim3(64 * kWaves), lds, s, a);
+  hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(p.grid + p.blocks + kOwnGrid), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
 template <typename Act, typename KV>
@@ -455,10 +516,10 @@ int w4a32_op_paged_prefix_attention(const w4a32_paged_cache* cache, const w4a32_
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   auto at = [&](size_t off) { return p.dealt ? (int*)(scratch + off) : nullptr; };
-  const Prefix x{d_group_start, d_prefix, n_groups, (int)p.grid, (OwnItem*)(scratch + p.item_off), (float*)(scratch + p.pre_part_off),
+  const Prefix x{d_group_start, d_prefix, n_groups, (int)p.grid, (int)p.blocks, (OwnItem*)(scratch + p.item_off), (float*)(scratch + p.pre_part_off),
                  (float*)(scratch + p.pre_state_off), at(128), (PrefixGroup*)at(p.group_off), at(p.from_off), at(p.of_off)};
   Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
-           rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, 0, rows->rows, 0, 0, 0, kLog2,
+           rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, 0, rows->rows, 0, 0, p.prompt_rows, kLog2,
            p.own.wide, p.own.slot_rows, (unsigned)p.own.items, (unsigned)p.own.tiles, scale * kLog2e, nullptr,
            (unsigned*)scratch, (float*)(scratch + p.part_off), (float*)(scratch + p.state_off), nullptr, nullptr, x};
   set_group(a);

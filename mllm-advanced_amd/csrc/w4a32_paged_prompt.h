@@ -57,9 +57,20 @@ __device__ __forceinline__ void load_lds(const void* from, unsigned to) {
 #pragma clang diagnostic pop
 static __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
-// kPrefix: a workgroup has a share of the keys of a prefix, for rows of all sequences of the group, and leaves its sums in scratch memory
-template <typename Act, typename KV, int DT, Form kForm, bool kPrefix>
-__device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, const PrefixGroup& g) {
+// kAllTokens: rows of one sequence and all that they see. kPrefixTokens: a share of the keys of a prefix, for rows of all sequences of the
+// group, which see all of it. kOwnTokens: rows of one sequence and what they see from `from` on. The last two leave their sums in scratch memory.
+enum Tokens { kAllTokens, kPrefixTokens, kOwnTokens };
+struct Piece {
+  int b;           // whose pages
+  Span s;          // rows, of which block `block` is this workgroup's
+  int hk, block;
+  int first, end;  // kPrefixTokens: tiles
+  int from;        // kOwnTokens
+  float *part, *state;  // for its first row
+};
+template <typename Act, typename KV, int DT, Form kForm, Tokens kTokens>
+__device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, const Piece& given) {
+  constexpr bool kPrefix = kTokens == kPrefixTokens;
   using M = Math<Act, KV>;
   using Sh = Shape<Act, KV, DT, kForm>;
   constexpr bool kSplit = kForm == kTeamsForm;
@@ -80,16 +91,12 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
   // ---- which rows ----
   const unsigned group = a.group, kv = a.c.kv_heads;
   Place p;
-  int block, hk, first_tile = 0, end_tile = 0;
-  if constexpr (kPrefix) {
-    const unsigned in = unit - g.first, in_kv = in / kv, share = in_kv / g.blocks;
-    hk = (int)(in - in_kv * kv);
-    block = (int)(in_kv - share * g.blocks);
-    const int tiles = (g.tokens + KB - 1) / KB;
-    first_tile = (int)((long long)tiles * share / g.shares);
-    end_tile = (int)((long long)tiles * (share + 1) / g.shares);
-    p.b = g.b;
-    p.q.s = {g.r0, g.n, g.tokens - 1};
+  int block, hk;
+  if constexpr (kTokens != kAllTokens) {
+    hk = given.hk;
+    block = given.block;
+    p.b = given.b;
+    p.q.s = given.s;
   } else {
     Seqs<KB, kPrompt> seqs;
     unsigned total = 0;
@@ -142,9 +149,9 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
   const int pos = kPrefix ? s.len : s.len + j, pos_min = slot_of(row0), pos_max = slot_of(row0 + 31);
   const int block_min = slot_of(of0), block_max = slot_of(of0 + kBlock - 1);
   // tiles that the workgroup's rows can see: [0, ft) and [w0, ..), of those that the table has
-  const int w0 = a.window ? max(0, min(block_min, a.c.cap - 1) - a.window + 1) / KB : 0;
+  const int w0 = kTokens == kOwnTokens ? min(given.from, a.c.cap - 1) / KB : a.window ? max(0, min(block_min, a.c.cap - 1) - a.window + 1) / KB : 0;
   const int ft = a.window ? min((min(a.first, a.c.cap) + KB - 1) / KB, w0) : 0;
-  const int nt = kPrefix ? end_tile : ft + min(block_max, a.c.cap - 1) / KB + 1 - w0;
+  const int first_tile = kPrefix ? given.first : 0, nt = kPrefix ? given.end : ft + min(block_max, a.c.cap - 1) / KB + 1 - w0;
   auto key_of = [&](int t) { return (t < ft ? t : t - ft + w0) * KB; };
 
   // ---- q ----
@@ -247,9 +254,10 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
     }
     return gone;
   };
+  auto in_front = [&](int key) { return kTokens == kOwnTokens && key < given.from; };  // in the prefix
   // Whether rows that stand from lo to hi all see all `keys` keys from k0 on
   auto seen_by = [&](int k0, int keys, int lo, int hi) {
-    return k0 + keys - 1 <= lo && (a.window == 0 || k0 > hi - a.window || k0 + keys - 1 < a.first);
+    return k0 + keys - 1 <= lo && !in_front(k0) && (a.window == 0 || k0 > hi - a.window || k0 + keys - 1 < a.first);
   };
   auto all_seen = [&](int k0, int lo, int hi) { return seen_by(k0, KB, lo, hi); };
   // The tile has arrived, for all wavefronts. Where not all rows see all of it: zeros for what no row sees, and for values that
@@ -271,7 +279,7 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
 #pragma unroll 1
     for (int i = team_tid; i < KB * kPerKey; i += kTeamThreads) {
       const int key = i / kPerKey, at = k0 + key;
-      const bool none = (gone >> key / 16 & 1) | (at > block_max) | ((a.window != 0) & (at <= block_min - a.window) & (at >= a.first));
+      const bool none = (gone >> key / 16 & 1) | (at > block_max) | in_front(at) | ((a.window != 0) & (at <= block_min - a.window) & (at >= a.first));
       u32x4 x = vs[i];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -349,7 +357,7 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
           for (int i = 0; i < 16; ++i) {
             const int key = first_key + 32 * u + 8 * (i / 4) + i % 4;
             const bool gone_key = gone_here >> (2 * u + i / 8) & 1;
-            const bool sees = real & (key <= pos) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !gone_key;
+            const bool sees = real & (key <= pos) & !in_front(key) & ((a.window == 0) | (key > pos - a.window) | (key < a.first)) & !gone_key;
             sc[u][i] = sees ? sc[u][i] : -INFINITY;
           }
       }
@@ -477,9 +485,8 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
     }
     return;
   }
-  if constexpr (kPrefix) {
-    const size_t at = (size_t)unit * kBlock + 32 * member + row;
-    float* part = a.prefix.part + at * DT;
+  if constexpr (kTokens != kAllTokens) {
+    float *part = given.part + (32 * member + row) * DT, *state = given.state + 2 * (32 * member + row);
     if (real) {
 #pragma unroll
       for (int d = 0; d < kDims; ++d)
@@ -487,8 +494,8 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
         for (int b = 0; b < 4; ++b)
           *(W4_GLOBAL f32x4*)(part + 32 * d + 8 * b + 4 * half) = f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
       if (half == 0) {
-        a.prefix.state[2 * at] = m - (float)kWeight;
-        a.prefix.state[2 * at + 1] = l;
+        state[0] = m - (float)kWeight;
+        state[1] = l;
       }
     }
     if (__builtin_expect(some_odd, 0)) {
@@ -497,12 +504,14 @@ __device__ __forceinline__ void prompt_body(const Attend& a, unsigned unit, cons
 #pragma unroll 1
       for (int add = 0; add < 2; ++add)
 #pragma unroll 1
-        for (t = first_tile; t < nt; ++t)
-          put_odd<M, KV, 32>(a, table, hk, key_of(t), min(KB, s.len + 1 - key_of(t)), s.len, row0, all_rows, [&](int r, int d, float v) {
+        for (t = first_tile; t < nt; ++t) {
+          const int k0 = kPrefix ? key_of(t) : max(key_of(t), given.from), end = key_of(t) + KB;
+          put_odd<M, KV, 32>(a, table, hk, k0, (kPrefix ? min(end, s.len + 1) : end) - k0, s.len, row0, all_rows, [&](int r, int d, float v) {
             if (!(numbers >> r & 1)) return;
-            float& sum = a.prefix.part[((size_t)unit * kBlock + 32 * member + r) * DT + d];
+            float& sum = given.part[(32 * member + r) * DT + d];
             sum = add ? sum + v : 0.0f;
           });
+        }
     }
     return;
   }

@@ -36,7 +36,7 @@ namespace paged {
 namespace {
 template <typename Act, typename KV, int DT, Form kForm>
 __global__ __launch_bounds__((Shape<Act, KV, DT, kForm>::kThreads), DT == 256 || kForm == kTeamsForm ? 1 : 2) void prompt_kernel(Attend a) {
-  prompt_body<Act, KV, DT, kForm, false>(a, blockIdx.x, {});
+  prompt_body<Act, KV, DT, kForm, kAllTokens>(a, blockIdx.x, {});
 }
 
 template <typename Act, typename KV, int DT, Form kForm>

@@ -15,7 +15,8 @@ constexpr int kFew = 16;          // tiles of a share up to which it has tiles o
 
 template <int KT, Which kWhich>
 __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT, kWhich>& s, unsigned grid) {
-  Deal d = {0, 0, 0, false};
+  Deal d = {0, 0, 0, true, false};
+  unsigned others = 0;  // items without tiles
   bool all_short = true;
   if (a.c.n_seqs == 1) {  // nothing to add up: a decode step of one sequence is all latency
     s.load(a, 0);
@@ -27,10 +28,12 @@ __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT, kWhich>& s, un
     d.total = add_sat(d.total, last_lane(wave_scan(s.tiles)));
     d.items = add_sat(d.items, last_lane(wave_scan(s.items)));
     all_short = all_short && !__any(s.q.nt > kAlone);
+    if constexpr (kWhich == kOwn) others = add_sat(others, last_lane(wave_scan(s.tiles ? 0 : s.items)));
   }
-  if (d.total == 0 || d.total > a.most_tiles || d.items > a.most_items) return d;
+  d.fits = d.total <= a.most_tiles && d.items <= a.most_items;
+  if (d.total == 0 || !d.fits) return d;
   d.per = max((d.total + grid - 1) / grid, (unsigned)kMinTiles);
-  const unsigned more = grid - min(grid, d.items);  // workgroups beyond one per item
+  const unsigned more = grid - min(grid, d.items - others);  // workgroups beyond one per item
   if (all_short) {  // a workgroup takes every grid-th
     d.per = kAlone;
     d.apart = true;
@@ -69,6 +72,13 @@ constexpr size_t lds_bytes() { return kWaves * (wave_lds<KV, DT>() + kRows * 2 *
 
 // DT: the head size rounded up to 64, 128 or 256. kDump: leave the scores for the launch that adds the weights up. kWhich == kOwn: the tokens
 // behind a prefix, whose sums another launch joins with the prefix's.
+// An item of a sequence with n rows, in its group (without rows, where it has none)
+__device__ __forceinline__ OwnItem own_item(const Attend& a, const Item& it, int n, const PrefixGroup& q) {
+  const int row = it.r0 - q.r0;
+  if (row < 0 || row + n > q.n) return {it, 0, 0, 0, 0};
+  return {it, row * a.group + it.row0, q.first + it.head, q.shares, q.blocks * a.c.kv_heads};
+}
+
 // own_from: where this lane's sequence's own tokens begin; group_at: the group of a sequence, without rows where it has none.
 template <typename Act, typename KV, int DT, bool kDump, Which kWhich, typename GroupAt>
 __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsigned grid, int own_from, GroupAt group_at) {
@@ -88,7 +98,7 @@ __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsig
   Seqs<KT, kWhich> seqs;
   seqs.own_from = own_from;
   const Deal deal = deal_of(a, seqs, grid);
-  if (block == 0 && threadIdx.x == 0) *a.count = deal.per ? deal.items : 0;
+  if (block == 0 && threadIdx.x == 0) *a.count = deal.fits ? deal.items : 0;
   if (deal.per == 0) return;
   unsigned u = block, u_end = max(deal.items, grid);
   if (!deal.apart) {
@@ -414,10 +424,7 @@ __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsig
     const int slot = 2 * (int)block + (t_lo == 0);
     if constexpr (kWhich == kOwn) {
       if (t_lo == 0 && wave == 0) {
-        const PrefixGroup q = group_at(p.b);
-        const int row = s.r0 - q.r0;
-        OwnItem o{{w_first, shares, s.r0, of0, rows, hk}, 0, 0, 0, 0};
-        if (row >= 0 && row + s.n <= q.n) o = {o.own, row * a.group + of0, q.first + hk, q.shares, q.blocks * a.c.kv_heads};
+        const OwnItem o = own_item(a, {w_first, shares, s.r0, of0, rows, hk}, s.n, group_at(p.b));
         if (lane == 0) a.prefix.item[p.item0 + item] = o;
       }
     } else {

@@ -84,6 +84,10 @@ SHAPES = [
     (28, 4, 128, 16, [20], [515], [i % 23 for i in range(20)], [1] * 20),                     # a workgroup of 256 rows, not all there
     (14, 2, 64, 16, [9, 8], [333, 260], list(range(17)), [3 + i % 3 for i in range(17)]),
     (16, 2, 256, 32, [10], [130], list(range(10)), [2] * 10),
+    (12, 2, 64, 16, [3, 2], [100, 31], [5, 0, 70, 0, 1], [50, 3, 130, 22, 21]),                # prompts of more rows than a workgroup has, and fewer
+    (12, 2, 128, 16, [2], [77], [0, 3], [64, 90]),                                            # and no others
+    (4, 2, 256, 32, [3], [130], [100, 0, 40], [90, 1, 65]),
+    (7, 1, 72, 16, [2, 2], [40, 0], [13, 0, 0, 50], [40, 19, 18, 60]),
     (12, 1, 128, 64, [30], [700], [3 * i for i in range(30)], [1 + i % 2 for i in range(30)]),
 ]
 
@@ -110,6 +114,11 @@ def test_one_sequence_and_many(pkg, act, kind):
     run(pkg, Groups(4, [1], [50], [3], [2], 2, 64, 16), act, kind, 6)
     counts = [3] * 50   # more than a wavefront's lanes of groups and sequences
     run(pkg, Groups(5, counts, [16 + 3 * i for i in range(50)], [i % 20 for i in range(150)], [(i * 7) % 3 for i in range(150)], 2, 64, 16), act, kind, 6)
+    for n in (64, 65):   # one wavefront's lanes of sequences, and more
+        run(pkg, Groups(5, [n - 7, 4, 3], [50, 0, 33], [i % 20 for i in range(n)], [i % 3 for i in range(n)], 2, 64, 16), act, kind, 6)
+    for n in (16, 17):   # as many groups as are gone through one by one, and more
+        run(pkg, Groups(5, [2] * n, [20 + i for i in range(n)], [i % 20 for i in range(2 * n)], [1 + i % 3 for i in range(2 * n)], 2, 64, 16), act, kind, 6)
+    run(pkg, Groups(5, [40, 40], [50, 33], [i % 20 for i in range(80)], [70 if i % 9 == 0 else 1 for i in range(80)], 1, 64, 16), act, kind, 2)
     run(pkg, Groups(6, [1] * 70 + [70], [20] * 71, [i % 5 for i in range(140)], [1] * 140, 1, 64, 16), act, kind, 2)
 
 
@@ -150,11 +159,10 @@ def test_lowest_and_infinite_values_where_nobody_sees_them(pkg, act, kind):
 
 
 @pytest.mark.parametrize("act,kind", TYPES)
-@pytest.mark.parametrize("wide", [False, True])
-def test_values_that_are_not_finite(pkg, act, kind, wide):
+@pytest.mark.parametrize("n,rows", [(2, 1), (24, 1), (2, 40)])
+def test_values_that_are_not_finite(pkg, act, kind, n, rows):
     """An infinite or NaN value of the prefix reaches all rows of the group and none of another, one behind it its sequence alone"""
-    n = 24 if wide else 2
-    B = Groups(11, [n, 2], [150, 40], [9] * n + [3, 3], [1] * (n + 2), 2, 64, 16)
+    B = Groups(11, [n, 2], [150, 40], [9] * n + [3, 3], [rows] * (n + 2), 2, 64, 16)
     heads = 12
     fill_new(B)
     p, i = B.slot(0, 77)
@@ -167,7 +175,7 @@ def test_values_that_are_not_finite(pkg, act, kind, wide):
     q = B.rng.standard_normal((B.total, heads * 64)) * 2.0
     q64, qt = held(q, act)
     cache, k64, v64 = on_gpu(pkg, B, kind)
-    out = pkg.op_paged_prefix_attention(cache, qt, dev(B.row_start), 1, heads, 0.125, dev(B.group_start), dev(np.array(B.prefix, np.int32)))
+    out = pkg.op_paged_prefix_attention(cache, qt, dev(B.row_start), rows, heads, 0.125, dev(B.group_start), dev(np.array(B.prefix, np.int32)))
     torch.cuda.synchronize()
     got = out.double().cpu().numpy().reshape(-1, heads, 64)
     with np.errstate(invalid="ignore"):
