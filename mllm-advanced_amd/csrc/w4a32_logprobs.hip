@@ -21,11 +21,12 @@ namespace w4 {
 namespace {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
-constexpr int kBlock = 1024, kEach = kBlock / 64;
+constexpr int kBlock = 1024;
 constexpr int kThreads = 1024;   // of the launch that finds the most probable tokens
 constexpr int kMaxima = 1024;    // blocks, or runs of them, whose maxima are compared
 constexpr int kList = 2048;      // logits that are put in order by counting
 constexpr int kMostTop = 1024;
+constexpr int kXcds = 8, kApart = 32;  // rows from which on those of the two launches meet in an XCD's L2
 
 struct Part {
   float top, sum, weighted;  // sum is NaN where a logit is NaN or +infinity
@@ -53,92 +54,120 @@ __device__ __forceinline__ float value_of(const void* row, int i) {
   return (float)__builtin_bit_cast(_Float16, h);
 }
 
-// A lane's 16 logits of the block that begins at `base`, -infinity behind the row's end, and their places.
-template <typename T>
-struct Lane {
-  static constexpr int kWide = 16 / (int)sizeof(T);
-  float v[kEach];
+// A lane's logits of kChunks chunks of 64 times 16 bytes that begin at base[c] (those from the row's end on: none), -infinity behind the row's end,
+// and their places. Bases are the same for all lanes. Rows may lie off 16 bytes: one branch for all chunks, so that their loads
+// are under way together.
+template <typename T, int kN>
+struct Chunks {
+  static constexpr int kWide = 16 / (int)sizeof(T), kChunk = 64 * kWide;
+  float v[kN][kWide];
   bool wide;
   __device__ __forceinline__ int place(int i) const {
     const int lane = threadIdx.x & 63;
-    return wide ? i / kWide * (64 * kWide) + lane * kWide + i % kWide : i * 64 + lane;
+    return wide ? lane * kWide + i : i * 64 + lane;
   }
-  __device__ __forceinline__ void load(const void* row, int base, int vocab) {
+  __device__ __forceinline__ void load(const T* row, const int (&base)[kN], int vocab) {
     const int lane = threadIdx.x & 63;
-    wide = ((uintptr_t)row & 15) == 0 && base + kBlock <= vocab;
-    if (wide) {
-      const u32x4* from = (const u32x4*)((const T*)row + base) + lane;
+    wide = ((uintptr_t)row & 15) == 0;
 #pragma unroll
-      for (int i = 0; i < kEach / kWide; ++i) {
-        const u32x4 x = load_global<u32x4>(from + 64 * i);
+    for (int c = 0; c < kN; ++c) wide = wide && (base[c] + kChunk <= vocab || base[c] >= vocab);
+    if (wide) {
+      u32x4 x[kN];
+#pragma unroll
+      for (int c = 0; c < kN; ++c) x[c] = load_global<u32x4>((const u32x4*)(row + (base[c] < vocab ? base[c] : 0)) + (base[c] < vocab ? lane : 0));
+#pragma unroll
+      for (int c = 0; c < kN; ++c)
 #pragma unroll
         for (int e = 0; e < kWide; ++e) {
+          float f;
           if constexpr (sizeof(T) == 4) {
-            v[kWide * i + e] = __uint_as_float(x[e]);
+            f = __uint_as_float(x[c][e]);
           } else {
-            const uint32_t h = e & 1 ? x[e / 2] >> 16 : x[e / 2] & 0xffffu;
+            const uint32_t h = e & 1 ? x[c][e / 2] >> 16 : x[c][e / 2] & 0xffffu;
             if constexpr (std::is_same<T, __bf16>::value)
-              v[kWide * i + e] = __uint_as_float(h << 16);
+              f = __uint_as_float(h << 16);
             else
-              v[kWide * i + e] = (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+              f = (float)__builtin_bit_cast(_Float16, (uint16_t)h);
           }
+          v[c][e] = base[c] < vocab ? f : -INFINITY;
         }
-      }
     } else {
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int at = base + i * 64 + lane;
-        const float x = value_of<T>(row, min(at, vocab - 1));
-        v[i] = at < vocab ? x : -INFINITY;
-      }
+      for (int c = 0; c < kN; ++c)
+#pragma unroll
+        for (int i = 0; i < kWide; ++i) {
+          const int at = base[c] + i * 64 + lane;
+          const float x = value_of<T>(row, min(at, vocab - 1));
+          v[c][i] = at < vocab ? x : -INFINITY;
+        }
     }
   }
 };
 
-__device__ __forceinline__ int wave_add(int x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-  return x;
+// By moves within the register file, as wave_add(double): six shuffles through LDS take 600 clocks
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ int moved(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRowMask, 0xf, false);
 }
-__device__ __forceinline__ float wave_add(float x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-  return x;
+template <int kCtrl, int kRowMask>
+__device__ __forceinline__ float moved(float x) {
+  return __int_as_float(moved<kCtrl, kRowMask>(__float_as_int(x)));
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T x) {
+  x += moved<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += moved<0x112, 0xf>(x);
+  x += moved<0x114, 0xf>(x);
+  x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x);  // row_bcast 15, 31
+  x += moved<0x143, 0xc>(x);
+  return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 // A wavefront per block
 template <typename T>
-__global__ __launch_bounds__(256) void blocks_kernel(Logprobs a, int groups) {
-  const int r = blockIdx.x / groups, block = (blockIdx.x - r * groups) * 4 + (threadIdx.x >> 6), base = block * kBlock;
-  if (block >= a.blocks) return;
+__global__ __launch_bounds__(256) void blocks_kernel(Logprobs a, int groups, bool apart) {
+  // kXcds rows go on side by side where `apart`: workgroups of numbers kXcds apart are one XCD's, and so are a row's here and in the next launch
+  const int unit = apart ? blockIdx.x / kXcds : blockIdx.x, of = unit / groups, r = apart ? of * kXcds + blockIdx.x % kXcds : of;
+  const int block = (unit - of * groups) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (block >= a.blocks || r >= a.rows) return;
   const T* row = (const T*)a.logits + (size_t)r * a.ldl;
   const int64_t token = a.tokens ? a.tokens[r] : -1;
   const bool known = token >= 0 && token < a.vocab;
-  Lane<T> x;
+  constexpr int kChunk = Chunks<T, 1>::kChunk, kN = kBlock / kChunk, kWide = Chunks<T, 1>::kWide;
+  int base[kN];
+#pragma unroll
+  for (int c = 0; c < kN; ++c) base[c] = block * kBlock + c * kChunk;
+  Chunks<T, kN> x;
   x.load(row, base, a.vocab);
   const float mine = value_of<T>(row, known ? (int)token : 0);
   float top = -INFINITY;
   bool odd = false;
   int before = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    top = fmaxf(top, x.v[i]);
-    odd |= !(x.v[i] < INFINITY);
-    before += x.v[i] > mine || (x.v[i] == mine && base + x.place(i) < (int)token);
-  }
+  for (int c = 0; c < kN; ++c)
+#pragma unroll
+    for (int i = 0; i < kWide; ++i) {
+      const float v = x.v[c][i];
+      top = fmaxf(top, v);
+      odd |= !(v < INFINITY);
+      before += v > mine || (v == mine && base[c] + x.place(i) < (int)token);
+    }
   top = wave_max(top);
   // the difference first: products of large logits would be off by their own rounding
   const float from = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, weighted = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const float d = fminf(from - x.v[i], FLT_MAX), e = __builtin_amdgcn_exp2f(-__fmaf_rn(d, a.scale_low, d * a.scale));
-    sum += e;
-    weighted += e > 0.0f ? e * d : 0.0f;
-  }
-  sum = wave_add(sum);
-  weighted = wave_add(weighted);
-  before = wave_add(before);
+  for (int c = 0; c < kN; ++c)
+#pragma unroll
+    for (int i = 0; i < kWide; ++i) {
+      const float d = fminf(from - x.v[c][i], FLT_MAX), e = __builtin_amdgcn_exp2f(-__fmaf_rn(d, a.scale_low, d * a.scale));
+      sum += e;
+      weighted += e > 0.0f ? e * d : 0.0f;
+    }
+  sum = wave_sum(sum);
+  weighted = wave_sum(weighted);
+  before = wave_sum(before);
   if (__any(odd)) sum = NAN;
   if ((threadIdx.x & 63) == 0) a.part[(size_t)r * a.blocks + block] = Part{top, sum, weighted, known ? before : -1};
 }
@@ -160,15 +189,21 @@ struct Shared {
 struct Row {
   double norm;  // ln S
   float top;
+  float mine;   // maximum of this thread's first block
   bool none;    // no distribution
 };
-// A row's sums from its blocks', by all threads; writes what belongs to the given token, and the entropy.
+// A row's sums from its blocks', by all threads. The last wavefront writes what belongs to the given token, and the entropy.
 template <typename T, int kN>
 __device__ __forceinline__ Row join(const Logprobs& a, int r, Shared<kN>& sh) {
   const Part* parts = a.part + (size_t)r * a.blocks;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < a.blocks; i += kN) top = fmaxf(top, parts[i].top);
+  const Part mine = (int)threadIdx.x < a.blocks ? parts[threadIdx.x] : Part{-INFINITY, 0.0f, 0.0f, 0};  // all there is up to kN blocks
+  const bool writes = threadIdx.x == kN - 64;
+  const int64_t token = writes && a.tokens ? a.tokens[r] : -1;
+  const bool known = token >= 0 && token < a.vocab;
+  const float x = writes ? value_of<T>((const T*)a.logits + (size_t)r * a.ldl, known ? (int)token : 0) : 0.0f;
+  float top = mine.top;
+  for (int i = threadIdx.x + kN; i < a.blocks; i += kN) top = fmaxf(top, parts[i].top);
   top = wave_max(top);
   if constexpr (kN > 64) {
     if (lane == 0) sh.top[wave] = top;
@@ -178,17 +213,18 @@ __device__ __forceinline__ Row join(const Logprobs& a, int r, Shared<kN>& sh) {
   }
   double sum = 0.0, weighted = 0.0;
   int before = 0;
-  for (int i = threadIdx.x; i < a.blocks; i += kN) {
-    const Part p = parts[i];
+  auto add = [&](const Part& p) {
     before += p.before;
-    if (p.top == -INFINITY && p.sum == p.sum) continue;
+    if (p.top == -INFINITY && p.sum == p.sum) return;
     const double d = (double)top - p.top, e = exp(-d * a.inv_t);
     sum += p.sum * e;
     weighted += (p.weighted + p.sum * d) * e;
-  }
-  sum = w4::wave_add(sum);
-  weighted = w4::wave_add(weighted);
-  before = wave_add(before);
+  };
+  add(mine);
+  for (int i = threadIdx.x + kN; i < a.blocks; i += kN) add(parts[i]);
+  sum = wave_add(sum);
+  weighted = wave_add(weighted);
+  before = wave_sum(before);
   if constexpr (kN > 64) {
     if (lane == 0) {
       sh.sum[wave] = sum;
@@ -207,17 +243,13 @@ __device__ __forceinline__ Row join(const Logprobs& a, int r, Shared<kN>& sh) {
   }
   Row row;
   row.top = top;
+  row.mine = mine.top;
   row.none = !(sum > 0.0);
   row.norm = log(sum);
-  if (threadIdx.x == 0) {
+  if (writes) {
     if (a.entropy) a.entropy[r] = row.none ? NAN : (float)(row.norm + weighted / sum * a.inv_t);
-    if (a.tokens) {
-      const int64_t token = a.tokens[r];
-      const bool known = token >= 0 && token < a.vocab;
-      const float x = value_of<T>((const T*)a.logits + (size_t)r * a.ldl, known ? (int)token : 0);
-      if (a.logprob) a.logprob[r] = row.none ? NAN : known ? (float)(((double)x - top) * a.inv_t - row.norm) : -INFINITY;
-      if (a.rank) a.rank[r] = row.none || !known ? -1 : before;
-    }
+    if (a.logprob) a.logprob[r] = row.none ? NAN : known ? (float)(((double)x - top) * a.inv_t - row.norm) : -INFINITY;
+    if (a.rank) a.rank[r] = row.none || !known ? -1 : before;
   }
   return row;
 }
@@ -235,10 +267,10 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Logprobs a) {
   __shared__ Shared<kThreads> sh;
   __shared__ uint32_t maxima[kMaxima];
   __shared__ unsigned list[2 * kList];  // keys, places; or 4096 counts
-  __shared__ int runs[kMaxima];
+  __shared__ int runs[kMaxima], ranks[kMaxima];
   __shared__ unsigned n_runs, n_list, state[2], in_wave[kThreads / 64];
   __shared__ uint32_t bound;
-  const int r = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, top = min(a.top, a.vocab);
+  const int r = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), top = min(a.top, a.vocab);
   const T* logits = (const T*)a.logits + (size_t)r * a.ldl;
   int64_t* out_token = a.top_token + (size_t)r * a.top;
   float* out_logprob = a.top_logprob + (size_t)r * a.top;
@@ -257,53 +289,92 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Logprobs a) {
   // ---- the bound: the top-th largest maximum ----
   const Part* parts = a.part + (size_t)r * a.blocks;
   const int run = (a.blocks + kMaxima - 1) / kMaxima, count = (a.blocks + run - 1) / run;
-  if (tid < count) {
-    float m = -INFINITY;
-    for (int i = tid * run; i < min((tid + 1) * run, a.blocks); ++i) m = fmaxf(m, parts[i].top);
-    maxima[tid] = key_of(m);
+  float most = row.mine;
+  if (run > 1 && tid < count) {
+    most = -INFINITY;
+    for (int i = tid * run; i < min((tid + 1) * run, a.blocks); ++i) most = fmaxf(most, parts[i].top);
   }
+  maxima[tid] = key_of(most);
   if (tid == 0) {
     n_runs = n_list = 0;
     bound = kNone + 1;
   }
+  ranks[tid] = 0;
   __syncthreads();
-  if (tid < count) {
-    const uint32_t mine = maxima[tid];
-    int larger = 0;
-    for (int i = 0; i < count; ++i) larger += maxima[i] > mine || (maxima[i] == mine && i < tid);
-    if (larger == top - 1 && mine > kNone) bound = mine;
-  }
+  // How many of n come before each, to ranks: n threads have the i-th of them, and what it is compared with is dealt to as many more as there are
+  auto rank = [&](int n, auto before) {
+    const int slices = max(kThreads / n, 1), each = (n + slices - 1) / slices;
+    for (int x = tid; x < n * slices; x += kThreads) {
+      const int slice = x / n, i = x - slice * n, end = min((slice + 1) * each, n);
+      int count = 0;
+#pragma unroll 8
+      for (int j = slice * each; j < end; ++j) count += before(j, i);
+      if (slices == 1)
+        ranks[i] = count;
+      else if (count)
+        atomicAdd(&ranks[i], count);
+    }
+    __syncthreads();
+  };
+  rank(count, [&](int j, int i) { return maxima[j] > maxima[i] || (maxima[j] == maxima[i] && j < i); });
+  if (tid < count && ranks[tid] == top - 1 && maxima[tid] > kNone) bound = maxima[tid];
   __syncthreads();
   const uint32_t least = bound;
+  ranks[tid] = 0;
   if (tid < count && maxima[tid] >= least) runs[atomicAdd(&n_runs, 1u)] = tid;
   __syncthreads();
-  const int blocks = (int)n_runs * run;  // to be read again
-  auto block_at = [&](int i) { return runs[i / run] * run + i % run; };
-  for (int i = wave; i < blocks; i += kThreads / 64) {
-    const int block = block_at(i);
-    if (block >= a.blocks) continue;
-    Lane<T> x;
-    x.load(logits, block * kBlock, a.vocab);
+  // What of them is to be read again, by put_one(key, place): a wavefront has every 16th chunk, several of them at once
+  constexpr int kChunk = Chunks<T, 1>::kChunk, kChunks = kBlock / kChunk, kAhead = sizeof(T) == 4 ? 8 : 4;
+  const float floor = of_key(least);
+  const int chunks = __builtin_amdgcn_readfirstlane((int)n_runs) * run * kChunks;
+  auto each = [&](auto put_one) {
+    for (int i0 = wave; i0 < chunks; i0 += kAhead * (kThreads / 64)) {
+      int base[kAhead];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const uint32_t k = key_of(x.v[e]);
-      if (k < least) continue;
-      const unsigned at = atomicAdd(&n_list, 1u);
-      if (at < kList) {
-        list[at] = k;
-        list[kList + at] = (unsigned)(block * kBlock + x.place(e));
+      for (int c = 0; c < kAhead; ++c) {
+        const int i = i0 + c * (kThreads / 64), block = i / kChunks;
+        base[c] = a.vocab;
+        if (i < chunks) {
+          const int at = run == 1 ? runs[block] : runs[block / run] * run + block % run;
+          base[c] = min(__builtin_amdgcn_readfirstlane(at) * kBlock + i % kChunks * kChunk, a.vocab);
+        }
+      }
+      Chunks<T, kAhead> x;
+      x.load(logits, base, a.vocab);
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) {
+        float most = x.v[c][0];
+#pragma unroll
+        for (int e = 1; e < Chunks<T, 1>::kWide; ++e) most = fmaxf(most, x.v[c][e]);
+        if (!__any(most >= floor)) continue;  // most chunks
+#pragma unroll
+        for (int e = 0; e < Chunks<T, 1>::kWide; ++e) put_one(key_of(x.v[c][e]), (unsigned)(base[c] + x.place(e)));
       }
     }
-  }
+  };
+  each([&](uint32_t k, unsigned place) {
+    if (k < least) return;
+    const unsigned at = atomicAdd(&n_list, 1u);
+    if (at < kList) {
+      list[at] = k;
+      list[kList + at] = place;
+    }
+  });
   __syncthreads();
   const unsigned found = n_list;
-  auto order = [&](unsigned n) {  // writes the first of the list's n
-    for (unsigned i = tid; i < n; i += kThreads) {
+  auto order = [&](int n) {  // writes the first of the list's n
+    if (n <= kMaxima) {
+      rank(n, [&](int j, int i) { return list[j] > list[i] || (list[j] == list[i] && list[kList + j] < list[kList + i]); });
+      if (tid < n && ranks[tid] < top) put((unsigned)ranks[tid], list[tid], list[kList + tid]);
+      return;
+    }
+    for (int i = tid; i < n; i += kThreads) {
       const uint32_t k = list[i];
       const unsigned place = list[kList + i];
-      unsigned first = 0;
-      for (unsigned j = 0; j < n; ++j) first += list[j] > k || (list[j] == k && list[kList + j] < place);
-      if (first < (unsigned)top) put(first, k, place);
+      int first = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) first += list[j] > k || (list[j] == k && list[kList + j] < place);
+      if (first < top) put((unsigned)first, k, place);
     }
   };
   for (unsigned i = min(found, (unsigned)top) + tid; i < (unsigned)a.top; i += kThreads) {
@@ -311,7 +382,7 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Logprobs a) {
     out_logprob[i] = -INFINITY;
   }
   if (found <= kList) {
-    order(found);
+    order((int)found);
     return;
   }
   // ---- too many: the top-th largest key, 12, 10 and 10 bits at a time ----
@@ -321,25 +392,17 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Logprobs a) {
     __syncthreads();
     for (int i = tid; i < 1 << bits; i += kThreads) list[i] = 0;
     __syncthreads();
-    for (int i = wave; i < blocks; i += kThreads / 64) {
-      const int block = block_at(i);
-      if (block >= a.blocks) continue;
-      Lane<T> x;
-      x.load(logits, block * kBlock, a.vocab);
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const uint32_t k = key_of(x.v[e]);
-        if (k >= least && (k & mask) == prefix) atomicAdd(&list[k >> shift & ((1u << bits) - 1)], 1u);
-      }
-    }
+    each([&](uint32_t k, unsigned) {
+      if (k >= least && (k & mask) == prefix) atomicAdd(&list[k >> shift & ((1u << bits) - 1)], 1u);
+    });
     __syncthreads();
-    const int each = (1 << bits) / kThreads, high = (1 << bits) - 1 - tid * each;  // thread i: the i-th `each` digits from the largest on
+    const int digits = (1 << bits) / kThreads, high = (1 << bits) - 1 - tid * digits;  // thread i: the i-th `digits` from the largest on
     unsigned sum = 0, all;
-    for (int i = 0; i < each; ++i) sum += list[high - i];
+    for (int i = 0; i < digits; ++i) sum += list[high - i];
     const unsigned upto = paged::block_scan<kThreads>(sum, in_wave, all);
     unsigned above = upto - sum;
     if (above < want && upto >= want)
-      for (int i = 0; i < each; ++i) {
+      for (int i = 0; i < digits; ++i) {
         const unsigned h = list[high - i];
         if (above < want && above + h >= want) {
           state[0] = (unsigned)(high - i);
@@ -356,23 +419,17 @@ __global__ __launch_bounds__(kThreads) void top_kernel(Logprobs a) {
   // the larger ones, fewer than top, and the first `want` of those that have this key, in the row's order
   if (tid == 0) n_list = 0;
   __syncthreads();
-  for (int i = wave; i < blocks; i += kThreads / 64) {
-    const int block = block_at(i);
-    if (block >= a.blocks) continue;
-    Lane<T> x;
-    x.load(logits, block * kBlock, a.vocab);
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const uint32_t k = key_of(x.v[e]);
-      if (k <= prefix) continue;
-      const unsigned at = atomicAdd(&n_list, 1u);
-      list[at] = k;
-      list[kList + at] = (unsigned)(block * kBlock + x.place(e));
-    }
-  }
+  each([&](uint32_t k, unsigned place) {
+    if (k <= prefix) return;
+    const unsigned at = atomicAdd(&n_list, 1u);
+    list[at] = k;
+    list[kList + at] = place;
+  });
   __syncthreads();
-  order(n_list);
   const unsigned larger = n_list;
+  ranks[tid] = 0;
+  __syncthreads();
+  if (larger) order((int)larger);
   unsigned taken = 0;
   for (int block = 0; block < a.blocks && taken < want; ++block) {
     if (maxima[block / run] < prefix) continue;
@@ -390,7 +447,7 @@ bool layout_of(int rows, int vocab, int top, int& blocks, size_t& total) {
   if (rows < 1 || vocab < 1 || top < 0 || rows >= 1 << 24 || vocab >= 1 << 30 || top > kMostTop) return false;
   blocks = (vocab + kBlock - 1) / kBlock;
   // a launch has less than 2^32 threads: 256 of four blocks, 1024 of a row
-  if ((long long)rows * ((blocks + 3) / 4) >= 1ll << 24 || (top && rows >= 1 << 22)) return false;
+  if (((long long)rows + kXcds) * ((blocks + 3) / 4) >= 1ll << 24 || (top && rows >= 1 << 22)) return false;
   total = (size_t)rows * blocks * sizeof(Part);
   return true;
 }
@@ -398,7 +455,9 @@ bool layout_of(int rows, int vocab, int top, int& blocks, size_t& total) {
 template <typename T>
 int launch(const Logprobs& a, hipStream_t s) {
   const int groups = (a.blocks + 3) / 4;
-  hipLaunchKernelGGL((blocks_kernel<T>), dim3((unsigned)a.rows * groups), dim3(256), 0, s, a, groups);
+  const bool apart = a.top && a.rows >= kApart;
+  const unsigned rows = apart ? (unsigned)(a.rows + kXcds - 1) / kXcds * kXcds : (unsigned)a.rows;
+  hipLaunchKernelGGL((blocks_kernel<T>), dim3(rows * groups), dim3(256), 0, s, a, groups, apart);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   if (a.top)
     hipLaunchKernelGGL((top_kernel<T>), dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
