@@ -13,13 +13,14 @@ constexpr int kSettle = 1024;         // threads of the one workgroup that hands
 constexpr int kMostPlaces = 1 << 26;  // places of a table: a place's number and two marks are an int
 // A page with a negative count, which is someone else's: changes by all places there are leave it below kHeldBelow.
 constexpr int kHeld = -0x7f000000, kHeldBelow = -(1 << 30);
-constexpr int kShared = 1 << 30, kStays = 1 << 29, kPlace = kMostPlaces - 1;
+constexpr int kShared = 1 << 30, kStays = 1 << 29, kGiven = 1 << 28, kPlace = kMostPlaces - 1;
 
 // ---------------------------------------------------------------------------------------------
-// Fork. What each sequence becomes follows from its parent's length alone, so places are gone through in parallel: a new table
-// and the pages' new counts go to scratch memory, by atomic sums of whole numbers. The rows' places (one or two of a sequence
-// that decodes) are then listed in order and settled by one workgroup: who has to leave a shared page, which pages are free. Where
-// there are enough the last launch makes it all true; else nothing has changed.
+// Fork. What each sequence becomes follows from its parent's length alone, so places are gone through in parallel, and the pages' new
+// counts are atomic sums of whole numbers. The places that rows write (one or two of a sequence that decodes) are then listed in
+// order and settled by one workgroup: who has to leave a shared page, which pages are free. Where there are enough it all becomes true;
+// else nothing has changed.
+// Where the counts fit into LDS: one launch of one workgroup, a chain of a few waits for memory. Else four launches, with the new table and the new counts in scratch memory.
 // ---------------------------------------------------------------------------------------------
 struct Seq {
   int parent, len;  // -1: none; tokens
@@ -58,128 +59,370 @@ __device__ __forceinline__ Seq seq_of(const Fork& a, int b) {
   s.first = n ? min(s.len >> a.shift, s.need) : s.need;
   return s;
 }
-
-__global__ __launch_bounds__(256) void fork_begin_kernel(Fork a) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < a.n_pages) {
-    const int r = a.refs[i];
-    a.left[i] = r < 0 ? kHeld : min(r, kMostPlaces);
-  }
-  if (i < a.n_seqs) a.seq[i] = seq_of(a, i);
+__device__ __forceinline__ int count_at_first(int refs) { return refs < 0 ? kHeld : min(refs, kMostPlaces); }
+// The page that a place gets before rows are looked at; `old`: what is there
+__device__ __forceinline__ int inherited(const Fork& a, const Seq& s, int b, int at, int old) {
+  if (at < s.kept) return s.parent == b ? old : a.table[(size_t)s.parent * a.width + at];
+  return at < s.need && s.parent == b ? old : -1;
 }
 
-__global__ __launch_bounds__(256) void fork_places_kernel(Fork a) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.n_seqs * a.width) return;
-  const int b = i / a.width, at = i - b * a.width;
-  const Seq s = a.seq[b];
-  const int old = a.table[i];
-  int page = -1;
-  if (at < s.kept)
-    page = s.parent == b ? old : a.table[(size_t)s.parent * a.width + at];
-  else if (at < s.need && s.parent == b)
-    page = old;
-  a.next[i] = page;
-  if (page == old) return;
-  if (named(a, old)) atomicSub(&a.left[old], 1);
-  if (named(a, page)) atomicAdd(&a.left[page], 1);
-}
+// Counts in LDS, and in memory that several compute units have written: past the caches of this one.
+struct NearCounts {
+  static constexpr bool kNear = true;
+  int* left;
+  __device__ __forceinline__ int get(int p) const { return left[p]; }
+  __device__ __forceinline__ void set(int p, int v) const { left[p] = v; }
+};
+struct FarCounts {
+  static constexpr bool kNear = false;
+  int* left;
+  __device__ __forceinline__ int get(int p) const { return __hip_atomic_load(&left[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+  __device__ __forceinline__ void set(int p, int v) const { __hip_atomic_store(&left[p], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+};
 
-__device__ __forceinline__ int count_of(const Fork& a, int page) {
-  return __hip_atomic_load(&a.left[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-__global__ __launch_bounds__(kSettle) void fork_settle_kernel(Fork a) {
+// Settles the places that rows write, by one workgroup. seq, page_at: what the sequences become, and the pages of their places; place, was, fresh:
+// room for a.most of each, in LDS or not. Returns how many places there are, of which those with kGiven get page was[..]; -1: it cannot be done.
+// leave(page): a page that a sequence leaves, its count being what it will be.
+template <typename Counts, typename SeqAt, typename PageAt, typename Leave>
+__device__ __forceinline__ int settle(const Fork& a, Counts left, SeqAt seq, PageAt page_at, int* place, int* was, int* fresh, Leave leave_page) {
   __shared__ unsigned in_wave[kSettle / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // ---- the places that rows write ----
+  const int tid = threadIdx.x;
   unsigned total = 0;
+  bool shared = false;
   for (int b0 = 0; b0 < a.n_seqs; b0 += kSettle) {
     const int b = b0 + tid;
     Seq s = {};
-    if (b < a.n_seqs) s = a.seq[b];
+    if (b < a.n_seqs) s = seq(b);
     const unsigned n = (unsigned)(s.need - s.first);
     unsigned all;
     const unsigned at = total + block_scan<kSettle>(n, in_wave, all) - n;
-    for (unsigned i = 0; i < n; ++i) {
-      if (at + i >= (unsigned)a.most) break;
-      const int place = b * a.width + s.first + (int)i, page = a.next[place];
-      a.place[at + i] = place;
+    for (unsigned i = 0; i < n && at + i < (unsigned)a.most; ++i) {
+      const int i_at = s.first + (int)i, page = page_at(s, b, i_at);
       // a sequence's last tokens that are not there stay so, and the place with them
-      a.was[at + i] = named(a, page) ? page : s.first + (int)i < s.kept ? -2 : -1;
+      was[at + i] = named(a, page) ? page : i_at < s.kept ? -2 : -1;
+      const bool more = named(a, page) && left.get(page) != 1;
+      place[at + i] = b * a.width + i_at + (more ? kShared : 0);
+      shared |= more;
     }
     total += all;
   }
   const int n = (int)min(total, (unsigned)a.most);
-  __syncthreads();
   // ---- who has to leave a shared page: all that write it, or, where nobody else has it, all but the last ----
-  for (int c = tid; c < n; c += kSettle)
-    if (a.was[c] >= 0 && count_of(a, a.was[c]) != 1) a.place[c] |= kShared;
-  __syncthreads();
-  for (int c = tid; c < n; c += kSettle)
-    if (a.place[c] & kShared && count_of(a, a.was[c]) >= kHeldBelow) atomicSub(&a.left[a.was[c]], 1);
-  __syncthreads();
-  for (int c = tid; c < n; c += kSettle)
-    if (a.place[c] & kShared) {
-      const int r = count_of(a, a.was[c]);
-      if (r <= 0 && r >= kHeldBelow) atomicMin(&a.left[a.was[c]], -2 - (a.place[c] & kPlace));
-    }
-  __syncthreads();
-  for (int c = tid; c < n; c += kSettle)
-    if (a.place[c] & kShared && count_of(a, a.was[c]) == -2 - (a.place[c] & kPlace)) a.place[c] |= kStays;
-  __syncthreads();
-  unsigned wanted = 0;
-  auto leaves = [&](int c) { return (a.place[c] & (kShared | kStays)) == kShared; };
-  for (int c = tid; c < n; c += kSettle) {
-    if (a.place[c] & kStays) __hip_atomic_store(&a.left[a.was[c]], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    wanted += leaves(c) || a.was[c] == -1;
+  if (__syncthreads_or(shared)) {
+    for (int c = tid; c < n; c += kSettle)
+      if (place[c] & kShared && left.get(was[c]) >= kHeldBelow) atomicSub(&left.left[was[c]], 1);
+    __syncthreads();
+    for (int c = tid; c < n; c += kSettle)
+      if (place[c] & kShared) {
+        const int r = left.get(was[c]);
+        if (r <= 0 && r >= kHeldBelow) atomicMin(&left.left[was[c]], -2 - (place[c] & kPlace));
+      }
+    __syncthreads();
+    for (int c = tid; c < n; c += kSettle)
+      if (place[c] & kShared && left.get(was[c]) == -2 - (place[c] & kPlace)) place[c] |= kStays;
+    __syncthreads();
+    for (int c = tid; c < n; c += kSettle)
+      if (place[c] & kStays) left.set(was[c], 1);
   }
-  unsigned all;
+  auto leaves = [&](int c) { return (place[c] & (kShared | kStays)) == kShared; };
+  unsigned wanted = 0, all;
+  for (int c = tid; c < n; c += kSettle) wanted += leaves(c) || was[c] == -1;
   block_scan<kSettle>(wanted, in_wave, all);  // its barriers stand behind the stores
   wanted = all;
-  // ---- free pages, the lowest first: a run of pages of each wavefront ----
-  const int run = (a.n_pages / (kSettle / 64) + 64) & -64, p0 = min(wave * run, a.n_pages), p1 = min(p0 + run, a.n_pages);
-  unsigned free = 0;
-  for (int p = p0; p < p1; p += 64) free += __popcll(__ballot(p + lane < p1 && count_of(a, min(p + lane, p1 - 1)) == 0));
-  unsigned nth = block_scan<kSettle>(lane == 0 ? free : 0, in_wave, all);
-  nth = (unsigned)__builtin_amdgcn_readfirstlane((int)nth) - free;
-  const bool ok = wanted <= all && total <= (unsigned)a.most;
-  if (ok) {
-    for (int p = p0; p < p1 && nth < wanted; p += 64) {
-      const bool here = p + lane < p1 && count_of(a, min(p + lane, p1 - 1)) == 0;
-      const unsigned long long who = __ballot(here);
-      const unsigned mine = nth + __popcll(who & ((1ull << lane) - 1));
-      if (here && mine < wanted) a.fresh[mine] = p + lane;
-      nth += __popcll(who);
+  // ---- free pages, the lowest first. In LDS a thread has the bits of up to 31 that follow each other, an odd number, so that its reads and those of the
+  // other threads meet in different banks; else a wavefront has a run of 64s, a lane the bits of one of these ----
+  constexpr int kAhead = Counts::kNear ? 8 : 16;
+  const int lane = tid & 63, wave = tid >> 6;
+  unsigned found = 0;
+  for (int p0 = 0, each; p0 < a.n_pages && found < wanted; p0 += each * kSettle) {
+    unsigned long long bits = 0;
+    int first;
+    if constexpr (Counts::kNear) {
+      each = min((a.n_pages - p0 + kSettle - 1) / kSettle | 1, 31);
+      first = p0 + tid * each;
+      for (int i0 = 0; i0 < each; i0 += kAhead) {
+        int counts[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) counts[i] = left.get(min(first + i0 + i, a.n_pages - 1));
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) bits |= (counts[i] == 0 && i0 + i < each && first + i0 + i < a.n_pages ? 1u : 0u) << ((i0 + i) & 31);
+      }
+    } else {
+      each = min((a.n_pages - p0 + kSettle - 1) / kSettle, 64);
+      first = p0 + wave * each * 64;
+      for (int i0 = 0; i0 < each; i0 += kAhead) {
+        int counts[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) counts[i] = left.get(min(first + 64 * (i0 + i) + lane, a.n_pages - 1));
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const unsigned long long b = __ballot(i0 + i < each && first + 64 * (i0 + i) + lane < a.n_pages && counts[i] == 0);
+          if (lane == i0 + i) bits = b;
+        }
+      }
+      first += 64 * lane;
     }
+    const unsigned mine = __popcll(bits), upto = block_scan<kSettle>(mine, in_wave, all);
+    for (unsigned at = found + upto - mine; bits && at < wanted; bits &= bits - 1) fresh[at++] = first + __builtin_ctzll(bits);
+    found += all;
   }
+  const bool ok = wanted <= found && total <= (unsigned)a.most;
   __syncthreads();
   // ---- and who gets them ----
   unsigned given = 0, copied = 0;
   for (int c0 = 0; ok && c0 < n; c0 += kSettle) {
     const int c = c0 + tid;
-    const bool leave = c < n && leaves(c), want = leave || (c < n && a.was[c] == -1);
-    const int place = c < n ? a.place[c] & kPlace : 0, b = place / a.width;
-    const bool copy = leave && place - b * a.width < a.seq[b].kept;
-    const unsigned x = (unsigned)want | (unsigned)copy << 16, upto = block_scan<kSettle>(x, in_wave, all);
+    const bool leave = c < n && leaves(c), want = leave || (c < n && was[c] == -1);
+    const int at = c < n ? place[c] & kPlace : 0, b = at / a.width;
+    const bool copy = leave && at - b * a.width < seq(b).kept;
+    unsigned upto = 0;
+    if (wanted) upto = block_scan<kSettle>((unsigned)want | (unsigned)copy << 16, in_wave, all);
     if (want) {
-      const int page = a.fresh[given + (upto & 0xffff) - 1];
-      a.next[place] = page;
-      __hip_atomic_store(&a.left[page], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int page = fresh[given + (upto & 0xffff) - 1];
+      left.set(page, 1);
       if (copy) {
         int* to = a.moves + 2 * (size_t)(copied + (upto >> 16) - 1);
-        to[0] = a.was[c];
+        to[0] = was[c];
         to[1] = page;
       }
+      if (leave) leave_page(was[c]);
+      place[c] = at | kGiven;
+      was[c] = page;
     }
-    given += all & 0xffff;
-    copied += all >> 16;
+    if (wanted) {
+      given += all & 0xffff;
+      copied += all >> 16;
+    }
   }
   for (unsigned i = copied + tid; i < (unsigned)a.n_seqs; i += kSettle) a.moves[2 * (size_t)i] = a.moves[2 * (size_t)i + 1] = -1;
   if (tid == 0) {
     a.counts[0] = (int)copied;
-    a.counts[1] = ok ? 0 : max((int)(wanted - min(wanted, all)), 1);
+    a.counts[1] = ok ? 0 : max((int)(wanted - min(wanted, found)), 1);
   }
+  return ok ? n : -1;
+}
+
+// ---- one launch ----
+constexpr int kNearPages = 32 * 1024, kNearSeqs = 512, kNearWritten = 1536, kNearPlaces = 32 * 1024;
+
+// A step that shares nothing and gives nothing back, as most are: rows' places that name no page get free ones, and that is all. Returns
+// false where there is more to do, with nothing changed. A thread has a sequence; a wavefront a run of pages, 64 of each lane, whose counts are under
+// way while the sequences' lengths are. Behind a sequence's tokens its pages follow each other: where the first place behind those that it needs names
+// -1, nothing is given back.
+__device__ __forceinline__ bool fork_nothing(const Fork& a, int* fresh) {
+  __shared__ unsigned in_wave[kSettle / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Seq s = {};
+  int had = 0;
+  if (tid < a.n_seqs) {
+    s = seq_of(a, tid);
+    had = min((min(max(a.len[tid], 0), kMost) + (1 << a.shift) - 1) >> a.shift, a.width);
+  }
+  constexpr int kAhead = 16;
+  const int run = (a.n_pages + 64 * (kSettle / 64) - 1) / (64 * (kSettle / 64)), first = wave * run * 64;  // at most 64 of 64
+  unsigned long long bits = 0;
+  for (int i0 = 0; i0 < run; i0 += kAhead) {
+    int refs[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) refs[i] = load_global<int>(a.refs + min(first + 64 * (i0 + i) + lane, a.n_pages - 1));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const unsigned long long b = __ballot(refs[i] == 0);
+      if (lane == i0 + i && i0 + i < run) bits = b;
+    }
+  }
+  const int left = a.n_pages - first - 64 * lane;  // the last page's count stands for those behind it
+  bits &= left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+  const int* row = a.table + (size_t)tid * a.width;
+  bool more = false;
+  unsigned wants = 0;
+  if (tid < a.n_seqs) {
+    more = s.need < a.width && (s.need < had || row[s.need] != -1);
+    for (int at = s.first; at < s.need; ++at) {
+      const int page = row[at];
+      if (named(a, page))
+        more |= a.refs[page] != 1;
+      else
+        wants += at >= s.kept;  // a sequence's last tokens that are not there stay so, and the place with them
+    }
+  }
+  if (__syncthreads_or(more)) return false;
+  unsigned wanted, found;
+  const unsigned mine = __popcll(bits);
+  unsigned nth = block_scan<kSettle>(wants, in_wave, wanted) - wants, at = block_scan<kSettle>(mine, in_wave, found) - mine;
+  const bool ok = wanted <= found && wanted <= (unsigned)a.most;
+  if (ok)
+    for (; bits && at < wanted; bits &= bits - 1) fresh[at++] = first + 64 * lane + __builtin_ctzll(bits);
+  __syncthreads();
+  if (ok && tid < a.n_seqs) {
+    for (int at = s.first; wants && at < s.need; ++at) {
+      if (at < s.kept || named(a, row[at])) continue;
+      const int page = fresh[nth++];
+      a.table[(size_t)tid * a.width + at] = page;
+      a.refs[page] = 1;
+    }
+    a.len[tid] = s.len;
+  }
+  for (int i = tid; i < 2 * a.n_seqs; i += kSettle) a.moves[i] = -1;
+  if (tid == 0) {
+    a.counts[0] = 0;
+    a.counts[1] = ok ? 0 : max((int)(wanted - min(wanted, found)), 1);
+  }
+  return true;
+}
+
+// kForked: sequences have parents; else each goes on from itself, and only places behind those that it needs change here.
+template <bool kForked>
+__global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
+  extern __shared__ int lds[];
+  int *left = lds, *place = left + a.n_pages, *was = place + a.most, *fresh = was + a.most;
+  Seq* seqs = (Seq*)(fresh + a.most);
+  if (!kForked && fork_nothing(a, fresh)) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int kAhead = 8;
+  for (int p0 = tid; p0 < a.n_pages; p0 += kAhead * kSettle) {
+    int refs[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) refs[i] = a.refs[min(p0 + i * kSettle, a.n_pages - 1)];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (p0 + i * kSettle < a.n_pages) left[p0 + i * kSettle] = count_at_first(refs[i]);
+  }
+  if (tid < a.n_seqs) seqs[tid] = seq_of(a, tid);
+  __syncthreads();
+  // Wavefronts have kSide sequences at a time, and kFar times 64 of their places: put(b, at, old, page) of those that may change
+  constexpr int kSide = kForked ? 2 : 4, kFar = 4;
+  auto places = [&](auto put) {
+    for (int b0 = wave * kSide; b0 < a.n_seqs; b0 += kSide * (kSettle / 64)) {
+      Seq s[kSide];
+      int least = a.width;
+#pragma unroll
+      for (int x = 0; x < kSide; ++x) {
+        s[x] = seqs[min(b0 + x, a.n_seqs - 1)];
+        const bool here = b0 + x < a.n_seqs;
+        s[x].need = __builtin_amdgcn_readfirstlane(here ? s[x].need : a.width);
+        s[x].kept = __builtin_amdgcn_readfirstlane(s[x].kept);
+        s[x].parent = __builtin_amdgcn_readfirstlane(here ? s[x].parent : b0 + x);
+        least = min(least, s[x].parent == b0 + x ? s[x].need : 0);
+      }
+      for (int at0 = least & -64; at0 < a.width; at0 += 64 * kFar) {
+        int old[kSide][kFar], page[kSide][kFar];
+#pragma unroll
+        for (int x = 0; x < kSide; ++x)
+#pragma unroll
+          for (int i = 0; i < kFar; ++i) {
+            const int at = at0 + 64 * i + lane, b = b0 + x;
+            const bool mine = at < a.width && (s[x].parent != b || at >= s[x].need);
+            old[x][i] = a.table[mine ? b * a.width + at : 0];
+            if (kForked) page[x][i] = a.table[mine && s[x].parent != b && at < s[x].kept ? s[x].parent * a.width + at : 0];
+          }
+#pragma unroll
+        for (int x = 0; x < kSide; ++x)
+#pragma unroll
+          for (int i = 0; i < kFar; ++i) {
+            const int at = at0 + 64 * i + lane, b = b0 + x;
+            if (at < a.width && (s[x].parent != b || at >= s[x].need))
+              put(b, at, old[x][i], kForked && s[x].parent != b && at < s[x].kept ? page[x][i] : -1);
+          }
+      }
+    }
+  };
+  bool changes = false;
+  places([&](int b, int at, int old, int page) {
+    if (kForked) a.next[b * a.width + at] = page;
+    if (old == page) return;
+    changes = true;
+    if (named(a, old)) atomicSub(&left[old], 1);
+    if (named(a, page)) atomicAdd(&left[page], 1);
+  });
+  changes = __syncthreads_or(changes);
+  auto count = [&](int p) {
+    if (named(a, p) && left[p] >= kHeldBelow) a.refs[p] = max(left[p], 0);
+  };
+  const int n = settle(
+      a, NearCounts{left}, [&](int b) { return seqs[b]; },
+      [&](const Seq& s, int b, int at) { return inherited(a, s, b, at, s.parent == b ? a.table[b * a.width + at] : -1); }, place, was, fresh, count);
+  if (n < 0) return;
+  __syncthreads();  // the counts
+  if (changes && kForked) {
+    for (int p = tid; p < a.n_pages; p += kSettle) count(p);
+    for (int b = wave; b < a.n_seqs; b += kSettle / 64) {
+      const int parent = __builtin_amdgcn_readfirstlane(seqs[b].parent), need = __builtin_amdgcn_readfirstlane(seqs[b].need);
+      for (int at0 = parent == b ? need & -64 : 0; at0 < a.width; at0 += 64 * kAhead) {
+        int page[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) page[i] = a.next[min(b * a.width + at0 + 64 * i + lane, a.n_seqs * a.width - 1)];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const int at = at0 + 64 * i + lane;
+          if (at < a.width && (parent != b || at >= need)) a.table[b * a.width + at] = page[i];
+        }
+      }
+    }
+  } else if (changes) {
+    places([&](int b, int at, int old, int) {
+      if (old == -1) return;
+      a.table[b * a.width + at] = -1;
+      count(old);
+    });
+  }
+  if (tid < a.n_seqs) a.len[tid] = seqs[tid].len;
+  __syncthreads();
+  for (int c = tid; c < n; c += kSettle) {
+    if (place[c] & kGiven) a.table[place[c] & kPlace] = was[c];
+    count(was[c]);
+  }
+}
+
+// ---- four launches ----
+__global__ __launch_bounds__(256) void fork_begin_kernel(Fork a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < a.n_pages) a.left[i] = count_at_first(a.refs[i]);
+  if (i < a.n_seqs) a.seq[i] = seq_of(a, i);
+}
+
+// A thread has the same place of kSide sequences that follow each other: children of one parent name one page there, and one atomic sum counts them
+// (32 prompts of up to 32000 tokens with eight children each: 13.6 us one by one).
+constexpr int kSide = 8;
+__global__ __launch_bounds__(256) void fork_places_kernel(Fork a, int chunks) {
+  const int b0 = blockIdx.x / chunks * kSide, at = (blockIdx.x % chunks) * 256 + threadIdx.x;
+  if (at >= a.width) return;
+  int old[kSide], page[kSide];
+#pragma unroll
+  for (int i = 0; i < kSide; ++i) {
+    const int b = b0 + i;
+    old[i] = page[i] = -1;
+    if (b >= a.n_seqs) continue;
+    old[i] = a.table[(size_t)b * a.width + at];
+    page[i] = inherited(a, a.seq[b], b, at, old[i]);
+    a.next[(size_t)b * a.width + at] = page[i];
+  }
+  int many = 0;
+#pragma unroll
+  for (int i = 0; i < kSide; ++i) {
+    if (old[i] != page[i]) {
+      if (named(a, old[i])) atomicSub(&a.left[old[i]], 1);
+      many += named(a, page[i]);
+    }
+    // the last of a run of equal pages
+    if (many && (i + 1 == kSide || page[i + 1] != page[i])) {
+      atomicAdd(&a.left[page[i]], many);
+      many = 0;
+    }
+  }
+}
+
+// kLists: the lists of places that rows write lie in LDS.
+template <bool kLists>
+__global__ __launch_bounds__(kSettle) void fork_settle_kernel(Fork a) {
+  __shared__ int lists[kLists ? 3 * kNearWritten : 1];
+  int *place = kLists ? lists : a.place, *was = kLists ? lists + kNearWritten : a.was, *fresh = kLists ? lists + 2 * kNearWritten : a.fresh;
+  const int n = settle(
+      a, FarCounts{a.left}, [&](int b) { return a.seq[b]; }, [&](const Seq&, int b, int at) { return a.next[(size_t)b * a.width + at]; }, place, was, fresh,
+      [](int) {});
+  __syncthreads();
+  for (int c = threadIdx.x; c < n; c += kSettle)
+    if (place[c] & kGiven) a.next[place[c] & kPlace] = was[c];
 }
 
 __global__ __launch_bounds__(256) void fork_end_kernel(Fork a) {
@@ -404,12 +647,20 @@ int w4a32_op_paged_fork(const w4a32_paged_cache* cache, const w4a32_paged_fork_a
                (int*)(s + r.left), (int*)(s + r.next), (int*)(s + r.place), (int*)(s + r.was), (int*)(s + r.fresh)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned places = (unsigned)cache->n_seqs * cache->table_ld, pages = (unsigned)cache->n_pages;
+  if (cache->n_pages <= kNearPages && cache->n_seqs <= kNearSeqs && a.most <= kNearWritten && places <= kNearPlaces) {
+    static w4::LdsLimitOnce limit[2];
+    auto kernel = a.parent ? fork_kernel<true> : fork_kernel<false>;
+    if (limit[a.parent != nullptr].raise((const void*)kernel, 4 * (kNearPages + 3 * kNearWritten) + kNearSeqs * sizeof(Seq)) != hipSuccess) return W4A32_ELAUNCH;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(kSettle), 4 * (size_t)(cache->n_pages + 3 * a.most) + cache->n_seqs * sizeof(Seq), st, a);
+    return from_hip(hipGetLastError());
+  }
   const unsigned seqs = (unsigned)cache->n_seqs, begin = pages > seqs ? pages : seqs, end = places > pages ? places : pages;
   hipLaunchKernelGGL(fork_begin_kernel, dim3((begin + 255) / 256), dim3(256), 0, st, a);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
-  hipLaunchKernelGGL(fork_places_kernel, dim3((places + 255) / 256), dim3(256), 0, st, a);
+  const unsigned chunks = ((unsigned)cache->table_ld + 255) / 256;
+  hipLaunchKernelGGL(fork_places_kernel, dim3((seqs + kSide - 1) / kSide * chunks), dim3(256), 0, st, a, (int)chunks);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
-  hipLaunchKernelGGL(fork_settle_kernel, dim3(1), dim3(kSettle), 0, st, a);
+  hipLaunchKernelGGL((a.most <= kNearWritten ? fork_settle_kernel<true> : fork_settle_kernel<false>), dim3(1), dim3(kSettle), 0, st, a);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   hipLaunchKernelGGL(fork_end_kernel, dim3((end + 255) / 256), dim3(256), 0, st, a);
   return from_hip(hipGetLastError());

@@ -95,7 +95,7 @@ def test_too_few_pages_change_nothing(pkg):
 
 def test_places_that_are_not_there(pkg):
     """Holes, numbers outside the pool, lengths past the table and below zero"""
-    table = np.array([[-1, 1, 9, -1], [3, 1 << 30, -7, 2], [4, 5, 6, 7], [-1, -1, -1, -1]])
+    table = np.array([[-1, 1, 9, -1], [3, 1 << 30, 2, -7], [4, 5, 6, 7], [-1, -1, -1, -1]])
     for lens in ([40, 40, 70, 0], [1, 30, -4, 3], [33, 1 << 30, 64, 5]):
         for rows in ([1, 1, 1, 1], [20, 0, 5, 70], None):
             check_fork(pkg, table, lens, model.count(table, 14), 16, rows=rows)
