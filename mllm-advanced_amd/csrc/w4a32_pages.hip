@@ -481,91 +481,138 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(Copy a) {
 
 // ---------------------------------------------------------------------------------------------
 // Compaction. Which pages are used and which may move are bits, 64 of a word, and a page's place among the movers or the holes
-// is the words' running sum and the bits below it. The i-th mover goes to the i-th hole.
+// is the words' running sum and the bits below it. The i-th mover goes to the i-th hole: the last word whose sum does not pass i has it. One
+// workgroup adds the words up; pages and places are then gone through by all. (Lists of movers and holes written by that one workgroup, a
+// store of every bit, took 23 us for 65536 pages.)
 // ---------------------------------------------------------------------------------------------
 typedef unsigned long long Bits64;
-struct Head {
-  int used, pairs;
-};
 struct Compact {
   int *table, *refs;
   int n_seqs, width, n_pages, words;
   int *moves, *counts;
-  Head* head;
-  Bits64 *used, *mover;  // [words]; the latter of all pages that may move, then of those behind the last that stays
-  int* before;           // [words]: movers in front of a word
+  Bits64 *hole, *mover;             // [words]; at first the pages in use, and those that may move
+  int *holes_before, *movers_before;  // [words]
 };
 
-__global__ __launch_bounds__(256) void compact_bits_kernel(Compact a) {
-  const int p = blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void compact_bits(const Compact& a, int p) {
   const int r = p < a.n_pages ? a.refs[p] : 0;
   const Bits64 used = __ballot(r != 0), mover = __ballot(r > 0);
   if ((threadIdx.x & 63) == 0 && p < a.n_pages) {
-    a.used[p >> 6] = used;
+    a.hole[p >> 6] = used;
     a.mover[p >> 6] = mover;
   }
 }
 
-__global__ __launch_bounds__(kSettle) void compact_lists_kernel(Compact a) {
+// By one workgroup; returns how many pages move
+__device__ __forceinline__ int compact_sums(const Compact& a) {
   __shared__ unsigned in_wave[kSettle / 64];
   __shared__ int last;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, each = (a.words + kSettle - 1) / kSettle, w0 = min(tid * each, a.words), w1 = min(w0 + each, a.words);
   if (tid == 0) last = 0;
   unsigned mine = 0, all;
-  for (int w = tid; w < a.words; w += kSettle) mine += __popcll(a.used[w]);
+  for (int w = w0; w < w1; ++w) mine += __popcll(a.hole[w]);
   block_scan<kSettle>(mine, in_wave, all);
   const int used = (int)all;
   auto below = [&](int w) { return used >= 64 * (w + 1) ? ~0ull : used <= 64 * w ? 0ull : (1ull << (used - 64 * w)) - 1; };
-  auto movers_of = [&](int w) { return a.mover[w] & ~below(w); };
-  mine = 0;
-  for (int w = tid; w < a.words; w += kSettle) {
-    mine += __popcll(movers_of(w));
-    const Bits64 held = a.used[w] & ~a.mover[w] & ~below(w);
-    if (held) atomicMax(&last, 64 * w + 64 - __builtin_clzll(held));
-  }
-  block_scan<kSettle>(mine, in_wave, all);
-  const unsigned pairs = all;  // as many holes as movers or more
   unsigned movers = 0, holes = 0;
-  for (int w0 = 0; w0 < a.words; w0 += kSettle) {
-    const int w = w0 + tid;
-    Bits64 from = w < a.words ? movers_of(w) : 0, to = w < a.words ? ~a.used[w] & below(w) : 0;
-    unsigned i = movers + block_scan<kSettle>(__popcll(from), in_wave, all) - __popcll(from);
-    movers += all;
-    if (w < a.words) {
-      a.before[w] = (int)i;
-      a.mover[w] = from;
-    }
-    for (; from; from &= from - 1) a.moves[2 * (size_t)i++] = 64 * w + __builtin_ctzll(from);
-    i = holes + block_scan<kSettle>(__popcll(to), in_wave, all) - __popcll(to);
-    holes += all;
-    for (; to && i < pairs; to &= to - 1) a.moves[2 * (size_t)i++ + 1] = 64 * w + __builtin_ctzll(to);
+  int held = 0;
+  for (int w = w0; w < w1; ++w) {
+    const Bits64 in_use = a.hole[w], may = a.mover[w], from = may & ~below(w), to = ~in_use & below(w), stays = in_use & ~may & ~below(w);
+    a.hole[w] = to;
+    a.mover[w] = from;
+    movers += __popcll(from);
+    holes += __popcll(to);
+    if (stays) held = 64 * w + 64 - __builtin_clzll(stays);
+  }
+  if (held) atomicMax(&last, held);
+  unsigned h = block_scan<kSettle>(holes, in_wave, all) - holes;
+  unsigned m = block_scan<kSettle>(movers, in_wave, all) - movers;
+  for (int w = w0; w < w1; ++w) {
+    a.holes_before[w] = (int)h;
+    a.movers_before[w] = (int)m;
+    h += __popcll(a.hole[w]);
+    m += __popcll(a.mover[w]);
   }
   if (tid == 0) {
-    a.head->used = used;
-    a.head->pairs = (int)pairs;
-    a.counts[0] = (int)pairs;
+    a.counts[0] = (int)all;  // as many holes as movers or more
     a.counts[1] = max(last, used);
   }
+  return (int)all;
 }
 
-__global__ __launch_bounds__(256) void compact_apply_kernel(Compact a) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  const int pairs = a.head->pairs;
+__device__ __forceinline__ int nth_hole(const Compact& a, int n) {
+  int lo = 0, hi = a.words;  // holes_before[lo] <= n < holes_before[hi]
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (a.holes_before[mid] <= n)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  const Bits64 both = a.hole[lo];
+  unsigned word = (unsigned)both;  // halves: a 64-bit shift by the last of a wavefront's registers is wrong now and then
+  int in = n - a.holes_before[lo], at = 64 * lo;
+  if (const int low = __popc(word); in >= low) {
+    in -= low;
+    at += 32;
+    word = (unsigned)(both >> 32);
+  }
+#pragma unroll
+  for (int half = 16; half; half /= 2) {
+    const int low = __popc(word & ((1u << half) - 1));
+    if (in >= low) {
+      in -= low;
+      at += half;
+      word >>= half;
+    }
+  }
+  return at;
+}
+// The number that a page gets; -1: it stays
+__device__ __forceinline__ int mover_number(const Compact& a, int page) {
+  const Bits64 word = a.mover[page >> 6], bit = 1ull << (page & 63);
+  return word & bit ? a.movers_before[page >> 6] + __popcll(word & (bit - 1)) : -1;
+}
+
+__device__ __forceinline__ void compact_apply(const Compact& a, int i, int pairs) {
   if (i < a.n_seqs * a.width) {
     const int page = a.table[i];
     if ((unsigned)page < (unsigned)a.n_pages) {
-      const Bits64 word = a.mover[page >> 6], bit = 1ull << (page & 63);
-      if (word & bit) a.table[i] = a.moves[2 * (size_t)(a.before[page >> 6] + __popcll(word & (bit - 1))) + 1];
+      const int n = mover_number(a, page);
+      if (n >= 0) a.table[i] = nth_hole(a, n);
     }
   }
-  if (i >= a.n_pages / 2) return;
-  int* move = a.moves + 2 * (size_t)i;
-  if (i < pairs) {
-    a.refs[move[1]] = a.refs[move[0]];
-    a.refs[move[0]] = 0;
-  } else {
-    move[0] = move[1] = -1;
+  if (i < a.n_pages) {
+    const int n = mover_number(a, i);
+    if (n >= 0) {
+      const int to = nth_hole(a, n);
+      a.moves[2 * (size_t)n] = i;
+      a.moves[2 * (size_t)n + 1] = to;
+      a.refs[to] = a.refs[i];
+      a.refs[i] = 0;
+    }
   }
+  if (i < a.n_pages / 2 && i >= pairs) a.moves[2 * (size_t)i] = a.moves[2 * (size_t)i + 1] = -1;
+}
+
+__global__ __launch_bounds__(256) void compact_bits_kernel(Compact a) { compact_bits(a, blockIdx.x * 256 + threadIdx.x); }
+__global__ __launch_bounds__(kSettle) void compact_sums_kernel(Compact a) { compact_sums(a); }
+__global__ __launch_bounds__(256) void compact_apply_kernel(Compact a) { compact_apply(a, blockIdx.x * 256 + threadIdx.x, a.counts[0]); }
+
+// All of it by one workgroup, where pages and places are few
+constexpr int kNearMoves = 8192;
+__global__ __launch_bounds__(kSettle) void compact_kernel(Compact a) {
+  __shared__ Bits64 hole[kNearMoves / 64], mover[kNearMoves / 64];
+  __shared__ int holes_before[kNearMoves / 64], movers_before[kNearMoves / 64];
+  a.hole = hole;
+  a.mover = mover;
+  a.holes_before = holes_before;
+  a.movers_before = movers_before;
+  for (int p = threadIdx.x; p < 64 * a.words; p += kSettle) compact_bits(a, p);
+  __syncthreads();
+  const int pairs = compact_sums(a);
+  __syncthreads();
+  for (int i = threadIdx.x; i < max(a.n_seqs * a.width, a.n_pages); i += kSettle) compact_apply(a, i, pairs);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -604,16 +651,16 @@ ForkRoom fork_room(const w4a32_paged_cache* c, int rows) {
 }
 
 struct CompactRoom {
-  size_t used, mover, before, total;
+  size_t mover, holes, movers, total;
   int words;
 };
 CompactRoom compact_room(const w4a32_paged_cache* c) {
   CompactRoom r;
   r.words = (c->n_pages + 63) / 64;
-  r.used = 256;
-  r.mover = r.used + up256((size_t)r.words * 8);
-  r.before = r.mover + up256((size_t)r.words * 8);
-  r.total = r.before + up256((size_t)r.words * 4);
+  r.mover = up256((size_t)r.words * 8);
+  r.holes = r.mover + up256((size_t)r.words * 8);
+  r.movers = r.holes + up256((size_t)r.words * 4);
+  r.total = r.movers + up256((size_t)r.words * 4);
   return r;
 }
 }  // namespace
@@ -714,13 +761,17 @@ int w4a32_op_paged_compact(const w4a32_paged_cache* cache, int* d_refs, int* d_m
   const CompactRoom r = compact_room(cache);
   if (scratch_bytes < r.total) return W4A32_EINVAL;
   uint8_t* s = static_cast<uint8_t*>(d_scratch);
-  const Compact a{const_cast<int*>(cache->d_table), d_refs, cache->n_seqs, cache->table_ld, cache->n_pages, r.words, d_moves, d_counts, (Head*)s,
-                  (Bits64*)(s + r.used), (Bits64*)(s + r.mover), (int*)(s + r.before)};
+  const Compact a{const_cast<int*>(cache->d_table), d_refs, cache->n_seqs, cache->table_ld, cache->n_pages, r.words, d_moves, d_counts, (Bits64*)s,
+                  (Bits64*)(s + r.mover), (int*)(s + r.holes), (int*)(s + r.movers)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned places = (unsigned)cache->n_seqs * cache->table_ld, pages = (unsigned)cache->n_pages, most = places > pages ? places : pages;
+  if (most <= kNearMoves) {
+    hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kSettle), 0, st, a);
+    return from_hip(hipGetLastError());
+  }
   hipLaunchKernelGGL(compact_bits_kernel, dim3((pages + 255) / 256), dim3(256), 0, st, a);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
-  hipLaunchKernelGGL(compact_lists_kernel, dim3(1), dim3(kSettle), 0, st, a);
+  hipLaunchKernelGGL(compact_sums_kernel, dim3(1), dim3(kSettle), 0, st, a);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   hipLaunchKernelGGL(compact_apply_kernel, dim3((most + 255) / 256), dim3(256), 0, st, a);
   return from_hip(hipGetLastError());
