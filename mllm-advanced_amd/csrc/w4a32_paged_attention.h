@@ -35,7 +35,7 @@ struct OwnItem {
 };
 struct Prefix {
   const int *group_start, *tokens;  // as they are given
-  int n_groups, grid, blocks;  // most workgroups that have a share of a prefix, or a block of own rows
+  int n_groups, grid, blocks, own_grid;  // most workgroups that have a share of a prefix, a block of own rows; those that own tokens are dealt to
   OwnItem* item;        // [items of the sequences' own tokens]
   float *part, *state;  // [workgroups][rows of an item][dt], [..][2]: as those of a share
   // Where a launch in front deals the batch; else every wavefront does
@@ -393,9 +393,7 @@ struct OwnPlan {
   int wide, slot_rows, dt;
 };
 int plan_own(const w4a32_paged_cache* c, const w4a32_paged_rows* r, OwnPlan& o);
-// Workgroups that own tokens are dealt to. More than are there at once, so that most of them have a share of one item and no more (64 sequences
-// of 16 to 1200 tokens behind 8003: 47 us with 768, 51 with 512, 57 with 320, of which most have the end of one item and the start of the next).
-constexpr int kOwnGrid = 768;
+constexpr int kOwnGrid = 768;            // most workgroups that own tokens are dealt to
 constexpr int kOwnSlots = 2 * kOwnGrid;  // of shares: two of a workgroup
 
 }  // namespace paged

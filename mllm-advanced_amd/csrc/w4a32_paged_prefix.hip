@@ -19,6 +19,7 @@ inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kPlan = 1024;      // threads of the workgroup that deals
 constexpr int kSlots = 512;      // workgroups that are there at once: two per CU
+constexpr int kMostShares = kSlots * 7 / 8;  // of prefixes, where their items are not more
 constexpr int kLog2 = 7;         // log2 of the rows of a workgroup of a prefix
 // Pairs of row and head from which on a sequence's own tokens go by blocks of 128 rows as well, and not by 16 of a wavefront (eight prompts of 60 to
 // 300 rows, 28 heads on 4, bf16: behind 64 tokens 46 us against 68, behind 4099 141 against 148; 64, 256, 512: the same).
@@ -70,7 +71,7 @@ __device__ __forceinline__ unsigned own_tiles(const Attend& a, const Span& s, in
 template <bool kF32, typename Count>
 __device__ __forceinline__ unsigned share_of(const Attend& a, unsigned tiles, unsigned items, unsigned pairs, unsigned own, Count count) {
   const float work = (float)tiles * 3.0f, rest = (float)own * a.c.kv_heads * (8.0f / kWaves);
-  unsigned most = min(max((unsigned)(kSlots * (work / (work + rest + 1.0f)) + 0.5f), (unsigned)kSlots / 4), (unsigned)kSlots * 7 / 8);
+  unsigned most = min(max((unsigned)(kSlots * (work / (work + rest + 1.0f)) + 0.5f), (unsigned)kSlots / 4), (unsigned)kMostShares);
   if (2 * items > most) most *= 2;  // in two rounds, so that what one leaves over is small
   most = min(most, (unsigned)a.prefix.grid);
   if (most <= items) return 1u << 30;
@@ -284,10 +285,10 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void both_kernel(At
       g = of_lane(m.q, __popcll(__ballot(lane < x.n_groups && m.q.first <= unit)) - 1);
     }
     const unsigned kv = a.c.kv_heads, in = (unsigned)(unit - g.first), in_kv = in / kv, share = in_kv / g.blocks;
-    const int tiles = (int)tiles_of<Sh::kKeys>(g);
+    const unsigned tiles = tiles_of<Sh::kKeys>(g), each = tiles / g.shares, more = tiles - each * g.shares, first = each * share + min(share, more);
     const size_t row = (size_t)unit << kLog2;
-    const Piece piece{g.b, {g.r0, g.n, g.tokens - 1}, (int)(in - in_kv * kv), (int)(in_kv - share * g.blocks), (int)((long long)tiles * share / g.shares),
-                      (int)((long long)tiles * (share + 1) / g.shares), 0, x.part + row * DT, x.state + 2 * row};
+    const Piece piece{g.b, {g.r0, g.n, g.tokens - 1}, (int)(in - in_kv * kv), (int)(in_kv - share * g.blocks), (int)first,
+                      (int)(first + each + (share < more)), 0, x.part + row * DT, x.state + 2 * row};
     prompt_body<Act, KV, DT, kHalfForm, kPrefixTokens>(a, 0, piece);
     return;
   }
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void both_kernel(At
     }
     unit -= (int)blocks;
   }
-  if (unit < kOwnGrid) rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)unit, kOwnGrid, m.from, group_at);
+  if (unit < x.own_grid) rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)unit, (unsigned)x.own_grid, m.from, group_at);
 }
 
 // Where rows are few: a workgroup per row and kSlice of its values, its threads four values of every 256 / (kSlice / 4)th share each
@@ -408,7 +409,7 @@ struct Plan {
   bool dealt;       // by a launch in front
   int prompt_rows;  // pairs of a sequence from which on it goes by blocks of them, of which there are `blocks`; 0: none does
   unsigned blocks;
-  unsigned grid;  // workgroups of the prefixes
+  unsigned grid, own_grid;  // workgroups of the prefixes, and of own tokens
   size_t group_off, from_off, of_off, item_off, part_off, state_off, pre_part_off, pre_state_off, total;
 };
 
@@ -418,11 +419,17 @@ int plan_of(const w4a32_paged_cache* c, const w4a32_paged_rows* r, int n_groups,
   const int dt = p.own.dt;
   p.dealt = c->n_seqs > kLanes || n_groups > kLaneGroups;
   const long long items = (((long long)r->rows * group >> kLog2) + n_groups) * c->kv_heads;
-  const long long grid = items > 2 * kSlots ? items : 2 * kSlots;
+  // No more workgroups than can have something to do: each that has nothing finds that out by dealing the batch
+  const long long grid = 2 * items <= kMostShares ? kMostShares : items > 2 * kMostShares ? items : 2 * kMostShares;
+  // Own tokens: more than are there at once where items are many, so that most of them have a share of one item and no more (64 sequences of 16 to
+  // 1200 tokens behind 8003, 4 kv heads: 47 us with 768, 51 with 512, 57 with 320, of which most have the end of one item and the start of the
+  // next), else one per CU (11 sequences: 29 us with 512, 32 with 768)
+  const long long own = 3 * p.own.items;
+  p.own_grid = (unsigned)(own < kSlots / 2 ? kSlots / 2 : own > kOwnGrid ? kOwnGrid : own);
   const long long most = r->max_rows < r->rows ? r->max_rows : r->rows;
   p.prompt_rows = most * group >= kOwnPromptRows ? kOwnPromptRows : 0;
   const long long blocks = p.prompt_rows ? (((long long)r->rows * group >> kLog2) + c->n_seqs) * c->kv_heads : 0;
-  if (grid + blocks + kOwnGrid > most_groups(64 * kWaves)) return W4A32_ESHAPE;
+  if (grid + blocks + p.own_grid > most_groups(64 * kWaves)) return W4A32_ESHAPE;
   p.blocks = (unsigned)blocks;
   p.grid = (unsigned)grid;
   size_t at = 256;
@@ -475,7 +482,7 @@ hipError_t launch_both(const Attend& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((deal_kernel<Shape<Act, KV, DT, kHalfForm>::kKeys, tile_keys<KV>(), sizeof(KV) == 4>), dim3(1), dim3(kPlan), 0, s, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(p.grid + p.blocks + kOwnGrid), dim3(64 * kWaves), lds, s, a);
+  hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(p.grid + p.blocks + p.own_grid), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
 template <typename Act, typename KV>
@@ -516,7 +523,7 @@ int w4a32_op_paged_prefix_attention(const w4a32_paged_cache* cache, const w4a32_
   if (scratch_bytes < p.total) return W4A32_EINVAL;
   uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
   auto at = [&](size_t off) { return p.dealt ? (int*)(scratch + off) : nullptr; };
-  const Prefix x{d_group_start, d_prefix, n_groups, (int)p.grid, (int)p.blocks, (OwnItem*)(scratch + p.item_off), (float*)(scratch + p.pre_part_off),
+  const Prefix x{d_group_start, d_prefix, n_groups, (int)p.grid, (int)p.blocks, (int)p.own_grid, (OwnItem*)(scratch + p.item_off), (float*)(scratch + p.pre_part_off),
                  (float*)(scratch + p.pre_state_off), at(128), (PrefixGroup*)at(p.group_off), at(p.from_off), at(p.of_off)};
   Attend a{view(cache), rows->d_q, rows->d_out, rows->d_row_start, rows->ldq, rows->ldo, rows->rows,
            rows->max_rows < rows->rows ? rows->max_rows : rows->rows, rows->heads, rows->heads / cache->kv_heads, 0, 0, 0, rows->rows, 0, 0, p.prompt_rows, kLog2,

@@ -121,9 +121,14 @@ __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsig
       shares = (int)((p.q.nt + deal.per - 1) / deal.per);
       item = (int)(p.inner / (unsigned)shares);
       const int mine = (int)p.inner - item * shares;
-      typedef typename std::conditional<kWhich == kOwn, u64, unsigned>::type U;  // else at most kFew kGrid tiles
-      t_lo = (int)((U)((U)p.q.nt * mine) / (unsigned)shares);
-      t_hi = (int)((U)((U)p.q.nt * (mine + 1)) / (unsigned)shares);
+      if constexpr (kWhich == kOwn) {
+        const int each = (int)((unsigned)p.q.nt / (unsigned)shares), more = p.q.nt - each * shares;
+        t_lo = each * mine + min(mine, more);
+        t_hi = t_lo + each + (mine < more);
+      } else {
+        t_lo = (int)((unsigned)(p.q.nt * mine) / (unsigned)shares);  // at most kFew kGrid tiles
+        t_hi = (int)((unsigned)(p.q.nt * (mine + 1)) / (unsigned)shares);
+      }
       w_first = (int)block - mine;
     } else {
       item = (int)(p.inner / p.q.nt);
