@@ -1153,6 +1153,7 @@ def op_token_logprobs(logits, tokens=None, top=0, temperature=1.0, scratch=None)
     if _torch is None:
         _setup()
     device, kind, f32 = _device(), _kinds.get(logits.dtype), _torch.float32
+    _sizes(top)
     if kind is None:
         raise W4A32Error(f"logits are f32, f16 or bf16, not {logits.dtype}")
     ldl = _row_ld(logits, "logits", logits.dtype, device)

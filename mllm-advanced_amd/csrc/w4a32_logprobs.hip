@@ -9,7 +9,6 @@
 // The k most probable tokens: of the blocks' maxima the k-th largest bounds them from below, so only blocks whose maximum reaches it
 // are read again, about k of them, and of their logits about k reach it; those are put in order by counting. Where many are alike and do
 // not fit into LDS, the k-th largest itself is found by its bits, and of equal ones the first are taken.
-#include <cfloat>
 #include <type_traits>
 
 #include "w4a32_decoder.h"
@@ -43,6 +42,7 @@ struct Logprobs {
   int rows, vocab, ldl, top, blocks;
   double inv_t;
   float scale, scale_low;  // log2(e) / T
+  float far;               // a difference of logits that leaves nothing, and whose products with these are finite
   Part* part;  // [rows][blocks]
 };
 
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256) void blocks_kernel(Logprobs a, int groups, boo
   for (int c = 0; c < kN; ++c)
 #pragma unroll
     for (int i = 0; i < kWide; ++i) {
-      const float d = fminf(from - x.v[c][i], FLT_MAX), e = __builtin_amdgcn_exp2f(-__fmaf_rn(d, a.scale_low, d * a.scale));
+      const float d = fminf(from - x.v[c][i], a.far), e = __builtin_amdgcn_exp2f(-__fmaf_rn(d, a.scale_low, d * a.scale));
       sum += e;
       weighted += e > 0.0f ? e * d : 0.0f;
     }
@@ -493,7 +493,7 @@ int w4a32_op_token_logprobs(const w4a32_logprobs_args* v, void* d_scratch, size_
   if (scratch_bytes < total) return W4A32_EINVAL;
   const double inv_t = 1.0 / v->temperature, scale = inv_t * 1.4426950408889634074;
   const Logprobs a{v->d_logits, v->d_tokens, v->d_logprob, v->d_rank, v->d_entropy, v->d_top_token, v->d_top_logprob, v->rows, v->vocab,
-                   v->ldl, v->top, blocks, inv_t, (float)scale, (float)(scale - (double)(float)scale), static_cast<Part*>(d_scratch)};
+                   v->ldl, v->top, blocks, inv_t, (float)scale, (float)(scale - (double)(float)scale), (float)(300.0 / scale), static_cast<Part*>(d_scratch)};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (v->dtype == W4A32_CACHE_F32) return launch<float>(a, s);
   if (v->dtype == W4A32_CACHE_F16) return launch<_Float16>(a, s);

@@ -164,6 +164,23 @@ def test_temperatures(pkg, T):
     assert np.array_equal(got[1].cpu().numpy(), want[1]) and np.array_equal(got[3].cpu().numpy(), want[3])
 
 
+@pytest.mark.parametrize("T", [1e-30, 1e-8, 1e30])
+def test_masked_logits_at_any_temperature(pkg, T):
+    """Differences that pass f32 once they are divided leave nothing, and no NaN"""
+    x = logits_of(5, 1500, "f32")
+    x[:, 100:900] = float("-inf")
+    x[1, 50] = -3e38
+    x[2, 7] = 3e38
+    tokens = torch.tensor([3, 50, 7, 500, 1499], device="cuda")
+    got = [g.double().cpu().numpy() for g in pkg.op_token_logprobs(x, tokens, top=4, temperature=T)]
+    want = definition(x.double().cpu().numpy(), tokens.cpu().numpy(), 4, T)
+    assert np.array_equal(got[1], want[1]) and np.array_equal(got[3], want[3])
+    for g, w in ((got[0], want[0]), (got[2], want[2]), (got[4], want[4])):
+        w = np.where(np.abs(w) > np.finfo(np.float32).max, np.sign(w) * np.inf, w)   # as f32 holds it
+        ok = np.isfinite(w)
+        assert np.array_equal(g[~ok], w[~ok]) and np.all(np.abs(g[ok] - w[ok]) <= 2.0 ** -19 + 2.0 ** -22 * np.abs(w[ok])), (T, g, w)
+
+
 def test_large_logits(pkg):
     x = logits_of(3, 2000, "f32", std=1.0)
     check(pkg, x + 5e4, some_tokens(3, 2000), 3, 1.0)

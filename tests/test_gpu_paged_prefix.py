@@ -265,3 +265,37 @@ def test_captured(pkg):
             stream.synchronize()
             assert torch.equal(got, scratch_too)
             assert (got.double() - alone.double()).abs().max() <= 2.0 ** -7 * 5
+
+
+def test_two_streams(pkg):
+    """Two batches at once, each with scratch memory of its own"""
+    both = []
+    for i in range(2):
+        B = Groups(16 + i, [5, 9], [300, 170], [7 * j for j in range(14)], [1 + (i + j) % 2 for j in range(14)], 2, 128, 16)
+        fill_new(B)
+        _, qt = held(B.rng.standard_normal((B.total, 12 * 128)), "bf16")
+        cache, *_ = on_gpu(pkg, B, "bf16")
+        args = (cache, qt, dev(B.row_start), 2, 12, 0.09, dev(B.group_start), dev(np.array(B.prefix, np.int32)))
+        both.append((args, pkg.op_paged_prefix_attention(*args), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for rep in range(5):
+        out = []
+        for args, _, stream in both:
+            with torch.cuda.stream(stream):
+                out.append(pkg.op_paged_prefix_attention(*args))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, (_, b, _) in zip(out, both))
+
+
+@pytest.mark.parametrize("act,kind", TYPES)
+def test_groups_that_overlap_stay_inside_the_arrays(pkg, act, kind):
+    """Group starts that decrease or pass the batch: what the rows get is unspecified, what lies around them is left as it is"""
+    B = Groups(18, [4, 4], [64, 48], [3, 0, 9, 20, 1, 1, 30, 2], [1, 2, 0, 3, 1, 1, 2, 1], 2, 64, 16)
+    fill_new(B)
+    _, qt = held(B.rng.standard_normal((B.total + 3, 6 * 64)), act)
+    cache, *_ = on_gpu(pkg, B, kind)
+    for starts in ([0, 6, 2], [5, 1, 8], [-7, 4, 1 << 30], [8, 0, 8], [0, 0, 0]):
+        out = torch.full_like(qt, 7.5)
+        pkg.op_paged_prefix_attention(cache, qt, dev(B.row_start), 3, 6, 0.125, dev(np.array(starts, np.int32)), dev(np.array(B.prefix, np.int32)), out=out)
+        torch.cuda.synchronize()
+        assert bool((out[B.total:] == 7.5).all())

@@ -301,3 +301,30 @@ def test_on_another_stream_beside_another_call(pkg):
     for (table, lens, refs, cache, r, *_), (moves, counts) in zip(both, out):
         t, n, c, pairs, missing = model.fork(table, lens, refs, 16, rows=[3] * 20)
         assert counts.tolist() == [len(pairs), missing] and np.array_equal(cache.table.cpu().numpy(), t) and np.array_equal(r.cpu().numpy(), c)
+
+
+@pytest.mark.parametrize("n_pages", [200, 9000])
+def test_compaction_captured(pkg, n_pages):
+    """One graph, replayed on other tables with eager work between"""
+    rng = np.random.default_rng(n_pages)
+    cache = cache_of(pkg, np.full((4, n_pages // 4), -1), [0] * 4, 16, n_pages)
+    refs, scratch = dev(np.zeros(n_pages)), pkg.op_paged_compact_scratch(cache)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        pkg.op_paged_compact(cache, refs, scratch=scratch)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            moves, counts = pkg.op_paged_compact(cache, refs, scratch=scratch)
+        for i in range(4):
+            table = np.full((4, n_pages // 4), -1)
+            table.ravel()[:n_pages // 3] = rng.permutation(n_pages)[:n_pages // 3]
+            before = model.count(table, n_pages)
+            cache.table.copy_(dev(table))
+            refs.copy_(dev(before))
+            graph.replay()
+            stream.synchronize()
+            want, after, pairs, end = model.compact(table, before)
+            assert counts.tolist() == [len(pairs), end] and np.array_equal(cache.table.cpu().numpy(), want) and np.array_equal(refs.cpu().numpy(), after)
+            assert moves.tolist()[:len(pairs)] == [list(p) for p in pairs]
