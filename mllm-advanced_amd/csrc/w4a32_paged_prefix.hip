@@ -2,9 +2,17 @@
 //
 // A row's softmax is joined from its sums over the prefix and those over its sequence's own tokens, each relative to its maximum:
 //   m = max(m_P, m_own),  l = 2^(m_P - m) l_P + 2^(m_own - m) l_own,  o = 2^(m_P - m) o_P + 2^(m_own - m) o_own.
-// The prefix is the prompts' kernel's with the rows of all of the group's sequences, which all see all of it, and its keys dealt to as many
-// workgroups as the chip has; the own tokens are the rows' kernel's. Four launches: who has what (the lengths and the groups are
-// device memory), the prefixes, the own tokens, the join.
+// The prefix is the prompts' kernel's with the rows of all of the group's sequences, which all see all of it, 128 rows of a workgroup, and its keys dealt to
+// as many workgroups as the chip has room for; the own tokens are the rows' kernel's, and those of long prompts the prompts' kernel's again. All
+// of these are workgroups of one launch, so that none waits for another kind, and each works out by itself what it has (the lengths and the
+// groups are device memory; a launch in front does that for batches that a wavefront's lanes cannot hold); a second launch joins the sums, in a
+// fixed order.
+// What bounds it. 64 sequences behind 8003 tokens with 16 to 1200 of their own (28 heads on 4 of 128, bf16): 97 MB, 20 us of memory; 35 us and 5.4 of
+// join. A workgroup of the own tokens takes 16 us, of which its loop over tiles is 8 (the deal 2, the first loads 4, its sums 2), and there are
+// three rounds of them beside the prefix. 48 sequences of two to five rows in six groups behind 1000 to 6000 tokens, 12 heads on 2, f32 on f16: 30 and 6
+// us, as an f32 operand is two f16 terms and a tile's product waits for its loads more than it takes. Eight prompts of 60 to 300 rows behind 4099
+// tokens, 28 heads on 4, bf16: 97 GFLOP, 130 and 13 us, 865 TFLOP/s for each further token of the prefix: products and softmax of a wavefront
+// take turns more than they overlap.
 #include "w4a32_paged_prompt.h"
 #include "w4a32_paged_rows.h"
 
@@ -27,8 +35,10 @@ constexpr int kOwnPromptRows = 128;
 constexpr int kManyRows = 1024;  // rows from which on a workgroup joins several of them
 constexpr int kJoins = 1 << 20;  // workgroups of the joining launch, beyond which they take more
 
-constexpr int kLanes = 64;        // sequences up to which every wavefront deals the batch by itself, one in each lane, where there are
-constexpr int kLaneGroups = 16;   // few groups, which it goes through one by one
+// Sequences up to which every wavefront deals the batch by itself, one in each lane, where there are few groups, which it goes through one by one (64
+// sequences behind prefixes of 500 tokens, 28 heads on 4, bf16: one group 18 us against 24 with a launch in front, 4 groups 20 against 23, 8 the same, 16 31
+// against 26; 12 heads on 2, f32 on f16, two to five rows each: 21 against 29, 22 against 29, 23 against 30, 24 against 29).
+constexpr int kLanes = 64, kLaneGroups = 8;
 
 __device__ __forceinline__ unsigned wave_sum(unsigned x) { return last_lane(wave_scan(x)); }  // sums that do not fit are the most
 __device__ __forceinline__ int wave_min(int x) {

@@ -20,7 +20,9 @@ constexpr int kShared = 1 << 30, kStays = 1 << 29, kGiven = 1 << 28, kPlace = kM
 // counts are atomic sums of whole numbers. The places that rows write (one or two of a sequence that decodes) are then listed in
 // order and settled by one workgroup: who has to leave a shared page, which pages are free. Where there are enough it all becomes true;
 // else nothing has changed.
-// Where the counts fit into LDS: one launch of one workgroup, a chain of a few waits for memory. Else four launches, with the new table and the new counts in scratch memory.
+// What is moved is small (4 bytes of a place and of a page); latency bounds all of it, waits for memory and barriers of 16 wavefronts one after the
+// other. Where the counts fit into LDS: one launch of one workgroup. Else four launches, with the new table and the new counts in scratch memory (32
+// prompts of up to 32000 tokens with eight children each, 2.9 MB: 2.4 + 8.1 + 14.6 + 4.3 us, of which the third is the one workgroup that settles).
 // ---------------------------------------------------------------------------------------------
 struct Seq {
   int parent, len;  // -1: none; tokens
@@ -203,7 +205,11 @@ __device__ __forceinline__ int settle(const Fork& a, Counts left, SeqAt seq, Pag
 }
 
 // ---- one launch ----
-constexpr int kNearPages = 32 * 1024, kNearSeqs = 512, kNearWritten = 1536, kNearPlaces = 32 * 1024;
+// One workgroup and four launches, us of a pass among others with a table's copy of 2: rows for sequences that go on, 64 of up to 2000 tokens (8064
+// places) 13 and 21, 500 of 1000 (31500 places) 13 and 23; with parents, eight children each, 64 of 1000 (4032 places) 13 and 24, 512 of 250 (8192) 18 and
+// 30, 128 of 2000 (16128) 21 to 23 and 25, 500 of 1000 (31500) 35 and 28; with kept lengths, 64 of 1000 13 and 20, 128 of 2000 19 and 20, 256 of 2000
+// (32256) 27 and 21. The rest is what there is room for.
+constexpr int kNearPages = 32 * 1024, kNearSeqs = 512, kNearWritten = 1536, kNearPlaces = 32 * 1024, kNearChanged = 16 * 1024;
 
 // A step that shares nothing and gives nothing back, as most are: rows' places that name no page get free ones, and that is all. Returns
 // false where there is more to do, with nothing changed. A thread has a sequence; a wavefront a run of pages, 64 of each lane, whose counts are under
@@ -278,7 +284,7 @@ __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
   int *left = lds, *place = left + a.n_pages, *was = place + a.most, *fresh = was + a.most;
   Seq* seqs = (Seq*)(fresh + a.most);
   if (!kForked && fork_nothing(a, fresh)) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tid = threadIdx.x;
   constexpr int kAhead = 8;
   for (int p0 = tid; p0 < a.n_pages; p0 += kAhead * kSettle) {
     int refs[kAhead];
@@ -290,52 +296,34 @@ __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
   }
   if (tid < a.n_seqs) seqs[tid] = seq_of(a, tid);
   __syncthreads();
-  // Wavefronts have kSide sequences at a time, and kFar times 64 of their places: put(b, at, old, page) of those that may change
-  constexpr int kSide = kForked ? 2 : 4, kFar = 4;
-  auto places = [&](auto put) {
-    for (int b0 = wave * kSide; b0 < a.n_seqs; b0 += kSide * (kSettle / 64)) {
-      Seq s[kSide];
-      int least = a.width;
+  // A thread has every kSettle-th place, kFar of them at a time, and a bit for each that changes
+  constexpr int kFar = 4;
+  static_assert(kNearPlaces <= 32 * kSettle, "a thread's places are bits of a word");
+  const int places = a.n_seqs * a.width;
+  const unsigned per_width = 0xffffffffu / (unsigned)a.width + 1;  // quotients of less than 2^15 by no more than that are exact
+  unsigned changed = 0;
+  for (int i0 = tid, j0 = 0; i0 < places; i0 += kFar * kSettle, j0 += kFar) {
+    int old[kFar], page[kFar];
+    bool mine[kFar];
 #pragma unroll
-      for (int x = 0; x < kSide; ++x) {
-        s[x] = seqs[min(b0 + x, a.n_seqs - 1)];
-        const bool here = b0 + x < a.n_seqs;
-        s[x].need = __builtin_amdgcn_readfirstlane(here ? s[x].need : a.width);
-        s[x].kept = __builtin_amdgcn_readfirstlane(s[x].kept);
-        s[x].parent = __builtin_amdgcn_readfirstlane(here ? s[x].parent : b0 + x);
-        least = min(least, s[x].parent == b0 + x ? s[x].need : 0);
-      }
-      for (int at0 = least & -64; at0 < a.width; at0 += 64 * kFar) {
-        int old[kSide][kFar], page[kSide][kFar];
-#pragma unroll
-        for (int x = 0; x < kSide; ++x)
-#pragma unroll
-          for (int i = 0; i < kFar; ++i) {
-            const int at = at0 + 64 * i + lane, b = b0 + x;
-            const bool mine = at < a.width && (s[x].parent != b || at >= s[x].need);
-            old[x][i] = a.table[mine ? b * a.width + at : 0];
-            if (kForked) page[x][i] = a.table[mine && s[x].parent != b && at < s[x].kept ? s[x].parent * a.width + at : 0];
-          }
-#pragma unroll
-        for (int x = 0; x < kSide; ++x)
-#pragma unroll
-          for (int i = 0; i < kFar; ++i) {
-            const int at = at0 + 64 * i + lane, b = b0 + x;
-            if (at < a.width && (s[x].parent != b || at >= s[x].need))
-              put(b, at, old[x][i], kForked && s[x].parent != b && at < s[x].kept ? page[x][i] : -1);
-          }
-      }
+    for (int x = 0; x < kFar; ++x) {
+      const int i = min(i0 + x * kSettle, places - 1), b = a.width == 1 ? i : (int)__umulhi((unsigned)i, per_width), at = i - b * a.width;
+      const int parent = seqs[b].parent;
+      mine[x] = i0 + x * kSettle < places && (parent != b || at >= seqs[b].need);
+      old[x] = page[x] = -1;
+      if (mine[x]) old[x] = a.table[i];
+      if (kForked && mine[x] && parent != b && at < seqs[b].kept) page[x] = a.table[parent * a.width + at];
     }
-  };
-  bool changes = false;
-  places([&](int b, int at, int old, int page) {
-    if (kForked) a.next[b * a.width + at] = page;
-    if (old == page) return;
-    changes = true;
-    if (named(a, old)) atomicSub(&left[old], 1);
-    if (named(a, page)) atomicAdd(&left[page], 1);
-  });
-  changes = __syncthreads_or(changes);
+#pragma unroll
+    for (int x = 0; x < kFar; ++x) {
+      if (kForked && mine[x]) a.next[i0 + x * kSettle] = page[x];
+      if (old[x] == page[x]) continue;
+      changed |= 1u << (j0 + x);
+      if (named(a, old[x])) atomicSub(&left[old[x]], 1);
+      if (named(a, page[x])) atomicAdd(&left[page[x]], 1);
+    }
+  }
+  __syncthreads();
   auto count = [&](int p) {
     if (named(a, p) && left[p] >= kHeldBelow) a.refs[p] = max(left[p], 0);
   };
@@ -344,27 +332,22 @@ __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
       [&](const Seq& s, int b, int at) { return inherited(a, s, b, at, s.parent == b ? a.table[b * a.width + at] : -1); }, place, was, fresh, count);
   if (n < 0) return;
   __syncthreads();  // the counts
-  if (changes && kForked) {
-    for (int p = tid; p < a.n_pages; p += kSettle) count(p);
-    for (int b = wave; b < a.n_seqs; b += kSettle / 64) {
-      const int parent = __builtin_amdgcn_readfirstlane(seqs[b].parent), need = __builtin_amdgcn_readfirstlane(seqs[b].need);
-      for (int at0 = parent == b ? need & -64 : 0; at0 < a.width; at0 += 64 * kAhead) {
-        int page[kAhead];
+  for (int i0 = tid; changed; i0 += kFar * kSettle, changed >>= kFar) {
+    int old[kFar], page[kFar];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) page[i] = a.next[min(b * a.width + at0 + 64 * i + lane, a.n_seqs * a.width - 1)];
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const int at = at0 + 64 * i + lane;
-          if (at < a.width && (parent != b || at >= need)) a.table[b * a.width + at] = page[i];
-        }
-      }
+    for (int x = 0; x < kFar; ++x) {
+      old[x] = page[x] = -1;
+      if (!(changed >> x & 1)) continue;
+      old[x] = a.table[i0 + x * kSettle];
+      if (kForked) page[x] = a.next[i0 + x * kSettle];
     }
-  } else if (changes) {
-    places([&](int b, int at, int old, int) {
-      if (old == -1) return;
-      a.table[b * a.width + at] = -1;
-      count(old);
-    });
+#pragma unroll
+    for (int x = 0; x < kFar; ++x) {
+      if (!(changed >> x & 1)) continue;
+      a.table[i0 + x * kSettle] = page[x];
+      count(old[x]);
+      if (kForked) count(page[x]);
+    }
   }
   if (tid < a.n_seqs) a.len[tid] = seqs[tid].len;
   __syncthreads();
@@ -435,7 +418,9 @@ __global__ __launch_bounds__(256) void fork_end_kernel(Fork a) {
 
 // ---------------------------------------------------------------------------------------------
 // Copies. A unit is kUnit bytes of one page's keys, values or weights in one cache; workgroups take every gridDim.x-th, so that a
-// captured launch serves as many pairs as the list then has.
+// captured launch serves as many pairs as the list then has. Memory bounds it: 64 pages of 64 KB and their weights in 28 caches, 237 MB read and
+// written, take 53 us among other passes, 4.5 TB/s where a copy of 2 GiB reaches 4.9, and 36 us where they are in the cache in front; eight pages of
+// 32 KB in one cache 3.1 us, a launch.
 // ---------------------------------------------------------------------------------------------
 constexpr int kUnit = 8192;
 constexpr int kAtOnce = 32;  // caches of a launch
@@ -483,7 +468,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(Copy a) {
 // Compaction. Which pages are used and which may move are bits, 64 of a word, and a page's place among the movers or the holes
 // is the words' running sum and the bits below it. The i-th mover goes to the i-th hole: the last word whose sum does not pass i has it. One
 // workgroup adds the words up; pages and places are then gone through by all. (Lists of movers and holes written by that one workgroup, a
-// store of every bit, took 23 us for 65536 pages.)
+// store of every bit, took 23 us for 65536 pages.) Latency bounds it: 2.4 + 4.4 + 6.5 us of three launches there, the last a
+// search of some ten dependent reads; 6.6 us of one launch for 2000 pages.
 // ---------------------------------------------------------------------------------------------
 typedef unsigned long long Bits64;
 struct Compact {
@@ -599,8 +585,9 @@ __global__ __launch_bounds__(256) void compact_bits_kernel(Compact a) { compact_
 __global__ __launch_bounds__(kSettle) void compact_sums_kernel(Compact a) { compact_sums(a); }
 __global__ __launch_bounds__(256) void compact_apply_kernel(Compact a) { compact_apply(a, blockIdx.x * 256 + threadIdx.x, a.counts[0]); }
 
-// All of it by one workgroup, where pages and places are few
-constexpr int kNearMoves = 8192;
+// All of it by one workgroup, where pages and places are few (2000 pages 12.8 us of a pass among others against 17.5 in three launches, 5000 13.9 against
+// 16.4, 6000 15.4 to 16.1 against 16.5, 8000 18.2 against 17.9)
+constexpr int kNearMoves = 6144;
 __global__ __launch_bounds__(kSettle) void compact_kernel(Compact a) {
   __shared__ Bits64 hole[kNearMoves / 64], mover[kNearMoves / 64];
   __shared__ int holes_before[kNearMoves / 64], movers_before[kNearMoves / 64];
@@ -694,7 +681,8 @@ int w4a32_op_paged_fork(const w4a32_paged_cache* cache, const w4a32_paged_fork_a
                (int*)(s + r.left), (int*)(s + r.next), (int*)(s + r.place), (int*)(s + r.was), (int*)(s + r.fresh)};
   hipStream_t st = static_cast<hipStream_t>(stream);
   const unsigned places = (unsigned)cache->n_seqs * cache->table_ld, pages = (unsigned)cache->n_pages;
-  if (cache->n_pages <= kNearPages && cache->n_seqs <= kNearSeqs && a.most <= kNearWritten && places <= kNearPlaces) {
+  if (cache->n_pages <= kNearPages && cache->n_seqs <= kNearSeqs && a.most <= kNearWritten &&
+      places <= (unsigned)(a.parent || a.keep ? kNearChanged : kNearPlaces)) {
     static w4::LdsLimitOnce limit[2];
     auto kernel = a.parent ? fork_kernel<true> : fork_kernel<false>;
     if (limit[a.parent != nullptr].raise((const void*)kernel, 4 * (kNearPages + 3 * kNearWritten) + kNearSeqs * sizeof(Seq)) != hipSuccess) return W4A32_ELAUNCH;

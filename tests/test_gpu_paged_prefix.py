@@ -116,7 +116,7 @@ def test_one_sequence_and_many(pkg, act, kind):
     run(pkg, Groups(5, counts, [16 + 3 * i for i in range(50)], [i % 20 for i in range(150)], [(i * 7) % 3 for i in range(150)], 2, 64, 16), act, kind, 6)
     for n in (64, 65):   # one wavefront's lanes of sequences, and more
         run(pkg, Groups(5, [n - 7, 4, 3], [50, 0, 33], [i % 20 for i in range(n)], [i % 3 for i in range(n)], 2, 64, 16), act, kind, 6)
-    for n in (16, 17):   # as many groups as are gone through one by one, and more
+    for n in (8, 9, 16, 17):   # as many groups as are gone through one by one, and more
         run(pkg, Groups(5, [2] * n, [20 + i for i in range(n)], [i % 20 for i in range(2 * n)], [1 + i % 3 for i in range(2 * n)], 2, 64, 16), act, kind, 6)
     run(pkg, Groups(5, [40, 40], [50, 33], [i % 20 for i in range(80)], [70 if i % 9 == 0 else 1 for i in range(80)], 1, 64, 16), act, kind, 2)
     run(pkg, Groups(6, [1] * 70 + [70], [20] * 71, [i % 5 for i in range(140)], [1] * 140, 1, 64, 16), act, kind, 2)

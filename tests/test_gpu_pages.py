@@ -120,6 +120,10 @@ def test_fork(pkg, seed):
     (1500, 5, 16, 12000),     # more sequences than the workgroup that settles them has threads
     (3, 20000, 16, 70000),    # long tables, many pages
     (300, 400, 16, 150000),
+    (256, 64, 16, 18000),     # as many places as one workgroup takes of sequences that change, and more
+    (257, 64, 16, 18000),
+    (500, 1, 16, 700),        # a place each
+    (512, 33, 32, 18000),
 ])
 def test_large_forks(pkg, B, W, page, n_pages):
     rng = np.random.default_rng(B)
@@ -127,6 +131,16 @@ def test_large_forks(pkg, B, W, page, n_pages):
     parent = [int(x) for x in rng.integers(0, B, B)]
     check_fork(pkg, table, lens, model.count(table, n_pages), page, parent, None, [int(x) for x in rng.integers(0, 60, B)])
     check_fork(pkg, table, lens, model.count(table, n_pages), page, None, [int(n * rng.random()) for n in lens], [1] * B)
+
+
+@pytest.mark.parametrize("B,W,n_pages", [(512, 64, 32768), (512, 61, 32000), (300, 109, 32768)])
+def test_many_sequences_that_end(pkg, B, W, n_pages):
+    """Some sequences have become shorter and give pages back, pages of others are shared: one workgroup, all that it has room for"""
+    rng = np.random.default_rng(W)
+    table, lens = model.pool(rng, B, W, 16, n_pages)
+    lens = [int(n * rng.random()) if b % 3 == 0 else n for b, n in enumerate(lens)]
+    table[7, :3], table[8, :3], lens[7], lens[8] = table[20, :3], table[20, :3], 40, 33
+    check_fork(pkg, table, lens, model.count(table, n_pages), 16, None, None, [b % 3 for b in range(B)])
 
 
 def test_a_prompt_of_many_pages(pkg):
@@ -213,7 +227,7 @@ def check_compact(pkg, table, refs):
     assert moves.tolist() == [list(p) for p in pairs] + [[-1, -1]] * (len(refs) // 2 - len(pairs))
 
 
-@pytest.mark.parametrize("n_pages", [1, 2, 63, 64, 65, 129, 1000, 5000, 8192, 8193, 70000])
+@pytest.mark.parametrize("n_pages", [1, 2, 63, 64, 65, 129, 1000, 5000, 6144, 6145, 8192, 8193, 70000])
 @pytest.mark.parametrize("held", [0, 3])
 def test_compact(pkg, n_pages, held):
     rng = np.random.default_rng(n_pages + held)
