@@ -219,3 +219,37 @@ def test_captured(pkg):
             eager = pkg.op_token_logprobs(x, tokens, top=10)
             stream.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_nan_of_either_sign(pkg, kind):
+    bits = torch.int32 if kind == "f32" else torch.int16
+    x = logits_of(6, 2500, kind)
+    minus = x[:, 0].clone().fill_(float("nan")).view(bits)
+    minus |= torch.iinfo(bits).min
+    for r, at in enumerate((0, 700, 1024, 2047, 2499)):
+        x.view(bits)[r, at] = minus[r]
+    assert bool(torch.signbit(x[:5][torch.isnan(x[:5])]).all()) and int(torch.isnan(x).sum()) == 5
+    check(pkg, x, some_tokens(6, 2500), 4, 1.0)
+    check(pkg, x, some_tokens(6, 2500), 0, 1.0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("V", [262144, 262145, 524288, 524289])
+def test_as_many_chunks_as_are_kept(pkg, kind, V):
+    """Vocabularies whose chunks' maxima just have room in LDS, and larger ones"""
+    for top in (1, 50):
+        check(pkg, logits_of(3, V, kind, V), some_tokens(3, V), top, 0.8)
+    check(pkg, (torch.arange(V, device="cuda") % 1000 == 999).to(TYPES[kind])[None], some_tokens(1, V), 700, 1.0)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_ranks_among_equal_logits(pkg, kind):
+    """The given token at blocks' borders: equal ones in front of it come before it, those behind it do not"""
+    V = 3500
+    tokens = torch.tensor([0, 1, 1023, 1024, 1025, 2047, 2048, 3071, 3073, 3499, 63, 64], device="cuda")
+    x = (torch.arange(V, device="cuda") % 2).to(TYPES[kind]).repeat(len(tokens), 1)
+    check(pkg, x, tokens, 0, 1.0)
+    check(pkg, x * 0, tokens, 2, 1.0)
+    x[:, ::3] = float("-inf")
+    check(pkg, x, tokens, 3, 1.0)
