@@ -420,10 +420,10 @@ __global__ __launch_bounds__(256) void fork_end_kernel(Fork a) {
 // ---------------------------------------------------------------------------------------------
 // Copies. A unit is kUnit bytes of one page's keys, values or weights in one cache; workgroups take every gridDim.x-th, so that a
 // captured launch serves as many pairs as the list then has. Memory bounds it: 64 pages of 64 KB and their weights in 28 caches, 237 MB read and
-// written, take 53 us among other passes, 4.5 TB/s where a copy of 2 GiB reaches 4.9, and 36 us where they are in the cache in front; eight pages of
-// 32 KB in one cache 3.1 us, a launch.
+// written, take 47 us among other passes (5.0 TB/s, where a copy of 2 GiB reaches 4.9), and 37 where they are in the cache in front; eight pages of
+// 32 KB in one cache 3 us, a launch. Copies are written past the caches, which keep what is read (52 us otherwise).
 // ---------------------------------------------------------------------------------------------
-constexpr int kUnit = 8192;
+constexpr int kUnit = 16384;
 constexpr int kAtOnce = 32;  // caches of a launch
 struct Copy {
   const int *moves, *count;
@@ -455,12 +455,12 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(Copy a) {
         if (lo + 4096 * i < a.row_bytes) x[i] = load_global<u32x4>(src + lo + 4096 * i);
 #pragma unroll
       for (int i = 0; i < kUnit / 4096; ++i)
-        if (lo + 4096 * i < a.row_bytes) *(W4_GLOBAL u32x4*)(dst + lo + 4096 * i) = x[i];
+        if (lo + 4096 * i < a.row_bytes) __builtin_nontemporal_store(x[i], (W4_GLOBAL u32x4*)(dst + lo + 4096 * i));
     } else {
       const unsigned words = a.weight_bytes / 4, lo = (unit - 2 * a.k_units) * (kUnit / 4);
       const float* src = a.w[cache] + (size_t)from * words;
       float* dst = a.w[cache] + (size_t)to * words;
-      for (unsigned i = lo + threadIdx.x; i < min(lo + kUnit / 4, words); i += 256) dst[i] = src[i];
+      for (unsigned i = lo + threadIdx.x; i < min(lo + kUnit / 4, words); i += 256) __builtin_nontemporal_store(src[i], (W4_GLOBAL float*)(dst + i));
     }
   }
 }
@@ -732,7 +732,7 @@ int w4a32_op_paged_copy(const w4a32_paged_cache* const* caches, int n_caches, co
       a.w[i] = caches[at + i]->d_weight;
     }
     const unsigned long long units = (unsigned long long)most * a.n_caches * a.units;
-    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(units < 2048 ? units : 2048)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(copy_pages_kernel, dim3((unsigned)(units < 8192 ? units : 8192)), dim3(256), 0, static_cast<hipStream_t>(stream), a);
     if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   }
   return W4A32_OK;
