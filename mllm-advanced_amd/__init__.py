@@ -900,7 +900,7 @@ class PagedCache:
         self.dtype, self.device, self.kv_heads, self.dim, self.n_seqs = k.dtype, device, kv, dim, table.shape[0]
         self.args = PagedCacheArgs(k.data_ptr(), v.data_ptr(), _ptr(weight), table.data_ptr(), length.data_ptr(), _kinds[k.dtype],
                                    pages, page, kv, dim, table.shape[0], table.shape[1])
-        self.starts = (table.shape[0] + 1,)   # shape of the row starts
+        self.starts, self.pages = (table.shape[0] + 1,), (pages,)   # shapes of the row starts, of the pages' counts
         self._ref, self._address = ctypes.byref(self.args), ctypes.addressof(self.args)
 
 
@@ -1042,7 +1042,7 @@ def op_paged_fork(cache, refs, parent=None, keep=None, row_start=None, rows=0, m
     device, i32, n = _device(), _torch.int32, cache.n_seqs
     if cache.device != device:
         raise W4A32Error(f"the cache is on device {cache.device}, the current one is {device}")
-    _need(refs, "refs", i32, device, cache.k.shape[:1])
+    _need(refs, "refs", i32, device, cache.pages)
     if parent is not None:
         _need(parent, "parent", i32, device, (n,))
     if keep is not None:
@@ -1062,16 +1062,19 @@ def op_paged_copy(caches, moves, counts):
     """In every one of `caches` (the layers', of the same sizes) page moves[i][1] becomes a copy of page moves[i][0], weights included, for
     i < counts[0]: what op_paged_fork() and op_paged_compact() return."""
     device, many = _device(), (caches,) if isinstance(caches, PagedCache) else tuple(caches)
-    if not many or any(c.device != device for c in many):
+    addresses = [c._address for c in many if c.device == device]
+    if not many or len(addresses) != len(many):
         raise W4A32Error(f"caches on device {device}, the current one, are wanted")
-    if moves.ndim != 2 or moves.shape[1] != 2 or counts.numel() < 1:
-        raise W4A32Error(f"moves is [pairs][2] and counts has their number first: got {tuple(moves.shape)}, {tuple(counts.shape)}")
+    shape = moves.shape
+    if len(shape) != 2 or shape[1] != 2 or counts.numel() < 1:
+        raise W4A32Error(f"moves is [pairs][2] and counts has their number first: got {tuple(shape)}, {tuple(counts.shape)}")
     _need(moves, "moves", _torch.int32, device), _need(counts, "counts", _torch.int32, device)
-    if moves.shape[0] == 0:
+    pairs = shape[0]
+    if pairs == 0:
         return
-    _sizes(*moves.shape)
-    refs = (ctypes.c_void_p * len(many))(*[c._address for c in many])
-    _check(lib().w4a32_op_paged_copy(refs, len(many), moves.data_ptr(), counts.data_ptr(), moves.shape[0], _stream()), "w4a32_op_paged_copy")
+    _sizes(pairs)
+    refs = (ctypes.c_void_p * len(many))(*addresses)
+    _check(lib().w4a32_op_paged_copy(refs, len(many), moves.data_ptr(), counts.data_ptr(), pairs, _stream()), "w4a32_op_paged_copy")
 
 
 def op_paged_compact_scratch(cache):
@@ -1089,10 +1092,10 @@ def op_paged_compact(cache, refs, scratch=None):
     device = _device()
     if cache.device != device:
         raise W4A32Error(f"the cache is on device {cache.device}, the current one is {device}")
-    _need(refs, "refs", _torch.int32, device, cache.k.shape[:1])
+    _need(refs, "refs", _torch.int32, device, cache.pages)
     if scratch is None:
         scratch = op_paged_compact_scratch(cache)
-    moves, counts = cache.table.new_empty((cache.k.shape[0] // 2, 2)), cache.table.new_empty(2)
+    moves, counts = cache.table.new_empty((cache.pages[0] // 2, 2)), cache.table.new_empty(2)
     _check(lib().w4a32_op_paged_compact(cache._ref, refs.data_ptr(), moves.data_ptr() or None, counts.data_ptr(), *_scratch_of(scratch, device),
                                         _stream()), "w4a32_op_paged_compact")
     return moves, counts
