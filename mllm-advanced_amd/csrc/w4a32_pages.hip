@@ -469,8 +469,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(Copy a) {
 // Compaction. Which pages are used and which may move are bits, 64 of a word, and a page's place among the movers or the holes
 // is the words' running sum and the bits below it. The i-th mover goes to the i-th hole: the last word whose sum does not pass i has it. One
 // workgroup adds the words up; pages and places are then gone through by all. (Lists of movers and holes written by that one workgroup, a
-// store of every bit, took 23 us for 65536 pages.) Latency bounds it: 2.4 + 4.4 + 6.5 us of three launches there, the last a
-// search of some ten dependent reads; 6.6 us of one launch for 2000 pages.
+// store of every bit, took 23 us for 65536 pages.) Latency bounds it: 2.5 + 8.1 us of two launches there, the second three
+// scans, a search of ten dependent reads and the names; 6.6 us of one launch for 2000 pages.
 // ---------------------------------------------------------------------------------------------
 typedef unsigned long long Bits64;
 struct Compact {
@@ -490,8 +490,8 @@ __device__ __forceinline__ void compact_bits(const Compact& a, int p) {
   }
 }
 
-// By one workgroup; returns how many pages move
-__device__ __forceinline__ int compact_sums(const Compact& a) {
+// By one workgroup; returns how many pages move, which is written where `writes`
+__device__ __forceinline__ int compact_sums(const Compact& a, bool writes) {
   __shared__ unsigned in_wave[kSettle / 64];
   __shared__ int last;
   const int tid = threadIdx.x, each = (a.words + kSettle - 1) / kSettle, w0 = min(tid * each, a.words), w1 = min(w0 + each, a.words);
@@ -520,7 +520,7 @@ __device__ __forceinline__ int compact_sums(const Compact& a) {
     h += __popcll(a.hole[w]);
     m += __popcll(a.mover[w]);
   }
-  if (tid == 0) {
+  if (writes && tid == 0) {
     a.counts[0] = (int)all;  // as many holes as movers or more
     a.counts[1] = max(last, used);
   }
@@ -583,12 +583,32 @@ __device__ __forceinline__ void compact_apply(const Compact& a, int i, int pairs
 }
 
 __global__ __launch_bounds__(256) void compact_bits_kernel(Compact a) { compact_bits(a, blockIdx.x * 256 + threadIdx.x); }
-__global__ __launch_bounds__(kSettle) void compact_sums_kernel(Compact a) { compact_sums(a); }
+__global__ __launch_bounds__(kSettle) void compact_sums_kernel(Compact a) { compact_sums(a, true); }
 __global__ __launch_bounds__(256) void compact_apply_kernel(Compact a) { compact_apply(a, blockIdx.x * 256 + threadIdx.x, a.counts[0]); }
 
-// All of it by one workgroup, where pages and places are few (2000 pages 12.8 us of a pass among others against 17.5 in three launches, 5000 13.9 against
-// 16.4, 6000 15.4 to 16.1 against 16.5, 8000 18.2 against 17.9)
-constexpr int kNearMoves = 6144;
+// The sums by every workgroup for itself, in LDS (65536 pages: 8.1 us where a launch of one workgroup and one of all with its searches in memory take 4.5
+// and 6.7; 14.4 against 16.6 of a pass among others, 10000 pages 13.2 against 15.8, 131072 17.6 either way)
+constexpr int kWords = 1024;
+__global__ __launch_bounds__(kSettle) void compact_both_kernel(Compact a) {
+  __shared__ Bits64 hole[kWords], mover[kWords];
+  __shared__ int holes_before[kWords], movers_before[kWords];
+  for (int w = threadIdx.x; w < a.words; w += kSettle) {
+    hole[w] = a.hole[w];
+    mover[w] = a.mover[w];
+  }
+  a.hole = hole;
+  a.mover = mover;
+  a.holes_before = holes_before;
+  a.movers_before = movers_before;
+  __syncthreads();
+  const int pairs = compact_sums(a, blockIdx.x == 0);
+  __syncthreads();
+  compact_apply(a, blockIdx.x * kSettle + threadIdx.x, pairs);
+}
+
+// All of it by one workgroup, where pages and places are few (2000 pages 12.2 us of a pass among others against 14.0 in two launches, 4096 12.3
+// against 14.4, 5000 the same, 6000 16.0 against 14.3)
+constexpr int kNearMoves = 4096;
 __global__ __launch_bounds__(kSettle) void compact_kernel(Compact a) {
   __shared__ Bits64 hole[kNearMoves / 64], mover[kNearMoves / 64];
   __shared__ int holes_before[kNearMoves / 64], movers_before[kNearMoves / 64];
@@ -598,7 +618,7 @@ __global__ __launch_bounds__(kSettle) void compact_kernel(Compact a) {
   a.movers_before = movers_before;
   for (int p = threadIdx.x; p < 64 * a.words; p += kSettle) compact_bits(a, p);
   __syncthreads();
-  const int pairs = compact_sums(a);
+  const int pairs = compact_sums(a, true);
   __syncthreads();
   for (int i = threadIdx.x; i < max(a.n_seqs * a.width, a.n_pages); i += kSettle) compact_apply(a, i, pairs);
 }
@@ -760,6 +780,10 @@ int w4a32_op_paged_compact(const w4a32_paged_cache* cache, int* d_refs, int* d_m
   }
   hipLaunchKernelGGL(compact_bits_kernel, dim3((pages + 255) / 256), dim3(256), 0, st, a);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
+  if (r.words <= kWords) {
+    hipLaunchKernelGGL(compact_both_kernel, dim3((most + kSettle - 1) / kSettle), dim3(kSettle), 0, st, a);
+    return from_hip(hipGetLastError());
+  }
   hipLaunchKernelGGL(compact_sums_kernel, dim3(1), dim3(kSettle), 0, st, a);
   if (hipGetLastError() != hipSuccess) return W4A32_ELAUNCH;
   hipLaunchKernelGGL(compact_apply_kernel, dim3((most + 255) / 256), dim3(256), 0, st, a);

@@ -227,7 +227,7 @@ def check_compact(pkg, table, refs):
     assert moves.tolist() == [list(p) for p in pairs] + [[-1, -1]] * (len(refs) // 2 - len(pairs))
 
 
-@pytest.mark.parametrize("n_pages", [1, 2, 63, 64, 65, 129, 1000, 5000, 6144, 6145, 8192, 8193, 70000])
+@pytest.mark.parametrize("n_pages", [1, 2, 63, 64, 65, 129, 1000, 4096, 4097, 5000, 8192, 8193, 65536, 65537, 70000])
 @pytest.mark.parametrize("held", [0, 3])
 def test_compact(pkg, n_pages, held):
     rng = np.random.default_rng(n_pages + held)
