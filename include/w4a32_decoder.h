@@ -364,7 +364,8 @@ int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache
  * 0 is a free page, and a page with a negative number is someone else's, never handed out, moved or counted (tables may name it: rows
  * that would be written to it get a copy). A fresh pool has zeros there, -1 in the table and lengths 0; these two operators keep
  * all of it true, and that behind a sequence's tokens its pages follow each other (the first -1 there is the end of
- * them). Layers have pools of their own and one table: they are called once, and w4a32_op_paged_copy for all layers.
+ * them): a sequence gives its pages back by a parent or a d_keep, not by a length that is made smaller by hand, which leaves it what stands behind
+ * a place without a page. Layers have pools of their own and one table: they are called once, and w4a32_op_paged_copy for all layers.
  *
  * Fork. Sequence b becomes the first min(length, d_keep[b]) tokens of sequence d_parent[b], as all of them were before the call,
  * with room for its rows of the coming step (d_row_start, as the step will have them):

@@ -215,7 +215,7 @@ constexpr int kNearPages = 32 * 1024, kNearSeqs = 512, kNearWritten = 1536, kNea
 // A step that shares nothing and gives nothing back, as most are: rows' places that name no page get free ones, and that is all. Returns
 // false where there is more to do, with nothing changed. A thread has a sequence; a wavefront a run of pages, 64 of each lane, whose counts are under
 // way while the sequences' lengths are. Behind a sequence's tokens its pages follow each other: where the first place behind those that it needs names
-// -1, nothing is given back.
+// -1, nothing is given back. (All places looked at instead, 128 KB by one workgroup: 11.9 us against 6.7.)
 __device__ __forceinline__ bool fork_nothing(const Fork& a, int* fresh) {
   __shared__ unsigned in_wave[kSettle / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -143,6 +143,18 @@ def test_many_sequences_that_end(pkg, B, W, n_pages):
     check_fork(pkg, table, lens, model.count(table, n_pages), 16, None, None, [b % 3 for b in range(B)])
 
 
+@pytest.mark.parametrize("B,W", [(3, 9), (40, 33), (1, 20000), (512, 64), (300, 200)])
+@pytest.mark.parametrize("forked", [False, True])
+def test_pages_behind_a_hole(pkg, B, W, forked):
+    """A sequence that keeps nothing, or has no parent, gives up all of its pages, those behind places that name none too"""
+    n_pages = B * W + 5
+    table = np.random.default_rng(W).permutation(n_pages)[:B * W].reshape(B, W)
+    table[:, :W // 2] = -1                       # pages that a window has left behind
+    lens, rows, ends = [W * 16] * B, [b % 2 for b in range(B)], [b % 2 == 0 for b in range(B)]
+    parent, keep = ([-1 if e else b for b, e in enumerate(ends)], None) if forked else (None, [0 if e else 1 << 30 for e in ends])
+    check_fork(pkg, table, lens, model.count(table, n_pages), 16, parent, keep, rows)
+
+
 def test_a_prompt_of_many_pages(pkg):
     table = np.full((2, 600), -1)
     table[1, :2] = [3, 4]
