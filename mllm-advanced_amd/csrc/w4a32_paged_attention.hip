@@ -59,7 +59,7 @@ constexpr int kLeastPass = 128;
 
 template <typename Act, typename KV, int DT, bool kDump>
 __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void rows_kernel(Attend a) {
-  rows_body<Act, KV, DT, kDump, kRest>(a, blockIdx.x, gridDim.x, 0, 0);
+  rows_body<Act, KV, DT, kDump, kRest>(a, blockIdx.x, gridDim.x, 0, 0, 0);
 }
 
 // Joins the shares of an item: a workgroup per query row and kSlice of its values, its threads four values of every 256 /
@@ -155,7 +155,7 @@ template <typename KV>
 __global__ __launch_bounds__(64 * kWaves) void weights_kernel(Attend a) {
   constexpr int KT = tile_keys<KV>(), kHalves = KT / 16;
   Seqs<KT> seqs;
-  if (deal_of(a, seqs, (unsigned)kGrid).per == 0) return;
+  if (deal_of(a, seqs, (unsigned)kGrid, 0).per == 0) return;
   const Place p = place_of(a, seqs, blockIdx.x, kKeyTiles, 1);
   if (!p.there) return;
   const int per_head = (p.q.nt + kWaves - 1) / kWaves, hk = (int)p.inner / per_head;

@@ -28,6 +28,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kPlan = 1024;      // threads of the workgroup that deals
 constexpr int kSlots = 512;      // workgroups that are there at once: two per CU
 constexpr int kMostShares = kSlots * 7 / 8;  // of prefixes, where their items are not more
+constexpr unsigned kUnits = 896;  // most workgroups where prefixes have kMostShares at most: those that find nothing take their time, too
 constexpr int kLog2 = 7;         // log2 of the rows of a workgroup of a prefix
 // Pairs of row and head from which on a sequence's own tokens go by blocks of 128 rows as well, and not by 16 of a wavefront (eight prompts of 60 to
 // 300 rows, 28 heads on 4, bf16: behind 64 tokens 46 us against 68, behind 4099 141 against 148; 64, 256, 512: the same).
@@ -345,8 +346,14 @@ __global__ __launch_bounds__(64 * kWaves, DT == 256 ? 1 : 2) void both_kernel(At
       return;
     }
     unit -= (int)blocks;
+    m.total += (int)blocks;
   }
-  if (unit < x.own_grid) rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)unit, (unsigned)x.own_grid, m.from, group_at);
+  // As many as there is room for beside the prefixes begin at once, if that leaves them short enough: shares are whole, and some four fifths of the
+  // workgroups that they are dealt to get one (64 sequences with 16 to 1200 tokens of their own, 28 heads on 4, bf16: behind eight prefixes of 1000 tokens 33 us
+  // against 38 with more and shorter ones; 48 behind six of 3000 32 against 36, of 6000 39 against 43).
+  const unsigned one_round = (unsigned)max(kSlots - m.total, 0) * 5 / 4;
+  const int own_grid = min(x.own_grid, (int)gridDim.x - m.total);
+  if (unit < own_grid) rows_body<Act, KV, DT, false, kOwn>(a, (unsigned)unit, (unsigned)own_grid, one_round, m.from, group_at);
 }
 
 // Where rows are few: a workgroup per row and kSlice of its values, its threads four values of every 256 / (kSlice / 4)th share each
@@ -492,7 +499,8 @@ hipError_t launch_both(const Attend& a, const Plan& p, hipStream_t s) {
     hipLaunchKernelGGL((deal_kernel<Shape<Act, KV, DT, kHalfForm>::kKeys, tile_keys<KV>(), sizeof(KV) == 4>), dim3(1), dim3(kPlan), 0, s, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(p.grid + p.blocks + p.own_grid), dim3(64 * kWaves), lds, s, a);
+  const unsigned units = p.grid + p.own_grid, most = p.grid == kMostShares && units > kUnits ? kUnits : units;
+  hipLaunchKernelGGL((both_kernel<Act, KV, DT>), dim3(most + p.blocks), dim3(64 * kWaves), lds, s, a);
   return hipGetLastError();
 }
 template <typename Act, typename KV>

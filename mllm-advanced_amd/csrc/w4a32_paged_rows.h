@@ -12,9 +12,11 @@ constexpr int kGrid = 512;
 constexpr int kMinTiles = kWaves; // least tiles of a share, where items have so many
 constexpr int kAlone = 8;         // tiles up to which items are not shared, where all are so short
 constexpr int kFew = 16;          // tiles of a share up to which it has tiles of one item only
+constexpr unsigned kRound = 24;
 
+// one_round (kOwn): to how many the shares are dealt so that all begin at once, if none has kRound tiles then
 template <int KT, Which kWhich>
-__device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT, kWhich>& s, unsigned grid) {
+__device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT, kWhich>& s, unsigned grid, unsigned one_round) {
   Deal d = {0, 0, 0, true, false};
   unsigned others = 0;  // items without tiles
   bool all_short = true;
@@ -32,6 +34,7 @@ __device__ __forceinline__ Deal deal_of(const Attend& a, Seqs<KT, kWhich>& s, un
   }
   d.fits = d.total <= a.most_tiles && d.items <= a.most_items;
   if (d.total == 0 || !d.fits) return d;
+  if (kWhich == kOwn && one_round < grid && one_round > d.items - others && d.total / (one_round - (d.items - others)) < kRound) grid = one_round;
   d.per = max((d.total + grid - 1) / grid, (unsigned)kMinTiles);
   const unsigned more = grid - min(grid, d.items - others);  // workgroups beyond one per item
   if (all_short) {  // a workgroup takes every grid-th
@@ -81,7 +84,7 @@ __device__ __forceinline__ OwnItem own_item(const Attend& a, const Item& it, int
 
 // own_from: where this lane's sequence's own tokens begin; group_at: the group of a sequence, without rows where it has none.
 template <typename Act, typename KV, int DT, bool kDump, Which kWhich, typename GroupAt>
-__device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsigned grid, int own_from, GroupAt group_at) {
+__device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsigned grid, unsigned one_round, int own_from, GroupAt group_at) {
   using M = Math<Act, KV>;
   constexpr int KT = tile_keys<KV>(), NT = M::kTerms, kHalves = KT / 16;
   constexpr bool k16 = sizeof(KV) == 2;
@@ -97,7 +100,7 @@ __device__ __forceinline__ void rows_body(const Attend& a, unsigned block, unsig
 
   Seqs<KT, kWhich> seqs;
   seqs.own_from = own_from;
-  const Deal deal = deal_of(a, seqs, grid);
+  const Deal deal = deal_of(a, seqs, grid, one_round);
   if (block == 0 && threadIdx.x == 0) *a.count = deal.fits ? deal.items : 0;
   if (deal.per == 0) return;
   unsigned u = block, u_end = max(deal.items, grid);
