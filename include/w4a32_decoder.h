@@ -333,10 +333,11 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
 
 /* w4a32_op_paged_attention (without window and added-up weights) for a batch whose sequences share prefixes: group g is sequences
  * d_group_start[g] .. d_group_start[g + 1] (n_groups of them, at most n_seqs; sequences outside all groups share nothing), and its first
- * d_prefix[g] tokens are read once for all of its rows, from the pages of the group's first sequence; each sequence has its own tokens
- * from there on, the rest of the page in which the prefix ends among them. As a fork of one sequence leaves it, the prefix being what they all had
- * then, or less. A prefix beyond the length of one of the group's sequences with rows is cut to that, so that a row sees what
- * it would see alone, as long as the tables name the same tokens. Same results as w4a32_op_paged_attention up to the order of sums: maxima and sums are
+ * d_prefix[g] tokens are read once for all of its rows, from the pages of the group's first sequence that has so many; each sequence has its own
+ * tokens from there on, the rest of the page in which the prefix ends among them. As a fork of one sequence leaves it, the prefix being what they
+ * all had then, or less. A prefix beyond the length of one of the group's sequences with rows is cut to that, so that a row sees what
+ * it would see alone, as long as the tables of the group's sequences that have it name the same tokens: one that has ended, with no length and no pages
+ * left, may stay in its group, wherever it stands. Same results as w4a32_op_paged_attention up to the order of sums: maxima and sums are
  * f32, and each of the two parts is divided by nothing until they are joined. Group starts do not decrease; where they do, what the
  * rows get is unspecified.
  *   d_scratch: w4a32_op_paged_prefix_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time; 0 for a call that is

@@ -987,7 +987,7 @@ def op_paged_prefix_attention_scratch(cache, rows, max_rows, heads, n_groups):
 def op_paged_prefix_attention(cache, q, row_start, max_rows, heads, scale, group_start, prefix, scratch=None, out=None):
     """op_paged_attention() of a batch whose sequences share prefixes: group_start int32 [groups + 1], sequences group_start[g] ..
     group_start[g + 1] have their first prefix[g] tokens (prefix int32 [groups]) in common. Those are read once for all of the group's rows, from the
-    pages of its first sequence, and the others from each sequence's own."""
+    pages of its first sequence that has so many, and the others from each sequence's own. Sequences that have ended may stay in their groups."""
     device, n = cache.device, prefix.numel()
     if scratch is None:
         scratch = op_paged_prefix_attention_scratch(cache, q.shape[0], max_rows, heads, n)

@@ -24,7 +24,7 @@ struct Item {
 
 // Groups of sequences with a prefix in common: what the first of their launches leaves to the others
 struct PrefixGroup {
-  int b, r0, n, tokens;       // the sequence whose pages have it, the group's rows, the prefix
+  int b, r0, n, tokens;       // the sequence whose pages are read, the group's rows, the prefix
   int first, shares, blocks;  // workgroup of its first share, shares of an item, items of a kv head
   int pad;
 };

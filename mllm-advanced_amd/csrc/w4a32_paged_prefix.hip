@@ -55,7 +55,8 @@ __device__ __forceinline__ int wave_min(int x) {
 }
 
 // A group whose sequences with rows, `with_rows` of them, have `least` tokens or more, rows from r0 to before r1: one such sequence alone has no
-// prefix.
+// prefix. Whose pages have it is for the caller to say: sequence b0's where they do, else those of the next that has so many tokens, as
+// each with rows does (b0 may have ended, and have given its pages back).
 __device__ __forceinline__ PrefixGroup group_of(const Attend& a, int b0, int with_rows, int least, int r0, int r1) {
   PrefixGroup q = {b0, 0, 0, 0, 0, 0, 0, 0};
   if (with_rows < 2 || least <= 0) return q;
@@ -132,8 +133,9 @@ __device__ __forceinline__ Mine deal_by_lanes(const Attend& a) {
     if (lo == hi) continue;
     const bool in = lane >= lo && lane < hi, has = in && s.n > 0;
     const int least = wave_min(has ? s.len : __builtin_amdgcn_readlane(want, g));
-    const PrefixGroup q = group_of(a, lo, __popcll(__ballot(has)), min(least, __builtin_amdgcn_readlane(want, g)), __builtin_amdgcn_readlane(s.r0, lo),
-                                   __builtin_amdgcn_readlane(end, hi - 1));
+    PrefixGroup q = group_of(a, lo, __popcll(__ballot(has)), min(least, __builtin_amdgcn_readlane(want, g)), __builtin_amdgcn_readlane(s.r0, lo),
+                             __builtin_amdgcn_readlane(end, hi - 1));
+    if (q.tokens) q.b = __builtin_ctzll(__ballot(in && s.len >= q.tokens));
     if (lane == g) m.q = q;
     if (in && q.tokens) {
       m.from = q.tokens;
@@ -172,7 +174,9 @@ __global__ __launch_bounds__(kPlan) void deal_kernel(Attend a) {
       with_rows += __popcll(__ballot(s.n > 0));
       if (s.n > 0) least = min(least, s.len);
     }
-    const PrefixGroup q = group_of(a, b0, with_rows, wave_min(least), min(max(a.row_start[b0], 0), a.rows), min(a.row_start[b1], a.rows));
+    PrefixGroup q = group_of(a, b0, with_rows, wave_min(least), min(max(a.row_start[b0], 0), a.rows), min(a.row_start[b1], a.rows));
+    for (u64 found = 0; q.tokens && !found && q.b < b1; q.b += found ? __builtin_ctzll(found) : 64)
+      found = __ballot(q.b + lane < b1 && a.c.len[min(q.b + lane, b1 - 1)] >= q.tokens);
     if (lane == 0) x.group[g] = q;
     if (q.tokens)
       for (int b = b0 + lane; b < b1; b += 64) {
