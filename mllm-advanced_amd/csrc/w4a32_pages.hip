@@ -1,4 +1,6 @@
 // The pages of a paged cache: which sequence has which (fork), their copies in all layers' pools, and their move to the pool's front.
+#include <climits>
+
 #include "w4a32_paged.h"
 
 namespace w4 {
@@ -11,8 +13,10 @@ inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 constexpr int kSettle = 1024;         // threads of the one workgroup that hands pages out
 constexpr int kMostPlaces = 1 << 26;  // places of a table: a place's number and two marks are an int
-// A page with a negative count, which is someone else's: changes by all places there are leave it below kHeldBelow.
-constexpr int kHeld = -0x7f000000, kHeldBelow = -(1 << 30);
+// A page with a negative count, which is someone else's: changes by all places there are, up or down, leave it an int and below kHeldBelow; other counts
+// stay above, with the marks of those that write such a page.
+constexpr int kHeld = -(3 << 29), kHeldBelow = -(1 << 30);
+static_assert((long long)kHeld - kMostPlaces >= INT_MIN && kHeld + kMostPlaces < kHeldBelow && -2 - 2 * kMostPlaces >= kHeldBelow, "counts of pages");
 constexpr int kShared = 1 << 30, kStays = 1 << 29, kGiven = 1 << 28, kPlace = kMostPlaces - 1;
 
 // ---------------------------------------------------------------------------------------------
