@@ -365,16 +365,17 @@ int w4a32_op_paged_evict(const w4a32_paged_cache* cache, const w4a32_paged_cache
  * 0 is a free page, and a page with a negative number is someone else's, never handed out, moved or counted (tables may name it: rows
  * that would be written to it get a copy). A fresh pool has zeros there, -1 in the table and lengths 0; these two operators keep
  * all of it true, and that behind a sequence's tokens its pages follow each other (the first -1 there is the end of
- * them): a sequence gives its pages back by a parent or a d_keep, not by a length that is made smaller by hand, which leaves it what stands behind
- * a place without a page. Layers have pools of their own and one table: they are called once, and w4a32_op_paged_copy for all layers.
+ * them): a sequence gives its pages back by another parent, by none, or by a d_keep that ends in an earlier page, not by a length that is made
+ * smaller by hand, which leaves it what stands behind a place without a page. Layers have pools of their own and one table: they are called once,
+ * and w4a32_op_paged_copy for all layers.
  *
  * Fork. Sequence b becomes the first min(length, d_keep[b]) tokens of sequence d_parent[b], as all of them were before the call,
  * with room for its rows of the coming step (d_row_start, as the step will have them):
  *   - places with its tokens name the parent's pages, which it shares from then on;
  *   - a page that its rows will write is its own: where others name it too (or it is someone else's) it is replaced, and what it
  *     holds of the sequence's tokens is to be copied. Of sequences that all leave a page the last one keeps it;
- *   - places behind its tokens that its rows need get free pages, places behind those are -1, and pages that nobody names any
- *     more are free. Pages are handed out in the order of the places, the lowest free number first.
+ *   - places behind its tokens that its rows need get free pages, places behind those are -1 (of a sequence that goes on from itself: up to the first
+ *     that was), and pages that nobody names any more are free. Pages are handed out in the order of the places, the lowest free number first.
  * d_parent NULL: each goes on from itself. A parent outside [0, n_seqs): an empty sequence (a sequence that has ended; a new one, if it has
  * rows). d_keep NULL: all tokens; fewer take back what a step wrote too much. d_row_start NULL: no rows (rows and max_rows unused).
  * A place whose page is not there stays so where the sequence has tokens; what the table has no place for gets none.

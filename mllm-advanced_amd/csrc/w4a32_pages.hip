@@ -32,6 +32,7 @@ struct Seq {
   int parent, len;  // -1: none; tokens
   int kept, need;   // places with tokens; with those and the rows
   int first;        // the first that the rows write; `need` where there are none
+  int end;          // places of its own in front of it stay, where it goes on from itself: end_of()
 };
 struct Fork {
   int *table, *len, *refs;
@@ -65,11 +66,19 @@ __device__ __forceinline__ Seq seq_of(const Fork& a, int b) {
   s.first = n ? min(s.len >> a.shift, s.need) : s.need;
   return s;
 }
+// Behind a sequence's tokens its pages follow each other: where one goes on from itself, with all places of its tokens, and the first place behind those that
+// it needs names -1, that is the end of them, and what may stand behind it is not looked at. So all ways of a fork leave the same, of which the
+// shortest has no time to look at all places.
+__device__ __forceinline__ int end_of(const Fork& a, int b, const Seq& s) {
+  if (s.parent != b || s.need >= a.width) return s.need;
+  const int had = min((min(max(a.len[b], 0), kMost) + (1 << a.shift) - 1) >> a.shift, a.width);
+  return s.need >= had && a.table[(size_t)b * a.width + s.need] == -1 ? a.width : s.need;
+}
 __device__ __forceinline__ int count_at_first(int refs) { return refs < 0 ? kHeld : min(refs, kMostPlaces); }
 // The page that a place gets before rows are looked at; `old`: what is there
 __device__ __forceinline__ int inherited(const Fork& a, const Seq& s, int b, int at, int old) {
   if (at < s.kept) return s.parent == b ? old : a.table[(size_t)s.parent * a.width + at];
-  return at < s.need && s.parent == b ? old : -1;
+  return at < s.end && s.parent == b ? old : -1;
 }
 
 // Counts in LDS, and in memory that several compute units have written: past the caches of this one.
@@ -218,17 +227,13 @@ constexpr int kNearPages = 32 * 1024, kNearSeqs = 512, kNearWritten = 1536, kNea
 
 // A step that shares nothing and gives nothing back, as most are: rows' places that name no page get free ones, and that is all. Returns
 // false where there is more to do, with nothing changed. A thread has a sequence; a wavefront a run of pages, 64 of each lane, whose counts are under
-// way while the sequences' lengths are. Behind a sequence's tokens its pages follow each other: where the first place behind those that it needs names
-// -1, nothing is given back. (All places looked at instead, 128 KB by one workgroup: 11.9 us against 6.7.)
+// way while the sequences' lengths are. Of the places behind those that a sequence needs only the first is looked at. (All of them instead, 128 KB by one
+// workgroup: 11.9 us against 6.7.)
 __device__ __forceinline__ bool fork_nothing(const Fork& a, int* fresh) {
   __shared__ unsigned in_wave[kSettle / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Seq s = {};
-  int had = 0;
-  if (tid < a.n_seqs) {
-    s = seq_of(a, tid);
-    had = min((min(max(a.len[tid], 0), kMost) + (1 << a.shift) - 1) >> a.shift, a.width);
-  }
+  if (tid < a.n_seqs) s = seq_of(a, tid);
   constexpr int kAhead = 16;
   const int run = (a.n_pages + 64 * (kSettle / 64) - 1) / (64 * (kSettle / 64)), first = wave * run * 64;  // at most 64 of 64
   unsigned long long bits = 0;
@@ -248,7 +253,7 @@ __device__ __forceinline__ bool fork_nothing(const Fork& a, int* fresh) {
   bool more = false;
   unsigned wants = 0;
   if (tid < a.n_seqs) {
-    more = s.need < a.width && (s.need < had || row[s.need] != -1);
+    more = end_of(a, tid, s) < a.width;
     for (int at = s.first; at < s.need; ++at) {
       const int page = row[at];
       if (named(a, page))
@@ -282,7 +287,7 @@ __device__ __forceinline__ bool fork_nothing(const Fork& a, int* fresh) {
   return true;
 }
 
-// kForked: sequences have parents; else each goes on from itself, and only places behind those that it needs change here.
+// kForked: sequences have parents; else each goes on from itself, and only places from Seq::end on change here.
 template <bool kForked>
 __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
   extern __shared__ int lds[];
@@ -299,7 +304,11 @@ __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
     for (int i = 0; i < kAhead; ++i)
       if (p0 + i * kSettle < a.n_pages) left[p0 + i * kSettle] = count_at_first(refs[i]);
   }
-  if (tid < a.n_seqs) seqs[tid] = seq_of(a, tid);
+  if (tid < a.n_seqs) {
+    Seq s = seq_of(a, tid);
+    s.end = end_of(a, tid, s);
+    seqs[tid] = s;
+  }
   __syncthreads();
   // A thread has every kSettle-th place, kFar of them at a time, and a bit for each that changes
   constexpr int kFar = 4;
@@ -314,7 +323,7 @@ __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
     for (int x = 0; x < kFar; ++x) {
       const int i = min(i0 + x * kSettle, places - 1), b = a.width == 1 ? i : (int)__umulhi((unsigned)i, per_width), at = i - b * a.width;
       const int parent = seqs[b].parent;
-      mine[x] = i0 + x * kSettle < places && (parent != b || at >= seqs[b].need);
+      mine[x] = i0 + x * kSettle < places && (parent != b || at >= seqs[b].end);
       old[x] = page[x] = -1;
       if (mine[x]) old[x] = a.table[i];
       if (kForked && mine[x] && parent != b && at < seqs[b].kept) page[x] = a.table[parent * a.width + at];
@@ -366,7 +375,11 @@ __global__ __launch_bounds__(kSettle) void fork_kernel(Fork a) {
 __global__ __launch_bounds__(256) void fork_begin_kernel(Fork a) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < a.n_pages) a.left[i] = count_at_first(a.refs[i]);
-  if (i < a.n_seqs) a.seq[i] = seq_of(a, i);
+  if (i < a.n_seqs) {
+    Seq s = seq_of(a, i);
+    s.end = end_of(a, i, s);
+    a.seq[i] = s;
+  }
 }
 
 // A thread has the same place of kSide sequences that follow each other: children of one parent name one page there, and one atomic sum counts them
