@@ -74,6 +74,11 @@ __device__ __forceinline__ unsigned own_tiles(const Attend& a, const Span& s, in
   const unsigned long long n = ((unsigned long long)s.n * a.group + 15) / 16 * (unsigned)((keys + kKeys - 1) / kKeys - first / kKeys);
   return (unsigned)min(n, 0xffffffffull);
 }
+// Numbers of shares and tiles, as sums of them: what does not fit is the most, so that a batch of too many is found to have too many
+constexpr __host__ __device__ unsigned times(unsigned a, unsigned b) { return (u64)a * b > 0xffffffffu ? 0xffffffffu : a * b; }
+constexpr __host__ __device__ unsigned parts(unsigned a, unsigned of) { return a / of + (a % of != 0); }  // of `of` each; a may be the most
+static_assert(times(128, 1u << 25) == 0xffffffffu && times(896, times(1u << 16, 1u << 16)) == 0xffffffffu && times(3, 5) == 15 && times(0, 7) == 0, "");
+static_assert(parts(0xffffffffu, 448) == 9586981 && parts(0, 3) == 0 && parts(6, 3) == 2 && parts(7, 3) == 3, "");
 // Tiles of a prefix that a share of it has: the slots of the chip go to the prefixes and to the own tokens as their work is estimated (a workgroup
 // takes 3 units of time for a tile of a prefix, 8 for kWaves tiles of own tokens), and an item gets as few shares as keep to that. But a share
 // costs as well: its sums are written and read again, some 50 ns where all of a workgroup's rows are there, against 1 us for a tile (f32: 5), so
@@ -89,7 +94,7 @@ __device__ __forceinline__ unsigned share_of(const Attend& a, unsigned tiles, un
   if (most <= items) return 1u << 30;
   const float rows = (float)pairs / ((float)max(items, 1u) * (1 << kLog2));  // of those that a workgroup has room for
   const unsigned least = max((unsigned)(__builtin_sqrtf((float)tiles * rows * (kF32 ? 0.01f : 0.05f)) + 0.5f), 1u);
-  unsigned lo = max((tiles + most - 1) / most, least), per = max((tiles + most - items - 1) / (most - items), lo);
+  unsigned lo = max(parts(tiles, most), least), per = max(parts(tiles, most - items), lo);
   while (lo < per) {
     const unsigned mid = (lo + per) / 2;
     if (count(mid) <= most)
@@ -144,10 +149,10 @@ __device__ __forceinline__ Mine deal_by_lanes(const Attend& a) {
   }
   const unsigned of_group = (unsigned)m.q.blocks * a.c.kv_heads, tiles = tiles_of<kKeys>(m.q);
   const unsigned pairs = (unsigned)(m.q.n * a.group) * a.c.kv_heads;
-  const unsigned per = share_of<kF32>(a, wave_sum(of_group * tiles), wave_sum(of_group), wave_sum(pairs), wave_sum(own_tiles<kOwnKeys>(a, s, m.from)),
-                                      [&](unsigned n) { return wave_sum(of_group * ((tiles + n - 1) / n)); });
+  const unsigned per = share_of<kF32>(a, wave_sum(times(of_group, tiles)), wave_sum(of_group), wave_sum(pairs), wave_sum(own_tiles<kOwnKeys>(a, s, m.from)),
+                                      [&](unsigned n) { return wave_sum(times(of_group, (tiles + n - 1) / n)); });
   m.q.shares = (int)((tiles + per - 1) / per);
-  const unsigned n = of_group * m.q.shares, upto = wave_scan(n);
+  const unsigned n = times(of_group, (unsigned)m.q.shares), upto = wave_scan(n);
   m.q.first = (int)(upto - n);
   m.total = (int)last_lane(upto);
   if ((unsigned)m.total > (unsigned)x.grid) m = {0, {}, 0, -1};  // row or group starts that decrease: all read everything by themselves
@@ -196,20 +201,20 @@ __global__ __launch_bounds__(kPlan) void deal_kernel(Attend a) {
   for (int w = 0; w < kPlan / 64; ++w) own = add_sat(own, of_wave[w]);
   auto all = [&](auto of) {  // of all groups together, per kv head
     unsigned sum = 0;
-    for (int g = lane; g < x.n_groups; g += 64) sum = add_sat(sum, of(x.group[g]) * a.c.kv_heads);
+    for (int g = lane; g < x.n_groups; g += 64) sum = add_sat(sum, times(of(x.group[g]), (unsigned)a.c.kv_heads));
     return wave_sum(sum);
   };
   typedef const PrefixGroup& Q;
-  const unsigned per = share_of<kF32>(a, all([](Q q) { return q.blocks * tiles_of<kKeys>(q); }), all([](Q q) { return (unsigned)q.blocks; }),
+  const unsigned per = share_of<kF32>(a, all([](Q q) { return times((unsigned)q.blocks, tiles_of<kKeys>(q)); }), all([](Q q) { return (unsigned)q.blocks; }),
                                       all([&](Q q) { return (unsigned)(q.n * a.group); }), own,
-                                      [&](unsigned n) { return all([&](Q q) { return q.blocks * ((tiles_of<kKeys>(q) + n - 1) / n); }); });
+                                      [&](unsigned n) { return all([&](Q q) { return times((unsigned)q.blocks, (tiles_of<kKeys>(q) + n - 1) / n); }); });
   unsigned total = 0;
   for (int g0 = 0; g0 < x.n_groups; g0 += 64) {
     const int g = g0 + lane;
     PrefixGroup q = {};
     if (g < x.n_groups) q = x.group[g];
     q.shares = (int)((tiles_of<kKeys>(q) + per - 1) / per);
-    const unsigned n = (unsigned)q.blocks * a.c.kv_heads * q.shares, upto = wave_scan(n);
+    const unsigned n = times((unsigned)q.blocks * a.c.kv_heads, (unsigned)q.shares), upto = wave_scan(n);
     q.first = (int)(total + upto - n);
     if (g < x.n_groups) x.group[g] = q;
     total = add_sat(total, last_lane(upto));
