@@ -77,7 +77,7 @@ struct Chunks {
   template <typename Meanwhile>
   __device__ __forceinline__ void load(const T* row, const int (&base)[kN], int vocab, Meanwhile meanwhile) {
     const int lane = threadIdx.x & 63;
-    wide = ((uintptr_t)row & 15) == 0;
+    wide = ((uintptr_t)row & 15) == 0 && vocab >= kWide;  // chunks that are not there read the row's first 16 bytes
 #pragma unroll
     for (int c = 0; c < kN; ++c) wide = wide && (base[c] + kChunk <= vocab || base[c] >= vocab);
     if (wide) {
