@@ -445,7 +445,8 @@ int w4a32_op_verify_drafts(const w4a32_verify_args* args, void* d_scratch, size_
  * order (equal ones by index) with their log probabilities. d_tokens NULL: no token is given; d_logprob, d_rank and d_entropy may be NULL,
  * d_top_* where top is 0. A token outside the vocabulary has log probability -infinity and rank -1, as have, with token -1, places
  * behind the last token of a probability above 0 (top may pass the vocabulary). Where a logit is NaN or +infinity, or all are
- * -infinity, there is no distribution: NaN, rank -1 and tokens -1. Natural logarithms; off by 1e-6 and the rounding of the result.
+ * -infinity, there is no distribution: NaN, rank -1 and tokens -1. Natural logarithms; off by the rounding of the result and, where many logits are
+ * alike and their roundings add up, by 6e-7 (an entropy 2.1e-6) as measured, 4e-6 (3e-5) at most.
  * temperature: 1e-30 .. 1e30; top <= 1024. Per row what AutoLLM.hpp:70-88 does without saying how sure it was.
  *   d_scratch: w4a32_op_token_logprobs_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time. */
 typedef struct {
