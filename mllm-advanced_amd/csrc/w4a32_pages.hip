@@ -498,6 +498,12 @@ struct Compact {
   int *holes_before, *movers_before;  // [words]
 };
 
+// The lowest n bits, by halves as all that follows: a 64-bit shift by the last of a wavefront's registers is wrong now and then
+__device__ __forceinline__ Bits64 first_bits(int n) {
+  auto half = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1; };
+  return (Bits64)half(n - 32) << 32 | half(n);
+}
+
 __device__ __forceinline__ void compact_bits(const Compact& a, int p) {
   const int r = p < a.n_pages ? a.refs[p] : 0;
   const Bits64 used = __ballot(r != 0), mover = __ballot(r > 0);
@@ -517,7 +523,7 @@ __device__ __forceinline__ int compact_sums(const Compact& a, bool writes) {
   for (int w = w0; w < w1; ++w) mine += __popcll(a.hole[w]);
   block_scan<kSettle>(mine, in_wave, all);
   const int used = (int)all;
-  auto below = [&](int w) { return used >= 64 * (w + 1) ? ~0ull : used <= 64 * w ? 0ull : (1ull << (used - 64 * w)) - 1; };
+  auto below = [&](int w) { return first_bits(used - 64 * w); };
   unsigned movers = 0, holes = 0;
   int held = 0;
   for (int w = w0; w < w1; ++w) {
@@ -554,7 +560,7 @@ __device__ __forceinline__ int nth_hole(const Compact& a, int n) {
       hi = mid;
   }
   const Bits64 both = a.hole[lo];
-  unsigned word = (unsigned)both;  // halves: a 64-bit shift by the last of a wavefront's registers is wrong now and then
+  unsigned word = (unsigned)both;
   int in = n - a.holes_before[lo], at = 64 * lo;
   if (const int low = __popc(word); in >= low) {
     in -= low;
@@ -574,8 +580,9 @@ __device__ __forceinline__ int nth_hole(const Compact& a, int n) {
 }
 // The number that a page gets; -1: it stays
 __device__ __forceinline__ int mover_number(const Compact& a, int page) {
-  const Bits64 word = a.mover[page >> 6], bit = 1ull << (page & 63);
-  return word & bit ? a.movers_before[page >> 6] + __popcll(word & (bit - 1)) : -1;
+  const Bits64 both = a.mover[page >> 6];
+  const unsigned low = (unsigned)both, bit = 1u << (page & 31), word = page & 32 ? (unsigned)(both >> 32) : low;
+  return word & bit ? a.movers_before[page >> 6] + __popc(word & (bit - 1)) + (page & 32 ? __popc(low) : 0) : -1;
 }
 
 __device__ __forceinline__ void compact_apply(const Compact& a, int i, int pairs) {
