@@ -337,12 +337,13 @@ int w4a32_op_paged_attention(const w4a32_paged_cache* cache, const w4a32_paged_r
  * tokens from there on, the rest of the page in which the prefix ends among them. As a fork of one sequence leaves it, the prefix being what they
  * all had then, or less. A prefix beyond the length of one of the group's sequences with rows is cut to that, so that a row sees what
  * it would see alone, as long as the tables of the group's sequences that have it name the same tokens: one that has ended, with no length and no pages
- * left, may stay in its group, wherever it stands. Same results as w4a32_op_paged_attention up to the order of sums: maxima and sums are
- * f32, and each of the two parts is divided by nothing until they are joined. Group starts do not decrease; where they do, what the
+ * left, may stay in its group, wherever it stands. Same results as w4a32_op_paged_attention, its roundings included, up to the order of sums: maxima and
+ * sums are f32, and each of the two parts is divided by nothing until they are joined. Group starts do not decrease; where they do, what the
  * rows get is unspecified.
  *   d_scratch: w4a32_op_paged_prefix_attention_scratch_bytes() bytes on 16 bytes, of any contents, for one call at a time; 0 for a call that is
- * refused. It holds the sums, dim (rounded up to 64, 128 or 256) * 4 bytes for each row of a head and, below 256 workgroups, for each
- * share of a prefix that the chip is filled with. */
+ * refused. It holds sums of dim (rounded up to 64, 128 or 256) * 4 bytes: of 128 rows for each workgroup that a prefix can have (448; 896 or as many as
+ * it takes to hold the batch's rows in blocks of 128 and the groups, where those blocks are more than 224), and of up to 64 rows for each of 1536 shares and each block
+ * of rows of the own tokens. Few rows take as much as the chip: four rows of 12 heads of 128 dims 35 MB, of 16 heads of 256 dims 66 MB. */
 size_t w4a32_op_paged_prefix_attention_scratch_bytes(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, int n_groups);
 int w4a32_op_paged_prefix_attention(const w4a32_paged_cache* cache, const w4a32_paged_rows* rows, float scale,
                                     const int* d_group_start, const int* d_prefix, int n_groups, void* d_scratch,

@@ -7,12 +7,16 @@
 // alone is off by the same 2^-25 of every exponent, which would add up.
 //
 // The k most probable tokens: of the blocks' maxima the k-th largest bounds them from below, so only chunks (1 KB) of such blocks whose own maximum reaches
-// it are read again, little more than k of them, and of their logits about k reach it; those are put in order by counting. Where many are alike and do
-// not fit into LDS, the k-th largest itself is found by its bits, and of equal ones the first are taken.
+// it are read again, little more than k of them, and of their logits about k reach it; those are put in order by counting. Where more reach it than fit
+// into LDS, the k-th largest itself is found by its bits, and of equal ones the first are taken. That holds while the blocks are a good deal more than k. With
+// k blocks the bound is the least of their maxima, and with fewer there is none: then all chunks are read again, each logit that reaches the bound
+// takes a place of the list by an atomic in LDS, and beyond 2048 of them the search by bits reads all of it four times more (64 rows of 32000: 16 us with the 31
+// largest, 30 with 32, 61 with 50, of which the first launch is 5; of 65536 35 with 64 and 104 with 65; of 152064 18 with 20, 22 with 64 and 255 with 200).
 //
 // Memory bounds the first launch where rows are many (500 rows of 151936, f32, 304 MB: 48.5 us, 6.3 TB/s, read only, part of it from the cache in front; the
 // second launch takes 5), instructions and latency where they are few: 64 rows of 152064 with their 20 largest, 9.4 us of the first launch, and 8.7 of
-// the second, a chain of the ranks of 149 maxima (2 us), some 25 chunks read again (2.5), their logits' order (1.5) and barriers.
+// the second, a chain of the ranks of 149 maxima (2 us), some 25 chunks read again (2.5), their logits' order (1.5) and barriers. Logits of 16 bits are half the
+// bytes, but as many instructions: the same rows in bf16 42 and 9.0 us of the first launch, 45 and 18 of both.
 #include <type_traits>
 
 #include "w4a32_decoder.h"

@@ -11,8 +11,12 @@
 // join. A workgroup of the own tokens takes 16 us, of which its loop over tiles is 8 (the deal 2, the first loads 4, its sums 2), and there are
 // three rounds of them beside the prefix. 48 sequences of two to five rows in six groups behind 1000 to 6000 tokens, 12 heads on 2, f32 on f16: 30 and 6
 // us, as an f32 operand is two f16 terms and a tile's product waits for its loads more than it takes. Eight prompts of 60 to 300 rows behind 4099
-// tokens, 28 heads on 4, bf16: 97 GFLOP, 130 and 13 us, 865 TFLOP/s for each further token of the prefix: products and softmax of a wavefront
+// tokens, 28 heads on 4, bf16: 97 GFLOP, 133 and 13 us, 865 TFLOP/s for each further token of the prefix: products and softmax of a wavefront
 // take turns more than they overlap.
+// 256 dims: one workgroup fits on a CU, and f32 rows on a bf16 cache do not fit into its registers (70 spilled; 4 with 128 dims). Prefixes go by this kernel all
+// the same. 16 heads on 4 of 256, both launches against those of the rows on their own, us: the 64 sequences bf16 85 and 226, f32 on f16 99 and
+// 240, f32 on bf16 120 and 272, f32 180 and 581; the 48 of two to five rows 83 and 187, 98 and 202, 141 and 223, 256 and 458; the prompts 243
+// and 239, 360 and 372, 558 and 609, 1251 and 1309; four rows behind 200 tokens 16 and 15, 18 and 17, 18 and 17, 23 and 17.
 #include "w4a32_paged_prompt.h"
 #include "w4a32_paged_rows.h"
 
@@ -26,7 +30,9 @@ inline size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kPlan = 1024;      // threads of the workgroup that deals
-constexpr int kSlots = 512;      // workgroups that are there at once: two per CU
+// Workgroups that are there at once: two per CU. (256 dims: one, so that the deal's round is two there. What follows from it, here and in the rows' deal,
+// was measured on 28 heads on 4 of 128 dims in bf16 and on 12 on 2 of 128, f32 on f16, and stands for all types and sizes.)
+constexpr int kSlots = 512;
 constexpr int kMostShares = kSlots * 7 / 8;  // of prefixes, where their items are not more
 constexpr unsigned kUnits = 896;  // most workgroups where prefixes have kMostShares at most: those that find nothing take their time, too
 constexpr int kLog2 = 7;         // log2 of the rows of a workgroup of a prefix

@@ -26,7 +26,7 @@ constexpr int kShared = 1 << 30, kStays = 1 << 29, kGiven = 1 << 28, kPlace = kM
 // else nothing has changed.
 // What is moved is small (4 bytes of a place and of a page); latency bounds all of it, waits for memory and barriers of 16 wavefronts one after the
 // other. Where the counts fit into LDS: one launch of one workgroup. Else four launches, with the new table and the new counts in scratch memory (32
-// prompts of up to 32000 tokens with eight children each, 2.9 MB: 2.4 + 8.6 + 11.6 + 4.2 us, of which the third is the one workgroup that settles).
+// prompts of up to 32000 tokens with eight children each, 2.9 MB: 2.6 + 8.2 + 11.9 + 4.0 us, of which the third is the one workgroup that settles).
 // ---------------------------------------------------------------------------------------------
 struct Seq {
   int parent, len;  // -1: none; tokens
@@ -222,7 +222,8 @@ __device__ __forceinline__ int settle(const Fork& a, Counts left, SeqAt seq, Pag
 // One workgroup and four launches, us of a pass among others with a table's copy of 2: rows for sequences that go on, 64 of up to 2000 tokens (8064
 // places) 13 and 21, 500 of 1000 (31500 places) 13 and 23; with parents, eight children each, 64 of 1000 (4032 places) 13 and 24, 512 of 250 (8192) 18 and
 // 30, 128 of 2000 (16128) 21 to 23 and 25, 500 of 1000 (31500) 35 and 28; with kept lengths, 64 of 1000 13 and 20, 128 of 2000 19 and 20, 256 of 2000
-// (32256) 27 and 21. The rest is what there is room for.
+// (32256) 27 and 21. The rest is what there is room for. fork_nothing() is a part of the one launch, though it goes through no places: a decode step of 64
+// sequences takes 8 us with tables of 512 places and 15 with 513 to 8192, or with pools of 100000 to 300000 pages.
 constexpr int kNearPages = 32 * 1024, kNearSeqs = 512, kNearWritten = 1536, kNearPlaces = 32 * 1024, kNearChanged = 16 * 1024;
 
 // A step that shares nothing and gives nothing back, as most are: rows' places that name no page get free ones, and that is all. Returns
@@ -486,8 +487,8 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(Copy a) {
 // Compaction. Which pages are used and which may move are bits, 64 of a word, and a page's place among the movers or the holes
 // is the words' running sum and the bits below it. The i-th mover goes to the i-th hole: the last word whose sum does not pass i has it. One
 // workgroup adds the words up; pages and places are then gone through by all. (Lists of movers and holes written by that one workgroup, a
-// store of every bit, took 23 us for 65536 pages.) Latency bounds it: 2.5 + 8.1 us of two launches there, the second three
-// scans, a search of ten dependent reads and the names; 6.6 us of one launch for 2000 pages.
+// store of every bit, took 23 us for 65536 pages.) Latency bounds it: 2.6 + 8.1 us of two launches for 65536 pages, the second three
+// scans, a search of ten dependent reads and the names; 2.5 + 4.4 + 6.7 of three for 65537; 6.6 us of one launch for 2000 pages.
 // ---------------------------------------------------------------------------------------------
 typedef unsigned long long Bits64;
 struct Compact {
@@ -611,7 +612,8 @@ __global__ __launch_bounds__(kSettle) void compact_sums_kernel(Compact a) { comp
 __global__ __launch_bounds__(256) void compact_apply_kernel(Compact a) { compact_apply(a, blockIdx.x * 256 + threadIdx.x, a.counts[0]); }
 
 // The sums by every workgroup for itself, in LDS (65536 pages: 8.1 us where a launch of one workgroup and one of all with its searches in memory take 4.5
-// and 6.7; 14.4 against 16.6 of a pass among others, 10000 pages 13.2 against 15.8, 131072 17.6 either way)
+// and 6.7; 14.4 against 16.6 of a pass among others, 10000 pages 13.2 against 15.8, 131072 17.6 either way; with tables of some thousand places. There are as
+// many workgroups as places by 1024, and where those are rounds of the chip so are the sums: 5000 pages and tables of 512 x 8192 places 29 us, 2048 x 8192 106)
 constexpr int kWords = 1024;
 __global__ __launch_bounds__(kSettle) void compact_both_kernel(Compact a) {
   __shared__ Bits64 hole[kWords], mover[kWords];
